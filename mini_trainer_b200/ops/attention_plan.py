@@ -7,6 +7,8 @@ average against the better form, always pairs would cost 19 % (at most 90 %), al
 """
 from __future__ import annotations
 
+from collections import Counter
+
 BLOCK = 128   # rows of a query block, keys of a key block
 
 # Forward, per head_dim. one: launch, a CTA, a key tile of it. two: launch; a pair of heads, a key tile of both; a pair of row
@@ -109,3 +111,53 @@ IN_ORDER_ITERATIONS = 20
 def backward_in_order(blocks: list, hq: int, hkv: int, d: int, splits: int) -> bool:
     """Backward: whether CTAs go round the chip in order, or come early to whatever SMs are free."""
     return d == 128 and sum(b * (b + 1) for b in blocks) * (hq // hkv) >= 2 * IN_ORDER_ITERATIONS * splits * sum(blocks) > 0
+
+
+# Under a rule (attention_rule.py) a unit's length no longer follows from its block's place alone.
+
+def key_tiles(q0: int, window: int, prefix: int) -> int:
+    """Key tiles that the query rows ``[q0, q0 + BLOCK)`` of a sample look at: the prefix's and the window's."""
+    tiles = -(-prefix // BLOCK)
+    return tiles + max(0, q0 // BLOCK + 1 - max(tiles, max(0, q0 + 1 - window) // BLOCK))
+
+
+def query_blocks(k0: int, n: int, window: int, prefix: int) -> int:
+    """Query blocks of a sample of ``n`` tokens that see one of the keys ``[k0, k0 + BLOCK)``."""
+    blocks = -(-n // BLOCK)
+    return blocks if k0 < prefix else min(blocks, (k0 + BLOCK - 2 + window) // BLOCK + 1) - k0 // BLOCK
+
+
+def rule_items(cu_host, prefixes, window: int, block: int, backward: bool) -> list:
+    """Work table of a batch under a rule: rows ``(seq_start, seq_len, block_start, prefix)``, most work first, and that work."""
+    items = []
+    for a, b, p in zip(cu_host[:-1], cu_host[1:], prefixes):
+        for s0 in range(0, b - a, block):
+            last = s0 + block - BLOCK
+            work = query_blocks(s0, b - a, window, p) if backward else key_tiles(last if last < b - a else s0, window, p)
+            items.append((work, a, b - a, s0, p))
+    items.sort(key=lambda it: -it[0])
+    return items
+
+
+def rule_splits(work: list, hq: int, hkv: int, sms: int, most: int) -> int:
+    """``backward_splits`` for key blocks of these numbers of query blocks."""
+    group = hq // hkv
+    if not work or group == 1 or most <= 1:
+        return 1
+    if len(work) * hq <= sms and most >= group:
+        return group if _BWD_PARTIAL < (group - 1) * max(work) else 1
+    counts = Counter(work)
+    best, splits = float("inf"), 1
+    for s in range(1, min(group, most) + 1):
+        if s > 1 and len(work) * hkv * (s - 1) >= 2 * sms:
+            break
+        cta = _BWD_CTA + (_BWD_PARTIAL if s > 1 else 0.0)
+        t = max(finish_time([(cta + group / s * n, c * hkv * s) for n, c in counts.items()], sms), cta + -(-group // s) * max(work))
+        if t < best:
+            best, splits = t, s
+    return splits
+
+
+def rule_in_order(work: list, hq: int, hkv: int, d: int, splits: int) -> bool:
+    """``backward_in_order`` for key blocks of these numbers of query blocks."""
+    return d == 128 and sum(work) * (hq // hkv) >= IN_ORDER_ITERATIONS * splits * len(work) > 0

@@ -1,0 +1,82 @@
+"""What attention does to its scores between ``q.k`` and the softmax, beyond the causal mask of the packed samples.
+
+``AttentionRule`` is handed to ``attention`` and ``attention_bwd`` of either backend. In the order in which they apply:
+
+* ``cap``     ``s -> cap * tanh(s / cap)`` of the scaled scores
+* ``slopes``  ``s -> s - slopes[head] * |i - j|``, a bias that falls with the distance of query and key (fp32, one slope per query head; constants of
+              the model: they get no gradient)
+* ``window``  query ``i`` sees the keys ``j <= i`` with ``i - j < window`` (itself among them)
+* ``prefix``  one length per sample: all tokens of the sample see its first ``prefix`` keys, whatever the window and on either side of them
+
+so that ``i`` sees ``j`` of its own sample iff ``(j <= i and i - j < window) or j < prefix``. The diagonal is always seen: no row is empty, whatever the rule.
+A window or a prefix of zero length, negative ones and prefixes longer than their sample are refused.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+import torch
+
+_NO_WINDOW = 1 << 30
+
+
+@dataclass(frozen=True)
+class AttentionRule:
+    cap: Optional[float] = None
+    window: Optional[int] = None
+    prefix: Optional[Sequence[int]] = None   # host integers, one per sample, like the host's list of sequence starts
+    slopes: Optional[torch.Tensor] = None    # [query heads] fp32, on the device of the activations
+
+    def __post_init__(self):
+        if self.cap is not None and not 0.0 < float(self.cap) < float("inf"):
+            raise ValueError(f"a score cap is a positive number, not {self.cap}")
+        if self.window is not None and int(self.window) < 1:
+            raise ValueError(f"a window has at least the query itself, one key, not {self.window}")
+
+    @property
+    def keys(self) -> int:
+        """Keys of the window; a number beyond any sequence where there is none."""
+        return _NO_WINDOW if self.window is None else min(int(self.window), _NO_WINDOW)
+
+    def layout(self) -> tuple:
+        """What decides which tiles there are: the key of a plan."""
+        return self.keys, None if self.prefix is None else tuple(self.prefix)
+
+    def prefixes(self, cu_host) -> list:
+        """The prefix of every sample, checked against its length."""
+        lens = [b - a for a, b in zip(cu_host[:-1], cu_host[1:])]
+        if self.prefix is None:
+            return [0] * len(lens)
+        p = [int(x) for x in self.prefix]
+        if len(p) != len(lens):
+            raise ValueError(f"{len(p)} prefixes for {len(lens)} samples")
+        for x, n in zip(p, lens):
+            if not 0 <= x <= n:
+                raise ValueError(f"a prefix of {x} tokens in a sample of {n}")
+        return p
+
+    def check(self, T: int, hq: int, device, cu_host) -> None:
+        """Refuses what neither backend computes; ``cu_host``: the samples' starts and the last one's end, at most ``T``."""
+        if len(cu_host) < 1 or cu_host[0] != 0 or cu_host[-1] > T or any(b < a for a, b in zip(cu_host[:-1], cu_host[1:])):
+            raise ValueError(f"sequence starts go from 0 to at most {T} without falling")
+        s = self.slopes
+        if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (hq,) or not s.is_contiguous() or s.device != torch.device(device)):
+            raise ValueError(f"slopes are {hq} contiguous fp32 numbers on {device}, not {tuple(s.shape)} {s.dtype} on {s.device}")
+
+    # -- plain form, one sample at a time -------------------------------------------------
+    def seen(self, n: int, prefix: int, device):
+        """``[n, n]``: whether a query (row) sees a key."""
+        i, j = torch.arange(n, device=device)[:, None], torch.arange(n, device=device)[None, :]
+        return ((j <= i) & (i - j < self.keys)) | (j < prefix)
+
+    def scores(self, s, seen):
+        """``(scores, derivative of the cap)`` of scaled products ``[heads, n, n]``; the derivative is ``None`` without a cap."""
+        n, d = s.shape[-1], None
+        if self.cap is not None:
+            t = torch.tanh(s / float(self.cap))
+            s, d = float(self.cap) * t, 1.0 - t * t
+        if self.slopes is not None:
+            i = torch.arange(n, device=s.device)
+            s = s - self.slopes.to(s.dtype).view(-1, 1, 1) * (i[:, None] - i[None, :]).abs()
+        return s.masked_fill(~seen, float("-inf")), d

@@ -101,6 +101,8 @@ class _Sig:
     mtb200_moe_route_bwd = [P, P, P, P, I, I, I, I, P, P]
     mtb200_attn_fwd_one = [P, L, P, L, P, P, I, I, I, I, I, F, P, P]
     mtb200_attn_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, F, P, P]
+    mtb200_attn_rule_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, I, F, F, I, P, P, P]
+    mtb200_attn_rule_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, I, P, U, P, L, F, F, I, P, I, P, P]
     mtb200_attn_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, P, U, P, L, F, I, P, P]
 
 
@@ -181,6 +183,7 @@ class NativeOps:
         self._gemm_plans = {}   # sizes of a product, or of a grouped one -> entry point and splits, or mode
         self._epoch = itertools.count(1)   # of the launches that may split
         self._attn_plan_cache = {}
+        self._captured_plans = []   # work tables of captured launches under a rule: a graph may be replayed for as long as there is one
         self._block_specs = {}   # sizes of a block -> its products' plans
         self._pairs = None
         self.sms = torch.cuda.get_device_properties(self._index).multi_processor_count
@@ -554,12 +557,113 @@ class NativeOps:
                 work = s0 if most_work_last_block else n - s0
                 items.append((work, a, n, s0))
         items.sort(key=lambda it: -it[0])
-        table = torch.tensor([it[1:] for it in items], dtype=torch.int32)
+        return self._move_table([it[1:] for it in items])
+
+    def _move_table(self, rows):
+        table = torch.tensor(rows, dtype=torch.int32)
         if table.numel() > 8192 or torch.cuda.is_current_stream_capturing():
             table = table.pin_memory()   # (the driver stages small copies, which is faster than pinning memory for them)
         return table.to(self.device, non_blocking=True)
 
-    def attention(self, qkv, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None):
+    # -- attention under a rule (attention_rule.py) -----------------------------------------
+    def _rule_plan(self, cu_host, hq, hkv, d, rule, backward):
+        """``(work table, row_pairs)`` of a batch's forward, ``(work table, CTAs per key block, bytes of their partials, launched in order)`` of its
+        backward. Kept like the plans of the causal form. A table that a capture makes is only filled when its graph runs, so it serves that
+        launch alone; it lives, with the host memory it is copied from, as long as this backend."""
+        what = ("rule_bwd" if backward else "rule_fwd", hq, hkv, d, rule.layout())
+        capturing = torch.cuda.is_current_stream_capturing()
+        plan = self._cached(cu_host, what)
+        if plan is None:
+            prefixes, window = rule.prefixes(cu_host), rule.keys
+            if backward:
+                items = attention_plan.rule_items(cu_host, prefixes, window, 128, True)
+                work, units = [it[0] for it in items], len(items) * hkv
+                most = 1 if units * 8 > _SPLIT_COUNTERS else min(hq // hkv, _SPLIT_FLOATS // max(1, units * 2 * 128 * d))
+                splits = attention_plan.rule_splits(work, hq, hkv, self.sms, most)
+                tail = (splits, splits * units * 2 * 128 * d * 4, int(attention_plan.rule_in_order(work, hq, hkv, d, splits)))
+            else:
+                row_pairs = (hq // hkv) % 2
+                items, tail = attention_plan.rule_items(cu_host, prefixes, window, 256 if row_pairs else 128, False), (row_pairs,)
+            rows = [it[1:] for it in items]
+            if capturing:
+                host = torch.tensor(rows, dtype=torch.int32).pin_memory()
+                self._captured_plans.append(host)
+                plan = (host.to(self.device, non_blocking=True), *tail)
+            else:
+                plan = self._keep(cu_host, what, (self._move_table(rows), *tail))
+        if capturing:
+            self._captured_plans.append(plan[0])
+        return plan
+
+    def _rule_check(self, qkv, cu_host, hq, hkv, d, scale, rule, *more):
+        if self.attention_impl == "flash_attn" or d not in NATIVE_HEAD_DIMS:
+            raise ValueError(f"attention under a rule runs on the kernels for head dimensions {NATIVE_HEAD_DIMS}, not {d}"
+                             + (" with library attention" if self.attention_impl == "flash_attn" else ""))
+        if hkv < 1 or hq < 1 or hq % hkv:
+            raise ValueError(f"{hq} query heads do not share {hkv} kv heads evenly")
+        T = qkv.shape[0]
+        for t, width in ((qkv, (hq + 2 * hkv) * d), *((m, hq * d) for m in more)):
+            if t.dtype != torch.bfloat16 or t.device != qkv.device or t.dim() != 2 or t.shape != (T, width) or t.stride(1) != 1 \
+                    or (T > 1 and (t.stride(0) < width or t.stride(0) % 8)) or t.data_ptr() % 16:
+                raise ValueError(f"expected bf16 rows of {width} on {qkv.device}, 16 bytes aligned, not {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
+        if qkv.device.index not in (None, self._index):
+            raise ValueError(f"this backend was made for {self.device}, the activations are on {qkv.device}")
+        if T * hq * d >= 1 << 40 or T >= 1 << 30:
+            raise ValueError(f"{T} tokens are more than the kernels count")
+        rule.check(T, hq, qkv.device, cu_host)
+        if not 0.0 < scale < float("inf"):
+            raise ValueError(f"attention under a rule wants a positive scale, not {scale}")
+        if rule.cap is not None and not 2.0 ** -13 <= scale / float(rule.cap) <= 2.0 ** 10:
+            raise ValueError(f"a cap of {rule.cap} for scores scaled by {scale}: the kernels take caps of 2^-10 to 2^13 times the scale")
+
+    @staticmethod
+    def _pitch(t):
+        """Leading dimension; of a single row whatever fits it, as its stride says nothing."""
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    def _attention_rule(self, qkv, cu_host, hq, hkv, d, scale, rule):
+        T, rows = qkv.shape[0], cu_host[-1] if len(cu_host) else 0
+        scale = d ** -0.5 if scale is None else float(scale)
+        self._rule_check(qkv, cu_host, hq, hkv, d, scale, rule)
+        out = torch.empty(T, hq * d, dtype=qkv.dtype, device=self.device)
+        lse = torch.empty(hq, T, dtype=torch.float32, device=self.device)
+        if rows < T:   # tokens behind the last sample
+            out[rows:].zero_()
+            lse[:, rows:].zero_()
+        if rows:
+            plan, row_pairs = self._rule_plan(cu_host, hq, hkv, d, rule, False)
+            self._call("mtb200_attn_rule_fwd", qkv.data_ptr(), self._pitch(qkv), out.data_ptr(), self._pitch(out), lse.data_ptr(), plan.data_ptr(), plan.shape[0], T,
+                       rows, hq, hkv, d, row_pairs, scale, float(rule.cap or 0.0), 0 if rule.window is None else rule.keys, _ptr(rule.slopes),
+                       self.status.data_ptr(), self._st(), tag="mtb200_attn_fwd")
+        return out, lse
+
+    def _attention_rule_bwd(self, dout, qkv, out, lse, cu_host, hq, hkv, d, scale, rule):
+        T, rows = qkv.shape[0], cu_host[-1] if len(cu_host) else 0
+        scale = d ** -0.5 if scale is None else float(scale)
+        self._rule_check(qkv, cu_host, hq, hkv, d, scale, rule, out, dout)
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (hq, T) or not lse.is_contiguous() or lse.device != qkv.device:
+            raise ValueError(f"lse is what the forward returned, contiguous fp32 [{hq}, {T}], not {tuple(lse.shape)} {lse.dtype}")
+        dqkv = torch.empty(T, qkv.shape[1], dtype=qkv.dtype, device=self.device)
+        if rows < T:
+            dqkv[rows:].zero_()
+        if not rows:
+            return dqkv
+        plan, splits, nbytes, in_order = self._rule_plan(cu_host, hq, hkv, d, rule, True)
+        scratch = torch.empty(hq * T * (d + 1), dtype=torch.float32, device=self.device)
+        dq_acc, st = scratch.data_ptr(), self._st()
+        split = self._split(st, nbytes) if splits > 1 else None
+        ws, epoch, part = split or (None, 0, None)
+        self._call("mtb200_attn_rule_bwd", qkv.data_ptr(), self._pitch(qkv), out.data_ptr(), self._pitch(out), dout.data_ptr(), self._pitch(dout), dqkv.data_ptr(),
+                   self._pitch(dqkv), lse.data_ptr(), dq_acc + 4 * hq * T * d, dq_acc, plan.data_ptr(), plan.shape[0], T, rows, hq, hkv, d,
+                   splits if split else 1, _ptr(ws), epoch, _ptr(part), 4 * part.numel() if split else 0, scale, float(rule.cap or 0.0),
+                   0 if rule.window is None else rule.keys, _ptr(rule.slopes), in_order, self.status.data_ptr(), st, n=3, tag="mtb200_attn_bwd")
+        return dqkv
+
+    def attention(self, qkv, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None, rule=None):
+        """``(out [T, hq * d], lse [hq, T])`` of causal attention inside each sample; under a ``rule`` (``AttentionRule``) scores and mask are the
+        rule's, and rows behind the last sample are zero in both."""
+        if rule is not None:
+            return self._attention_rule(qkv, cu_host, hq, hkv, d, scale, rule)
         T = qkv.shape[0]
         scale = d ** -0.5 if scale is None else float(scale)
         if self.attention_impl == "flash_attn" or d not in NATIVE_HEAD_DIMS:
@@ -571,7 +675,10 @@ class NativeOps:
                    plan.data_ptr(), plan.shape[0], T, hq, hkv, d, *tail, scale, self.status.data_ptr(), self._st(), tag="mtb200_attn_fwd")
         return out, lse
 
-    def attention_bwd(self, dout, qkv, out, lse, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None):
+    def attention_bwd(self, dout, qkv, out, lse, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None, rule=None):
+        """Gradient of ``qkv``; ``rule``: the forward's. Rows behind the last sample are zero under a rule."""
+        if rule is not None:
+            return self._attention_rule_bwd(dout, qkv, out, lse, cu_host, hq, hkv, d, scale, rule)
         T = qkv.shape[0]
         scale = d ** -0.5 if scale is None else float(scale)
         if self.attention_impl == "flash_attn" or d not in NATIVE_HEAD_DIMS:

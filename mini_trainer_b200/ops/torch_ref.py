@@ -144,8 +144,11 @@ class TorchOps:
         v = qkv[:, (hq + hkv) * d:].reshape(T, hkv, d)
         return q, k, v
 
-    def attention(self, qkv, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None):
-        """Causal attention inside each ``cu_seqlens`` segment. Returns ``out [T, hq*d]``, ``lse [hq, T]``."""
+    def attention(self, qkv, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None, rule=None):
+        """Causal attention inside each ``cu_seqlens`` segment. Returns ``out [T, hq*d]``, ``lse [hq, T]``. Under a ``rule`` (``AttentionRule``)
+        scores and mask are the rule's, and rows behind the last segment are zero in both."""
+        if rule is not None:
+            return self._attention_rule(qkv, cu_seqlens, cu_host, hq, hkv, d, scale, rule)
         T = qkv.shape[0]
         q, k, v = self._split(qkv, hq, hkv, d)
         g = hq // hkv
@@ -167,7 +170,54 @@ class TorchOps:
             lse[:, a:b] = l
         return out.reshape(T, hq * d), lse
 
-    def attention_bwd(self, dout, qkv, out, lse, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None):
+    def _rule_samples(self, qkv, cu_seqlens, cu_host, hq, rule):
+        bounds = list(cu_host) if cu_host is not None else cu_seqlens.tolist()
+        rule.check(qkv.shape[0], hq, qkv.device, bounds)
+        return [(a, b, rule.seen(b - a, p, qkv.device)) for a, b, p in zip(bounds[:-1], bounds[1:], rule.prefixes(bounds)) if b > a]
+
+    def _attention_rule(self, qkv, cu_seqlens, cu_host, hq, hkv, d, scale, rule):
+        T = qkv.shape[0]
+        q, k, v = self._split(qkv, hq, hkv, d)
+        g = hq // hkv
+        scale = d ** -0.5 if scale is None else float(scale)
+        out = torch.zeros(T, hq, d, dtype=qkv.dtype, device=qkv.device)
+        lse = torch.zeros(hq, T, dtype=torch.float32, device=qkv.device)
+        for a, b, seen in self._rule_samples(qkv, cu_seqlens, cu_host, hq, rule):
+            qs = q[a:b].float().transpose(0, 1)
+            ks = k[a:b].float().transpose(0, 1).repeat_interleave(g, 0)
+            vs = v[a:b].float().transpose(0, 1).repeat_interleave(g, 0)
+            s, _ = rule.scores((qs @ ks.transpose(1, 2)) * scale, seen)
+            l = torch.logsumexp(s, -1)
+            out[a:b] = (torch.exp(s - l.unsqueeze(-1)) @ vs).transpose(0, 1).to(qkv.dtype)
+            lse[:, a:b] = l
+        return out.reshape(T, hq * d), lse
+
+    def _attention_rule_bwd(self, dout, qkv, out, lse, cu_seqlens, cu_host, hq, hkv, d, scale, rule):
+        T = qkv.shape[0]
+        q, k, v = self._split(qkv, hq, hkv, d)
+        g = hq // hkv
+        scale = d ** -0.5 if scale is None else float(scale)
+        grads = torch.zeros(T, hq + 2 * hkv, d, dtype=qkv.dtype, device=qkv.device)
+        do, o = dout.reshape(T, hq, d), out.reshape(T, hq, d)
+        for a, b, seen in self._rule_samples(qkv, cu_seqlens, cu_host, hq, rule):
+            n = b - a
+            qs = q[a:b].float().transpose(0, 1)
+            ks = k[a:b].float().transpose(0, 1).repeat_interleave(g, 0)
+            vs = v[a:b].float().transpose(0, 1).repeat_interleave(g, 0)
+            dos, os_ = do[a:b].float().transpose(0, 1), o[a:b].float().transpose(0, 1)
+            s, slope = rule.scores((qs @ ks.transpose(1, 2)) * scale, seen)
+            p = torch.exp(s - lse[:, a:b].unsqueeze(-1))
+            ds = p * (dos @ vs.transpose(1, 2) - (dos * os_).sum(-1, keepdim=True)) * scale
+            if slope is not None:
+                ds = ds * slope
+            grads[a:b, :hq] = (ds @ ks).transpose(0, 1).to(qkv.dtype)
+            grads[a:b, hq: hq + hkv] = (ds.transpose(1, 2) @ qs).reshape(hkv, g, n, d).sum(1).transpose(0, 1).to(qkv.dtype)
+            grads[a:b, hq + hkv:] = (p.transpose(1, 2) @ dos).reshape(hkv, g, n, d).sum(1).transpose(0, 1).to(qkv.dtype)
+        return grads.reshape(T, -1)
+
+    def attention_bwd(self, dout, qkv, out, lse, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None, rule=None):
+        if rule is not None:
+            return self._attention_rule_bwd(dout, qkv, out, lse, cu_seqlens, cu_host, hq, hkv, d, scale, rule)
         T = qkv.shape[0]
         q, k, v = self._split(qkv, hq, hkv, d)
         g = hq // hkv
