@@ -364,6 +364,292 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __nv_bfloat16* __re
   }
 }
 
+// ------------------------------------------------------------------------------ norms around a branch: residual sum between two RMSNorms
+// n = y * rstd_y * w_post  (POST; else n = y),   h = x + scale * gate[row] * n,   z = h * rstd_h * w_pre  (PRE)
+// in one pass: x and y are read once, h and z written once (8 bytes an element; as norm, sum and norm 14, and the first two round n in between). All of it is fp32
+// but for h, which is rounded before its norm: the norm is that of the residual stream that backward and every later block read.
+// Rows are laid out over threads as in norm_fwd_kernel, x and y side by side in a stage; BULK as there.
+template <int VPT, bool POST, bool PRE, bool BULK>
+__global__ void __launch_bounds__(EW_THREADS) residual_norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ y,
+                                                                      const __nv_bfloat16* __restrict__ w_post, const __nv_bfloat16* __restrict__ w_pre,
+                                                                      const float* __restrict__ gate, __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ z,
+                                                                      float* __restrict__ rstd_y, float* __restrict__ rstd_h, float scale, float eps, int T, int H,
+                                                                      int lanes, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  extern __shared__ __align__(128) uint8_t norm_smem[];
+  __shared__ uint64_t full[NORM_STAGES];
+  __shared__ float red[2][2][EW_THREADS / 32];   // [parity of the row set][y, h]
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int rows_per_block = EW_THREADS / lanes;
+  const int sub = threadIdx.x / lanes, l = threadIdx.x % lanes;
+  const uint32_t set_bytes = static_cast<uint32_t>(rows_per_block) * H * 2;
+  const long long step = static_cast<long long>(gridDim.x) * rows_per_block;
+  const long long first0 = static_cast<long long>(blockIdx.x) * rows_per_block;
+  auto request = [&](long long first, int s) {   // one thread
+    if (first >= T) return;
+    const uint32_t bytes = static_cast<uint32_t>(T - first < rows_per_block ? T - first : rows_per_block) * H * 2;
+    mbar_arrive_expect_tx(&full[s], 2 * bytes);
+    bulk_load(norm_smem + 2 * s * set_bytes, y + first * H, bytes, &full[s]);
+    bulk_load(norm_smem + (2 * s + 1) * set_bytes, x + first * H, bytes, &full[s]);
+  };
+  if (BULK && threadIdx.x == 0) {
+    for (int s = 0; s < NORM_STAGES; ++s) mbar_init(&full[s], 1);
+    abort_word = 0;
+    fence_mbar_init();
+    for (int s = 0; s < NORM_STAGES; ++s) request(first0 + s * step, s);
+  }
+  bf16x8 wq[POST && BULK ? VPT : 1], wz[PRE && BULK ? VPT : 1];   // weights: once per persistent block, or behind the row's own loads
+  if constexpr (BULK) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int c = (l + k * lanes) * 8;
+      if (c < H) { if constexpr (POST) wq[k].load(w_post + c); if constexpr (PRE) wz[k].load(w_pre + c); }
+    }
+    __syncthreads();
+  }
+  int it = 0;
+  for (long long first = first0; first < T; first += step, ++it) {
+    const int s = it % NORM_STAGES, par = it & 1;
+    const long long row = first + sub;
+    const bool row_ok = row < T;
+    if (BULK && !mbar_wait(&full[s], (it / NORM_STAGES) & 1, abort_flag)) { atomicExch(status, 72); break; }
+    const __nv_bfloat16* sy = BULK ? reinterpret_cast<const __nv_bfloat16*>(norm_smem + 2 * s * set_bytes) + sub * H : y + row * H;
+    const __nv_bfloat16* sx = BULK ? reinterpret_cast<const __nv_bfloat16*>(norm_smem + (2 * s + 1) * set_bytes) + sub * H : x + row * H;
+    float f[VPT][8];
+    bf16x8 xv[VPT];
+    float acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int c = (l + k * lanes) * 8;
+      bf16x8 v; v.u = xv[k].u = make_uint4(0u, 0u, 0u, 0u);
+      if (row_ok && c < H) { v.load(sy + c); xv[k].load(sx + c); }
+      v.to_float(f[k]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc += f[k][i] * f[k][i];
+    }
+    const float by = scale * (gate != nullptr && row_ok ? gate[row] : 1.f);
+    float ry = 1.f;
+    if constexpr (POST) {
+      ry = rsqrtf(group_sum(acc, red[par][0], lanes, sub) / H + eps);
+      if (row_ok && l == 0) rstd_y[row] = ry;
+    }
+    acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int c = (l + k * lanes) * 8;
+      float g[8], r[8];
+      if constexpr (POST) {
+        if (!BULK && c < H) wq[0].load(w_post + c);
+        wq[BULK ? k : 0].to_float(g);
+      }
+      xv[k].to_float(r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[k][i] = fmaf(by, POST ? f[k][i] * ry * g[i] : f[k][i], r[i]);
+      bf16x8 o; o.from_float(f[k]);
+      if (row_ok && c < H) o.store(h + row * H + c);
+      if constexpr (PRE) {
+        o.to_float(f[k]);
+        if (c < H) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc += f[k][i] * f[k][i];
+        }
+      }
+    }
+    float ss = 0.f;
+    if constexpr (PRE) ss = group_sum(acc, red[par][1], lanes, sub);
+    if (BULK) {
+      if (!PRE || lanes <= 32) __syncthreads();
+      // every thread has its part of the rows in registers: the stage may be refilled
+      if (threadIdx.x == 0) request(first + NORM_STAGES * step, s);
+    }
+    if constexpr (PRE) {
+      if (!row_ok) continue;
+      const float rh = rsqrtf(ss / H + eps);
+      if (l == 0) rstd_h[row] = rh;
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        const int c = (l + k * lanes) * 8;
+        if (c < H) {
+          float g[8];
+          if constexpr (!BULK) wz[0].load(w_pre + c);
+          wz[BULK ? k : 0].to_float(g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[k][i] = f[k][i] * rh * g[i];
+          bf16x8 o; o.from_float(f[k]); o.store(z + row * H + c);
+        }
+      }
+    }
+  }
+}
+
+// Its gradient, from that of h (dh, may be null: zero) and z (dz):
+//   dx = dh + rstd_h (g - hhat mean(g hhat)),  g = dz w_pre, hhat = h rstd_h                      (dx = dh without PRE)
+//   c = sum(dx n),  dgate = scale c,  dy = rstd_y b (dx w_post - yhat c / H),  b = scale gate     (dy = b dx without POST)
+//   partial rows of dw_post += b dx yhat and dw_pre += dz hhat, per block, behind each other
+// dx stays in fp32 between its two uses. The second reduction is the gate's gradient and the norm's correction at once. Rows arrive by bulk copies as in
+// norm_bwd_kernel, up to four of them (dh, dz, h, y) to a stage; two barriers a row. Bound by reading them and writing dx and dy, 12 bytes an element.
+template <int VPT, bool POST, bool PRE>
+__global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloat16* __restrict__ dh, const __nv_bfloat16* __restrict__ dz,
+                                                               const __nv_bfloat16* __restrict__ y, const __nv_bfloat16* __restrict__ h,
+                                                               const float* __restrict__ rstd_y, const float* __restrict__ rstd_h,
+                                                               const __nv_bfloat16* __restrict__ w_post, const __nv_bfloat16* __restrict__ w_pre,
+                                                               const float* __restrict__ gate, __nv_bfloat16* __restrict__ dx, __nv_bfloat16* __restrict__ dy,
+                                                               float* __restrict__ dgate, float* __restrict__ part, float scale, int T, int H, int stages, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  extern __shared__ __align__(128) uint8_t norm_smem[];
+  __shared__ uint64_t full[8];
+  __shared__ float red[2][2][16];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int nt = blockDim.x, wid = threadIdx.x >> 5;
+  const bool want_c = POST || dgate != nullptr, have_dh = dh != nullptr;   // y is read for c alone where there is no norm
+  const uint32_t row_bytes = static_cast<uint32_t>(H) * 2;
+  // rows of a stage: dz and h, y, dh, each where it is wanted
+  const uint32_t at_y = PRE ? 2 * row_bytes : 0u, at_dh = at_y + (want_c ? row_bytes : 0u), stage_bytes = at_dh + (have_dh ? row_bytes : 0u);
+  auto request = [&](long long row, int s) {   // one thread
+    if (row >= T) return;
+    mbar_arrive_expect_tx(&full[s], stage_bytes);
+    uint8_t* d = norm_smem + s * stage_bytes;
+    if (PRE) { bulk_load(d, dz + row * H, row_bytes, &full[s]); bulk_load(d + row_bytes, h + row * H, row_bytes, &full[s]); }
+    if (want_c) bulk_load(d + at_y, y + row * H, row_bytes, &full[s]);
+    if (have_dh) bulk_load(d + at_dh, dh + row * H, row_bytes, &full[s]);
+  };
+  for (int i = threadIdx.x; i < 64; i += nt) red[i >> 5][(i >> 4) & 1][i & 15] = 0.f;   // warps that do not exist add zeros
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    abort_word = 0;
+    fence_mbar_init();
+    for (int s = 0; s < stages; ++s) request(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+  }
+  float2 accq[POST ? VPT : 1][4], accz[PRE ? VPT : 1][4];
+  bf16x8 wq[POST ? VPT : 1], wz[PRE ? VPT : 1];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int c = (threadIdx.x + v * nt) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { if constexpr (POST) accq[v][i] = make_float2(0.f, 0.f); if constexpr (PRE) accz[v][i] = make_float2(0.f, 0.f); }
+    if constexpr (POST) { wq[v].u = make_uint4(0u, 0u, 0u, 0u); if (c < H) wq[v].load(w_post + c); }
+    if constexpr (PRE) { wz[v].u = make_uint4(0u, 0u, 0u, 0u); if (c < H) wz[v].load(w_pre + c); }
+  }
+  auto stat = [&](const float* p, long long row, float none) { return p != nullptr && row < T ? p[row] : none; };
+  float ry = POST ? stat(rstd_y, blockIdx.x, 0.f) : 1.f, rh = PRE ? stat(rstd_h, blockIdx.x, 0.f) : 0.f, by = scale * stat(gate, blockIdx.x, 1.f);
+  __syncthreads();
+  const float inv_h = 1.f / H;
+  int s = 0, it = 0;
+  uint32_t ph = 0;
+  auto load2 = [&](const uint8_t* p, int c, float2 (&f)[4]) {
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    if (c < H) u = *reinterpret_cast<const uint4*>(p + c * 2);
+    f[0] = unpack_bf16(u.x); f[1] = unpack_bf16(u.y); f[2] = unpack_bf16(u.z); f[3] = unpack_bf16(u.w);
+  };
+  auto w2 = [&](const bf16x8& w, int i) { return unpack_bf16(i == 0 ? w.u.x : i == 1 ? w.u.y : i == 2 ? w.u.z : w.u.w); };
+  auto total = [&](float d, float (&rd)[16]) {   // over the block
+    d = warp_sum(d);
+    if ((threadIdx.x & 31) == 0) rd[wid] = d;
+    __syncthreads();
+    float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 16; k += 2) t = fadd2(t, make_float2(rd[k], rd[k + 1]));
+    return t.x + t.y;
+  };
+  for (long long row = blockIdx.x; row < T; row += gridDim.x, ++it) {
+    const long long next = row + gridDim.x;
+    const float nry = POST ? stat(rstd_y, next, 0.f) : 1.f, nrh = PRE ? stat(rstd_h, next, 0.f) : 0.f, nby = scale * stat(gate, next, 1.f);
+    if (!mbar_wait(&full[s], ph, abort_flag)) { atomicExch(status, 73); break; }
+    const uint8_t* st = norm_smem + s * stage_bytes;
+    const float2 rh2 = make_float2(rh, rh), ry2 = make_float2(ry, ry), by2 = make_float2(by, by);
+    float2 dxv[VPT][4];
+    float m = 0.f;
+    if constexpr (PRE) {
+      float2 d = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        const int c = (threadIdx.x + v * nt) * 8;
+        float2 a[4], b[4];
+        load2(st, c, a); load2(st + row_bytes, c, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 hh = fmul2(b[i], rh2), g = fmul2(a[i], w2(wz[v], i));
+          d = ffma2(g, hh, d);
+          accz[v][i] = ffma2(a[i], hh, accz[v][i]);
+        }
+      }
+      m = total(d.x + d.y, red[it & 1][0]) * inv_h;
+    }
+    float2 d = make_float2(0.f, 0.f);
+    const float2 nm = make_float2(-m, -m);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int c = (threadIdx.x + v * nt) * 8;
+      float2 a[4], b[4], t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = make_float2(0.f, 0.f);
+      if (have_dh) load2(st + at_dh, c, t);
+      if constexpr (PRE) { load2(st, c, a); load2(st + row_bytes, c, b); }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (PRE) t[i] = ffma2(ffma2(fmul2(b[i], rh2), nm, fmul2(a[i], w2(wz[v], i))), rh2, t[i]);
+        dxv[v][i] = t[i];
+      }
+      if (c < H) *reinterpret_cast<uint4*>(dx + row * H + c) = make_uint4(pack_bf16(t[0].x, t[0].y), pack_bf16(t[1].x, t[1].y), pack_bf16(t[2].x, t[2].y), pack_bf16(t[3].x, t[3].y));
+      if (want_c) {
+        load2(st + at_y, c, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (POST) {
+            const float2 yh = fmul2(b[i], ry2);
+            accq[v][i] = ffma2(fmul2(t[i], by2), yh, accq[v][i]);
+            d = ffma2(fmul2(t[i], w2(wq[v], i)), yh, d);
+          } else d = ffma2(t[i], b[i], d);
+        }
+      }
+    }
+    float cn = 0.f;
+    if (want_c) {
+      cn = total(d.x + d.y, red[it & 1][1]);
+      if (dgate != nullptr && threadIdx.x == 0) dgate[row] = scale * cn;
+    }
+    // all threads are past the previous row's last reads: its stage may be refilled
+    if (threadIdx.x == 0 && it > 0) request(row + static_cast<long long>(stages - 1) * gridDim.x, s == 0 ? stages - 1 : s - 1);
+    const float2 nc = make_float2(-cn * inv_h, -cn * inv_h), f2 = make_float2(ry * by, ry * by);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int c = (threadIdx.x + v * nt) * 8;
+      if (c < H) {
+        float2 b[4], o[4];
+        if constexpr (POST) load2(st + at_y, c, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (POST) o[i] = fmul2(ffma2(fmul2(b[i], ry2), nc, fmul2(dxv[v][i], w2(wq[v], i))), f2);
+          else o[i] = fmul2(dxv[v][i], by2);
+        }
+        *reinterpret_cast<uint4*>(dy + row * H + c) = make_uint4(pack_bf16(o[0].x, o[0].y), pack_bf16(o[1].x, o[1].y), pack_bf16(o[2].x, o[2].y), pack_bf16(o[3].x, o[3].y));
+      }
+    }
+    ry = nry; rh = nrh; by = nby;
+    if (++s == stages) { s = 0; ph ^= 1; }
+  }
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int c = (threadIdx.x + v * nt) * 8;
+    if (c < H) {
+      float* dst = part + static_cast<long long>(blockIdx.x) * ((POST ? 1 : 0) + (PRE ? 1 : 0)) * H + c;
+      if constexpr (POST) {
+        *reinterpret_cast<float4*>(dst) = make_float4(accq[v][0].x, accq[v][0].y, accq[v][1].x, accq[v][1].y);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(accq[v][2].x, accq[v][2].y, accq[v][3].x, accq[v][3].y);
+        dst += H;
+      }
+      if constexpr (PRE) {
+        *reinterpret_cast<float4*>(dst) = make_float4(accz[v][0].x, accz[v][0].y, accz[v][1].x, accz[v][1].y);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(accz[v][2].x, accz[v][2].y, accz[v][3].x, accz[v][3].y);
+      }
+    }
+  }
+}
+
 // Sums of R partial rows of C columns; columns [0, D) go to out_a, the rest to out_b (a row may hold the partials of two
 // vectors; D = C when it holds one). 32 columns per block, 16 warps share the rows: a chain of R / 16 loads instead of R
 // (296 rows of 4096: 15 -> 5 us). Few rows are one thread's work per column (reduce_few_rows_kernel): with a batch of eight tokens the
@@ -1337,6 +1623,50 @@ static int launch_norm_bwd(const void* dy, const void* x, const float* mean, con
   return launch_ok();
 }
 
+template <int VPT, bool POST, bool PRE, bool BULK>
+static int launch_residual_norm_fwd(const void* x, const void* y, const void* w_post, const void* w_pre, const float* gate, void* h, void* z, float* rstd_y, float* rstd_h,
+                                    float scale, float eps, int T, int H, int lanes, int* status, cudaStream_t st) {
+  auto kern = residual_norm_fwd_kernel<VPT, POST, PRE, BULK>;
+  const int rows = EW_THREADS / lanes, smem = BULK ? NORM_STAGES * rows * H * 4 : 0;
+  int grid = cdiv(T, rows);
+  if constexpr (BULK) {
+    static bool configured = false;
+    if (!configured) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) return -4;
+      configured = true;
+    }
+    static thread_local int for_smem = -1, resident = 0;   // the occupancy of the last shape this thread launched
+    if (for_smem != smem) {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, EW_THREADS, smem) != cudaSuccess || resident < 1) return -4;
+      for_smem = smem;
+    }
+    if (grid > num_sms() * resident) grid = num_sms() * resident;
+  }
+  launch_pdl(kern, grid, EW_THREADS, smem, st, (const bf16*)x, (const bf16*)y, (const bf16*)w_post, (const bf16*)w_pre, gate, (bf16*)h, (bf16*)z, rstd_y, rstd_h, scale, eps,
+             T, H, lanes, status);
+  return launch_ok();
+}
+
+template <int VPT, bool POST, bool PRE>
+static int launch_residual_norm_bwd(const void* dh, const void* dz, const void* y, const void* h, const float* rstd_y, const float* rstd_h, const void* w_post,
+                                    const void* w_pre, const float* gate, void* dx, void* dy, float* dgate, float* part, float scale, int T, int H, int blocks, int threads,
+                                    int* status, cudaStream_t st) {
+  auto kern = residual_norm_bwd_kernel<VPT, POST, PRE>;
+  constexpr int most = 200 * 1024;
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return -4;
+    configured = true;
+  }
+  // up to four rows ahead in the block's share of the SM, two at least (8192 columns: 64 KB a stage, and one block on an SM at a time)
+  const int stage = H * 2 * ((PRE ? 2 : 0) + (POST || dgate != nullptr ? 1 : 0) + (dh != nullptr ? 1 : 0)), per_sm = cdiv(blocks, num_sms());
+  int stages = most / (per_sm * stage);
+  stages = stages > 4 ? 4 : (stages < 2 ? 2 : stages);
+  launch_pdl(kern, blocks, threads, stages * stage, st, (const bf16*)dh, (const bf16*)dz, (const bf16*)y, (const bf16*)h, rstd_y, rstd_h, (const bf16*)w_post,
+             (const bf16*)w_pre, gate, (bf16*)dx, (bf16*)dy, dgate, part, scale, T, H, stages, status);
+  return launch_ok();
+}
+
 static bool aligned16(const void* a, const void* b, const void* c) {
   return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 15) == 0;
 }
@@ -1381,6 +1711,49 @@ int mtb200_layernorm_bwd(const void* dy, const void* x, const float* mean, const
 #undef LB
   if (rc) return rc;
   reduce_rows(dw_partial, dw_out, db_out, blocks, 2 * H, H, st);
+  return launch_ok();
+}
+
+// Norms around a branch (residual_norm_fwd_kernel). w_post, w_pre, gate: null for none, not both weights null; z and rstd_h go with w_pre, rstd_y with w_post.
+int mtb200_residual_norm_fwd(const void* x, const void* y, const void* w_post, const void* w_pre, const float* gate, void* h, void* z, float* rstd_y, float* rstd_h,
+                             float scale, float eps, int T, int H, int* status, cudaStream_t st) {
+  if (T <= 0) return 0;
+  if (H <= 0 || H % 8 || H > 4 * 8 * EW_THREADS || (w_post == nullptr && w_pre == nullptr)) return -10;
+  if (!aligned16(x, y, h) || !aligned16(z, w_post, w_pre)) return -11;
+  const int vecs = H / 8;
+  int lanes = 32;
+  while (lanes < EW_THREADS && lanes * 4 < vecs) lanes *= 2;
+  const int vpt = cdiv(vecs, lanes), rows = EW_THREADS / lanes, stages = NORM_STAGES * rows * H * 4 + 1280;
+  const int fit = 227 * 1024 / stages < 8 ? 227 * 1024 / stages : 8;
+  const bool bulk = fit > 0 && 2 * cdiv(T, rows) > 5 * fit * num_sms();
+#define RF(V, A, B) (bulk ? launch_residual_norm_fwd<V, A, B, true>(x, y, w_post, w_pre, gate, h, z, rstd_y, rstd_h, scale, eps, T, H, lanes, status, st) \
+                          : launch_residual_norm_fwd<V, A, B, false>(x, y, w_post, w_pre, gate, h, z, rstd_y, rstd_h, scale, eps, T, H, lanes, status, st))
+#define RW(V) return w_post == nullptr ? RF(V, false, true) : w_pre == nullptr ? RF(V, true, false) : RF(V, true, true)
+  if (vpt <= 1) RW(1);
+  if (vpt <= 2) RW(2);
+  if (vpt <= 3) RW(3);
+  RW(4);
+#undef RW
+#undef RF
+}
+
+// part: fp32 scratch [mtb200_norm_bwd_blocks(T, H), weights, H]; dw_post / dw_pre: [H] bf16, as their weights.
+int mtb200_residual_norm_bwd(const void* dh, const void* dz, const void* y, const void* h, const float* rstd_y, const float* rstd_h, const void* w_post, const void* w_pre,
+                             const float* gate, void* dx, void* dy, float* dgate, float* part, void* dw_post, void* dw_pre, float scale, int T, int H, int* status,
+                             cudaStream_t st) {
+  if (T <= 0) return 0;
+  if (H <= 0 || H % 8 || H > 4 * 8 * EW_THREADS || (w_post == nullptr && w_pre == nullptr)) return -10;
+  if (!aligned16(dh, dz, y) || !aligned16(h, dx, dy) || !aligned16(w_post, w_pre, part)) return -11;
+  const int blocks = mtb200_norm_bwd_blocks(T, H), vpt = norm_bwd_vpt(H), threads = norm_bwd_threads(H);
+  int rc;
+#define RB(V, A, B) launch_residual_norm_bwd<V, A, B>(dh, dz, y, h, rstd_y, rstd_h, w_post, w_pre, gate, dx, dy, dgate, part, scale, T, H, blocks, threads, status, st)
+#define RW(V) rc = w_post == nullptr ? RB(V, false, true) : w_pre == nullptr ? RB(V, true, false) : RB(V, true, true)
+  if (vpt <= 1) RW(1); else RW(2);
+#undef RW
+#undef RB
+  if (rc) return rc;
+  const bool both = w_post != nullptr && w_pre != nullptr;
+  reduce_rows(part, w_post != nullptr ? dw_post : dw_pre, dw_pre, blocks, both ? 2 * H : H, H, st);
   return launch_ok();
 }
 

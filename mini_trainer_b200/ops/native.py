@@ -60,6 +60,8 @@ class _Sig:
     mtb200_rmsnorm_fwd = [P, P, P, P, F, I, I, P, P]
     mtb200_norm_bwd_blocks = [I, I]
     mtb200_rmsnorm_bwd = [P, P, P, P, P, P, P, P, I, I, P, P]
+    mtb200_residual_norm_fwd = [P, P, P, P, P, P, P, P, P, F, F, I, I, P, P]
+    mtb200_residual_norm_bwd = [P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, F, I, I, P, P]
     mtb200_layernorm_fwd = [P, P, P, P, P, P, F, I, I, P, P]
     mtb200_layernorm_bwd = [P, P, P, P, P, P, P, P, P, P, I, I, P, P]
     mtb200_rope = [P, P, P, I, L, I, I, I, P]
@@ -386,6 +388,60 @@ class NativeOps:
         self._call("mtb200_rmsnorm_bwd", dy.data_ptr(), x.data_ptr(), rstd.data_ptr(), w.data_ptr(), _ptr(add_to),
                    dx.data_ptr(), part.data_ptr(), dw_out.data_ptr(), T, H, self.status.data_ptr(), self._st(), n=2)
         return dx
+
+    # -- norms around a branch: residual sum between two RMSNorms ----------------------------
+    def _residual_norm_check(self, rows: dict, weights: dict, fp32: dict):
+        """Shapes of every argument against ``y``'s; what is ``None`` is not there."""
+        T, H = rows["y"].shape if rows["y"].dim() == 2 else (0, 0)
+        if H < 8 or H % 8 or H > 8192:
+            raise ValueError(f"rows of a multiple of 8 up to 8192 elements, not {tuple(rows['y'].shape)}")
+        for want, dtype, group in (((T, H), torch.bfloat16, rows), ((H,), torch.bfloat16, weights), ((T,), torch.float32, fp32)):
+            for name, t in group.items():
+                if t is not None and (t.dtype != dtype or tuple(t.shape) != want or not t.is_contiguous() or t.device != rows["y"].device or t.data_ptr() % 16 * (dtype == torch.bfloat16)):
+                    raise ValueError(f"{name}: expected contiguous, aligned {dtype} {want} on {rows['y'].device}, not {tuple(t.shape)} {t.dtype} on {t.device}")
+        if rows["y"].device.index not in (None, self._index):
+            raise ValueError(f"this backend was made for {self.device}, the activations are on {rows['y'].device}")
+        return T, H
+
+    def residual_norm(self, x, y, w_post, w_pre, eps, scale=1.0, gate=None):
+        """``(h, z, (rstd_y, rstd_h))`` of ``h = x + scale * gate * RMSNorm(y; w_post)`` and ``z = RMSNorm(h; w_pre)`` in one pass over ``[T, H]`` rows. ``w_post``
+        ``None``: the branch is added as it is; ``w_pre`` ``None``: no ``z``; one of them is there. ``gate`` [T] fp32, one factor per token.
+        ``h`` is rounded before its norm, nothing else on the way."""
+        if w_post is None and w_pre is None:
+            raise ValueError("a norm behind the branch, in front of the next or both: without either this is a sum")
+        T, H = self._residual_norm_check({"y": y, "x": x}, {"w_post": w_post, "w_pre": w_pre}, {"gate": gate})
+        h, z = torch.empty_like(y), None if w_pre is None else torch.empty_like(y)
+        ry, rh = (None if w is None else torch.empty(T, dtype=torch.float32, device=y.device) for w in (w_post, w_pre))
+        self._call("mtb200_residual_norm_fwd", x.data_ptr(), y.data_ptr(), _ptr(w_post), _ptr(w_pre), _ptr(gate), h.data_ptr(), _ptr(z), _ptr(ry), _ptr(rh),
+                   float(scale), eps, T, H, self.status.data_ptr(), self._st())
+        return h, z, (ry, rh)
+
+    def residual_norm_bwd(self, dh, dz, y, h, stats, w_post, w_pre, dw_post_out, dw_pre_out, scale=1.0, gate=None):
+        """``(dx, dy, dgate)`` from the gradients of ``h`` (``dh``, ``None`` for zero) and ``z`` (``dz``, ``None`` without ``w_pre``); the weights' go to ``dw_post_out`` and
+        ``dw_pre_out`` (``None`` where the weight is). ``h`` and ``stats``: what the forward returned. ``dgate`` [T] fp32, ``None`` without a gate."""
+        if w_post is None and w_pre is None:
+            raise ValueError("a norm behind the branch, in front of the next or both: without either this is a sum")
+        for name, w, others in (("w_post", w_post, (stats[0], dw_post_out)), ("w_pre", w_pre, (stats[1], dw_pre_out, dz))):
+            if any((w is None) != (t is None) for t in others):
+                raise ValueError(f"{name}, its statistics and its gradients are there together or not at all")
+        T, H = self._residual_norm_check({"y": y, "h": h, "dh": dh, "dz": dz},
+                                         {"w_post": w_post, "w_pre": w_pre, "dw_post_out": dw_post_out, "dw_pre_out": dw_pre_out},
+                                         {"gate": gate, "rstd_y": stats[0], "rstd_h": stats[1]})
+        if dh is None and w_pre is None:
+            raise ValueError("without a gradient of h or z there is nothing to do")
+        dx, dy = torch.empty_like(y), torch.empty_like(y)
+        dgate = None if gate is None else torch.empty(T, dtype=torch.float32, device=y.device)
+        if T == 0:
+            for w in (dw_post_out, dw_pre_out):
+                if w is not None:
+                    w.zero_()
+            return dx, dy, dgate
+        weights = (w_post is not None) + (w_pre is not None)
+        part = torch.empty(self._fn["mtb200_norm_bwd_blocks"](T, H) * weights * H, dtype=torch.float32, device=y.device)
+        self._call("mtb200_residual_norm_bwd", _ptr(dh), _ptr(dz), y.data_ptr(), h.data_ptr(), _ptr(stats[0]), _ptr(stats[1]), _ptr(w_post), _ptr(w_pre), _ptr(gate),
+                   dx.data_ptr(), dy.data_ptr(), _ptr(dgate), part.data_ptr(), _ptr(dw_post_out), _ptr(dw_pre_out), float(scale), T, H, self.status.data_ptr(),
+                   self._st(), n=2)
+        return dx, dy, dgate
 
     # -- layernorm (Starcoder2) -----------------------------------------------------------
     def layernorm(self, x, w, b, eps):

@@ -52,6 +52,48 @@ class TorchOps:
             dx = dx + add_to.float()
         return dx.to(x.dtype)
 
+    # -- norms around a branch: residual sum between two RMSNorms ----------------------------
+    def residual_norm(self, x, y, w_post, w_pre, eps, scale=1.0, gate=None):
+        """``(h, z, (rstd_y, rstd_h))`` of ``h = x + scale * gate * RMSNorm(y; w_post)`` and ``z = RMSNorm(h; w_pre)``; either weight may be ``None``."""
+        if w_post is None and w_pre is None:
+            raise ValueError("a norm behind the branch, in front of the next or both: without either this is a sum")
+        b = float(scale) if gate is None else float(scale) * gate.unsqueeze(1)
+        n, ry, z, rh = y.float(), None, None, None
+        if w_post is not None:
+            ry = torch.rsqrt(n.pow(2).mean(-1) + eps)
+            n = n * ry.unsqueeze(1) * w_post.float()
+        h = (x.float() + b * n).to(x.dtype)
+        if w_pre is not None:
+            rh = torch.rsqrt(h.float().pow(2).mean(-1) + eps)
+            z = (h.float() * rh.unsqueeze(1) * w_pre.float()).to(x.dtype)
+        return h, z, (ry, rh)
+
+    def residual_norm_bwd(self, dh, dz, y, h, stats, w_post, w_pre, dw_post_out, dw_pre_out, scale=1.0, gate=None):
+        """``(dx, dy, dgate)``; ``dh`` may be ``None`` (zero). Weight gradients go to ``dw_post_out`` and ``dw_pre_out``."""
+        if w_post is None and w_pre is None:
+            raise ValueError("a norm behind the branch, in front of the next or both: without either this is a sum")
+        for name, w, others in (("w_post", w_post, (stats[0], dw_post_out)), ("w_pre", w_pre, (stats[1], dw_pre_out, dz))):
+            if any((w is None) != (t is None) for t in others):
+                raise ValueError(f"{name}, its statistics and its gradients are there together or not at all")
+        if dh is None and w_pre is None:
+            raise ValueError("without a gradient of h or z there is nothing to do")
+        b = float(scale) if gate is None else float(scale) * gate.unsqueeze(1)
+        d = torch.zeros_like(y, dtype=torch.float32) if dh is None else dh.float()
+        if w_pre is not None:
+            r = stats[1].unsqueeze(1)
+            hh, g = h.float() * r, dz.float() * w_pre.float()
+            dw_pre_out.copy_((dz.float() * hh).sum(0))
+            d = d + r * (g - hh * (g * hh).mean(-1, keepdim=True))
+        n, dy = y.float(), b * d
+        if w_post is not None:
+            r = stats[0].unsqueeze(1)
+            yh = n * r
+            n, g = yh * w_post.float(), dy * w_post.float()
+            dw_post_out.copy_((dy * yh).sum(0))
+            dy = r * (g - yh * (g * yh).mean(-1, keepdim=True))
+        dgate = None if gate is None else float(scale) * (d * n).sum(-1)
+        return d.to(y.dtype), dy.to(y.dtype), dgate
+
     # -- layernorm (Starcoder2) -----------------------------------------------------------
     def layernorm(self, x, w, b, eps):
         xf = x.float()
