@@ -395,16 +395,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
           for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
             for (int x = 0; x < 32; x += 2) big[cc] = fmax3(big[cc], fabsf(__uint_as_float(sv[cc][x])), fabsf(__uint_as_float(sv[cc][x + 1])));
-          if (__all_sync(0xffffffffu, fmaxf(big[0], big[1]) <= p.r.most)) {
+          if (__all_sync(0xffffffffu, fmaxf(big[0], big[1]) <= p.r.cap.most)) {
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
               for (int x = 0; x < 32; x += 2) {
-                const float2 s = make_float2(__uint_as_float(sv[cc][x]), __uint_as_float(sv[cc][x + 1])), v = fmul2(s, cap_poly(p.r, s));
+                const float2 s = make_float2(__uint_as_float(sv[cc][x]), __uint_as_float(sv[cc][x + 1])), v = cap_pair(p.r.cap, s);
                 sv[cc][x] = __float_as_uint(v.x); sv[cc][x + 1] = __float_as_uint(v.y);
               }
           } else {
-            cap_in_place(p.r, ts, 4);
+            cap_in_place(p.r.cap, ts, 4);
             tmem_ld_32x32(ts, sv[0]);
             tmem_ld_32x32(ts + 32, sv[1]);
             tmem_ld_wait();
@@ -432,7 +432,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
               }
               const float2 e = make_float2(ex2_mufu(a.x), !EDGE && (x & 2) ? ex2_fma(a.y) : ex2_mufu(a.y));   // masked scores want exact zeros
               pk[x >> 1] = pack_bf16(e.x, e.y);
-              pr[cc * 16 + (x >> 1)] = R::CAP ? fmul2(e, ffma2(fmul2(s, splat(p.r.inv2)), s, splat(1.f))) : e;
+              pr[cc * 16 + (x >> 1)] = R::CAP ? fmul2(e, ffma2(fmul2(s, splat(p.r.cap.inv2)), s, splat(1.f))) : e;
             }
             tmem_st_32x16(ts + cc * 16, pk);
           }

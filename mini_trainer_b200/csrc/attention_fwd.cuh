@@ -454,15 +454,15 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_kernel(const __grid_c
 #pragma unroll
               for (int i = 0; i < 32; i += 2) big[c] = fmax3(big[c], fabsf(__uint_as_float(sv[c][i])), fabsf(__uint_as_float(sv[c][i + 1])));
             }
-            if (__all_sync(0xffffffffu, fmax3(fmaxf(big[0], big[1]), big[2], big[3]) <= p.r.most)) {
+            if (__all_sync(0xffffffffu, fmax3(fmaxf(big[0], big[1]), big[2], big[3]) <= p.r.cap.most)) {
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 if (EDGE && !any[c]) continue;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) put(c, i, fmul2(pair(c, i), cap_poly(p.r, pair(c, i))));
+                for (int i = 0; i < 16; ++i) put(c, i, cap_pair(p.r.cap, pair(c, i)));
               }
             } else {
-              cap_in_place(p.r, ts, 8);
+              cap_in_place(p.r.cap, ts, 8);
 #pragma unroll
               for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, sv[c]);
               tmem_ld_wait();

@@ -8,7 +8,7 @@ extern "C" int mtb200_attn_rule_bwd(const void* qkv, long long ld, const void* o
                                     const float* slopes, int in_order, int* status, cudaStream_t st) {
   using namespace mtb;
   if (n_items <= 0 || rows <= 0) return 0;
-  if (Hkv <= 0 || rows > T || !(scale > 0.f) || !att_cap_ok(scale, cap) || window < 0) return -10;
+  if (Hkv <= 0 || rows > T || !(scale > 0.f) || (cap != 0.f && !cap_ok(scale, cap)) || window < 0) return -10;
   const AttRuleArgs args = att_rule_args(scale, cap, window, slopes);
 #define BWD(C, B) bwd<Rule<C, B>>(qkv, ld, out, ldo, dout, lddo, rows, n_items, D, part_bytes, in_order != 0, delta, {reinterpret_cast<__nv_bfloat16*>(dqkv), ldq, lse, delta, dq_acc, plan, T, Hq, Hkv, Hq / Hkv, 0xffffffffu / static_cast<unsigned>(Hkv), splits, part, counters, epoch, scale, status, args}, st)
   return cap > 0.f ? (slopes ? BWD(true, true) : BWD(true, false)) : (slopes ? BWD(false, true) : BWD(false, false));

@@ -7,7 +7,7 @@ extern "C" int mtb200_attn_rule_fwd(const void* qkv, long long ld, void* out, lo
                                     int Hkv, int D, int row_pairs, float scale, float cap, int window, const float* slopes, int* status, cudaStream_t st) {
   using namespace mtb;
   if (n_items <= 0 || rows <= 0) return 0;
-  if (rows > T || !(scale > 0.f) || !att_cap_ok(scale, cap) || window < 0) return -10;
+  if (rows > T || !(scale > 0.f) || (cap != 0.f && !cap_ok(scale, cap)) || window < 0) return -10;
   const AttRuleArgs args = att_rule_args(scale, cap, window, slopes);
 #define FWD(C, B) fwd<Rule<C, B>>(qkv, ld, out, ldo, rows, D, {reinterpret_cast<__nv_bfloat16*>(out), ldo, lse, plan, n_items, T, Hq, Hkv, row_pairs, scale, status, args}, st)
   return cap > 0.f ? (slopes ? FWD(true, true) : FWD(true, false)) : (slopes ? FWD(false, true) : FWD(false, false));

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "cap.cuh"
 #include "entries.h"
 #include "ptx.cuh"
 
@@ -1295,6 +1296,71 @@ __global__ void __launch_bounds__(1024, 1) ce_row_kernel(const __nv_bfloat16* lo
   pdl_trigger();
 }
 
+// Cross-entropy of logits capped by a tanh, l = cap tanh(z / cap), from fp32 products z [R, V]: loss and dz = (softmax(l) - onehot) (1 - tanh^2) scale, rounded to
+// bf16. The products come in fp32 because the loss is a difference of numbers of their size: rounded to bf16 they would be off by up to 2^-8 of themselves,
+// and the loss with them. One block per row, two passes over it; the capped numbers are formed again in the second.
+__device__ __forceinline__ void cap8(const CapArgs& r, const float* p, float (&f)[8]) {
+  load8(p, f);
+  const float big = fmax3(fmax3(fabsf(f[0]), fabsf(f[1]), fabsf(f[2])), fmax3(fabsf(f[3]), fabsf(f[4]), fabsf(f[5])), fmaxf(fabsf(f[6]), fabsf(f[7])));
+  if (big <= r.most) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float2 v = cap_pair(r, make_float2(f[i], f[i + 1]));
+      f[i] = v.x; f[i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = cap_exact(r, f[i]);
+  }
+}
+
+__global__ void __launch_bounds__(1024) ce_capped_kernel(const float* __restrict__ logits, long long ld, const long long* __restrict__ targets, float* __restrict__ loss,
+                                                        __nv_bfloat16* __restrict__ dlogits, long long ldd, int V, CapArgs cap, float grad_scale, long long ignore_index) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float red[32];
+  const long long row = blockIdx.x;
+  const float* lr = logits + row * ld;
+  __nv_bfloat16* dr = dlogits + row * ldd;
+  const long long tgt = targets[row];
+  if (tgt == ignore_index) {
+    for (int c = threadIdx.x * 8; c < V; c += blockDim.x * 8) *reinterpret_cast<uint4*>(dr + c) = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) loss[row] = 0.f;
+    return;
+  }
+  float m = -INFINITY, s = 0.f;
+  for (int c = threadIdx.x * 8; c < V; c += blockDim.x * 8) {
+    float v[8];
+    cap8(cap, lr + c, v);
+    const float mx = fmax3(fmax3(v[0], v[1], v[2]), fmax3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
+    if (mx > m) { s *= ex2_mufu(m - mx); m = mx; }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += ex2_mufu(v[i] - m);
+  }
+  const float gm = block_max(m, red);
+  const float gs = block_sum(m == -INFINITY ? 0.f : s * ex2_mufu(m - gm), red);   // (a thread without columns)
+  if (threadIdx.x == 0) {
+    float t = NAN;   // of a target that is no column
+    if (tgt >= 0 && tgt < V) {
+      const float z = lr[tgt];
+      t = fabsf(z) <= cap.most ? cap_pair(cap, splat(z)).x : cap_exact(cap, z);
+    }
+    loss[row] = 0.6931471805599453f * ((gm - t) + log2f(gs));
+  }
+  const float inv = grad_scale / gs;
+  for (int c = threadIdx.x * 8; c < V; c += blockDim.x * 8) {
+    float v[8];
+    cap8(cap, lr + c, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float p = ex2_mufu(v[i] - gm) * inv;
+      if (tgt - c == i) p -= grad_scale;
+      v[i] = p * fmaf(v[i] * cap.inv2, v[i], 1.f);
+    }
+    bf16x8 o; o.from_float(v); o.store(dr + c);
+  }
+}
+
 // ------------------------------------------------------------------------------ column sums (bias grad)
 // part[split, c] = sum over this split's rows of x[r, c]; then reduce_rows_kernel. A lane adds V neighbouring columns of every
 // eighth row: V = 8 (16-byte loads) where rows are 16-byte aligned, V = 2 for any even width, and for few columns and rows, where more
@@ -1931,6 +1997,17 @@ int mtb200_ce_fwd_bwd(const void* logits, long long ld, int logits_bf16, const f
   }
   if (stats) CE(bf16, true); else if (logits_bf16) CE(bf16, false); else CE(float, false);
 #undef CE
+  return launch_ok();
+}
+
+// logits: fp32 [R, ld]; dlogits: bf16 [R, ldd], another buffer.
+int mtb200_ce_capped(const float* logits, long long ld, const long long* targets, float* loss, void* dlogits, long long ldd, int R, int V, float cap, float grad_scale,
+                     long long ignore_index, cudaStream_t st) {
+  if (R <= 0) return 0;
+  if (V <= 0 || V % 8 || ld % 8 || ldd % 8 || !cap_ok(1.f, cap)) return -10;
+  if (!aligned16(logits, dlogits, nullptr)) return -11;
+  const int threads = cdiv(V, 8 * 32) * 32;
+  launch_pdl(ce_capped_kernel, R, threads < 1024 ? threads : 1024, 0, st, logits, ld, targets, loss, (bf16*)dlogits, ldd, V, cap_args(1.f, cap), grad_scale, ignore_index);
   return launch_ok();
 }
 

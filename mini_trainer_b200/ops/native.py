@@ -82,6 +82,7 @@ class _Sig:
     mtb200_embedding_bwd_scan = [P, P, P, I, I, I, P, P]
     mtb200_scatter_rows = [P, P, P, P, P, I, I, I, P, P]
     mtb200_ce_fwd_bwd = [P, L, I, P, P, P, P, L, I, I, F, L, P]
+    mtb200_ce_capped = [P, L, P, P, P, L, I, I, F, F, L, P]
     mtb200_colsum = [P, L, P, P, I, I, P]
     mtb200_accumulate = [P, P, L, I, I, P]
     mtb200_f32_to_bf16 = [P, P, L, I, P]
@@ -669,7 +670,7 @@ class NativeOps:
         rule.check(T, hq, qkv.device, cu_host)
         if not 0.0 < scale < float("inf"):
             raise ValueError(f"attention under a rule wants a positive scale, not {scale}")
-        if rule.cap is not None and not 2.0 ** -13 <= scale / float(rule.cap) <= 2.0 ** 10:
+        if rule.cap is not None and not 2.0 ** -13 <= scale / float(rule.cap) <= 2.0 ** 10:   # cap_ok of csrc/cap.cuh
             raise ValueError(f"a cap of {rule.cap} for scores scaled by {scale}: the kernels take caps of 2^-10 to 2^13 times the scale")
 
     @staticmethod
@@ -955,12 +956,54 @@ class NativeOps:
         # and 1777 us, 8000 x 32000 x 2048 899 and 1002, x 1536 744 and 821, but x 1024 702 and 622; 8000 x 512 x 64 50 and 15.
         return V > 16384 and H >= 1536
 
-    def linear_ce(self, x, w, targets, grad_scale, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0):
+    def _linear_ce_capped(self, x, w, targets, grad_scale, dw_out, accumulate_dw, ignore_index, logit_scale, softcap):
+        """``linear_ce`` with capped logits. The products are kept in fp32 until they are capped, in half as many rows at a time, and their gradient goes to a
+        buffer of its own; nothing is held between calls."""
+        ok = x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1]
+        if not ok or any(t.dtype != torch.bfloat16 or t.device != x.device or not t.is_contiguous() or t.data_ptr() % 16 for t in (x, w, dw_out)) or dw_out.shape != w.shape:
+            raise ValueError("expected contiguous bf16 rows [T, H], a weight [V, H] and its gradient on one device")
+        T, H = x.shape
+        V = w.shape[0]
+        if H < 8 or H % 8 or V < 8 or V % 8:
+            raise ValueError(f"a weight of multiples of 8, not {V} x {H}")
+        if targets.dtype != torch.int64 or tuple(targets.shape) != (T,) or not targets.is_contiguous() or targets.device != x.device:
+            raise ValueError(f"targets are {T} contiguous int64 numbers on {x.device}")
+        if x.device.index not in (None, self._index):
+            raise ValueError(f"this backend was made for {self.device}, the activations are on {x.device}")
+        if not 2.0 ** -10 <= softcap <= 2.0 ** 13:
+            raise ValueError(f"logits are capped at 2^-10 to 2^13, not {softcap}")
+        loss, dx = torch.empty(T, dtype=torch.float32, device=x.device), torch.empty_like(x)
+        if T == 0:
+            if not accumulate_dw:
+                dw_out.zero_()
+            return loss, dx
+        ck = min(max(1, self.ce_chunk // 2), T)
+        z, dz = torch.empty(ck, V, dtype=torch.float32, device=x.device), torch.empty(ck, V, dtype=torch.bfloat16, device=x.device)
+        dw32 = None if T <= ck else torch.empty(V, H, dtype=torch.float32, device=x.device)
+        for a in range(0, T, ck):
+            n = min(ck, T - a)
+            xc = x[a:a + n]
+            self.gemm(xc, False, w, False, z, n, V, H, alpha=logit_scale)
+            self._call("mtb200_ce_capped", z.data_ptr(), V, targets[a:a + n].data_ptr(), loss[a:a + n].data_ptr(), dz.data_ptr(), V, n, V, softcap, float(grad_scale),
+                       ignore_index, self._st())
+            self.gemm(dz, False, w, True, dx[a:a + n], n, H, V, alpha=logit_scale)
+            if dw32 is None:
+                self.gemm(dz, True, x, True, dw_out, V, H, n, residual=dw_out if accumulate_dw else None, alpha=logit_scale)
+            else:
+                self.gemm(dz, True, xc, True, dw32, V, H, n, residual=dw32 if a else None, alpha=logit_scale)
+        if dw32 is not None:
+            self._call("mtb200_f32_to_bf16", dw_out.data_ptr(), dw32.data_ptr(), V * H, int(accumulate_dw), self._st())
+        return loss, dx
+
+    def linear_ce(self, x, w, targets, grad_scale, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0, softcap=None):
         """Per-token CE of ``logit_scale * x @ w.T``. Chunked over tokens (8192 rows): bf16 logits chunk
         by the tcgen05 GEMM (fp32 accumulation, one rounding: what the reference's fused linear-CE holds
         too), whose epilogue also leaves softmax statistics where that pays -> loss and the bf16 gradient written over the logits -> dX
         chunk and dW accumulation, again on the tcgen05 GEMM. Only ``[chunk, V]`` logits ever exist.
-        dW is accumulated in fp32 over the chunks and rounded to bf16 once."""
+        dW is accumulated in fp32 over the chunks and rounded to bf16 once.
+        ``softcap``: the logits are ``softcap * tanh(logit_scale * x @ w.T / softcap)``."""
+        if softcap is not None:
+            return self._linear_ce_capped(x, w, targets, grad_scale, dw_out, accumulate_dw, ignore_index, logit_scale, float(softcap))
         T, H = x.shape
         V = w.shape[0]
         loss = torch.empty(T, dtype=torch.float32, device=self.device)

@@ -331,14 +331,16 @@ class TorchOps:
         return self.gelu_bwd(dy, x), self.gelu(x)
 
     # -- fused linear + cross-entropy ---------------------------------------------------
-    def linear_ce(self, x, w, targets, grad_scale, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0):
+    def linear_ce(self, x, w, targets, grad_scale, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0, softcap=None):
         """Per-token CE of ``logit_scale * x @ w.T`` against ``targets`` without materialising all logits.
 
         Returns ``(loss [T] fp32, dx [T, H])``; ``dw_out`` receives (or accumulates) ``dW``.
         Gradients are those of ``grad_scale * sum(loss)``, the uniform upstream scale the
-        training loop applies (reference train.py:98-102).
+        training loop applies (reference train.py:98-102). ``softcap``: the logits are ``softcap * tanh(logit_scale * x @ w.T / softcap)``.
         """
         T = x.shape[0]
+        if softcap is not None and not 0.0 < float(softcap) < float("inf"):
+            raise ValueError(f"a cap of the logits is a positive number, not {softcap}")
         loss = torch.zeros(T, dtype=torch.float32, device=x.device)
         dx = torch.empty_like(x)
         dw = torch.zeros(w.shape, dtype=torch.float32, device=x.device)
@@ -347,6 +349,9 @@ class TorchOps:
             b = min(T, a + self.ce_chunk)
             xc, tc = x[a:b].float(), targets[a:b]
             logits = (xc @ wf.t()) * logit_scale
+            if softcap is not None:
+                t = torch.tanh(logits / softcap)
+                logits = softcap * t
             valid = tc != ignore_index
             safe = tc.clamp_min(0)
             lse = torch.logsumexp(logits, -1)
@@ -354,6 +359,8 @@ class TorchOps:
             loss[a:b] = torch.where(valid, lse - picked, torch.zeros_like(lse))
             dl = torch.softmax(logits, -1)
             dl[torch.arange(b - a, device=x.device), safe] -= 1.0
+            if softcap is not None:
+                dl = dl * (1.0 - t * t)
             dl = dl * (valid.float() * grad_scale).unsqueeze(1)
             dl = dl.to(x.dtype).float() * logit_scale  # the kernels round dlogits to the storage dtype
             dx[a:b] = (dl @ wf).to(x.dtype)

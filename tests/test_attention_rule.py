@@ -1,7 +1,7 @@
 """Attention under a rule (score cap, bias by distance, window, prefix): the plain backend on the CPU and the kernels, against 64 bits.
 
 Tolerances count roundings. A rounding to bf16 is off by at most U = 2^-8 of the value. out = sum p v: every p is rounded once and the sum once;
-an exponential is off by at most 1.0e-4 (the cubic), a capped score by 6.1e-6 of itself. dS = p (dP - delta) c is rounded once, its delta is formed
+an exponential is off by at most 1.0e-4 (the cubic), a capped score by 5.1e-7 of itself within the cap and 2^-21 of the cap beyond it. dS = p (dP - delta) c is rounded once, its delta is formed
 with the rounded out; dQ, dK and dV are rounded once. ``bounds`` adds these up entry by entry."""
 import math
 
@@ -14,7 +14,7 @@ from mini_trainer_b200.ops.torch_ref import TorchOps
 
 U = torch.finfo(torch.bfloat16).eps / 2
 EXP = 1.0e-4 + 2.0 ** -20
-CAP = 6.1e-6
+CAP = 5.1e-7
 
 
 def starts(lens):
@@ -72,7 +72,7 @@ def exact(qkv, cu, hq, hkv, d, rule, dout=None, scale=None):
             p = torch.exp(z - l[:, None])
             o = p @ v
             # a score's own error: the product of rows in fp32, the cap's polynomial, its place in the bias
-            dz = (2.0 ** -18 * (q.abs() @ k.abs().t()) * scale + CAP * size + 2.0 ** -21 * size).masked_fill(~see, 0.0)
+            dz = (2.0 ** -18 * (q.abs() @ k.abs().t()) * scale + CAP * size + 2.0 ** -21 * (rule.cap or 0.0) + 2.0 ** -21 * size).masked_fill(~see, 0.0)
             rel = EXP + dz + (p * (dz + EXP)).sum(1, keepdim=True)   # of p, normalised
             out[a:b, h], lse[h, a:b] = o, l
             eo = (p * (U + rel)) @ v.abs() + U * o.abs()
@@ -83,7 +83,7 @@ def exact(qkv, cu, hq, hkv, d, rule, dout=None, scale=None):
             dp, delta = do @ v.t(), (do * o).sum(1, keepdim=True)
             ds = p * (dp - delta) * c * scale
             edelta = (do.abs() * 1.1 * eo).sum(1, keepdim=True) + 2.0 ** -18 * (do.abs() * o.abs()).sum(1, keepdim=True)
-            eds = (U + 2 * rel) * ds.abs() + p * c * scale * (edelta + 2.0 ** -18 * (do.abs() @ v.abs().t())) + 3 * CAP * p * (dp - delta).abs() * scale
+            eds = (U + 2 * rel) * ds.abs() + p * c * scale * (edelta + 2.0 ** -18 * (do.abs() @ v.abs().t())) + (3 * CAP + 2.0 ** -20) * p * (dp - delta).abs() * scale
             grad[a:b, h] += ds @ k
             grad[a:b, hq + h // g] += ds.t() @ q
             grad[a:b, hq + hkv + h // g] += p.t() @ do
