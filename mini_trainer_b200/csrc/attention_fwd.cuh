@@ -430,79 +430,13 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_kernel(const __grid_c
         if constexpr (R::BIAS) slope2 = p.r.slopes[g == 0 ? w.h[0] : w.h[1]] * 1.4426950408889634f;
         auto rule_tile = [&](auto edge, int j, int k0) -> bool {
           constexpr bool EDGE = decltype(edge)::value, FORM = R::BIAS || R::CAP;
-          constexpr int FMA = EDGE ? 32 : POLY;   // masked scores want exact zeros, which the cubic does not give
-          uint32_t sv[4][32];
+          constexpr int FMA = EDGE || R::CAP ? 32 : POLY;   // masked scores want exact zeros, which the cubic does not give; the cap's polynomial fills the FMA pipe as it is
+          uint32_t sv[4][32], seen[4];
+          bool any[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, sv[c]);
           tmem_ld_wait();
-          uint32_t seen[4];
-          bool any[4];   // of the warp's rows
-          if constexpr (EDGE) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              seen[c] = att_keys_seen(p.r, qpos, k0 + c * 32, w.prefix);
-              any[c] = __any_sync(0xffffffffu, seen[c] != 0u);
-            }
-          }
-          auto pair = [&](int c, int i) { return make_float2(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1])); };
-          auto put = [&](int c, int i, float2 v) { sv[c][2 * i] = __float_as_uint(v.x); sv[c][2 * i + 1] = __float_as_uint(v.y); };
-          if constexpr (R::CAP) {
-            float big[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              big[c] = 0.f;
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) big[c] = fmax3(big[c], fabsf(__uint_as_float(sv[c][i])), fabsf(__uint_as_float(sv[c][i + 1])));
-            }
-            if (__all_sync(0xffffffffu, fmax3(fmaxf(big[0], big[1]), big[2], big[3]) <= p.r.cap.most)) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                if (EDGE && !any[c]) continue;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) put(c, i, cap_pair(p.r.cap, pair(c, i)));
-              }
-            } else {
-              cap_in_place(p.r.cap, ts, 8);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, sv[c]);
-              tmem_ld_wait();
-            }
-          }
-          if constexpr (R::BIAS) {
-            auto add = [&](int c, int i, float2 b) { put(c, i, R::CAP ? fadd2(pair(c, i), b) : ffma2(pair(c, i), sl2v, b)); };
-            const float from = static_cast<float>(k0 - qpos);
-            if (w.prefix > k0 && k0 + ATT_B - 1 > qpos - r) {   // keys behind the query are only seen in a prefix
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) add(c, i, make_float2(-slope2 * fabsf(from + (c * 32 + 2 * i)), -slope2 * fabsf(from + (c * 32 + 2 * i + 1))));
-            } else {
-              float2 off[4];   // within 8 keys
-#pragma unroll
-              for (int i = 0; i < 4; ++i) off[i] = make_float2(slope2 * (2 * i), slope2 * (2 * i + 1));
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                if (EDGE && !any[c]) continue;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) add(c, i, fadd2(off[i & 3], splat(slope2 * (from + (c * 32 + (i >> 2) * 8)))));
-              }
-            }
-          }
-          float mc[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            mc[c] = -INFINITY;
-            if constexpr (EDGE) {
-              if (!any[c]) continue;
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(seen[c] >> i & 1u)) sv[c][i] = 0xff800000u;   // -inf
-            }
-            mc[c] = fmaxf(__uint_as_float(sv[c][0]), __uint_as_float(sv[c][1]));
-#pragma unroll
-            for (int i = 2; i < 32; i += 2) mc[c] = fmax3(mc[c], __uint_as_float(sv[c][i]), __uint_as_float(sv[c][i + 1]));
-          }
-        float mt = fmax3(fmaxf(mc[0], mc[1]), mc[2], mc[3]);
+          float mt = att_form<R, EDGE, 4>(p.r, sv, seen, any, qpos, k0, w.prefix, w.prefix > k0 && k0 + ATT_B - 1 > qpos - r, slope2, sl2v, ts);
           if constexpr (!FORM) mt *= sl2;   // (-inf stays: the scale is positive)
           float factor = 1.f;
           bool rescale = false;
@@ -533,7 +467,8 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_kernel(const __grid_c
             if (!EDGE || any[c]) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                const float2 x = FORM ? fadd2(pair(c, i), nmo) : ffma2(pair(c, i), sl2v, nmo);
+                const float2 s = make_float2(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1]));
+                const float2 x = FORM ? fadd2(s, nmo) : ffma2(s, sl2v, nmo);
                 const float2 e = (i % FMA == FMA - 1) ? ex2_fma2(x) : make_float2(ex2_mufu(x.x), ex2_mufu(x.y));
                 l2[i & 1] = fadd2(l2[i & 1], e);
                 pk[i] = pack_bf16(e.x, e.y);

@@ -139,6 +139,23 @@ def rule_items(cu_host, prefixes, window: int, block: int, backward: bool) -> li
     return items
 
 
+def rule_in_pairs(work: list, pair_work, hq: int, hkv: int, d: int, sms: int) -> bool:
+    """``forward_in_pairs`` for row blocks of these numbers of key tiles. ``pair_work()``: where heads do not pair up, ``(tiles, has a partner)`` of every pair
+    of row blocks."""
+    if not work:
+        return True
+    if len(work) * hq <= sms:
+        return False
+    launch, a, b = _ONE[d]
+    one = launch + finish_time([(a + b * n, c * hq) for n, c in Counter(work).items()], sms)
+    launch, a, b, ra, rb, la, lb = _TWO[d]
+    if (hq // hkv) % 2 == 0:
+        units = [(a + b * n, c * hq // 2) for n, c in Counter(work).items()]
+    else:
+        units = [((ra + rb * n) if two else (la + lb * n), c * hq) for (n, two), c in Counter(pair_work()).items()]
+    return launch + finish_time(units, sms) <= one
+
+
 def rule_splits(work: list, hq: int, hkv: int, sms: int, most: int) -> int:
     """``backward_splits`` for key blocks of these numbers of query blocks."""
     group = hq // hkv

@@ -33,22 +33,17 @@ class AttentionRule:
             raise ValueError(f"a score cap is a positive number, not {self.cap}")
         if self.window is not None and int(self.window) < 1:
             raise ValueError(f"a window has at least the query itself, one key, not {self.window}")
-
-    @property
-    def keys(self) -> int:
-        """Keys of the window; a number beyond any sequence where there is none."""
-        return _NO_WINDOW if self.window is None else min(int(self.window), _NO_WINDOW)
-
-    def layout(self) -> tuple:
-        """What decides which tiles there are: the key of a plan."""
-        return self.keys, None if self.prefix is None else tuple(self.prefix)
+        own = object.__setattr__
+        own(self, "prefix", None if self.prefix is None else tuple(int(x) for x in self.prefix))
+        own(self, "keys", _NO_WINDOW if self.window is None else min(int(self.window), _NO_WINDOW))   # of the window; beyond any sample where there is none
+        own(self, "key", (0.0 if self.cap is None else float(self.cap), 0 if self.window is None else self.keys, self.prefix))   # what a plan depends on
 
     def prefixes(self, cu_host) -> list:
         """The prefix of every sample, checked against its length."""
         lens = [b - a for a, b in zip(cu_host[:-1], cu_host[1:])]
         if self.prefix is None:
             return [0] * len(lens)
-        p = [int(x) for x in self.prefix]
+        p = list(self.prefix)
         if len(p) != len(lens):
             raise ValueError(f"{len(p)} prefixes for {len(lens)} samples")
         for x, n in zip(p, lens):
@@ -56,13 +51,16 @@ class AttentionRule:
                 raise ValueError(f"a prefix of {x} tokens in a sample of {n}")
         return p
 
-    def check(self, T: int, hq: int, device, cu_host) -> None:
-        """Refuses what neither backend computes; ``cu_host``: the samples' starts and the last one's end, at most ``T``."""
+    def check_slopes(self, hq: int, like) -> None:
+        s = self.slopes
+        if s is not None and (s.dtype is not torch.float32 or s.shape != (hq,) or not s.is_contiguous() or s.get_device() != like.get_device()):
+            raise ValueError(f"slopes are {hq} contiguous fp32 numbers on {like.device}, not {tuple(s.shape)} {s.dtype} on {s.device}")
+
+    @staticmethod
+    def check_starts(cu_host, T: int) -> None:
+        """``cu_host``: the samples' starts and the last one's end, at most ``T``."""
         if len(cu_host) < 1 or cu_host[0] != 0 or cu_host[-1] > T or any(b < a for a, b in zip(cu_host[:-1], cu_host[1:])):
             raise ValueError(f"sequence starts go from 0 to at most {T} without falling")
-        s = self.slopes
-        if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (hq,) or not s.is_contiguous() or s.device != torch.device(device)):
-            raise ValueError(f"slopes are {hq} contiguous fp32 numbers on {device}, not {tuple(s.shape)} {s.dtype} on {s.device}")
 
     # -- plain form, one sample at a time -------------------------------------------------
     def seen(self, n: int, prefix: int, device):

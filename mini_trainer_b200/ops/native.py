@@ -105,6 +105,7 @@ class _Sig:
     mtb200_attn_fwd_one = [P, L, P, L, P, P, I, I, I, I, I, F, P, P]
     mtb200_attn_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, F, P, P]
     mtb200_attn_rule_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, I, F, F, I, P, P, P]
+    mtb200_attn_rule_fwd_one = [P, L, P, L, P, P, I, I, I, I, I, I, F, F, I, P, P, P]
     mtb200_attn_rule_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, I, P, U, P, L, F, F, I, P, I, P, P]
     mtb200_attn_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, P, U, P, L, F, I, P, P]
 
@@ -391,18 +392,29 @@ class NativeOps:
         return dx
 
     # -- norms around a branch: residual sum between two RMSNorms ----------------------------
-    def _residual_norm_check(self, rows: dict, weights: dict, fp32: dict):
-        """Shapes of every argument against ``y``'s; what is ``None`` is not there."""
-        T, H = rows["y"].shape if rows["y"].dim() == 2 else (0, 0)
-        if H < 8 or H % 8 or H > 8192:
-            raise ValueError(f"rows of a multiple of 8 up to 8192 elements, not {tuple(rows['y'].shape)}")
-        for want, dtype, group in (((T, H), torch.bfloat16, rows), ((H,), torch.bfloat16, weights), ((T,), torch.float32, fp32)):
-            for name, t in group.items():
-                if t is not None and (t.dtype != dtype or tuple(t.shape) != want or not t.is_contiguous() or t.device != rows["y"].device or t.data_ptr() % 16 * (dtype == torch.bfloat16)):
-                    raise ValueError(f"{name}: expected contiguous, aligned {dtype} {want} on {rows['y'].device}, not {tuple(t.shape)} {t.dtype} on {t.device}")
-        if rows["y"].device.index not in (None, self._index):
-            raise ValueError(f"this backend was made for {self.device}, the activations are on {rows['y'].device}")
-        return T, H
+    @staticmethod
+    def _is(t, shape, dtype, index):
+        return t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index
+
+    def _residual_norm_check(self, y, rows, weights, fp32):
+        """``(T, H)`` of ``y``; the other arguments against it. What is ``None`` is not there."""
+        shape, index, bf, ok = y.shape, y.get_device(), torch.bfloat16, self._is
+        if len(shape) != 2 or shape[1] < 8 or shape[1] & 7 or shape[1] > 8192:
+            raise ValueError(f"rows of a multiple of 8 up to 8192 elements, not {tuple(shape)}")
+        if index != self._index and self._index is not None:
+            raise ValueError(f"this backend was made for {self.device}, the activations are on {y.device}")
+        bits = y.data_ptr()
+        for want, dtype, group in ((shape, bf, (y, *rows)), (shape[1:], bf, weights), (shape[:1], torch.float32, fp32)):
+            for t in group:
+                if t is None:
+                    continue
+                if not ok(t, want, dtype, index):
+                    raise ValueError(f"expected contiguous {dtype} {tuple(want)} on {y.device}, not {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
+                if dtype is bf:
+                    bits |= t.data_ptr()
+        if bits & 15:
+            raise ValueError("rows and weights start on 16 bytes")
+        return shape
 
     def residual_norm(self, x, y, w_post, w_pre, eps, scale=1.0, gate=None):
         """``(h, z, (rstd_y, rstd_h))`` of ``h = x + scale * gate * RMSNorm(y; w_post)`` and ``z = RMSNorm(h; w_pre)`` in one pass over ``[T, H]`` rows. ``w_post``
@@ -410,11 +422,12 @@ class NativeOps:
         ``h`` is rounded before its norm, nothing else on the way."""
         if w_post is None and w_pre is None:
             raise ValueError("a norm behind the branch, in front of the next or both: without either this is a sum")
-        T, H = self._residual_norm_check({"y": y, "x": x}, {"w_post": w_post, "w_pre": w_pre}, {"gate": gate})
+        T, H = self._residual_norm_check(y, (x,), (w_post, w_pre), (gate,))
         h, z = torch.empty_like(y), None if w_pre is None else torch.empty_like(y)
-        ry, rh = (None if w is None else torch.empty(T, dtype=torch.float32, device=y.device) for w in (w_post, w_pre))
+        ry = None if w_post is None else torch.empty(T, dtype=torch.float32, device=y.device)
+        rh = None if w_pre is None else torch.empty(T, dtype=torch.float32, device=y.device)
         self._call("mtb200_residual_norm_fwd", x.data_ptr(), y.data_ptr(), _ptr(w_post), _ptr(w_pre), _ptr(gate), h.data_ptr(), _ptr(z), _ptr(ry), _ptr(rh),
-                   float(scale), eps, T, H, self.status.data_ptr(), self._st())
+                   scale, eps, T, H, self.status.data_ptr(), self._st())
         return h, z, (ry, rh)
 
     def residual_norm_bwd(self, dh, dz, y, h, stats, w_post, w_pre, dw_post_out, dw_pre_out, scale=1.0, gate=None):
@@ -422,12 +435,10 @@ class NativeOps:
         ``dw_pre_out`` (``None`` where the weight is). ``h`` and ``stats``: what the forward returned. ``dgate`` [T] fp32, ``None`` without a gate."""
         if w_post is None and w_pre is None:
             raise ValueError("a norm behind the branch, in front of the next or both: without either this is a sum")
-        for name, w, others in (("w_post", w_post, (stats[0], dw_post_out)), ("w_pre", w_pre, (stats[1], dw_pre_out, dz))):
-            if any((w is None) != (t is None) for t in others):
-                raise ValueError(f"{name}, its statistics and its gradients are there together or not at all")
-        T, H = self._residual_norm_check({"y": y, "h": h, "dh": dh, "dz": dz},
-                                         {"w_post": w_post, "w_pre": w_pre, "dw_post_out": dw_post_out, "dw_pre_out": dw_pre_out},
-                                         {"gate": gate, "rstd_y": stats[0], "rstd_h": stats[1]})
+        ry, rh = stats
+        if not (w_post is None) == (ry is None) == (dw_post_out is None) or not (w_pre is None) == (rh is None) == (dw_pre_out is None) == (dz is None):
+            raise ValueError("a weight, its statistics and its gradients are there together or not at all")
+        T, H = self._residual_norm_check(y, (h, dh, dz), (w_post, w_pre, dw_post_out, dw_pre_out), (gate, ry, rh))
         if dh is None and w_pre is None:
             raise ValueError("without a gradient of h or z there is nothing to do")
         dx, dy = torch.empty_like(y), torch.empty_like(y)
@@ -439,8 +450,8 @@ class NativeOps:
             return dx, dy, dgate
         weights = (w_post is not None) + (w_pre is not None)
         part = torch.empty(self._fn["mtb200_norm_bwd_blocks"](T, H) * weights * H, dtype=torch.float32, device=y.device)
-        self._call("mtb200_residual_norm_bwd", _ptr(dh), _ptr(dz), y.data_ptr(), h.data_ptr(), _ptr(stats[0]), _ptr(stats[1]), _ptr(w_post), _ptr(w_pre), _ptr(gate),
-                   dx.data_ptr(), dy.data_ptr(), _ptr(dgate), part.data_ptr(), _ptr(dw_post_out), _ptr(dw_pre_out), float(scale), T, H, self.status.data_ptr(),
+        self._call("mtb200_residual_norm_bwd", _ptr(dh), _ptr(dz), y.data_ptr(), h.data_ptr(), _ptr(ry), _ptr(rh), _ptr(w_post), _ptr(w_pre), _ptr(gate),
+                   dx.data_ptr(), dy.data_ptr(), _ptr(dgate), part.data_ptr(), _ptr(dw_post_out), _ptr(dw_pre_out), scale, T, H, self.status.data_ptr(),
                    self._st(), n=2)
         return dx, dy, dgate
 
@@ -623,97 +634,110 @@ class NativeOps:
         return table.to(self.device, non_blocking=True)
 
     # -- attention under a rule (attention_rule.py) -----------------------------------------
-    def _rule_plan(self, cu_host, hq, hkv, d, rule, backward):
-        """``(work table, row_pairs)`` of a batch's forward, ``(work table, CTAs per key block, bytes of their partials, launched in order)`` of its
-        backward. Kept like the plans of the causal form. A table that a capture makes is only filled when its graph runs, so it serves that
-        launch alone; it lives, with the host memory it is copied from, as long as this backend."""
-        what = ("rule_bwd" if backward else "rule_fwd", hq, hkv, d, rule.layout())
+    def _rule_plan(self, cu_host, hq, hkv, d, scale, rule, T, backward):
+        """``(work table, tokens of the samples, entry point, its row_pairs argument)`` of a batch's forward, ``(work table, tokens of the samples, CTAs per key
+        block, bytes of their partials, launched in order)`` of its backward. Checked when it is made and kept like the plans of the causal form, by the values
+        it depends on. A table that a capture makes is only filled when its graph runs, so it serves that launch alone; it lives, with the host
+        memory it is copied from, as long as this backend."""
+        what = (backward, hq, hkv, d, scale, rule.key)
         capturing = torch.cuda.is_current_stream_capturing()
         plan = self._cached(cu_host, what)
         if plan is None:
-            prefixes, window = rule.prefixes(cu_host), rule.keys
-            if backward:
-                items = attention_plan.rule_items(cu_host, prefixes, window, 128, True)
-                work, units = [it[0] for it in items], len(items) * hkv
-                most = 1 if units * 8 > _SPLIT_COUNTERS else min(hq // hkv, _SPLIT_FLOATS // max(1, units * 2 * 128 * d))
-                splits = attention_plan.rule_splits(work, hq, hkv, self.sms, most)
-                tail = (splits, splits * units * 2 * 128 * d * 4, int(attention_plan.rule_in_order(work, hq, hkv, d, splits)))
-            else:
-                row_pairs = (hq // hkv) % 2
-                items, tail = attention_plan.rule_items(cu_host, prefixes, window, 256 if row_pairs else 128, False), (row_pairs,)
-            rows = [it[1:] for it in items]
-            if capturing:
-                host = torch.tensor(rows, dtype=torch.int32).pin_memory()
-                self._captured_plans.append(host)
-                plan = (host.to(self.device, non_blocking=True), *tail)
-            else:
-                plan = self._keep(cu_host, what, (self._move_table(rows), *tail))
+            plan = self._make_rule_plan(cu_host, hq, hkv, d, scale, rule, T, backward, capturing)
+            if not capturing:
+                self._keep(cu_host, what, plan)
+        elif plan[1] > T:
+            rule.check_starts(cu_host, T)
         if capturing:
             self._captured_plans.append(plan[0])
         return plan
 
-    def _rule_check(self, qkv, cu_host, hq, hkv, d, scale, rule, *more):
-        if self.attention_impl == "flash_attn" or d not in NATIVE_HEAD_DIMS:
-            raise ValueError(f"attention under a rule runs on the kernels for head dimensions {NATIVE_HEAD_DIMS}, not {d}"
-                             + (" with library attention" if self.attention_impl == "flash_attn" else ""))
+    def _make_rule_plan(self, cu_host, hq, hkv, d, scale, rule, T, backward, capturing):
+        if d not in NATIVE_HEAD_DIMS:
+            raise ValueError(f"attention under a rule runs on the kernels for head dimensions {NATIVE_HEAD_DIMS}, not {d}")
         if hkv < 1 or hq < 1 or hq % hkv:
             raise ValueError(f"{hq} query heads do not share {hkv} kv heads evenly")
-        T = qkv.shape[0]
-        for t, width in ((qkv, (hq + 2 * hkv) * d), *((m, hq * d) for m in more)):
-            if t.dtype != torch.bfloat16 or t.device != qkv.device or t.dim() != 2 or t.shape != (T, width) or t.stride(1) != 1 \
-                    or (T > 1 and (t.stride(0) < width or t.stride(0) % 8)) or t.data_ptr() % 16:
-                raise ValueError(f"expected bf16 rows of {width} on {qkv.device}, 16 bytes aligned, not {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
-        if qkv.device.index not in (None, self._index):
-            raise ValueError(f"this backend was made for {self.device}, the activations are on {qkv.device}")
         if T * hq * d >= 1 << 40 or T >= 1 << 30:
             raise ValueError(f"{T} tokens are more than the kernels count")
-        rule.check(T, hq, qkv.device, cu_host)
+        rule.check_starts(cu_host, T)
+        prefixes, window = rule.prefixes(cu_host), rule.keys
         if not 0.0 < scale < float("inf"):
             raise ValueError(f"attention under a rule wants a positive scale, not {scale}")
         if rule.cap is not None and not 2.0 ** -13 <= scale / float(rule.cap) <= 2.0 ** 10:   # cap_ok of csrc/cap.cuh
             raise ValueError(f"a cap of {rule.cap} for scores scaled by {scale}: the kernels take caps of 2^-10 to 2^13 times the scale")
+        items = attention_plan.rule_items(cu_host, prefixes, window, 128, backward)
+        work = [it[0] for it in items]
+        if backward:
+            units = len(items) * hkv
+            most = 1 if units * 8 > _SPLIT_COUNTERS else min(hq // hkv, _SPLIT_FLOATS // max(1, units * 2 * 128 * d))
+            splits = attention_plan.rule_splits(work, hq, hkv, self.sms, most)
+            tail = (splits, splits * units * 2 * 128 * d * 4, int(attention_plan.rule_in_order(work, hq, hkv, d, splits)))
+        else:
+            pairs = attention_plan.rule_items(cu_host, prefixes, window, 256, False) if (hq // hkv) % 2 else []
+            if attention_plan.rule_in_pairs(work, lambda: [(it[0], it[3] + 128 < it[2]) for it in pairs], hq, hkv, d, self.sms):
+                items, tail = pairs or items, ("mtb200_attn_rule_fwd", ((hq // hkv) % 2,))
+            else:
+                tail = ("mtb200_attn_rule_fwd_one", ())
+        rows = [it[1:] for it in items]
+        if not rows:
+            table = None
+        elif capturing:
+            host = torch.tensor(rows, dtype=torch.int32).pin_memory()
+            self._captured_plans.append(host)
+            table = host.to(self.device, non_blocking=True)
+        else:
+            table = self._move_table(rows)
+        return (table, cu_host[-1], *tail)
 
-    @staticmethod
-    def _pitch(t):
-        """Leading dimension; of a single row whatever fits it, as its stride says nothing."""
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    def _rule_rows(self, t, T, width):
+        """Leading dimension of bf16 rows ``[T, width]`` on this backend's device, 16 bytes aligned; anything else is refused."""
+        if t.dtype is torch.bfloat16 and t.shape == (T, width) and not t.data_ptr() & 15 and (t.get_device() == self._index or self._index is None):
+            if t.is_contiguous():   # of a single row too, whose stride says nothing
+                return width
+            if t.stride(1) == 1 and t.stride(0) >= width and not t.stride(0) & 7:
+                return t.stride(0)
+        raise ValueError(f"expected bf16 rows of {width} on {self.device}, 16 bytes aligned, not {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
 
     def _attention_rule(self, qkv, cu_host, hq, hkv, d, scale, rule):
-        T, rows = qkv.shape[0], cu_host[-1] if len(cu_host) else 0
+        if self.attention_impl == "flash_attn":
+            raise ValueError("attention under a rule runs on the kernels, not on library attention")
+        T, width = qkv.shape[0], hq * d
         scale = d ** -0.5 if scale is None else float(scale)
-        self._rule_check(qkv, cu_host, hq, hkv, d, scale, rule)
-        out = torch.empty(T, hq * d, dtype=qkv.dtype, device=self.device)
+        table, rows, name, tail = self._rule_plan(cu_host, hq, hkv, d, scale, rule, T, False)
+        ld = self._rule_rows(qkv, T, width + 2 * hkv * d)
+        rule.check_slopes(hq, qkv)
+        out = torch.empty(T, width, dtype=qkv.dtype, device=self.device)
         lse = torch.empty(hq, T, dtype=torch.float32, device=self.device)
         if rows < T:   # tokens behind the last sample
             out[rows:].zero_()
             lse[:, rows:].zero_()
         if rows:
-            plan, row_pairs = self._rule_plan(cu_host, hq, hkv, d, rule, False)
-            self._call("mtb200_attn_rule_fwd", qkv.data_ptr(), self._pitch(qkv), out.data_ptr(), self._pitch(out), lse.data_ptr(), plan.data_ptr(), plan.shape[0], T,
-                       rows, hq, hkv, d, row_pairs, scale, float(rule.cap or 0.0), 0 if rule.window is None else rule.keys, _ptr(rule.slopes),
-                       self.status.data_ptr(), self._st(), tag="mtb200_attn_fwd")
+            self._call(name, qkv.data_ptr(), ld, out.data_ptr(), width, lse.data_ptr(), table.data_ptr(), table.shape[0], T, rows, hq, hkv, d, *tail, scale,
+                       rule.key[0], rule.key[1], _ptr(rule.slopes), self.status.data_ptr(), self._st(), tag="mtb200_attn_fwd")
         return out, lse
 
     def _attention_rule_bwd(self, dout, qkv, out, lse, cu_host, hq, hkv, d, scale, rule):
-        T, rows = qkv.shape[0], cu_host[-1] if len(cu_host) else 0
+        if self.attention_impl == "flash_attn":
+            raise ValueError("attention under a rule runs on the kernels, not on library attention")
+        T, width = qkv.shape[0], hq * d
         scale = d ** -0.5 if scale is None else float(scale)
-        self._rule_check(qkv, cu_host, hq, hkv, d, scale, rule, out, dout)
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (hq, T) or not lse.is_contiguous() or lse.device != qkv.device:
-            raise ValueError(f"lse is what the forward returned, contiguous fp32 [{hq}, {T}], not {tuple(lse.shape)} {lse.dtype}")
+        table, rows, splits, nbytes, in_order = self._rule_plan(cu_host, hq, hkv, d, scale, rule, T, True)
+        ld, ldo, lddo = self._rule_rows(qkv, T, width + 2 * hkv * d), self._rule_rows(out, T, width), self._rule_rows(dout, T, width)
+        rule.check_slopes(hq, qkv)
+        if lse.dtype is not torch.float32 or lse.shape != (hq, T) or not lse.is_contiguous() or lse.get_device() != qkv.get_device():
+            raise ValueError(f"lse is what the forward returned, contiguous fp32 [{hq}, {T}], not {tuple(lse.shape)} {lse.dtype} on {lse.device}")
         dqkv = torch.empty(T, qkv.shape[1], dtype=qkv.dtype, device=self.device)
         if rows < T:
             dqkv[rows:].zero_()
         if not rows:
             return dqkv
-        plan, splits, nbytes, in_order = self._rule_plan(cu_host, hq, hkv, d, rule, True)
-        scratch = torch.empty(hq * T * (d + 1), dtype=torch.float32, device=self.device)
+        scratch = torch.empty(hq * T * (d + 1), dtype=torch.float32, device=self.device)   # dQ's accumulator [T, hq * d] and delta [hq, T]
         dq_acc, st = scratch.data_ptr(), self._st()
         split = self._split(st, nbytes) if splits > 1 else None
         ws, epoch, part = split or (None, 0, None)
-        self._call("mtb200_attn_rule_bwd", qkv.data_ptr(), self._pitch(qkv), out.data_ptr(), self._pitch(out), dout.data_ptr(), self._pitch(dout), dqkv.data_ptr(),
-                   self._pitch(dqkv), lse.data_ptr(), dq_acc + 4 * hq * T * d, dq_acc, plan.data_ptr(), plan.shape[0], T, rows, hq, hkv, d,
-                   splits if split else 1, _ptr(ws), epoch, _ptr(part), 4 * part.numel() if split else 0, scale, float(rule.cap or 0.0),
-                   0 if rule.window is None else rule.keys, _ptr(rule.slopes), in_order, self.status.data_ptr(), st, n=3, tag="mtb200_attn_bwd")
+        self._call("mtb200_attn_rule_bwd", qkv.data_ptr(), ld, out.data_ptr(), ldo, dout.data_ptr(), lddo, dqkv.data_ptr(), qkv.shape[1], lse.data_ptr(),
+                   dq_acc + 4 * hq * T * d, dq_acc, table.data_ptr(), table.shape[0], T, rows, hq, hkv, d, splits if split else 1, _ptr(ws), epoch, _ptr(part),
+                   4 * part.numel() if split else 0, scale, rule.key[0], rule.key[1], _ptr(rule.slopes), in_order, self.status.data_ptr(), st, n=3, tag="mtb200_attn_bwd")
         return dqkv
 
     def attention(self, qkv, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None, rule=None):

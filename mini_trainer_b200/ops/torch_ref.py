@@ -214,7 +214,8 @@ class TorchOps:
 
     def _rule_samples(self, qkv, cu_seqlens, cu_host, hq, rule):
         bounds = list(cu_host) if cu_host is not None else cu_seqlens.tolist()
-        rule.check(qkv.shape[0], hq, qkv.device, bounds)
+        rule.check_starts(bounds, qkv.shape[0])
+        rule.check_slopes(hq, qkv)
         return [(a, b, rule.seen(b - a, p, qkv.device)) for a, b, p in zip(bounds[:-1], bounds[1:], rule.prefixes(bounds)) if b > a]
 
     def _attention_rule(self, qkv, cu_seqlens, cu_host, hq, hkv, d, scale, rule):

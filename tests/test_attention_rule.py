@@ -219,6 +219,15 @@ def test_backward_of_a_rule_without_edges_is_planned_as_the_causal_one():
     assert A.rule_splits([], 4, 1, 148, 4) == 1
 
 
+def test_forward_of_a_rule_without_edges_takes_the_causal_form():
+    for lens, hq, hkv, d in (([2048], 16, 4, 64), ([16384], 2, 1, 128), ([300] * 41, 16, 4, 64), ([128] * 100, 32, 8, 128), ([5000] * 4, 9, 3, 128), ([1024], 14, 2, 128), ([700] * 30, 3, 1, 64)):
+        cu = starts(lens)
+        work = [it[0] for it in A.rule_items(cu, [0] * len(lens), 1 << 30, 128, False)]
+        pairs = [(it[0], it[3] + 128 < it[2]) for it in A.rule_items(cu, [0] * len(lens), 1 << 30, 256, False)]
+        assert A.rule_in_pairs(work, lambda: pairs, hq, hkv, d, 148) == A.forward_in_pairs(A.blocks_per_sequence(cu), hq, hkv, d, 148)
+    assert A.rule_in_pairs([], list, 4, 1, 64, 148)
+
+
 def host_ops():
     from .test_native_host import make_ops
     ops = make_ops()
@@ -236,9 +245,9 @@ def test_kernel_calls_get_the_rule_and_its_table(monkeypatch):
     rule = AttentionRule(cap=30.0, window=50, prefix=[3, 0], slopes=slopes_of(4))
     out, lse = ops.attention(qkv, None, cu, 200, 4, 2, 64, rule=rule)
     name, args = ops.calls[-1]
-    assert name == "mtb200_attn_rule_fwd" and args[6:13] == (4, 336, 330, 4, 2, 64, 0) and args[14:16] == (30.0, 50) and args[16] == rule.slopes.data_ptr()
+    assert name == "mtb200_attn_rule_fwd_one" and args[6:12] == (4, 336, 330, 4, 2, 64) and args[13:15] == (30.0, 50) and args[15] == rule.slopes.data_ptr()
     assert not out[330:].any() and not lse[:, 330:].any()
-    table = ops._cached(cu, ("rule_fwd", 4, 2, 64, rule.layout()))[0]
+    table = ops._cached(cu, (False, 4, 2, 64, 0.125, rule.key))[0]
     assert sorted(map(tuple, table.tolist())) == [(0, 200, 0, 3), (0, 200, 128, 3), (200, 130, 0, 0), (200, 130, 128, 0)]
     ops.attention(qkv, None, cu, 200, 4, 2, 64, rule=AttentionRule(window=50, prefix=[4, 0]))   # another prefix is another table
     assert ops.calls[-1][1][5] != args[5]
@@ -264,7 +273,7 @@ def test_kernel_calls_refuse_what_they_cannot_address(monkeypatch):
 
     wide = torch.zeros(64, 516, dtype=torch.bfloat16)
     for bad in (qkv.float(), qkv[:, :-64], wide[:, 1:513], wide[:, :512], qkv.t().contiguous().t(), qkv[None], torch.zeros(64 * 512 + 4, dtype=torch.bfloat16)[4:].view(64, 512)):
-        refused("expected bf16 rows", lambda: ops.attention(bad, None, cu, 64, 4, 2, 64, rule=rule))
+        refused("expected bf16 rows|sequence starts", lambda: ops.attention(bad, None, cu, 64, 4, 2, 64, rule=rule))
     refused("head dimensions", lambda: ops.attention(qkv, None, cu, 64, 2, 1, 128 + 128, rule=rule))
     refused("share", lambda: ops.attention(qkv, None, cu, 64, 4, 3, 64, rule=rule))
     refused("scale", lambda: ops.attention(qkv, None, cu, 64, 4, 2, 64, scale=0.0, rule=rule))
@@ -299,9 +308,12 @@ def run(ops, case, qkv, dout, scale=None):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pairs", "one"])
 @pytest.mark.parametrize("gain", [1.0, 40.0])   # scores within the cap, and far beyond it
 @pytest.mark.parametrize("case", CASES)
-def test_kernels_against_64_bits(ops, case, gain):
+def test_kernels_against_64_bits(ops, case, gain, form, monkeypatch):
+    monkeypatch.setattr(A, "rule_in_pairs", lambda *a: form == "pairs")
+    ops._attn_plan_cache.clear()
     lens, hq, hkv, d = case[:4]
     qkv, dout = make(lens, hq, hkv, d, gain=gain, tail=5, device="cuda")
     want, bound = exact(qkv, starts(lens), hq, hkv, d, rule_of(case), dout)
@@ -310,9 +322,12 @@ def test_kernels_against_64_bits(ops, case, gain):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pairs", "one"])
 @pytest.mark.parametrize("d", [64, 128])
-def test_every_combination_on_ragged_samples(ops, d):
+def test_every_combination_on_ragged_samples(ops, d, form, monkeypatch):
     import itertools
+    monkeypatch.setattr(A, "rule_in_pairs", lambda *a: form == "pairs")
+    ops._attn_plan_cache.clear()
     for cap, window, prefix, bias, (hq, hkv) in itertools.product([None, 35.0], [None, 77], [None, [0, 140, 9]], [False, True], [(4, 2), (3, 1)]):
         case = ([201, 333, 45], hq, hkv, d, cap, window, prefix, bias)
         qkv, dout = make(case[0], hq, hkv, d, seed=hq, device="cuda")
@@ -435,8 +450,9 @@ def test_a_table_that_does_not_fit_the_batch_is_reported(ops):
     out, lse = torch.zeros(64, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 64, device="cuda")
     for row in ([0, 65, 0, 0], [-1, 64, 0, 0], [0, 64, 64, 0], [0, 64, 0, 65], [0, 64, 0, -1]):
         plan = torch.tensor([row], dtype=torch.int32, device="cuda")
-        ops._call("mtb200_attn_rule_fwd", qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), lse.data_ptr(), plan.data_ptr(), 1, 64, 64, 2, 1, 64, 0,
-                  0.125, 0.0, 5, None, ops.status.data_ptr(), ops._st())
-        with pytest.raises(RuntimeError, match="work item"):
-            ops.check_status()
+        for name, tail in (("mtb200_attn_rule_fwd", (0,)), ("mtb200_attn_rule_fwd_one", ())):
+            ops._call(name, qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), lse.data_ptr(), plan.data_ptr(), 1, 64, 64, 2, 1, 64, *tail,
+                      0.125, 0.0, 5, None, ops.status.data_ptr(), ops._st())
+            with pytest.raises(RuntimeError, match="work item"):
+                ops.check_status()
     assert not out.any() and not lse.any()
