@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __nv_bfloat16* __re
 // but for h, which is rounded before its norm: the norm is that of the residual stream that backward and every later block read.
 // Rows are laid out over threads as in norm_fwd_kernel, x and y side by side in a stage; BULK as there.
 template <int VPT, bool POST, bool PRE, bool BULK>
-__global__ void __launch_bounds__(EW_THREADS) residual_norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ y,
+__global__ void __launch_bounds__(EW_THREADS, BULK ? (VPT <= 2 ? 3 : 2) : 1) residual_norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ y,
                                                                       const __nv_bfloat16* __restrict__ w_post, const __nv_bfloat16* __restrict__ w_pre,
                                                                       const float* __restrict__ gate, __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ z,
                                                                       float* __restrict__ rstd_y, float* __restrict__ rstd_h, float scale, float eps, int T, int H,
@@ -406,6 +406,8 @@ __global__ void __launch_bounds__(EW_THREADS) residual_norm_fwd_kernel(const __n
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int c = (l + k * lanes) * 8;
+      if constexpr (POST) wq[k].u = make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (PRE) wz[k].u = make_uint4(0u, 0u, 0u, 0u);
       if (c < H) { if constexpr (POST) wq[k].load(w_post + c); if constexpr (PRE) wz[k].load(w_pre + c); }
     }
     __syncthreads();
@@ -418,48 +420,45 @@ __global__ void __launch_bounds__(EW_THREADS) residual_norm_fwd_kernel(const __n
     if (BULK && !mbar_wait(&full[s], (it / NORM_STAGES) & 1, abort_flag)) { atomicExch(status, 72); break; }
     const __nv_bfloat16* sy = BULK ? reinterpret_cast<const __nv_bfloat16*>(norm_smem + 2 * s * set_bytes) + sub * H : y + row * H;
     const __nv_bfloat16* sx = BULK ? reinterpret_cast<const __nv_bfloat16*>(norm_smem + (2 * s + 1) * set_bytes) + sub * H : x + row * H;
-    float f[VPT][8];
-    bf16x8 xv[VPT];
-    float acc = 0.f;
+    auto two = [](const uint4& u, int i) { return unpack_bf16(i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w); };
+    float2 f[VPT][4];
+    uint4 xv[VPT];
+    float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int c = (l + k * lanes) * 8;
-      bf16x8 v; v.u = xv[k].u = make_uint4(0u, 0u, 0u, 0u);
-      if (row_ok && c < H) { v.load(sy + c); xv[k].load(sx + c); }
-      v.to_float(f[k]);
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      xv[k] = v;
+      if (row_ok && c < H) { v = *reinterpret_cast<const uint4*>(sy + c); xv[k] = *reinterpret_cast<const uint4*>(sx + c); }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc += f[k][i] * f[k][i];
+      for (int i = 0; i < 4; ++i) { f[k][i] = two(v, i); if (POST) acc = ffma2(f[k][i], f[k][i], acc); }
     }
-    const float by = scale * (gate != nullptr && row_ok ? gate[row] : 1.f);
-    float ry = 1.f;
+    float by = scale * (gate != nullptr && row_ok ? gate[row] : 1.f);
     if constexpr (POST) {
-      ry = rsqrtf(group_sum(acc, red[par][0], lanes, sub) / H + eps);
+      const float ry = rsqrtf(group_sum(acc.x + acc.y, red[par][0], lanes, sub) / H + eps);
       if (row_ok && l == 0) rstd_y[row] = ry;
+      by *= ry;
     }
-    acc = 0.f;
+    const float2 by2 = make_float2(by, by);
+    acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int c = (l + k * lanes) * 8;
-      float g[8], r[8];
-      if constexpr (POST) {
-        if (!BULK && c < H) wq[0].load(w_post + c);
-        wq[BULK ? k : 0].to_float(g);
+      if constexpr (POST && !BULK) { wq[0].u = make_uint4(0u, 0u, 0u, 0u); if (c < H) wq[0].load(w_post + c); }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (POST) f[k][i] = ffma2(fmul2(f[k][i], by2), two(wq[BULK ? k : 0].u, i), two(xv[k], i));
+        else f[k][i] = ffma2(f[k][i], by2, two(xv[k], i));
       }
-      xv[k].to_float(r);
+      const uint4 o = make_uint4(pack_bf16(f[k][0].x, f[k][0].y), pack_bf16(f[k][1].x, f[k][1].y), pack_bf16(f[k][2].x, f[k][2].y), pack_bf16(f[k][3].x, f[k][3].y));
+      if (row_ok && c < H) *reinterpret_cast<uint4*>(h + row * H + c) = o;
+      if constexpr (PRE) {   // columns that do not exist are zeros throughout
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[k][i] = fmaf(by, POST ? f[k][i] * ry * g[i] : f[k][i], r[i]);
-      bf16x8 o; o.from_float(f[k]);
-      if (row_ok && c < H) o.store(h + row * H + c);
-      if constexpr (PRE) {
-        o.to_float(f[k]);
-        if (c < H) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc += f[k][i] * f[k][i];
-        }
+        for (int i = 0; i < 4; ++i) { f[k][i] = two(o, i); acc = ffma2(f[k][i], f[k][i], acc); }
       }
     }
     float ss = 0.f;
-    if constexpr (PRE) ss = group_sum(acc, red[par][1], lanes, sub);
+    if constexpr (PRE) ss = group_sum(acc.x + acc.y, red[par][1], lanes, sub);
     if (BULK) {
       if (!PRE || lanes <= 32) __syncthreads();
       // every thread has its part of the rows in registers: the stage may be refilled
@@ -469,16 +468,16 @@ __global__ void __launch_bounds__(EW_THREADS) residual_norm_fwd_kernel(const __n
       if (!row_ok) continue;
       const float rh = rsqrtf(ss / H + eps);
       if (l == 0) rstd_h[row] = rh;
+      const float2 rh2 = make_float2(rh, rh);
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int c = (l + k * lanes) * 8;
         if (c < H) {
-          float g[8];
           if constexpr (!BULK) wz[0].load(w_pre + c);
-          wz[BULK ? k : 0].to_float(g);
+          float2 o[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[k][i] = f[k][i] * rh * g[i];
-          bf16x8 o; o.from_float(f[k]); o.store(z + row * H + c);
+          for (int i = 0; i < 4; ++i) o[i] = fmul2(fmul2(f[k][i], rh2), two(wz[BULK ? k : 0].u, i));
+          *reinterpret_cast<uint4*>(z + row * H + c) = make_uint4(pack_bf16(o[0].x, o[0].y), pack_bf16(o[1].x, o[1].y), pack_bf16(o[2].x, o[2].y), pack_bf16(o[3].x, o[3].y));
         }
       }
     }
@@ -491,7 +490,8 @@ __global__ void __launch_bounds__(EW_THREADS) residual_norm_fwd_kernel(const __n
 //   partial rows of dw_post += b dx yhat and dw_pre += dz hhat, per block, behind each other
 // dx stays in fp32 between its two uses. The second reduction is the gate's gradient and the norm's correction at once. Rows arrive by bulk copies as in
 // norm_bwd_kernel, up to four of them (dh, dz, h, y) to a stage; two barriers a row. Bound by reading them and writing dx and dy, 12 bytes an element.
-template <int VPT, bool POST, bool PRE>
+constexpr int RN_VPT = 2;
+template <bool POST, bool PRE>
 __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloat16* __restrict__ dh, const __nv_bfloat16* __restrict__ dz,
                                                                const __nv_bfloat16* __restrict__ y, const __nv_bfloat16* __restrict__ h,
                                                                const float* __restrict__ rstd_y, const float* __restrict__ rstd_h,
@@ -500,9 +500,10 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloa
                                                                float* __restrict__ dgate, float* __restrict__ part, float scale, int T, int H, int stages, int* status) {
   pdl_trigger();
   pdl_wait();
+  constexpr int VPT = RN_VPT;
   extern __shared__ __align__(128) uint8_t norm_smem[];
   __shared__ uint64_t full[8];
-  __shared__ float red[2][2][16];
+  __shared__ __align__(16) float red[2][2][16];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int nt = blockDim.x, wid = threadIdx.x >> 5;
@@ -526,14 +527,15 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloa
     for (int s = 0; s < stages; ++s) request(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
   }
   float2 accq[POST ? VPT : 1][4], accz[PRE ? VPT : 1][4];
-  bf16x8 wq[POST ? VPT : 1], wz[PRE ? VPT : 1];
+  uint4 wq[POST ? VPT : 1], wz[PRE ? VPT : 1];
+  const int c0 = threadIdx.x * 8;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int c = (threadIdx.x + v * nt) * 8;
+    const int c = c0 + v * nt * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i) { if constexpr (POST) accq[v][i] = make_float2(0.f, 0.f); if constexpr (PRE) accz[v][i] = make_float2(0.f, 0.f); }
-    if constexpr (POST) { wq[v].u = make_uint4(0u, 0u, 0u, 0u); if (c < H) wq[v].load(w_post + c); }
-    if constexpr (PRE) { wz[v].u = make_uint4(0u, 0u, 0u, 0u); if (c < H) wz[v].load(w_pre + c); }
+    if constexpr (POST) { wq[v] = make_uint4(0u, 0u, 0u, 0u); if (c < H) wq[v] = *reinterpret_cast<const uint4*>(w_post + c); }
+    if constexpr (PRE) { wz[v] = make_uint4(0u, 0u, 0u, 0u); if (c < H) wz[v] = *reinterpret_cast<const uint4*>(w_pre + c); }
   }
   auto stat = [&](const float* p, long long row, float none) { return p != nullptr && row < T ? p[row] : none; };
   float ry = POST ? stat(rstd_y, blockIdx.x, 0.f) : 1.f, rh = PRE ? stat(rstd_h, blockIdx.x, 0.f) : 0.f, by = scale * stat(gate, blockIdx.x, 1.f);
@@ -541,71 +543,70 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloa
   const float inv_h = 1.f / H;
   int s = 0, it = 0;
   uint32_t ph = 0;
-  auto load2 = [&](const uint8_t* p, int c, float2 (&f)[4]) {
-    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (c < H) u = *reinterpret_cast<const uint4*>(p + c * 2);
-    f[0] = unpack_bf16(u.x); f[1] = unpack_bf16(u.y); f[2] = unpack_bf16(u.z); f[3] = unpack_bf16(u.w);
-  };
-  auto w2 = [&](const bf16x8& w, int i) { return unpack_bf16(i == 0 ? w.u.x : i == 1 ? w.u.y : i == 2 ? w.u.z : w.u.w); };
+  auto load = [&](const uint8_t* p, int c) { return c < H ? *reinterpret_cast<const uint4*>(p + c * 2) : make_uint4(0u, 0u, 0u, 0u); };
+  auto two = [&](const uint4& u, int i) { return unpack_bf16(i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w); };
   auto total = [&](float d, float (&rd)[16]) {   // over the block
     d = warp_sum(d);
+    if (nt == 32) return d;
     if ((threadIdx.x & 31) == 0) rd[wid] = d;
     __syncthreads();
-    float2 t = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < 16; k += 2) t = fadd2(t, make_float2(rd[k], rd[k + 1]));
-    return t.x + t.y;
+    float4 t = *reinterpret_cast<const float4*>(rd);
+    for (int k = 4; k < nt >> 5; k += 4) {
+      const float4 u = *reinterpret_cast<const float4*>(rd + k);
+      t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
+    }
+    return (t.x + t.y) + (t.z + t.w);
   };
-  for (long long row = blockIdx.x; row < T; row += gridDim.x, ++it) {
+  __nv_bfloat16 *dxr = dx + blockIdx.x * static_cast<long long>(H) + c0, *dyr = dy + blockIdx.x * static_cast<long long>(H) + c0;
+  const long long hop = static_cast<long long>(gridDim.x) * H;
+  for (long long row = blockIdx.x; row < T; row += gridDim.x, ++it, dxr += hop, dyr += hop) {
     const long long next = row + gridDim.x;
     const float nry = POST ? stat(rstd_y, next, 0.f) : 1.f, nrh = PRE ? stat(rstd_h, next, 0.f) : 0.f, nby = scale * stat(gate, next, 1.f);
     if (!mbar_wait(&full[s], ph, abort_flag)) { atomicExch(status, 73); break; }
     const uint8_t* st = norm_smem + s * stage_bytes;
     const float2 rh2 = make_float2(rh, rh), ry2 = make_float2(ry, ry), by2 = make_float2(by, by);
-    float2 dxv[VPT][4];
+    float2 g[PRE ? VPT : 1][4], hh[PRE ? VPT : 1][4];   // dz w_pre and hhat; then g is dx
     float m = 0.f;
     if constexpr (PRE) {
       float2 d = make_float2(0.f, 0.f);
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
-        const int c = (threadIdx.x + v * nt) * 8;
-        float2 a[4], b[4];
-        load2(st, c, a); load2(st + row_bytes, c, b);
+        const int c = c0 + v * nt * 8;
+        const uint4 a = load(st, c), b = load(st + row_bytes, c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 hh = fmul2(b[i], rh2), g = fmul2(a[i], w2(wz[v], i));
-          d = ffma2(g, hh, d);
-          accz[v][i] = ffma2(a[i], hh, accz[v][i]);
+          const float2 av = two(a, i);
+          hh[v][i] = fmul2(two(b, i), rh2);
+          g[v][i] = fmul2(av, two(wz[v], i));
+          d = ffma2(g[v][i], hh[v][i], d);
+          accz[v][i] = ffma2(av, hh[v][i], accz[v][i]);
         }
       }
       m = total(d.x + d.y, red[it & 1][0]) * inv_h;
     }
-    float2 d = make_float2(0.f, 0.f);
+    float2 d = make_float2(0.f, 0.f), dxv[VPT][4], yh[POST ? VPT : 1][4];
     const float2 nm = make_float2(-m, -m);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int c = (threadIdx.x + v * nt) * 8;
-      float2 a[4], b[4], t[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = make_float2(0.f, 0.f);
-      if (have_dh) load2(st + at_dh, c, t);
-      if constexpr (PRE) { load2(st, c, a); load2(st + row_bytes, c, b); }
+      const int c = c0 + v * nt * 8;
+      uint4 u = make_uint4(0u, 0u, 0u, 0u), b = u;
+      if (have_dh) u = load(st + at_dh, c);
+      if (want_c) b = load(st + at_y, c);
+      float2 (&t)[4] = dxv[v];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (PRE) t[i] = ffma2(ffma2(fmul2(b[i], rh2), nm, fmul2(a[i], w2(wz[v], i))), rh2, t[i]);
-        dxv[v][i] = t[i];
+        t[i] = two(u, i);
+        if constexpr (PRE) t[i] = ffma2(ffma2(hh[v][i], nm, g[v][i]), rh2, t[i]);
       }
-      if (c < H) *reinterpret_cast<uint4*>(dx + row * H + c) = make_uint4(pack_bf16(t[0].x, t[0].y), pack_bf16(t[1].x, t[1].y), pack_bf16(t[2].x, t[2].y), pack_bf16(t[3].x, t[3].y));
-      if (want_c) {
-        load2(st + at_y, c, b);
+      if (c < H) *reinterpret_cast<uint4*>(dxr + v * nt * 8) = make_uint4(pack_bf16(t[0].x, t[0].y), pack_bf16(t[1].x, t[1].y), pack_bf16(t[2].x, t[2].y), pack_bf16(t[3].x, t[3].y));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (POST) {
-            const float2 yh = fmul2(b[i], ry2);
-            accq[v][i] = ffma2(fmul2(t[i], by2), yh, accq[v][i]);
-            d = ffma2(fmul2(t[i], w2(wq[v], i)), yh, d);
-          } else d = ffma2(t[i], b[i], d);
-        }
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (POST) {   // from here on dx w_post, and yhat
+          yh[v][i] = fmul2(two(b, i), ry2);
+          accq[v][i] = ffma2(fmul2(t[i], by2), yh[v][i], accq[v][i]);
+          t[i] = fmul2(t[i], two(wq[v], i));
+          d = ffma2(t[i], yh[v][i], d);
+        } else d = ffma2(t[i], two(b, i), d);
       }
     }
     float cn = 0.f;
@@ -613,21 +614,23 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloa
       cn = total(d.x + d.y, red[it & 1][1]);
       if (dgate != nullptr && threadIdx.x == 0) dgate[row] = scale * cn;
     }
-    // all threads are past the previous row's last reads: its stage may be refilled
-    if (threadIdx.x == 0 && it > 0) request(row + static_cast<long long>(stages - 1) * gridDim.x, s == 0 ? stages - 1 : s - 1);
+    if (nt == 32) __syncwarp();
+    // behind the second reduction this row is in registers and its stage may be refilled; without one the row before it is
+    if (threadIdx.x == 0) {
+      if (want_c) request(row + static_cast<long long>(stages) * gridDim.x, s);
+      else if (it > 0) request(row + static_cast<long long>(stages - 1) * gridDim.x, s == 0 ? stages - 1 : s - 1);
+    }
     const float2 nc = make_float2(-cn * inv_h, -cn * inv_h), f2 = make_float2(ry * by, ry * by);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int c = (threadIdx.x + v * nt) * 8;
-      if (c < H) {
-        float2 b[4], o[4];
-        if constexpr (POST) load2(st + at_y, c, b);
+      if (c0 + v * nt * 8 < H) {
+        float2 o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (POST) o[i] = fmul2(ffma2(fmul2(b[i], ry2), nc, fmul2(dxv[v][i], w2(wq[v], i))), f2);
+          if constexpr (POST) o[i] = fmul2(ffma2(yh[v][i], nc, dxv[v][i]), f2);
           else o[i] = fmul2(dxv[v][i], by2);
         }
-        *reinterpret_cast<uint4*>(dy + row * H + c) = make_uint4(pack_bf16(o[0].x, o[0].y), pack_bf16(o[1].x, o[1].y), pack_bf16(o[2].x, o[2].y), pack_bf16(o[3].x, o[3].y));
+        *reinterpret_cast<uint4*>(dyr + v * nt * 8) = make_uint4(pack_bf16(o[0].x, o[0].y), pack_bf16(o[1].x, o[1].y), pack_bf16(o[2].x, o[2].y), pack_bf16(o[3].x, o[3].y));
       }
     }
     ry = nry; rh = nrh; by = nby;
@@ -635,7 +638,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloa
   }
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int c = (threadIdx.x + v * nt) * 8;
+    const int c = c0 + v * nt * 8;
     if (c < H) {
       float* dst = part + static_cast<long long>(blockIdx.x) * ((POST ? 1 : 0) + (PRE ? 1 : 0)) * H + c;
       if constexpr (POST) {
@@ -684,6 +687,28 @@ __global__ void __launch_bounds__(256) reduce_few_rows_kernel(const float* __res
   float s = 0.f;
   for (int r = 0; r < R; ++r) s += part[static_cast<long long>(r) * C + c];
   if (c < D) out_a[c] = __float2bfloat16(s); else out_b[c - D] = __float2bfloat16(s);
+}
+
+// The same for the many partial rows of residual_norm_bwd_kernel: 8 columns per block, 64 threads share the rows of each (740 rows of 3072 columns).
+__global__ void __launch_bounds__(512) reduce_many_rows_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ out_a, __nv_bfloat16* __restrict__ out_b,
+                                                              int R, int C, int D) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float sm[16][8];
+  const int c = blockIdx.x * 8 + (threadIdx.x & 7);   // C is a multiple of 8
+  float s = 0.f;
+#pragma unroll 4
+  for (int r = threadIdx.x >> 3; r < R; r += 64) s += part[static_cast<long long>(r) * C + c];
+  s += __shfl_xor_sync(0xffffffffu, s, 8);
+  s += __shfl_xor_sync(0xffffffffu, s, 16);
+  if ((threadIdx.x & 31) < 8) sm[threadIdx.x >> 5][threadIdx.x & 7] = s;
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += sm[k][threadIdx.x];
+    if (c < D) out_a[c] = __float2bfloat16(s); else out_b[c - D] = __float2bfloat16(s);
+  }
 }
 
 // ------------------------------------------------------------------------------ RoPE
@@ -1713,23 +1738,32 @@ static int launch_residual_norm_fwd(const void* x, const void* y, const void* w_
   return launch_ok();
 }
 
-template <int VPT, bool POST, bool PRE>
+// Blocks of the backward of norms around a branch, as many as are resident, and the rows of its partials. A thread has two vectors of a row.
+static int residual_norm_threads(int H) { return cdiv(H, 8 * RN_VPT * 32) * 32; }
+extern "C" int mtb200_residual_norm_bwd_blocks(int T, int H) {
+  const int per_sm = 512 / residual_norm_threads(H);
+  const int b = num_sms() * (per_sm < 1 ? 1 : (per_sm > 8 ? 8 : per_sm));
+  return T < b ? (T > 0 ? T : 1) : b;
+}
+
+template <bool POST, bool PRE>
 static int launch_residual_norm_bwd(const void* dh, const void* dz, const void* y, const void* h, const float* rstd_y, const float* rstd_h, const void* w_post,
-                                    const void* w_pre, const float* gate, void* dx, void* dy, float* dgate, float* part, float scale, int T, int H, int blocks, int threads,
-                                    int* status, cudaStream_t st) {
-  auto kern = residual_norm_bwd_kernel<VPT, POST, PRE>;
+                                    const void* w_pre, const float* gate, void* dx, void* dy, float* dgate, float* part, float scale, int T, int H, int* status,
+                                    cudaStream_t st) {
+  auto kern = residual_norm_bwd_kernel<POST, PRE>;
   constexpr int most = 200 * 1024;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return -4;
     configured = true;
   }
-  // up to four rows ahead in the block's share of the SM, two at least (8192 columns: 64 KB a stage, and one block on an SM at a time)
-  const int stage = H * 2 * ((PRE ? 2 : 0) + (POST || dgate != nullptr ? 1 : 0) + (dh != nullptr ? 1 : 0)), per_sm = cdiv(blocks, num_sms());
+  // up to four rows ahead in the block's share of the SM, two at least
+  const int blocks = mtb200_residual_norm_bwd_blocks(T, H), per_sm = cdiv(blocks, num_sms());
+  const int stage = H * 2 * ((PRE ? 2 : 0) + (POST || dgate != nullptr ? 1 : 0) + (dh != nullptr ? 1 : 0));
   int stages = most / (per_sm * stage);
   stages = stages > 4 ? 4 : (stages < 2 ? 2 : stages);
-  launch_pdl(kern, blocks, threads, stages * stage, st, (const bf16*)dh, (const bf16*)dz, (const bf16*)y, (const bf16*)h, rstd_y, rstd_h, (const bf16*)w_post,
-             (const bf16*)w_pre, gate, (bf16*)dx, (bf16*)dy, dgate, part, scale, T, H, stages, status);
+  launch_pdl(kern, blocks, residual_norm_threads(H), stages * stage, st, (const bf16*)dh, (const bf16*)dz, (const bf16*)y, (const bf16*)h, rstd_y, rstd_h,
+             (const bf16*)w_post, (const bf16*)w_pre, gate, (bf16*)dx, (bf16*)dy, dgate, part, scale, T, H, stages, status);
   return launch_ok();
 }
 
@@ -1788,7 +1822,7 @@ int mtb200_residual_norm_fwd(const void* x, const void* y, const void* w_post, c
   if (!aligned16(x, y, h) || !aligned16(z, w_post, w_pre)) return -11;
   const int vecs = H / 8;
   int lanes = 32;
-  while (lanes < EW_THREADS && lanes * 4 < vecs) lanes *= 2;
+  while (lanes < EW_THREADS && lanes * 2 < vecs) lanes *= 2;   // two rows' worth of registers per thread: half as many vectors as a norm alone has
   const int vpt = cdiv(vecs, lanes), rows = EW_THREADS / lanes, stages = NORM_STAGES * rows * H * 4 + 1280;
   const int fit = 227 * 1024 / stages < 8 ? 227 * 1024 / stages : 8;
   const bool bulk = fit > 0 && 2 * cdiv(T, rows) > 5 * fit * num_sms();
@@ -1803,23 +1837,21 @@ int mtb200_residual_norm_fwd(const void* x, const void* y, const void* w_post, c
 #undef RF
 }
 
-// part: fp32 scratch [mtb200_norm_bwd_blocks(T, H), weights, H]; dw_post / dw_pre: [H] bf16, as their weights.
+// part: fp32 scratch [mtb200_residual_norm_bwd_blocks(T, H), weights, H]; dw_post / dw_pre: [H] bf16, as their weights.
 int mtb200_residual_norm_bwd(const void* dh, const void* dz, const void* y, const void* h, const float* rstd_y, const float* rstd_h, const void* w_post, const void* w_pre,
                              const float* gate, void* dx, void* dy, float* dgate, float* part, void* dw_post, void* dw_pre, float scale, int T, int H, int* status,
                              cudaStream_t st) {
   if (T <= 0) return 0;
   if (H <= 0 || H % 8 || H > 4 * 8 * EW_THREADS || (w_post == nullptr && w_pre == nullptr)) return -10;
   if (!aligned16(dh, dz, y) || !aligned16(h, dx, dy) || !aligned16(w_post, w_pre, part)) return -11;
-  const int blocks = mtb200_norm_bwd_blocks(T, H), vpt = norm_bwd_vpt(H), threads = norm_bwd_threads(H);
-  int rc;
-#define RB(V, A, B) launch_residual_norm_bwd<V, A, B>(dh, dz, y, h, rstd_y, rstd_h, w_post, w_pre, gate, dx, dy, dgate, part, scale, T, H, blocks, threads, status, st)
-#define RW(V) rc = w_post == nullptr ? RB(V, false, true) : w_pre == nullptr ? RB(V, true, false) : RB(V, true, true)
-  if (vpt <= 1) RW(1); else RW(2);
-#undef RW
+#define RB(A, B) launch_residual_norm_bwd<A, B>(dh, dz, y, h, rstd_y, rstd_h, w_post, w_pre, gate, dx, dy, dgate, part, scale, T, H, status, st)
+  const int rc = w_post == nullptr ? RB(false, true) : w_pre == nullptr ? RB(true, false) : RB(true, true);
 #undef RB
   if (rc) return rc;
-  const bool both = w_post != nullptr && w_pre != nullptr;
-  reduce_rows(part, w_post != nullptr ? dw_post : dw_pre, dw_pre, blocks, both ? 2 * H : H, H, st);
+  const int blocks = mtb200_residual_norm_bwd_blocks(T, H), C = w_post != nullptr && w_pre != nullptr ? 2 * H : H;
+  void* first = w_post != nullptr ? dw_post : dw_pre;
+  if (blocks > 64) launch_pdl(reduce_many_rows_kernel, C / 8, 512, 0, st, part, (bf16*)first, (bf16*)dw_pre, blocks, C, H);
+  else reduce_rows(part, first, dw_pre, blocks, C, H, st);
   return launch_ok();
 }
 

@@ -61,6 +61,7 @@ class _Sig:
     mtb200_norm_bwd_blocks = [I, I]
     mtb200_rmsnorm_bwd = [P, P, P, P, P, P, P, P, I, I, P, P]
     mtb200_residual_norm_fwd = [P, P, P, P, P, P, P, P, P, F, F, I, I, P, P]
+    mtb200_residual_norm_bwd_blocks = [I, I]
     mtb200_residual_norm_bwd = [P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, F, I, I, P, P]
     mtb200_layernorm_fwd = [P, P, P, P, P, P, F, I, I, P, P]
     mtb200_layernorm_bwd = [P, P, P, P, P, P, P, P, P, P, I, I, P, P]
@@ -449,7 +450,7 @@ class NativeOps:
                     w.zero_()
             return dx, dy, dgate
         weights = (w_post is not None) + (w_pre is not None)
-        part = torch.empty(self._fn["mtb200_norm_bwd_blocks"](T, H) * weights * H, dtype=torch.float32, device=y.device)
+        part = torch.empty(self._fn["mtb200_residual_norm_bwd_blocks"](T, H) * weights * H, dtype=torch.float32, device=y.device)
         self._call("mtb200_residual_norm_bwd", _ptr(dh), _ptr(dz), y.data_ptr(), h.data_ptr(), _ptr(ry), _ptr(rh), _ptr(w_post), _ptr(w_pre), _ptr(gate),
                    dx.data_ptr(), dy.data_ptr(), _ptr(dgate), part.data_ptr(), _ptr(dw_post_out), _ptr(dw_pre_out), scale, T, H, self.status.data_ptr(),
                    self._st(), n=2)

@@ -135,7 +135,7 @@ def test_formula_against_differences():
 
 def host_ops():
     from .test_native_host import make_ops
-    ops = make_ops(mtb200_norm_bwd_blocks=lambda T, H: 3)
+    ops = make_ops(mtb200_residual_norm_bwd_blocks=lambda T, H: 3)
     ops._index = None
     return ops
 
