@@ -28,7 +28,7 @@ inline AttRuleArgs att_rule_args(float scale, float cap, int window, const float
   AttRuleArgs r{};
   r.window = window > 0 && window < (1 << 30) ? window : 1 << 30;
   r.slopes = slopes;
-  if (cap > 0.f) r.cap = cap_args(scale, cap);
+  if (cap > 0.f) r.cap = cap_args(scale, cap, static_cast<double>(cap) * 1.4426950408889634);
   return r;
 }
 

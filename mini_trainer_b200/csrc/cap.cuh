@@ -1,4 +1,4 @@
-// Numbers capped by a tanh, cap tanh(scale s / cap), in units of log2 e, as the exponentials of a softmax want them.
+// Numbers capped by a tanh, unit tanh(scale s / cap): attention wants them in units of log2 e, as its exponentials do (unit = cap log2 e), the head as a part of the cap (1).
 //
 // Up to the cap (|scale s| <= cap; bigger ones are rare) an odd polynomial of degree eleven, fitted to the least relative error on [-1, 1] (5.1e-7), with the powers of
 // scale / cap in its coefficients: seven packed instructions for two numbers. Beyond it tanh as 1 - 2 / (1 + e^2x), two operations on the special-function
@@ -10,26 +10,28 @@
 
 namespace mtb {
 
+// The polynomial: tanh(x) = x (C0 + C1 x^2 + ...).
+constexpr float CAP_C[6] = {0.99999949f, -0.33329398f, 0.13284259f, -0.05168433f, 0.01683263f, -0.00310275f};
+
 struct CapArgs {
   float2 a[6];       // twice each, for packed arithmetic: s (a0 + a1 s^2 + ...)
   float most;        // |s| up to which that holds
-  float cap2, k2;    // cap log2 e; 2 scale / cap log2 e
-  float inv2;        // -1 / cap2^2: the derivative is 1 + inv2 v^2 of a capped number v
+  float unit, k2;    // k2: 2 scale / cap log2 e
+  float inv2;        // -1 / unit^2: the derivative is 1 + inv2 v^2 of a capped number v
 };
 
 // Range of caps. Above it the exact form's error would pass 1e-3 of the scale's unit.
 inline bool cap_ok(float scale, float cap) { return scale > 0.f && cap > 0.f && scale >= cap * 0x1p-13f && scale <= cap * 0x1p10f; }
 
-inline CapArgs cap_args(float scale, float cap) {
-  constexpr double C[6] = {0.99999949, -0.33329398, 0.13284259, -0.05168433, 0.01683263, -0.00310275};
+inline CapArgs cap_args(float scale, float cap, double unit) {
   CapArgs r{};
-  const double k = static_cast<double>(scale) / cap, c2 = static_cast<double>(cap) * 1.4426950408889634;
+  const double k = static_cast<double>(scale) / cap;
   double p = k;
-  for (int i = 0; i < 6; ++i, p *= k * k) r.a[i].x = r.a[i].y = static_cast<float>(c2 * C[i] * p);
+  for (int i = 0; i < 6; ++i, p *= k * k) r.a[i].x = r.a[i].y = static_cast<float>(unit * CAP_C[i] * p);
   r.most = k >= 0x1p-11 ? static_cast<float>(1.0 / k) : -1.f;   // below, k^11 is no normal number: the exact form throughout
-  r.cap2 = static_cast<float>(c2);
+  r.unit = static_cast<float>(unit);
   r.k2 = static_cast<float>(2.0 * k * 1.4426950408889634);
-  r.inv2 = static_cast<float>(-1.0 / (c2 * c2));
+  r.inv2 = static_cast<float>(-1.0 / (unit * unit));
   return r;
 }
 
@@ -37,7 +39,7 @@ inline CapArgs cap_args(float scale, float cap) {
 __device__ __forceinline__ float cap_exact(const CapArgs& r, float s) {
   float q;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + ex2_mufu(s * r.k2)));
-  return fmaf(-2.f * r.cap2, q, r.cap2);
+  return fmaf(-2.f * r.unit, q, r.unit);
 }
 __device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
 // A pair within the cap.
@@ -48,6 +50,21 @@ __device__ __forceinline__ float2 cap_pair(const CapArgs& r, float2 s) {
   p = ffma2(u, p, r.a[2]);
   p = ffma2(u, p, r.a[1]);
   return fmul2(s, ffma2(u, p, r.a[0]));
+}
+// The same of numbers that are parts of the cap already, tanh(x).
+__device__ __forceinline__ float2 tanh_pair(float2 x) {
+  const float2 u = fmul2(x, x);
+  constexpr float C0 = CAP_C[0], C1 = CAP_C[1], C2 = CAP_C[2], C3 = CAP_C[3], C4 = CAP_C[4], C5 = CAP_C[5];
+  float2 p = ffma2(u, splat(C5), splat(C4));
+  p = ffma2(u, p, splat(C3));
+  p = ffma2(u, p, splat(C2));
+  p = ffma2(u, p, splat(C1));
+  return fmul2(x, ffma2(u, p, splat(C0)));
+}
+__device__ __forceinline__ float tanh_exact(float x) {
+  float q;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + ex2_mufu(x * 2.8853900817779268f)));
+  return fmaf(-2.f, q, 1.f);
 }
 // A warp's numbers in tensor memory, n x 16 columns of its lanes, capped in place by the exact form. A loop of its own, so that the polynomial's code is all that
 // tiles within the cap fetch.

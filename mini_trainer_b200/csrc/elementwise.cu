@@ -5,6 +5,7 @@
 // These replace what the reference gets from Liger's Triton kernels (rms_norm, rope, swiglu,
 // cross_entropy) and ATen foreach ops (clip, AdamW).
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -1321,68 +1322,80 @@ __global__ void __launch_bounds__(1024, 1) ce_row_kernel(const __nv_bfloat16* lo
   pdl_trigger();
 }
 
-// Cross-entropy of logits capped by a tanh, l = cap tanh(z / cap), from fp32 products z [R, V]: loss and dz = (softmax(l) - onehot) (1 - tanh^2) scale, rounded to
-// bf16. The products come in fp32 because the loss is a difference of numbers of their size: rounded to bf16 they would be off by up to 2^-8 of themselves,
-// and the loss with them. One block per row, two passes over it; the capped numbers are formed again in the second.
-__device__ __forceinline__ void cap8(const CapArgs& r, const float* p, float (&f)[8]) {
-  load8(p, f);
-  const float big = fmax3(fmax3(fabsf(f[0]), fabsf(f[1]), fabsf(f[2])), fmax3(fabsf(f[3]), fabsf(f[4]), fabsf(f[5])), fmaxf(fabsf(f[6]), fabsf(f[7])));
-  if (big <= r.most) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float2 v = cap_pair(r, make_float2(f[i], f[i + 1]));
-      f[i] = v.x; f[i + 1] = v.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = cap_exact(r, f[i]);
-  }
-}
+// Cross-entropy of logits capped by a tanh, l = cap t: loss and dz = (softmax(l) - onehot) (1 - t^2) scale, rounded to bf16, over t [R, V] in fp16, in place. The
+// product that left t has left the softmax's statistics of every 128 columns too, formed before its rounding (gemm_act.cuh, ACT_CAP), and the target's logit is
+// formed again from its rows of x and w: the loss, a difference of numbers many times a rounding apart, sees none. The gradient is that of t as it is
+// rounded (2^-11 of itself, where bf16 logits are off by 2^-8). One block per row; bound by reading and writing it.
+__device__ __forceinline__ float2 unpack_half(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-__global__ void __launch_bounds__(1024) ce_capped_kernel(const float* __restrict__ logits, long long ld, const long long* __restrict__ targets, float* __restrict__ loss,
-                                                        __nv_bfloat16* __restrict__ dlogits, long long ldd, int V, CapArgs cap, float grad_scale, long long ignore_index) {
+__global__ void __launch_bounds__(1024) ce_capped_kernel(__nv_bfloat16* t, const float2* __restrict__ stats, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
+                                                        const long long* __restrict__ targets, float* __restrict__ loss, int V, int H, float alpha, float cap2, float grad_scale,
+                                                        long long ignore_index) {
   pdl_trigger();
   pdl_wait();
   __shared__ float red[32];
   const long long row = blockIdx.x;
-  const float* lr = logits + row * ld;
-  __nv_bfloat16* dr = dlogits + row * ldd;
+  __nv_bfloat16* tr = t + row * V;
   const long long tgt = targets[row];
+  const int c0 = threadIdx.x * 8, step = blockDim.x * 8;
   if (tgt == ignore_index) {
-    for (int c = threadIdx.x * 8; c < V; c += blockDim.x * 8) *reinterpret_cast<uint4*>(dr + c) = make_uint4(0, 0, 0, 0);
+    for (int c = c0; c < V; c += step) *reinterpret_cast<uint4*>(tr + c) = make_uint4(0, 0, 0, 0);
     if (threadIdx.x == 0) loss[row] = 0.f;
     return;
   }
-  float m = -INFINITY, s = 0.f;
-  for (int c = threadIdx.x * 8; c < V; c += blockDim.x * 8) {
-    float v[8];
-    cap8(cap, lr + c, v);
-    const float mx = fmax3(fmax3(v[0], v[1], v[2]), fmax3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
-    if (mx > m) { s *= ex2_mufu(m - mx); m = mx; }
+  const bool there = tgt >= 0 && tgt < V;
+  float m = -2.f, s = 0.f, dot = 0.f;
+  const int tiles = (V + 127) / 128;
+  for (int c = threadIdx.x; c < tiles; c += blockDim.x) {
+    const float2 q = stats[row * tiles + c];
+    if (q.x > m) { s *= ex2_mufu((m - q.x) * cap2); m = q.x; }
+    s += q.y * ex2_mufu((q.x - m) * cap2);
+  }
+  for (int c = c0; there && c < H; c += step) {
+    const uint4 a = *reinterpret_cast<const uint4*>(x + row * H + c), b = *reinterpret_cast<const uint4*>(w + tgt * H + c);
+    const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += ex2_mufu(v[i] - m);
+    for (int i = 0; i < 4; ++i) {
+      const float2 u = unpack_bf16(av[i]), v = unpack_bf16(bv[i]);
+      dot = fmaf(u.x, v.x, fmaf(u.y, v.y, dot));
+    }
   }
   const float gm = block_max(m, red);
-  const float gs = block_sum(m == -INFINITY ? 0.f : s * ex2_mufu(m - gm), red);   // (a thread without columns)
+  const float gs = block_sum(s * ex2_mufu((m - gm) * cap2), red);   // (zero for a thread without columns)
+  dot = block_sum(dot, red) * alpha;
   if (threadIdx.x == 0) {
-    float t = NAN;   // of a target that is no column
-    if (tgt >= 0 && tgt < V) {
-      const float z = lr[tgt];
-      t = fabsf(z) <= cap.most ? cap_pair(cap, splat(z)).x : cap_exact(cap, z);
-    }
-    loss[row] = 0.6931471805599453f * ((gm - t) + log2f(gs));
+    const float tt = !there ? NAN : fabsf(dot) <= 1.f ? tanh_pair(splat(dot)).x : tanh_exact(dot);   // NaN of a target that is no column
+    loss[row] = 0.6931471805599453f * ((gm - tt) * cap2 + log2f(gs));
   }
-  const float inv = grad_scale / gs;
-  for (int c = threadIdx.x * 8; c < V; c += blockDim.x * 8) {
-    float v[8];
-    cap8(cap, lr + c, v);
+  const float2 inv = splat(grad_scale / gs), nm = splat(-gm * cap2), one = splat(1.f), c2 = splat(cap2);
+  auto gradient = [&](uint4 u, int c) {
+    const float2 f[4] = {unpack_half(u.x), unpack_half(u.y), unpack_half(u.z), unpack_half(u.w)};
+    float2 p[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float p = ex2_mufu(v[i] - gm) * inv;
-      if (tgt - c == i) p -= grad_scale;
-      v[i] = p * fmaf(v[i] * cap.inv2, v[i], 1.f);
+    for (int i = 0; i < 4; ++i) {
+      const float2 e = ffma2(f[i], c2, nm);
+      p[i] = fmul2(make_float2(ex2_mufu(e.x), ex2_mufu(e.y)), inv);
     }
-    bf16x8 o; o.from_float(v); o.store(dr + c);
+    if (tgt >= c && tgt < c + 8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (tgt - c == 2 * i) p[i].x -= grad_scale;
+        if (tgt - c == 2 * i + 1) p[i].y -= grad_scale;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = fmul2(p[i], ffma2(make_float2(-f[i].x, -f[i].y), f[i], one));
+    *reinterpret_cast<uint4*>(tr + c) = make_uint4(pack_bf16(p[0].x, p[0].y), pack_bf16(p[1].x, p[1].y), pack_bf16(p[2].x, p[2].y), pack_bf16(p[3].x, p[3].y));
+  };
+  // four vectors are on their way before the first is overwritten
+  for (int c = c0; c < V; c += 4 * step) {
+    uint4 u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k * step < V) u[k] = *reinterpret_cast<const uint4*>(tr + c + k * step);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c + k * step < V) gradient(u[k], c + k * step);
   }
 }
 
@@ -2032,14 +2045,16 @@ int mtb200_ce_fwd_bwd(const void* logits, long long ld, int logits_bf16, const f
   return launch_ok();
 }
 
-// logits: fp32 [R, ld]; dlogits: bf16 [R, ldd], another buffer.
-int mtb200_ce_capped(const float* logits, long long ld, const long long* targets, float* loss, void* dlogits, long long ldd, int R, int V, float cap, float grad_scale,
-                     long long ignore_index, cudaStream_t st) {
+// t: fp16 [R, V] and stats [R, ceil(V / 128)], of mtb200_gemm_capped for these x [R, H], w [V, H], alpha and cap2; bf16 gradients of the products come in t's place.
+int mtb200_ce_capped(void* t, const float2* stats, const void* x, const void* w, const long long* targets, float* loss, int R, int V, int H, float alpha, float cap2,
+                     float grad_scale, long long ignore_index, cudaStream_t st) {
   if (R <= 0) return 0;
-  if (V <= 0 || V % 8 || ld % 8 || ldd % 8 || !cap_ok(1.f, cap)) return -10;
-  if (!aligned16(logits, dlogits, nullptr)) return -11;
-  const int threads = cdiv(V, 8 * 32) * 32;
-  launch_pdl(ce_capped_kernel, R, threads < 1024 ? threads : 1024, 0, st, logits, ld, targets, loss, (bf16*)dlogits, ldd, V, cap_args(1.f, cap), grad_scale, ignore_index);
+  if (V <= 0 || V % 8 || H <= 0 || H % 8) return -10;
+  if (!aligned16(t, x, w)) return -11;
+  const int threads = cdiv(V, 8 * 4 * 32) * 32;   // four vectors each, up to the most threads
+  const int most = R >= 6 * num_sms() ? 512 : 1024;   // rows enough: several at a time on an SM hide each other's reductions
+  launch_pdl(ce_capped_kernel, R, threads < most ? threads : most, 0, st, (bf16*)t, stats, (const bf16*)x, (const bf16*)w, targets, loss, V, H, alpha, cap2, grad_scale,
+             ignore_index);
   return launch_ok();
 }
 

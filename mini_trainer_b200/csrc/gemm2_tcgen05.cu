@@ -365,7 +365,8 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__
         __syncwarp();
         if (lane == 0) mbar_arrive_cta0(&tempty_bar[h]);
       };
-      if constexpr (ACT != ACT_NONE) epilogue_act_wide<ACT>(p.e, p.act, maps, out, taddr, row0, row_end, col0 / BN + h, q, lane, drained);
+      if constexpr (ACT == ACT_CAP) drained();   // (never wide)
+      else if constexpr (ACT != ACT_NONE) epilogue_act_wide<ACT>(p.e, p.act, maps, out, taddr, row0, row_end, col0 / BN + h, q, lane, drained);
       else epilogue_wide<OUT_F32, !GROUP, STATS, EXTRA>(p.e, out, taddr, row0, row_end, col0 + h * BN, q, lane, 2 * (tm * tiles_n + col0 / BN + h) + static_cast<int>(rank),
                                                 splits > 1 ? w / wide_tiles : 0, GROUP == GROUP_REDUCE && kb1 == 0, drained);
     }
@@ -577,11 +578,13 @@ int launch_gather(const void* A, long long lda, void* D, long long ldd, const vo
   return launch<false, false, false, true>(ta, tb, td, p, stream, &g);
 }
 
-// Products with an activation in the epilogue; called by mtb200_gemm_act.
+// Products with an activation or a cap in the epilogue; called by mtb200_gemm_act and mtb200_gemm_capped.
 int launch_act(int mode, bool wide, const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_GLU>& m, const EpiParams& e, const ActParams& a, int K,
                int* status, cudaStream_t stream) {
   const Params p{e.M, e.N, K, status, 0, 0, 0, e, a};
   const ActMaps<ACT_PLAIN> plain{m.gate, m.up, m.act};
+  const ActMaps<ACT_CAP> capped{m.gate};
+  if (mode == ACT_CAP) return launch<false, false, false, false, false, false, ACT_CAP>(ta, tb, m.gate, p, stream, nullptr, 0, capped);
   if (wide) return mode == ACT_GLU ? launch<false, false, false, false, false, false, ACT_GLU, true>(ta, tb, m.gate, p, stream, nullptr, 0, m)
                                    : launch<false, false, false, false, false, false, ACT_PLAIN, true>(ta, tb, m.gate, p, stream, nullptr, 0, plain);
   if (mode == ACT_GLU) return launch<false, false, false, false, false, false, ACT_GLU>(ta, tb, m.gate, p, stream, nullptr, 0, m);

@@ -2,6 +2,10 @@
 // a bandwidth-bound kernel. They are rounded to bf16 before the activation reads them, as if they had been stored in between.
 //   ACT_GLU    pre = A * [Wg; Wu]^T, act = f(g) * u. A tile's 256 columns are 128 of the gate and the same 128 of up, so that one thread has both.
 //   ACT_PLAIN  pre = A * B (+ bias), act = f(pre): an MLP without a gate
+//   ACT_CAP    t = tanh(alpha A * B^T) alone, rounded to fp16, and of every row and 128 columns the largest t and the sum of 2^((t - largest) cap2): what
+//              the cross-entropy of capped logits (cap t, cap2 = cap log2 e) reads instead of products in fp32. The statistics are formed before
+//              the rounding. 3720 x 151936 x 1536 1153 us (the product alone 1128), 5000 x 8192 x 512 62 (54), where the exponentials do not hide. Wide tiles, whose one
+//              warp per quarter would form them before it gives the accumulator back, took 1876 us.
 // Eight warps, two per 32-row quarter: with four (one per scheduler) the arithmetic of a tile took longer than short reductions. They work on
 // 32 columns at a time, staged as boxes of 32 rows x 64 bytes (64B-swizzled). Bound by the product. With its activation, in a loop of its own on a B200:
 // 5987 x 17920 x 1536 272 -> 231 us (product alone 220), 4099 x 12288 x 2048 167 -> 153, 16384 x 28672 x 4096 3.16 -> 2.8 ms, 7001 x 12288 x 3072 without
@@ -15,21 +19,27 @@
 // longer ones run at the power cap, where the time is given by what is computed and moved.
 #pragma once
 #include <cuda.h>
+#include <cuda_fp16.h>
 
+#include "cap.cuh"
 #include "gemm_epilogue.cuh"
 #include "ptx.cuh"
 
 namespace mtb {
 
-enum { ACT_NONE = 0, ACT_GLU = 1, ACT_PLAIN = 2 };
+enum { ACT_NONE = 0, ACT_GLU = 1, ACT_PLAIN = 2, ACT_CAP = 3 };
 
 struct ActParams {
   int F;          // width of the activation
-  int gelu;       // 0: SiLU, 1: tanh-approximated GELU
+  union {
+    int gelu;     // 0: SiLU, 1: tanh-approximated GELU
+    float cap2;   // ACT_CAP
+  };
 };
 // Tensor maps of gate (or x), up and act, boxes of 32 rows x 32 columns, 64B-swizzled; nothing in instances without an activation.
 template <int ACT> struct ActMaps { CUtensorMap gate, up, act; };
 template <> struct ActMaps<ACT_NONE> {};
+template <> struct ActMaps<ACT_CAP> { CUtensorMap gate; };
 
 constexpr int ACT_WARPS = 8;
 constexpr int ACT_BOX = 32 * 64;                     // bytes of a box
@@ -59,6 +69,54 @@ __device__ __forceinline__ uint32_t act_pair(uint32_t g, uint32_t u, bool gelu) 
   if (GATED) f = fmul2(f, unpack_bf16(u));
   return pack2(f);
 }
+__device__ __forceinline__ uint32_t pack_half(float2 v) {
+  const __half2 h = __float22half2_rn(v);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+constexpr float CAP_NONE = -2.f;   // below any t: no column yet
+// ACT_CAP: 32 columns of a thread's row, from `col` on, and their part of the row's statistics {largest t, sum}; columns past N count for nothing.
+__device__ __forceinline__ void cap_columns32(const EpiParams& p, float cap2, const uint32_t (&v)[32], int col, uint32_t (&d)[16], float2& st) {
+  float2 t[16];
+  float big[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    t[i] = fmul2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f2(p.alpha));
+    big[i & 1] = fmax3(big[i & 1], fabsf(t[i].x), fabsf(t[i].y));
+  }
+  if (fmaxf(big[0], big[1]) <= 1.f) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] = tanh_pair(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] = make_float2(tanh_exact(t[i].x), tanh_exact(t[i].y));
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) d[i] = pack_half(t[i]);
+  if (col + 32 > p.N) {   // N is a multiple of 8
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (col + (i & ~3) * 2 >= p.N) t[i] = f2(-INFINITY);
+  }
+  float mx[2] = {CAP_NONE, CAP_NONE};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mx[i & 1] = fmax3(mx[i & 1], t[i].x, t[i].y);
+  const float m = fmax3(st.x, mx[0], mx[1]);
+  st.y *= ex2_mufu((st.x - m) * cap2);
+  st.x = m;
+  const float2 nm = f2(-m * cap2);
+  float2 s[2] = {f2(0.f), f2(0.f)};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 x = ffma2(t[i], f2(cap2), nm);
+    s[i & 1] = fadd2(s[i & 1], make_float2(ex2_mufu(x.x), ex2_mufu(x.y)));
+  }
+  const float2 q = fadd2(s[0], s[1]);
+  st.y += q.x + q.y;
+}
+__device__ __forceinline__ void cap_stats(const EpiParams& p, int row, int row_end, int col, float2 st) {
+  if (row < row_end && col < p.N) p.stats[static_cast<long long>(row) * ((p.N + 127) / 128) + col / 128] = st;
+}
+
 // One warp's part of a tile, `half` of its columns (gated: 64 of the gate and the same of up, else 128). `out`: this warp's two boxes.
 template <int ACT>
 __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams& ap, const ActMaps<ACT>& maps, EpiOut& out, uint32_t taddr, int row0,
@@ -66,6 +124,7 @@ __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams
   constexpr bool GLU = ACT == ACT_GLU;
   const int y0 = row0 + q * 32;
   if (y0 >= p.M) return;
+  float2 st = make_float2(CAP_NONE, 0.f);
   auto send = [&](const CUtensorMap& map, const uint32_t (&d)[16], int col) {
     if (lane == 0) bulk_wait_read<1>();
     __syncwarp();
@@ -82,6 +141,11 @@ __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams
     uint32_t v[32], g[16], u[GLU ? 16 : 1];
     tmem_ld_32x32(taddr + at, v);
     tmem_ld_wait();
+    if constexpr (ACT == ACT_CAP) {
+      cap_columns32(p, ap.cap2, v, col, g, st);
+      send(maps.gate, g, col);
+      continue;
+    }
     if (ACT == ACT_PLAIN && p.bias != nullptr) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -107,15 +171,18 @@ __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams
       for (int j = 0; j < 16; ++j) u[j] = pack_bf16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
       send(maps.up, u, col);
     }
-    if (ap.gelu) {
+    if constexpr (ACT != ACT_CAP) {
+      if (ap.gelu) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) g[j] = act_pair<GLU>(g[j], u[GLU ? j : 0], true);
-    } else {
+        for (int j = 0; j < 16; ++j) g[j] = act_pair<GLU>(g[j], u[GLU ? j : 0], true);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) g[j] = act_pair<GLU>(g[j], u[GLU ? j : 0], false);
+        for (int j = 0; j < 16; ++j) g[j] = act_pair<GLU>(g[j], u[GLU ? j : 0], false);
+      }
+      send(maps.act, g, col);
     }
-    send(maps.act, g, col);
   }
+  if constexpr (ACT == ACT_CAP) cap_stats(p, y0 + lane, p.M, tn * 256 + half * 128, st);
 }
 
 // The same for wide tiles: one warp has all 256 columns of its quarter and reads them before it works on any; boxes of 32 rows x 128 bytes, one per

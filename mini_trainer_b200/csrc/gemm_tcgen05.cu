@@ -555,13 +555,37 @@ int mtb200_gemm_act(const void* A, long long lda, const void* W, void* out, void
   if (!rc) rc = make_tmap_act(&m.act, act, F, M, F, wide);
   if (rc) return rc - 20;
   const EpiParams e{M, N, nullptr, 0, reinterpret_cast<const __nv_bfloat16*>(bias), 1.0f, 1, nullptr, nullptr, nullptr, 0};
-  const ActParams a{F, gelu};
+  ActParams a{F, {}};
+  a.gelu = gelu;
   if (form != FORM_ONE) return g2::launch_act(mode, wide, ta, tb, m, e, a, K, status, stream);
   const GemmParams p{M, N, K, status, tune_group_m(), tune_wait_hint(), 0u, e, a};
   if (mode == ACT_GLU)
     return launch<false, false, false, false, false, GROUP_NONE, false, false, ACT_GLU>(ta, tb, m.gate, p, stream, nullptr, 0, nullptr, m);
   return launch<false, false, false, false, false, GROUP_NONE, false, false, ACT_PLAIN>(ta, tb, m.gate, p, stream, nullptr, 0, nullptr,
                                                                                      ActMaps<ACT_PLAIN>{m.gate, m.up, m.act});
+}
+
+// t[M, N] = tanh(alpha A[M, K] * W[N, K]^T) in fp16, and stats[M, ceil(N / 128)] = {largest t, sum of 2^((t - largest) cap2)} of its rows (gemm_act.cuh). All row-major,
+// without padding between rows but in A. `form`: FORM_ONE or FORM_PAIR.
+int mtb200_gemm_capped(const void* A, long long lda, const void* W, void* t, float2* stats, int M, int N, int K, float alpha, float cap2, int form, int* status,
+                       cudaStream_t stream) {
+  using namespace mtb;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if ((form != FORM_ONE && form != FORM_PAIR) || N % 8 || K % 8 || stats == nullptr) return -10;
+  CUtensorMap ta, tb;
+  ActMaps<ACT_GLU> m{};
+  int rc = make_tmap_2d_bf16(&ta, A, K, M, lda, 64, 128);
+  if (rc) return rc;
+  rc = make_tmap_2d_bf16(&tb, W, K, N, K, 64, form != FORM_ONE ? 128 : 256);
+  if (rc) return rc - 10;
+  rc = make_tmap_act(&m.gate, t, N, M, N, false);   // (16-bit elements: the map does not care which)
+  if (rc) return rc - 20;
+  const EpiParams e{M, N, nullptr, 0, nullptr, alpha, 1, nullptr, stats, nullptr, 0};
+  ActParams a{N, {}};
+  a.cap2 = cap2;
+  if (form != FORM_ONE) return g2::launch_act(ACT_CAP, false, ta, tb, m, e, a, K, status, stream);
+  const GemmParams p{M, N, K, status, tune_group_m(), tune_wait_hint(), 0u, e, a};
+  return launch<false, false, false, false, false, GROUP_NONE, false, false, ACT_CAP>(ta, tb, m.gate, p, stream, nullptr, 0, nullptr, ActMaps<ACT_CAP>{m.gate});
 }
 
 enum { GROUPED_WIDE = 4 };
@@ -591,7 +615,8 @@ int mtb200_gemm_grouped(const void* A, long long lda, const void* B, long long l
   else rc = make_tmap_out(&td, D, rows, N, ldd, 0);
   if (rc) return rc - 20;
   const EpiParams ep{out_rows, N, nullptr, 0, nullptr, 1.0f, 1, nullptr, nullptr, nullptr, 0};
-  const ActParams ap{N / 2, gelu};
+  ActParams ap{N / 2, {}};
+  ap.gelu = gelu;
   GroupParams g{starts, counts, E, static_cast<float>(2.0 * rows * N * (mode == 2 ? M : K))};
   ActMaps<ACT_GLU> m{};
   if (mode == 3) {

@@ -26,6 +26,13 @@ def partial_bytes(M: int, N: int, pair: bool, splits: int) -> int:
 FORMS = {"mtb200_gemm_bf16": 0, "mtb200_gemm2_bf16": 1, "mtb200_gemm2_wide_bf16": 2, "mtb200_gemm_n64_bf16": 3, "mtb200_gemm_n128_bf16": 4}
 
 
+def capped_form(M: int, K: int, pairs_only: bool, pairs: int) -> int:
+    """Kernel of a product whose epilogue caps it (csrc/gemm_act.cuh, ACT_CAP), for one with many columns. Pairs need two row tiles and a reduction that hides
+    their epilogue: 2048 x 128256 x 1024 389 us on pairs and 434 on single CTAs, 3720 x 151936 x 1536 1153 and 1295, 700 x 65536 x 4096 278 and 302; the other way
+    round 5000 x 8192 x 512 72 and 62, 1000 x 65536 x 512 79 and 72, 129 x 32000 x 256 16 and 14."""
+    return int(pairs > 0 and (pairs_only or (M > 128 and K >= 1024)))
+
+
 def _best_split(tiles: int, units: int, kblocks: int, workers: int, max_units: int, t: tuple):
     launch, block, item, least, split, partial = t
     best = launch + -(-tiles // workers) * max(kblocks * block + item, least)

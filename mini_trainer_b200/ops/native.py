@@ -83,7 +83,8 @@ class _Sig:
     mtb200_embedding_bwd_scan = [P, P, P, I, I, I, P, P]
     mtb200_scatter_rows = [P, P, P, P, P, I, I, I, P, P]
     mtb200_ce_fwd_bwd = [P, L, I, P, P, P, P, L, I, I, F, L, P]
-    mtb200_ce_capped = [P, L, P, P, P, L, I, I, F, F, L, P]
+    mtb200_gemm_capped = [P, L, P, P, P, I, I, I, F, F, I, P, P]
+    mtb200_ce_capped = [P, P, P, P, P, P, I, I, I, F, F, F, L, P]
     mtb200_colsum = [P, L, P, P, I, I, P]
     mtb200_accumulate = [P, P, L, I, I, P]
     mtb200_f32_to_bf16 = [P, P, L, I, P]
@@ -393,29 +394,35 @@ class NativeOps:
         return dx
 
     # -- norms around a branch: residual sum between two RMSNorms ----------------------------
-    @staticmethod
-    def _is(t, shape, dtype, index):
-        return t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index
-
     def _residual_norm_check(self, y, rows, weights, fp32):
         """``(T, H)`` of ``y``; the other arguments against it. What is ``None`` is not there."""
-        shape, index, bf, ok = y.shape, y.get_device(), torch.bfloat16, self._is
+        shape, index, bf = y.shape, y.get_device(), torch.bfloat16
         if len(shape) != 2 or shape[1] < 8 or shape[1] & 7 or shape[1] > 8192:
             raise ValueError(f"rows of a multiple of 8 up to 8192 elements, not {tuple(shape)}")
         if index != self._index and self._index is not None:
             raise ValueError(f"this backend was made for {self.device}, the activations are on {y.device}")
-        bits = y.data_ptr()
-        for want, dtype, group in ((shape, bf, (y, *rows)), (shape[1:], bf, weights), (shape[:1], torch.float32, fp32)):
-            for t in group:
-                if t is None:
-                    continue
-                if not ok(t, want, dtype, index):
-                    raise ValueError(f"expected contiguous {dtype} {tuple(want)} on {y.device}, not {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
-                if dtype is bf:
-                    bits |= t.data_ptr()
+        bits = 0
+        for t in rows:
+            if t is not None:
+                if t.dtype is not bf or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+                    self._residual_norm_refuse(t, bf, shape, y)
+                bits |= t.data_ptr()
+        T, H = shape
+        for t in weights:
+            if t is not None:
+                if t.dtype is not bf or t.shape != (H,) or not t.is_contiguous() or t.get_device() != index:
+                    self._residual_norm_refuse(t, bf, (H,), y)
+                bits |= t.data_ptr()
+        for t in fp32:
+            if t is not None and (t.dtype is not torch.float32 or t.shape != (T,) or not t.is_contiguous() or t.get_device() != index):
+                self._residual_norm_refuse(t, torch.float32, (T,), y)
         if bits & 15:
             raise ValueError("rows and weights start on 16 bytes")
-        return shape
+        return T, H
+
+    @staticmethod
+    def _residual_norm_refuse(t, dtype, shape, y):
+        raise ValueError(f"expected contiguous {dtype} {tuple(shape)} on {y.device}, not {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
 
     def residual_norm(self, x, y, w_post, w_pre, eps, scale=1.0, gate=None):
         """``(h, z, (rstd_y, rstd_h))`` of ``h = x + scale * gate * RMSNorm(y; w_post)`` and ``z = RMSNorm(h; w_pre)`` in one pass over ``[T, H]`` rows. ``w_post``
@@ -423,10 +430,10 @@ class NativeOps:
         ``h`` is rounded before its norm, nothing else on the way."""
         if w_post is None and w_pre is None:
             raise ValueError("a norm behind the branch, in front of the next or both: without either this is a sum")
-        T, H = self._residual_norm_check(y, (x,), (w_post, w_pre), (gate,))
+        T, H = self._residual_norm_check(y, (y, x), (w_post, w_pre), (gate,))
         h, z = torch.empty_like(y), None if w_pre is None else torch.empty_like(y)
-        ry = None if w_post is None else torch.empty(T, dtype=torch.float32, device=y.device)
-        rh = None if w_pre is None else torch.empty(T, dtype=torch.float32, device=y.device)
+        ry = None if w_post is None else torch.empty(T, dtype=torch.float32, device=self.device)
+        rh = None if w_pre is None else torch.empty(T, dtype=torch.float32, device=self.device)
         self._call("mtb200_residual_norm_fwd", x.data_ptr(), y.data_ptr(), _ptr(w_post), _ptr(w_pre), _ptr(gate), h.data_ptr(), _ptr(z), _ptr(ry), _ptr(rh),
                    scale, eps, T, H, self.status.data_ptr(), self._st())
         return h, z, (ry, rh)
@@ -439,7 +446,7 @@ class NativeOps:
         ry, rh = stats
         if not (w_post is None) == (ry is None) == (dw_post_out is None) or not (w_pre is None) == (rh is None) == (dw_pre_out is None) == (dz is None):
             raise ValueError("a weight, its statistics and its gradients are there together or not at all")
-        T, H = self._residual_norm_check(y, (h, dh, dz), (w_post, w_pre, dw_post_out, dw_pre_out), (gate, ry, rh))
+        T, H = self._residual_norm_check(y, (y, h, dh, dz), (w_post, w_pre, dw_post_out, dw_pre_out), (gate, ry, rh))
         if dh is None and w_pre is None:
             raise ValueError("without a gradient of h or z there is nothing to do")
         dx, dy = torch.empty_like(y), torch.empty_like(y)
@@ -982,8 +989,8 @@ class NativeOps:
         return V > 16384 and H >= 1536
 
     def _linear_ce_capped(self, x, w, targets, grad_scale, dw_out, accumulate_dw, ignore_index, logit_scale, softcap):
-        """``linear_ce`` with capped logits. The products are kept in fp32 until they are capped, in half as many rows at a time, and their gradient goes to a
-        buffer of its own; nothing is held between calls."""
+        """``linear_ce`` with capped logits. The product leaves them as parts of the cap, in fp16, with the softmax's statistics formed in fp32 before that
+        rounding; the loss kernel writes their gradient over them. Nothing is held between calls."""
         ok = x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1]
         if not ok or any(t.dtype != torch.bfloat16 or t.device != x.device or not t.is_contiguous() or t.data_ptr() % 16 for t in (x, w, dw_out)) or dw_out.shape != w.shape:
             raise ValueError("expected contiguous bf16 rows [T, H], a weight [V, H] and its gradient on one device")
@@ -1002,15 +1009,18 @@ class NativeOps:
             if not accumulate_dw:
                 dw_out.zero_()
             return loss, dx
-        ck = min(max(1, self.ce_chunk // 2), T)
-        z, dz = torch.empty(ck, V, dtype=torch.float32, device=x.device), torch.empty(ck, V, dtype=torch.bfloat16, device=x.device)
+        ck = min(self.ce_chunk, T)
+        dz, stats = torch.empty(ck, V, dtype=torch.bfloat16, device=x.device), torch.empty(ck, -(-V // 128), 2, dtype=torch.float32, device=x.device)
         dw32 = None if T <= ck else torch.empty(V, H, dtype=torch.float32, device=x.device)
+        alpha, cap2 = logit_scale / softcap, softcap * 1.4426950408889634
         for a in range(0, T, ck):
             n = min(ck, T - a)
             xc = x[a:a + n]
-            self.gemm(xc, False, w, False, z, n, V, H, alpha=logit_scale)
-            self._call("mtb200_ce_capped", z.data_ptr(), V, targets[a:a + n].data_ptr(), loss[a:a + n].data_ptr(), dz.data_ptr(), V, n, V, softcap, float(grad_scale),
-                       ignore_index, self._st())
+            form = gemm_plan.capped_form(n, H, self.use_gemm2, 0 if self.pair_max_flops <= 0 and not self.use_gemm2 else self.cta_pairs())
+            self._call("mtb200_gemm_capped", xc.data_ptr(), H, w.data_ptr(), dz.data_ptr(), stats.data_ptr(), n, V, H, alpha, cap2, form, self.status.data_ptr(),
+                       self._st(), tag="gemm_nt_capped")
+            self._call("mtb200_ce_capped", dz.data_ptr(), stats.data_ptr(), xc.data_ptr(), w.data_ptr(), targets[a:a + n].data_ptr(), loss[a:a + n].data_ptr(), n, V, H,
+                       alpha, cap2, float(grad_scale), ignore_index, self._st())
             self.gemm(dz, False, w, True, dx[a:a + n], n, H, V, alpha=logit_scale)
             if dw32 is None:
                 self.gemm(dz, True, x, True, dw_out, V, H, n, residual=dw_out if accumulate_dw else None, alpha=logit_scale)

@@ -2,13 +2,14 @@
 
 Tolerances count roundings. The products z = x w come in fp32: off by at most 2^-17 of sum |x w| (sums of up to 4096 terms, added up in blocks). A capped logit is off by 5.1e-7 of
 itself within the cap and 2^-21 of the cap beyond it (and for caps over 2048), and by the product's error; the loss by those of its target and of the others on average, and
-by 2^-18 of the logits' size. Its gradient is rounded to bf16 once (U = 2^-8) before the products that dx and dw are, which are rounded once more."""
+by 2^-18 of the logits' size. The gradient is formed from l / cap rounded to fp16 (2^-11), and rounded to bf16 once (U = 2^-8) before the products that dx and dw are, which are rounded once more."""
 import pytest
 import torch
 
 from mini_trainer_b200.ops.torch_ref import TorchOps
 
 U = torch.finfo(torch.bfloat16).eps / 2
+H = torch.finfo(torch.float16).eps / 2
 IGNORE = -100
 
 
@@ -34,7 +35,10 @@ def exact(x, w, t, cap, scale, grad_scale):
     mean = (p * el).sum(1)
     bl = valid * (mean + el.gather(1, safe)[:, 0] + 2.0 ** -18 * l.abs().amax(1) + 2.0 ** -20)
     dz = (p - one) * c * (valid * grad_scale)[:, None]
-    edz = U * dz.abs() + ((p * (el + mean[:, None] + 2.0 ** -18) * c) + (p - one).abs() * (2 * el.clamp_max(cap) / cap + 2.0 ** -21)) * (valid * abs(grad_scale))[:, None]
+    # t = l / cap is rounded to fp16, H of itself or 2^-25 below its normal numbers: the exponential is off by the logit's error, the derivative 1 - t^2 by 2 |t| dt
+    et = H * th.abs().clamp_min(2.0 ** -14)
+    edz = U * dz.abs() + (1.02 * p * (el + mean[:, None] + cap * et + 2.0 ** -18) * c + (p - one).abs() * (2 * th.abs() * et + et * et + 2 * el.clamp_max(cap) / cap + 2.0 ** -21)) \
+        * (valid * abs(grad_scale))[:, None]
     dx, dw = dz @ w * scale, dz.t() @ x * scale
     bx, bw = (1.01 * edz + 2.0 ** -17 * dz.abs()) @ w.abs() * abs(scale), (1.01 * edz + 2.0 ** -17 * dz.abs()).t() @ x.abs() * abs(scale)
     return (loss, dx, dw), (bl, bx + U * dx.abs() + 1e-30, bw + U * dw.abs() + 1e-30)
@@ -88,10 +92,10 @@ def test_calls_of_the_kernels_and_their_refusals():
     ops.ce_chunk, ops._index = 64, None
     x, w, t = inputs(70, 32, 72)
     dw = torch.empty_like(w)
-    ops.linear_ce(x, w, t, 0.1, dw, softcap=30.0)   # three chunks of 32 rows: products, loss, two gradients each, the sum of dw rounded at the end
-    assert [n for n, _ in ops.calls].count("mtb200_ce_capped") == 3 and ops.calls[-1][0] == "mtb200_f32_to_bf16"
-    rows = [a[6] for n, a in ops.calls if n == "mtb200_ce_capped"]
-    assert rows == [32, 32, 6] and all(a[8] == 30.0 for n, a in ops.calls if n == "mtb200_ce_capped")
+    ops.linear_ce(x, w, t, 0.1, dw, logit_scale=0.5, softcap=30.0)   # two chunks: products, loss, two gradients each, the sum of dw rounded at the end
+    names = [n for n, _ in ops.calls]
+    assert names[:2] == names[4:6] == ["mtb200_gemm_capped", "mtb200_ce_capped"] and names[-1] == "mtb200_f32_to_bf16" and len(names) == 9
+    assert [a[6:11] for n, a in ops.calls if n == "mtb200_ce_capped"] == [(k, 72, 32, 0.5 / 30.0, 30.0 * 1.4426950408889634) for k in (64, 6)]
     n = len(ops.calls)
     dw.fill_(1.0)
     loss, dx = ops.linear_ce(x[:0], w, t[:0], 0.1, dw, accumulate_dw=True, softcap=30.0)
@@ -108,6 +112,12 @@ def test_calls_of_the_kernels_and_their_refusals():
     assert len(ops.calls) == n
 
 
+def test_choice_of_the_product():
+    from mini_trainer_b200.ops import gemm_plan
+    assert [gemm_plan.capped_form(*c, False, 74) for c in ((3720, 1536), (128, 4096), (5000, 512))] == [1, 0, 0]
+    assert gemm_plan.capped_form(3720, 1536, True, 0) == 0 and gemm_plan.capped_form(100, 64, True, 74) == 1
+
+
 # ------------------------------------------------------------------------------------------ GPU
 @pytest.fixture(scope="module")
 def ops():
@@ -117,8 +127,11 @@ def ops():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("cap,gain,scale", [(30.0, 3.0, 1.0), (2.0, 3.0, 1.0), (15.0, 100.0, 0.5), (4096.0, 3.0, 1.0), (0.01, 1.0, 1.0)])
-@pytest.mark.parametrize("T,H,V", [(1, 8, 8), (5, 64, 264), (129, 72, 1000), (33, 256, 8200), (300, 512, 4096), (17, 128, 40008)])
-def test_kernels_against_64_bits(ops, T, H, V, cap, gain, scale):
+@pytest.mark.parametrize("pair", [0, 1])
+@pytest.mark.parametrize("T,H,V", [(1, 8, 8), (5, 64, 264), (129, 72, 1000), (33, 256, 8200), (300, 512, 4096), (17, 128, 40008), (257, 1032, 520)])
+def test_kernels_against_64_bits(ops, T, H, V, cap, gain, scale, pair, monkeypatch):
+    from mini_trainer_b200.ops import gemm_plan
+    monkeypatch.setattr(gemm_plan, "capped_form", lambda *a: pair)
     check(ops, *inputs(T, H, V, gain, seed=T, device="cuda"), cap, scale, 1.0 / T)
     ops.check_status()
 
