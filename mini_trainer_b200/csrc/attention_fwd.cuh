@@ -151,6 +151,7 @@ __device__ __forceinline__ void att_unit(const AttFwdParams<R>& p, const AttDiv&
     const int a = w.q0[0] / ATT_B + 1 - from, b = w.q0[1] / ATT_B + 1 - from;
     w.n[0] = tiles + (a > 0 ? a : 0);
     w.n[1] = w.q0[1] < w.seq_len ? tiles + (b > 0 ? b : 0) : 0;
+    if (R::BIAS && w.n[1] > 0) w.n[0] = w.n[1];   // from B's diagonal back: A sees nothing of that tile
   } else {
     w.n[0] = q0 / ATT_B + 1;
     w.n[1] = w.q0[1] < w.seq_len ? w.q0[1] / ATT_B + 1 : 0;
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_kernel(const __grid_c
           for (int j = 0; j < n; ++j, ++kt) {
             const int s = kt & 1;
             const uint32_t ph = ((kt >> 1) & 1) ^ 1;
-            const int row = w.seq_start + (R::ON ? w.at(j) : j) * ATT_B;
+            const int row = w.seq_start + (R::ON ? w.at.tile<R>(j, n) : j) * ATT_B;
             if (!mbar_wait(&k_empty[s], ph, abort_flag)) { atomicExch(p.status, 11); goto done; }
             mbar_arrive_expect_tx(&k_full[s], L::TILE);
 #pragma unroll
@@ -424,20 +425,16 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_kernel(const __grid_c
           if (!ok) { atomicExch(p.status, 18); goto done; }
         }
       } else {
-        // The same under a rule, with m_ref in units of log2 e. EDGE: an edge of the mask crosses the tile. Capped or biased scores are formed in place (FORM) before
-        // their maximum; without either the scale goes into the exponential's argument as above.
+        // The same under a rule, with m_ref in units of log2 e (attention_rule.cuh).
         float slope2 = 0.f;
         if constexpr (R::BIAS) slope2 = p.r.slopes[g == 0 ? w.h[0] : w.h[1]] * 1.4426950408889634f;
         auto rule_tile = [&](auto edge, int j, int k0) -> bool {
-          constexpr bool EDGE = decltype(edge)::value, FORM = R::BIAS || R::CAP;
-          constexpr int FMA = EDGE || R::CAP ? 32 : POLY;   // masked scores want exact zeros, which the cubic does not give; the cap's polynomial fills the FMA pipe as it is
-          uint32_t sv[4][32], seen[4];
-          bool any[4];
+          AttScores<R, decltype(edge)::value, 4> s;
+          s.slope2 = slope2; s.sl2 = sl2;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, sv[c]);
+          for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, s.sv[c]);
           tmem_ld_wait();
-          float mt = att_form<R, EDGE, 4>(p.r, sv, seen, any, qpos, k0, w.prefix, w.prefix > k0 && k0 + ATT_B - 1 > qpos - r, slope2, sl2v, ts);
-          if constexpr (!FORM) mt *= sl2;   // (-inf stays: the scale is positive)
+          const float mt = s.reference(p.r, qpos, k0, qpos - r, k0, w.prefix, ts);
           float factor = 1.f;
           bool rescale = false;
           if (mt > m_ref && mt - m_ref > 8.f) {
@@ -459,39 +456,29 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_kernel(const __grid_c
               tmem_st_32x16(to + c * 16, v);
             }
           }
-          const float2 nmo = splat(m_ref == -INFINITY ? 0.f : -m_ref);
+          const float ref = m_ref == -INFINITY ? 0.f : m_ref;
           float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          att_by_way<R>(s.way, [&](auto way) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
-            if (!EDGE || any[c]) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 s = make_float2(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1]));
-                const float2 x = FORM ? fadd2(s, nmo) : ffma2(s, sl2v, nmo);
-                const float2 e = (i % FMA == FMA - 1) ? ex2_fma2(x) : make_float2(ex2_mufu(x.x), ex2_mufu(x.y));
-                l2[i & 1] = fadd2(l2[i & 1], e);
-                pk[i] = pack_bf16(e.x, e.y);
+            for (int c = 0; c < 4; ++c) {
+              uint32_t pk[16];
+              s.template probabilities<POLY, decltype(way)::value>(p.r, c, ref, pk, l2);
+              tmem_st_32x16(ts + c * 16, pk);
+              if (c & 1) {
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[2 * g + (c >> 1)]);
               }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) pk[i] = 0u;
             }
-            tmem_st_32x16(ts + c * 16, pk);
-            if (c & 1) {
-              tmem_st_wait();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_ready[2 * g + (c >> 1)]);
-            }
-          }
+          });
           l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
           return true;
         };
         for (int j = 0; j < n; ++j, ++cnt) {
           if (!mbar_wait(&s_full[g], cnt & 1, abort_flag)) { atomicExch(p.status, 17); goto done; }
           tc_fence_after();
-          const int k0 = w.at(j) * ATT_B;
+          const int k0 = w.at.tile<R>(j, n) * ATT_B;
           if (j == n - 1) att_fetch<R>(p, per_item, round, f);
           const bool ok = att_all_seen(p.r, qpos - r, k0, w.prefix) ? rule_tile(AttFalse{}, j, k0) : rule_tile(AttTrue{}, j, k0);
           if (!ok) { atomicExch(p.status, 18); goto done; }
@@ -552,7 +539,7 @@ done:
 }
 
 template <int D, class R>
-static int launch_fwd(const CUtensorMap& tm, const CUtensorMap& to, const AttFwdParams<R>& p, cudaStream_t st) {
+int launch_fwd(const CUtensorMap& tm, const CUtensorMap& to, const AttFwdParams<R>& p, cudaStream_t st) {
   static bool configured = false;
   static int sms = 0;
   auto kern = attn_fwd_kernel<D, R>;
@@ -570,7 +557,7 @@ static int launch_fwd(const CUtensorMap& tm, const CUtensorMap& to, const AttFwd
 }
 
 template <class R>
-static int fwd(const void* qkv, long long ld, void* out, long long ldo, int rows, int D, const AttFwdParams<R>& p, cudaStream_t st) {
+int fwd(const void* qkv, long long ld, void* out, long long ldo, int rows, int D, const AttFwdParams<R>& p, cudaStream_t st) {
   if ((D != 64 && D != 128) || p.Hkv <= 0 || p.Hq % p.Hkv || ld % 8 || ldo % 8 || (!p.row_pairs && (p.Hq / p.Hkv) % 2)) return -10;
   CUtensorMap tm;
   CUtensorMap to;

@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_one_kernel(const __gr
       for (int j = 0; j < n_tiles; ++j) {
         const int s = j & 1;
         if (!mbar_wait(&k_empty[s], ((j >> 1) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 11); goto done; }
-        const int row = seq_start + (R::ON ? at(j) : j) * ATT_BN;
+        const int row = seq_start + (R::ON ? at.tile<R>(j, n_tiles) : j) * ATT_BN;
         mbar_arrive_expect_tx(&k_full[s], L::KV_BYTES);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -231,16 +231,12 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_one_kernel(const __gr
       if constexpr (R::ON) {
         // Under a rule, with m_ref in units of log2 e: attention_rule.cuh; EDGE: an edge of the mask crosses the tile.
         auto rule_tile = [&](auto edge, int k0) -> bool {
-          constexpr bool EDGE = decltype(edge)::value, FORM = R::BIAS || R::CAP;
-          constexpr int FMA = EDGE || R::CAP ? 32 : POLY;
-          uint32_t sv[2][32], seen[2];
-          bool any[2];
-          tmem_ld_32x32(ts + half * 64, sv[0]);
-          tmem_ld_32x32(ts + half * 64 + 32, sv[1]);
+          AttScores<R, decltype(edge)::value, 2> s;
+          s.slope2 = slope2; s.sl2 = sl2;
+          tmem_ld_32x32(ts + half * 64, s.sv[0]);
+          tmem_ld_32x32(ts + half * 64 + 32, s.sv[1]);
           tmem_ld_wait();
-          const float2 sl2v = make_float2(sl2, sl2);
-          float mt = att_form<R, EDGE, 2>(p.r, sv, seen, any, qpos, k0 + half * 64, prefix, prefix > k0 && k0 + ATT_BN - 1 > q0, slope2, sl2v, ts + half * 64);
-          if constexpr (!FORM) mt *= sl2;
+          const float mt = s.reference(p.r, qpos, k0 + half * 64, q0, k0, prefix, ts + half * 64);
           float factor = 1.f;
           bool rescale = false;
           if (mt > m_ref && mt - m_ref > 8.f) {
@@ -263,30 +259,20 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_one_kernel(const __gr
             }
             tmem_st_wait();
           }
-          const float2 nmo = splat(m_ref == -INFINITY ? 0.f : -m_ref);
-          float2 l2 = make_float2(0.f, 0.f);
+          const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+          float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          att_by_way<R>(s.way, [&](auto way) {
 #pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            uint32_t pk[16];
-            if (!EDGE || any[cc]) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 s = make_float2(__uint_as_float(sv[cc][2 * i]), __uint_as_float(sv[cc][2 * i + 1]));
-                const float2 x = FORM ? fadd2(s, nmo) : ffma2(s, sl2v, nmo);
-                const float2 e = (i % FMA == FMA - 1) ? ex2_fma2(x) : make_float2(ex2_mufu(x.x), ex2_mufu(x.y));
-                l2 = fadd2(l2, e);
-                pk[i] = pack_bf16(e.x, e.y);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) pk[i] = 0u;
+            for (int cc = 0; cc < 2; ++cc) {
+              uint32_t pk[16];
+              s.template probabilities<POLY, decltype(way)::value>(p.r, cc, ref, pk, l2);
+              tmem_st_32x16(ts + half * 64 + cc * 16, pk);
             }
-            tmem_st_32x16(ts + half * 64 + cc * 16, pk);
-          }
-          l += l2.x + l2.y;
+          });
+          l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
           return true;
         };
-        const int k0 = at(j) * ATT_BN;
+        const int k0 = at.tile<R>(j, n_tiles) * ATT_BN;
         if (!(att_all_seen(p.r, q0, k0, prefix) ? rule_tile(No{}, k0) : rule_tile(Yes{}, k0))) { atomicExch(p.status, 18); goto done; }
       } else {
         const bool diag = (j == n_tiles - 1);

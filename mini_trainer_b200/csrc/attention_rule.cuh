@@ -38,7 +38,13 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 
 // Key tiles of 128 that a tile of query rows [q0, q0 + 128) looks at: the prefix's, then those from `skip` on behind them.
 struct AttTiles {
   int prefix_tiles, skip;
-  __device__ __forceinline__ int operator()(int j) const { return j >= prefix_tiles ? j + skip : j; }
+  // The j-th of n. With a bias from the diagonal back: near keys have the larger scores, so the reference maximum is found at once and the accumulator hardly ever
+  // rescaled (the other way round it was in nearly every tile: 280 us where it takes 215, 8192 tokens in three samples, 32/8 heads of 128).
+  template <class R>
+  __device__ __forceinline__ int tile(int j, int n) const {
+    if (R::BIAS) j = n - 1 - j;
+    return j >= prefix_tiles ? j + skip : j;
+  }
 };
 // Whether every row of [q0, q0 + 128) sees every key of [k0, k0 + 128).
 __device__ __forceinline__ bool att_all_seen(const AttRuleArgs& r, int q0, int k0, int prefix) {
@@ -54,80 +60,182 @@ __device__ __forceinline__ uint32_t att_queries_seen(const AttRuleArgs& r, int j
 }
 
 
-// Scores of one query and C x 32 keys from `key` on, formed in place, and their maximum. EDGE: an edge of the mask crosses the tile; masked scores become -inf, `seen` and `any`
-// (whether one of the warp's rows sees a key of 32) are left for the exponentials. With a cap or a bias the scores and the maximum come in units of log2 e
-// (FORM); without either they stay products, which the scale still has to be applied to. taddr: where the products came from in tensor memory.
+// One query's scores against C x 32 keys from `key` on, raw products in registers, on their way to probabilities.
+//
+// The reference of the exponentials does not have to be the largest score, only near it and the same throughout. A cap is monotonic, so the largest product capped is
+// the largest capped score; a bias is not, but within 32 keys it changes by 31 slopes: the largest product of each 32, capped, with the bias of the nearer
+// end is a bound that is too high by at most that. Where capped scores are small, up to 2^+-30 as exponentials, their largest absolute value, which has to be known for the cap's
+// polynomial anyhow, is bound enough: 2^60 too high at most, which fp32 has room for. So the scores themselves are only formed on their way into the exponentials, which
+// keeps the FMA pipe and the special-function unit busy at once; formed in place first, capped scores took 286 us where they take 250 (8192 tokens in three samples,
+// 32/8 heads of 128; 194 without a cap). They are formed in place, and their largest taken, where this does not hold (`formed`):
+// products beyond the cap, slopes so steep that the bound could be 2^40 too high for them alone, and biased keys behind the query.
+constexpr float ATT_STEEP = 40.f / 31.f;
+// Which way a tile takes is decided once for all of it: branches for every 32 keys kept the compiler from mixing their instructions (bias 247 -> 279 us).
+enum { ATT_RAW = 0, ATT_LOW = 1, ATT_FORMED = 2 };   // from products; the same within half of the cap; scores formed in place
+// EDGE: an edge of the mask crosses the tile. Left for the exponentials: `seen`, `any` (whether one of the warp's rows sees a key of 32), the bias.
 template <class R, bool EDGE, int C>
-__device__ __forceinline__ float att_form(const AttRuleArgs& r, uint32_t (&sv)[C][32], uint32_t (&seen)[C], bool (&any)[C], int query, int key, int prefix, bool right,
-                                          float slope2, float2 sl2v, uint32_t taddr) {
-  auto pair = [&](int c, int i) { return make_float2(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1])); };
-  auto put = [&](int c, int i, float2 v) { sv[c][2 * i] = __float_as_uint(v.x); sv[c][2 * i + 1] = __float_as_uint(v.y); };
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    seen[c] = EDGE ? att_keys_seen(r, query, key + c * 32, prefix) : 0xffffffffu;
-    any[c] = !EDGE || __any_sync(0xffffffffu, seen[c] != 0u);
-  }
-  if constexpr (R::CAP) {
-    float big = 0.f;
+struct AttScores {
+  uint32_t sv[C][32], seen[C];
+  bool any[C];
+  int way;
+  float slope2, from, sl2;   // slope in units of log2 e (negated where keys are behind the queries), first key minus query
+
+  __device__ __forceinline__ float2 pair(int c, int i) const { return make_float2(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1])); }
+  __device__ __forceinline__ bool sees(int c, int i) const { return !EDGE || (seen[c] >> i & 1u); }
+
+  // Forms the scores, masked ones -inf, and returns their maximum.
+  __device__ __forceinline__ float form(const AttRuleArgs& r, bool small) {
+    float m[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      float b = 0.f;
+      m[c] = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) b = fmax3(b, fabsf(__uint_as_float(sv[c][i])), fabsf(__uint_as_float(sv[c][i + 1])));
-      big = fmaxf(big, b);
+      for (int i = 0; i < 16; ++i) {
+        float2 v = pair(c, i);
+        if constexpr (R::CAP) { if (small) v = cap_pair(r.cap, v); }
+        else v = fmul2(v, splat(sl2));
+        if constexpr (R::BIAS) {
+          const float x = from + (c * 32 + 2 * i), y = from + (c * 32 + 2 * i + 1);
+          v = ffma2(splat(-slope2), make_float2(fabsf(x), fabsf(y)), v);
+        }
+        if (!sees(c, 2 * i)) v.x = -INFINITY;
+        if (!sees(c, 2 * i + 1)) v.y = -INFINITY;
+        sv[c][2 * i] = __float_as_uint(v.x); sv[c][2 * i + 1] = __float_as_uint(v.y);
+        m[c] = fmax3(m[c], v.x, v.y);
+      }
     }
-    if (__all_sync(0xffffffffu, big <= r.cap.most)) {
+    float most = fmaxf(m[0], m[1]);
+#pragma unroll
+    for (int c = 2; c < C; c += 2) most = fmax3(most, m[c], m[c + 1]);
+    return most;
+  }
+
+  // The reference: largest score, or the bound, in units of log2 e; -inf where nothing is seen. The tile: 128 queries from q0, keys from k0 on, of which this thread
+  // has those from `key` on.
+  __device__ __forceinline__ float reference(const AttRuleArgs& r, int query, int key, int q0, int k0, int prefix, uint32_t taddr) {
+    from = static_cast<float>(key - query);
+    bool small = true, low = false;
+    float big[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      seen[c] = EDGE ? att_keys_seen(r, query, key + c * 32, prefix) : 0xffffffffu;
+      any[c] = !EDGE || __any_sync(0xffffffffu, seen[c] != 0u);
+    }
+    if constexpr (R::CAP) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        big[c] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) big[c] = fmax3(big[c], fabsf(__uint_as_float(sv[c][i])), fabsf(__uint_as_float(sv[c][i + 1])));
+      }
+      float most = big[0];
+#pragma unroll
+      for (int c = 1; c < C; ++c) most = fmaxf(most, big[c]);
+      low = __all_sync(0xffffffffu, most <= r.cap.low);
+      small = low || __all_sync(0xffffffffu, most <= r.cap.most);
+      if (!small) {
+        cap_in_place(r.cap, taddr, 2 * C);
+#pragma unroll
+        for (int c = 0; c < C; ++c) tmem_ld_32x32(taddr + c * 32, sv[c]);
+        tmem_ld_wait();
+      }
+    }
+    way = low ? ATT_LOW : ATT_RAW;
+    if constexpr (R::CAP || R::BIAS) {
+      bool formed = !small;
+      if constexpr (R::BIAS) {   // keys behind their query are only seen in a prefix; the tile on the diagonal has both kinds
+        const bool right = prefix > k0 && k0 + 127 > q0;
+        formed = formed || (right && k0 < q0 + 128) || fabsf(slope2) > ATT_STEEP;
+        if (right && !formed) slope2 = -slope2;
+      }
+      if (formed) {
+        way = ATT_FORMED;
+        return form(r, small);
+      }
+    }
+    float mc[C];   // independent chains
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      mc[c] = -INFINITY;
+      if (EDGE && !any[c]) continue;
+      if (EDGE && !R::CAP) {   // (a masked product that stayed infinite would be NaN when it is capped)
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (!sees(c, i)) sv[c][i] = 0xff800000u;   // -inf
+      }
+    }
+    if (R::CAP && !EDGE && low) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) mc[c] = big[c];
+    } else {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         if (EDGE && !any[c]) continue;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) put(c, i, cap_pair(r.cap, pair(c, i)));
+        for (int i = 0; i < 32; i += 2) {
+          float x = __uint_as_float(sv[c][i]), y = __uint_as_float(sv[c][i + 1]);
+          if (R::CAP && !sees(c, i)) x = -INFINITY;
+          if (R::CAP && !sees(c, i + 1)) y = -INFINITY;
+          mc[c] = fmax3(mc[c], x, y);
+        }
       }
-    } else {
-      cap_in_place(r.cap, taddr, 2 * C);
-#pragma unroll
-      for (int c = 0; c < C; ++c) tmem_ld_32x32(taddr + c * 32, sv[c]);
-      tmem_ld_wait();
     }
+    if constexpr (R::BIAS) {   // of 32 keys the nearest has the larger bias unless the slope is negative
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float near = fmaxf(slope2 * (from + (c * 32)), slope2 * (from + (c * 32 + 31)));
+        if (mc[c] > -INFINITY) mc[c] = R::CAP ? cap_exact(r.cap, mc[c]) + near : fmaf(mc[c], sl2, near);
+      }
+    }
+    float m = fmaxf(mc[0], mc[1]);
+#pragma unroll
+    for (int c = 2; c < C; c += 2) m = fmax3(m, mc[c], mc[c + 1]);
+    if constexpr (!R::BIAS) m = m == -INFINITY ? m : R::CAP ? cap_exact(r.cap, m) : m * sl2;
+    return m;
   }
-  if constexpr (R::BIAS) {
-    auto add = [&](int c, int i, float2 b) { put(c, i, R::CAP ? fadd2(pair(c, i), b) : ffma2(pair(c, i), sl2v, b)); };
-    const float from = static_cast<float>(key - query);
-    if (right) {   // keys behind the query, which only a prefix shows it
+
+  // 32 probabilities, exp2(score - ref), of piece c: rounded to bf16 pairs, and their sum. Every FMA_EVERY-th pair is formed on the FMA pipe, where nothing is
+  // masked, which wants exact zeros, and the cap's polynomial does not fill that pipe as it is.
+  template <int FMA_EVERY, int WAY>
+  __device__ __forceinline__ void probabilities(const AttRuleArgs& r, int c, float ref, uint32_t (&pk)[16], float2 (&l2)[2]) const {
+    if (EDGE && !any[c]) {
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) add(c, i, make_float2(-slope2 * fabsf(from + (c * 32 + 2 * i)), -slope2 * fabsf(from + (c * 32 + 2 * i + 1))));
-    } else {
-      float2 off[4];   // within 8 keys
+      for (int i = 0; i < 16; ++i) pk[i] = 0u;
+      return;
+    }
+    constexpr int FMA = EDGE || R::CAP ? 32 : FMA_EVERY;
+    [[maybe_unused]] float2 off[4] = {};   // of the bias, within 8 keys
+    if constexpr (R::BIAS) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) off[i] = make_float2(slope2 * (2 * i), slope2 * (2 * i + 1));
+    }
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (EDGE && !any[c]) continue;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) add(c, i, fadd2(off[i & 3], splat(slope2 * (from + (c * 32 + (i >> 2) * 8)))));
+    for (int i = 0; i < 16; ++i) {
+      float2 x;
+      if constexpr (WAY == ATT_FORMED) x = fadd2(pair(c, i), splat(-ref));
+      else {
+        const float2 b = R::BIAS ? fadd2(off[i & 3], splat(fmaf(slope2, from + (c * 32 + (i >> 2) * 8), -ref))) : splat(-ref);
+        x = WAY == ATT_LOW ? cap_half(r.cap, pair(c, i), b) : R::CAP ? cap_pair(r.cap, pair(c, i), b) : ffma2(pair(c, i), splat(sl2), b);
+        if (R::CAP && !sees(c, 2 * i)) x.x = -INFINITY;
+        if (R::CAP && !sees(c, 2 * i + 1)) x.y = -INFINITY;
       }
+      const float2 e = (i % FMA == FMA - 1) ? ex2_fma2(x) : make_float2(ex2_mufu(x.x), ex2_mufu(x.y));
+      l2[i & 1] = fadd2(l2[i & 1], e);
+      pk[i] = pack_bf16(e.x, e.y);
     }
   }
-  float mc[C];   // independent chains
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    mc[c] = -INFINITY;
-    if constexpr (EDGE) {
-      if (!any[c]) continue;
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (!(seen[c] >> i & 1u)) sv[c][i] = 0xff800000u;   // -inf
-    }
-    mc[c] = fmaxf(__uint_as_float(sv[c][0]), __uint_as_float(sv[c][1]));
-#pragma unroll
-    for (int i = 2; i < 32; i += 2) mc[c] = fmax3(mc[c], __uint_as_float(sv[c][i]), __uint_as_float(sv[c][i + 1]));
+};
+template <int W> struct AttWay { static constexpr int value = W; };
+// emit(AttWay) for the way a tile takes.
+template <class R, typename Emit>
+__device__ __forceinline__ void att_by_way(int way, Emit emit) {
+  if constexpr (R::CAP) {
+    if (way == ATT_LOW) { emit(AttWay<ATT_LOW>{}); return; }
   }
-  float m = fmaxf(mc[0], mc[1]);
-#pragma unroll
-  for (int c = 2; c < C; c += 2) m = fmax3(m, mc[c], mc[c + 1]);
-  return m;
+  if constexpr (R::CAP || R::BIAS) {
+    if (way == ATT_FORMED) { emit(AttWay<ATT_FORMED>{}); return; }
+  }
+  emit(AttWay<ATT_RAW>{});
 }
 
 }  // namespace mtb

@@ -1,6 +1,14 @@
 // Attention forward under a rule: instances of the kernel in attention_fwd.cuh (mathematics and masks: attention_rule.cuh).
 #include "attention_fwd.cuh"
 
+namespace mtb {
+// the instances with a cap take the compiler longest: attention_rule_fwd_cap*.cu
+extern template int launch_fwd<64, Rule<true, false>>(const CUtensorMap&, const CUtensorMap&, const AttFwdParams<Rule<true, false>>&, cudaStream_t);
+extern template int launch_fwd<128, Rule<true, false>>(const CUtensorMap&, const CUtensorMap&, const AttFwdParams<Rule<true, false>>&, cudaStream_t);
+extern template int launch_fwd<64, Rule<true, true>>(const CUtensorMap&, const CUtensorMap&, const AttFwdParams<Rule<true, true>>&, cudaStream_t);
+extern template int launch_fwd<128, Rule<true, true>>(const CUtensorMap&, const CUtensorMap&, const AttFwdParams<Rule<true, true>>&, cudaStream_t);
+}  // namespace mtb
+
 // Under a rule (attention_rule.cuh). plan: [n_items, 4] = (seq_start, seq_len, q0, prefix). rows <= T: those of the samples; what lies behind them is neither
 // read (the loads give zeros there) nor written. cap, window: 0 for none; slopes [Hq] fp32 or null.
 extern "C" int mtb200_attn_rule_fwd(const void* qkv, long long ld, void* out, long long ldo, float* lse, const int* plan, int n_items, int T, int rows, int Hq,

@@ -1,7 +1,7 @@
 // Numbers capped by a tanh, unit tanh(scale s / cap): attention wants them in units of log2 e, as its exponentials do (unit = cap log2 e), the head as a part of the cap (1).
 //
 // Up to the cap (|scale s| <= cap; bigger ones are rare) an odd polynomial of degree eleven, fitted to the least relative error on [-1, 1] (5.1e-7), with the powers of
-// scale / cap in its coefficients: seven packed instructions for two numbers. Beyond it tanh as 1 - 2 / (1 + e^2x), two operations on the special-function
+// scale / cap in its coefficients: seven packed instructions for two numbers; up to half of it one of degree seven on [-1/2, 1/2] (5.4e-7), five. Beyond the cap tanh as 1 - 2 / (1 + e^2x), two operations on the special-function
 // unit each, whose error is 2^-22 of the cap: a softmax that is bound by that unit as it is would do three times the work there.
 #pragma once
 #include <stdint.h>
@@ -12,10 +12,12 @@ namespace mtb {
 
 // The polynomial: tanh(x) = x (C0 + C1 x^2 + ...).
 constexpr float CAP_C[6] = {0.99999949f, -0.33329398f, 0.13284259f, -0.05168433f, 0.01683263f, -0.00310275f};
+constexpr float CAP_HALF[4] = {0.99999948f, -0.33326467f, 0.13191882f, -0.04444443f};
 
 struct CapArgs {
   float2 a[6];       // twice each, for packed arithmetic: s (a0 + a1 s^2 + ...)
-  float most;        // |s| up to which that holds
+  float2 b[4];       // the same of degree seven
+  float most, low;   // |s| up to which they hold; `low` also keeps capped numbers within +-30
   float unit, k2;    // k2: 2 scale / cap log2 e
   float inv2;        // -1 / unit^2: the derivative is 1 + inv2 v^2 of a capped number v
 };
@@ -27,8 +29,11 @@ inline CapArgs cap_args(float scale, float cap, double unit) {
   CapArgs r{};
   const double k = static_cast<double>(scale) / cap;
   double p = k;
+  for (int i = 0; i < 4; ++i, p *= k * k) r.b[i].x = r.b[i].y = static_cast<float>(unit * CAP_HALF[i] * p);
+  p = k;
   for (int i = 0; i < 6; ++i, p *= k * k) r.a[i].x = r.a[i].y = static_cast<float>(unit * CAP_C[i] * p);
   r.most = k >= 0x1p-11 ? static_cast<float>(1.0 / k) : -1.f;   // below, k^11 is no normal number: the exact form throughout
+  r.low = r.most * static_cast<float>(unit > 60.0 ? 30.0 / unit : 0.5);
   r.unit = static_cast<float>(unit);
   r.k2 = static_cast<float>(2.0 * k * 1.4426950408889634);
   r.inv2 = static_cast<float>(-1.0 / (unit * unit));
@@ -42,15 +47,24 @@ __device__ __forceinline__ float cap_exact(const CapArgs& r, float s) {
   return fmaf(-2.f * r.unit, q, r.unit);
 }
 __device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
-// A pair within the cap.
-__device__ __forceinline__ float2 cap_pair(const CapArgs& r, float2 s) {
+// A pair within the cap, over s; then the pair itself, and with something added.
+__device__ __forceinline__ float2 cap_part(const CapArgs& r, float2 s) {
   const float2 u = fmul2(s, s);
   float2 p = ffma2(u, r.a[5], r.a[4]);
   p = ffma2(u, p, r.a[3]);
   p = ffma2(u, p, r.a[2]);
   p = ffma2(u, p, r.a[1]);
-  return fmul2(s, ffma2(u, p, r.a[0]));
+  return ffma2(u, p, r.a[0]);
 }
+// Up to half of the cap.
+__device__ __forceinline__ float2 cap_half(const CapArgs& r, float2 s, float2 plus) {
+  const float2 u = fmul2(s, s);
+  float2 p = ffma2(u, r.b[3], r.b[2]);
+  p = ffma2(u, p, r.b[1]);
+  return ffma2(s, ffma2(u, p, r.b[0]), plus);
+}
+__device__ __forceinline__ float2 cap_pair(const CapArgs& r, float2 s) { return fmul2(s, cap_part(r, s)); }
+__device__ __forceinline__ float2 cap_pair(const CapArgs& r, float2 s, float2 plus) { return ffma2(s, cap_part(r, s), plus); }
 // The same of numbers that are parts of the cap already, tanh(x).
 __device__ __forceinline__ float2 tanh_pair(float2 x) {
   const float2 u = fmul2(x, x);
