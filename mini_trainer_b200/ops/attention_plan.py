@@ -139,20 +139,25 @@ def rule_items(cu_host, prefixes, window: int, block: int, backward: bool) -> li
     return items
 
 
-def rule_in_pairs(work: list, pair_work, hq: int, hkv: int, d: int, sms: int) -> bool:
+# Forward, a key tile of one and of two query tiles with (cap, bias) over one without: batches of two to forty samples at both head dimensions.
+_RULE_TILE = {(False, False): (1.0, 1.0), (True, False): (1.27, 1.27), (False, True): (1.12, 1.17), (True, True): (1.45, 1.65)}
+
+
+def rule_in_pairs(work: list, pair_work, hq: int, hkv: int, d: int, sms: int, cap: bool = False, bias: bool = False) -> bool:
     """``forward_in_pairs`` for row blocks of these numbers of key tiles. ``pair_work()``: where heads do not pair up, ``(tiles, has a partner)`` of every pair
     of row blocks."""
     if not work:
         return True
     if len(work) * hq <= sms:
         return False
+    one_tile, two_tiles = _RULE_TILE[cap, bias]
     launch, a, b = _ONE[d]
-    one = launch + finish_time([(a + b * n, c * hq) for n, c in Counter(work).items()], sms)
+    one = launch + finish_time([(a + one_tile * b * n, c * hq) for n, c in Counter(work).items()], sms)
     launch, a, b, ra, rb, la, lb = _TWO[d]
     if (hq // hkv) % 2 == 0:
-        units = [(a + b * n, c * hq // 2) for n, c in Counter(work).items()]
+        units = [(a + two_tiles * b * n, c * hq // 2) for n, c in Counter(work).items()]
     else:
-        units = [((ra + rb * n) if two else (la + lb * n), c * hq) for (n, two), c in Counter(pair_work()).items()]
+        units = [((ra + two_tiles * rb * n) if two else (la + two_tiles * lb * n), c * hq) for (n, two), c in Counter(pair_work()).items()]
     return launch + finish_time(units, sms) <= one
 
 

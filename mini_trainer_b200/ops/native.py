@@ -189,7 +189,7 @@ class NativeOps:
         self._gemm_plans = {}   # sizes of a product, or of a grouped one -> entry point and splits, or mode
         self._epoch = itertools.count(1)   # of the launches that may split
         self._attn_plan_cache = {}
-        self._captured_plans = []   # work tables of captured launches under a rule: a graph may be replayed for as long as there is one
+        self._captured = []   # what captured launches under a rule read and copy: a graph may be replayed for as long as there is one
         self._block_specs = {}   # sizes of a block -> its products' plans
         self._pairs = None
         self.sms = torch.cuda.get_device_properties(self._index).multi_processor_count
@@ -645,19 +645,20 @@ class NativeOps:
     def _rule_plan(self, cu_host, hq, hkv, d, scale, rule, T, backward):
         """``(work table, tokens of the samples, entry point, its row_pairs argument)`` of a batch's forward, ``(work table, tokens of the samples, CTAs per key
         block, bytes of their partials, launched in order)`` of its backward. Checked when it is made and kept like the plans of the causal form, by the values
-        it depends on. A table that a capture makes is only filled when its graph runs, so it serves that launch alone; it lives, with the host
-        memory it is copied from, as long as this backend."""
-        what = (backward, hq, hkv, d, scale, rule.key)
+        it depends on, and for the stream that fills the table and gives it back. A table that a capture makes is only filled when its graph runs, so it
+        serves that launch alone; what a graph reads, the host memory that such a table is copied from or a table made before, lives as long as this backend."""
+        what = (backward, hq, hkv, d, scale, rule.key, rule.slopes is None, self._st())
         capturing = torch.cuda.is_current_stream_capturing()
         plan = self._cached(cu_host, what)
         if plan is None:
             plan = self._make_rule_plan(cu_host, hq, hkv, d, scale, rule, T, backward, capturing)
             if not capturing:
                 self._keep(cu_host, what, plan)
-        elif plan[1] > T:
+            return plan
+        if plan[1] > T:
             rule.check_starts(cu_host, T)
         if capturing:
-            self._captured_plans.append(plan[0])
+            self._captured.append(plan[0])
         return plan
 
     def _make_rule_plan(self, cu_host, hq, hkv, d, scale, rule, T, backward, capturing):
@@ -682,7 +683,8 @@ class NativeOps:
             tail = (splits, splits * units * 2 * 128 * d * 4, int(attention_plan.rule_in_order(work, hq, hkv, d, splits)))
         else:
             pairs = attention_plan.rule_items(cu_host, prefixes, window, 256, False) if (hq // hkv) % 2 else []
-            if attention_plan.rule_in_pairs(work, lambda: [(it[0], it[3] + 128 < it[2]) for it in pairs], hq, hkv, d, self.sms):
+            if attention_plan.rule_in_pairs(work, lambda: [(it[0], it[3] + 128 < it[2]) for it in pairs], hq, hkv, d, self.sms,
+                                            rule.cap is not None, rule.slopes is not None):
                 items, tail = pairs or items, ("mtb200_attn_rule_fwd", ((hq // hkv) % 2,))
             else:
                 tail = ("mtb200_attn_rule_fwd_one", ())
@@ -691,7 +693,7 @@ class NativeOps:
             table = None
         elif capturing:
             host = torch.tensor(rows, dtype=torch.int32).pin_memory()
-            self._captured_plans.append(host)
+            self._captured.append(host)
             table = host.to(self.device, non_blocking=True)
         else:
             table = self._move_table(rows)

@@ -231,7 +231,7 @@ def test_forward_of_a_rule_without_edges_takes_the_causal_form():
 def host_ops():
     from .test_native_host import make_ops
     ops = make_ops()
-    ops.attention_impl, ops._captured_plans = "native", []
+    ops.attention_impl, ops._captured = "native", []
     ops._move_table = lambda rows: torch.tensor(rows, dtype=torch.int32)
     ops._index = None
     return ops
@@ -247,7 +247,7 @@ def test_kernel_calls_get_the_rule_and_its_table(monkeypatch):
     name, args = ops.calls[-1]
     assert name == "mtb200_attn_rule_fwd_one" and args[6:12] == (4, 336, 330, 4, 2, 64) and args[13:15] == (30.0, 50) and args[15] == rule.slopes.data_ptr()
     assert not out[330:].any() and not lse[:, 330:].any()
-    table = ops._cached(cu, (False, 4, 2, 64, 0.125, rule.key))[0]
+    table = ops._cached(cu, (False, 4, 2, 64, 0.125, rule.key, False, 0))[0]
     assert sorted(map(tuple, table.tolist())) == [(0, 200, 0, 3), (0, 200, 128, 3), (200, 130, 0, 0), (200, 130, 128, 0)]
     ops.attention(qkv, None, cu, 200, 4, 2, 64, rule=AttentionRule(window=50, prefix=[4, 0]))   # another prefix is another table
     assert ops.calls[-1][1][5] != args[5]
@@ -334,6 +334,62 @@ def test_every_combination_on_ragged_samples(ops, d, form, monkeypatch):
         want, bound = exact(qkv, starts(case[0]), hq, hkv, d, rule_of(case), dout)
         for g, w, b in zip(run(ops, case, qkv, dout), want, bound):
             within(g, w, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pairs", "one"])
+@pytest.mark.parametrize("cap", [None, 25.0, 120.0])
+def test_slopes_of_every_size_and_sign(ops, cap, form, monkeypatch):
+    """Zero, so steep that only the query itself counts, and negative ones, which favour the far end; a prefix with keys behind the query."""
+    monkeypatch.setattr(A, "rule_in_pairs", lambda *a: form == "pairs")
+    ops._attn_plan_cache.clear()
+    lens, hq, hkv, d = [400, 131], 6, 2, 64
+    cu, qkv_dout = starts(lens), make(lens, hq, hkv, d, gain=3.0, device="cuda")
+    for prefix, window in ((None, None), ([390, 7], 50)):
+        slopes = torch.tensor([0.0, 1e-4, 0.6, 4.0, 60.0, -0.05], device="cuda")
+        rule = AttentionRule(cap=cap, window=window, prefix=prefix, slopes=slopes)
+        qkv, dout = qkv_dout
+        o, l = ops.attention(qkv, None, cu, 400, hq, hkv, d, rule=rule)
+        g = ops.attention_bwd(dout, qkv, o, l, None, cu, 400, hq, hkv, d, rule=rule)
+        want, bound = exact(qkv, cu, hq, hkv, d, rule, dout)
+        for x, w, b in zip((o, l, g), want, bound):
+            within(x, w, b)
+    ops.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [0.02, 1.0, 60.0, 300.0])
+def test_caps_of_every_size(ops, cap):
+    """Around the border between the polynomials, the exact form, and caps beyond the polynomials' coefficients."""
+    lens, hq, hkv, d = [200, 129], 2, 1, 128
+    for gain in (0.2, 4.0, 14.0):
+        case = (lens, hq, hkv, d, cap, None, None, False)
+        qkv, dout = make(lens, hq, hkv, d, gain=gain, device="cuda")
+        want, bound = exact(qkv, starts(lens), hq, hkv, d, rule_of(case), dout)
+        for x, w, b in zip(run(ops, case, qkv, dout), want, bound):
+            within(x, w, b)
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(ops):
+    """One batch, the same host list, on streams that do not wait for each other: each fills a work table of its own."""
+    case = ([900, 77, 300], 6, 2, 128, 30.0, 300, [100, 0, 300], True)
+    qkv, dout = make(case[0], 6, 2, 128, device="cuda")
+    rule, cu = rule_of(case, "cuda"), starts(case[0])
+    want = ops.attention(qkv, None, cu, 900, 6, 2, 128, rule=rule)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                o, l = ops.attention(qkv, None, cu, 900, 6, 2, 128, rule=rule)
+                got.append((o, l, ops.attention_bwd(dout, qkv, o, l, None, cu, 900, 6, 2, 128, rule=rule)))
+    torch.cuda.synchronize()
+    exactly, bound = exact(qkv, cu, 6, 2, 128, rule_of(case), dout)
+    for o, l, g in got:
+        assert torch.equal(o, want[0]) and torch.equal(l, want[1])
+        within(g, exactly[2], bound[2])
+    ops.check_status()
 
 
 @pytest.mark.gpu
