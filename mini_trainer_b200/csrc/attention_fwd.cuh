@@ -325,12 +325,14 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_kernel(const __grid_c
     uint8_t* box = smem + L::OFF_OUT + (warp - 4) * 4096;
     const float2 sl2v = make_float2(sl2, sl2);
     uint32_t cnt = 0;
+    [[maybe_unused]] uint32_t kt = 0, kt_next = 0;   // key tiles of the CTA before this unit, and behind it
     AttWork w;
     AttNext f;
     att_fetch<R>(p, per_item, 0, f);
     for (int round = 1; f.more; ++round) {
       att_unit<R>(p, group, f, w);
       const int n = g == 0 ? w.n[0] : w.n[1];
+      if constexpr (R::ON) { kt = kt_next; kt_next += w.tiles(); }
       if (n == 0) { att_fetch<R>(p, per_item, round, f); continue; }
       const int qpos = (g == 0 ? w.q0[0] : w.q0[1]) + r;
       float m_ref = -INFINITY, l = 0.f;
@@ -455,6 +457,12 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_kernel(const __grid_c
               for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
               tmem_st_32x16(to + c * 16, v);
             }
+          }
+          // the sample's last tile: V's rows behind it, once for the pair, whose products A's come before
+          if (decltype(edge)::value && k0 + ATT_B > w.seq_len && (g == 0 || j >= w.n[0])) {
+            const uint32_t t = kt + j;
+            if (!mbar_wait(&v_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
+            zero_rows<KB>(smem + L::OFF_V + (t & 1) * L::TILE, w.seq_len - k0, r, 128);
           }
           const float ref = m_ref == -INFINITY ? 0.f : m_ref;
           float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};

@@ -259,6 +259,10 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) attn_fwd_one_kernel(const __gr
             }
             tmem_st_wait();
           }
+          if (decltype(edge)::value && k0 + ATT_BN > seq_len) {   // the sample's last tile: V's rows behind it
+            if (!mbar_wait(&v_full[j & 1], (j >> 1) & 1, abort_flag)) return false;
+            zero_rows<KB>(smem + L::OFF_V + (j & 1) * L::KV_BYTES, seq_len - k0, threadIdx.x - 64, 256);
+          }
           const float ref = m_ref == -INFINITY ? 0.f : m_ref;
           float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           att_by_way<R>(s.way, [&](auto way) {

@@ -70,6 +70,19 @@ __device__ __forceinline__ uint32_t att_queries_seen(const AttRuleArgs& r, int j
 // 32/8 heads of 128; 194 without a cap). They are formed in place, and their largest taken, where this does not hold (`formed`):
 // products beyond the cap, slopes so steep that the bound could be 2^40 too high for them alone, and biased keys on the diagonal.
 constexpr float ATT_STEEP = 40.f / 31.f;
+// Rows [first, 128) of a [128, 64 KB] tile in shared memory (128B swizzle: a row's bytes stay together) set to zero by `n` threads, for reads by the tensor core behind
+// the caller's next arrival. A tile at a sample's end holds rows of the next sample, which meet probabilities and gradients of zero; a product
+// with zero is only zero for finite numbers, and one sample's infinities are not another's. (The backward has no such rows zeroed:
+// it took a tenth of its time, and the gradient of the weights is the batch's whatever its samples keep to themselves.)
+template <int KB>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int first, int thread, int n) {
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll 8
+    for (int at = first * 128 + thread * 16; at < 128 * 128; at += n * 16) *reinterpret_cast<uint4*>(tile + kb * 16384 + at) = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+}
+
 // Which way a tile takes is decided once for all of it: branches for every 32 keys kept the compiler from mixing their instructions (bias 247 -> 279 us).
 enum { ATT_RAW = 0, ATT_LOW = 1, ATT_FORMED = 2 };   // from products; the same within half of the cap; scores formed in place
 // EDGE: an edge of the mask crosses the tile. Left for the exponentials: `seen`, `any` (whether one of the warp's rows sees a key of 32), the bias.

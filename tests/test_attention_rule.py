@@ -455,6 +455,30 @@ def test_strided_rows_and_rows_behind_the_last_sample(ops):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pairs", "one"])
+@pytest.mark.parametrize("case", [([200, 77, 300], 4, 2, 64, None, 90, None, False), ([129, 1, 130], 3, 1, 128, 30.0, None, [60, 1, 130], True),
+                                  ([100, 140, 383], 4, 1, 128, 25.0, 150, None, False), ([300, 300, 300], 6, 2, 64, None, None, [0, 9, 299], True)])
+def test_infinities_of_one_sample_stay_there(ops, case, form, monkeypatch):
+    """Tiles at a sample's end hold rows of the next one: the other samples' outputs are those of finite neighbours."""
+    monkeypatch.setattr(A, "rule_in_pairs", lambda *a: form == "pairs")
+    ops._attn_plan_cache.clear()
+    lens, hq, hkv, d = case[:4]
+    qkv, _ = make(lens, hq, hkv, d, device="cuda")
+    cu = starts(lens)
+    want, bound = exact(qkv, cu, hq, hkv, d, rule_of(case))
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for s in range(3):
+            q = qkv.clone()
+            q[cu[s]: cu[s + 1]] = bad
+            o, l = ops.attention(q, None, cu, max(lens), hq, hkv, d, rule=rule_of(case, "cuda"))
+            ops.check_status()
+            for k in {0, 1, 2} - {s}:
+                rows = slice(cu[k], cu[k + 1])
+                for x, w, b in ((o, want[0], bound[0]), (l.t(), want[1].t(), bound[1].t())):
+                    within(x[rows], w[rows], b[rows])
+
+
+@pytest.mark.gpu
 def test_rules_on_side_streams_and_in_captured_graphs(ops):
     """Two graphs captured from one backend, replayed in turn with eager calls between them, on other inputs than they were captured with."""
     cases = [CASES[8], CASES[12]]
