@@ -395,15 +395,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
           for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
             for (int x = 0; x < 32; x += 2) big[cc] = fmax3(big[cc], fabsf(__uint_as_float(sv[cc][x])), fabsf(__uint_as_float(sv[cc][x + 1])));
-          if (__all_sync(0xffffffffu, fmaxf(big[0], big[1]) <= p.r.cap.most)) {
+          auto form = [&](auto low) {
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
               for (int x = 0; x < 32; x += 2) {
-                const float2 s = make_float2(__uint_as_float(sv[cc][x]), __uint_as_float(sv[cc][x + 1])), v = cap_pair(p.r.cap, s);
+                const float2 s = make_float2(__uint_as_float(sv[cc][x]), __uint_as_float(sv[cc][x + 1]));
+                const float2 v = decltype(low)::value ? fmul2(s, cap_half_part(p.r.cap, s)) : cap_pair(p.r.cap, s);
                 sv[cc][x] = __float_as_uint(v.x); sv[cc][x + 1] = __float_as_uint(v.y);
               }
-          } else {
+          };
+          if (__all_sync(0xffffffffu, fmaxf(big[0], big[1]) <= p.r.cap.low)) form(AbTrue{});
+          else if (__all_sync(0xffffffffu, fmaxf(big[0], big[1]) <= p.r.cap.most)) form(AbFalse{});
+          else {
             cap_in_place(p.r.cap, ts, 4);
             tmem_ld_32x32(ts, sv[0]);
             tmem_ld_32x32(ts + 32, sv[1]);

@@ -57,12 +57,13 @@ __device__ __forceinline__ float2 cap_part(const CapArgs& r, float2 s) {
   return ffma2(u, p, r.a[0]);
 }
 // Up to half of the cap.
-__device__ __forceinline__ float2 cap_half(const CapArgs& r, float2 s, float2 plus) {
+__device__ __forceinline__ float2 cap_half_part(const CapArgs& r, float2 s) {
   const float2 u = fmul2(s, s);
   float2 p = ffma2(u, r.b[3], r.b[2]);
   p = ffma2(u, p, r.b[1]);
-  return ffma2(s, ffma2(u, p, r.b[0]), plus);
+  return ffma2(u, p, r.b[0]);
 }
+__device__ __forceinline__ float2 cap_half(const CapArgs& r, float2 s, float2 plus) { return ffma2(s, cap_half_part(r, s), plus); }
 __device__ __forceinline__ float2 cap_pair(const CapArgs& r, float2 s) { return fmul2(s, cap_part(r, s)); }
 __device__ __forceinline__ float2 cap_pair(const CapArgs& r, float2 s, float2 plus) { return ffma2(s, cap_part(r, s), plus); }
 // The same of numbers that are parts of the cap already, tanh(x).

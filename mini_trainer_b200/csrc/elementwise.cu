@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(256) reduce_few_rows_kernel(const float* __res
   if (c < D) out_a[c] = __float2bfloat16(s); else out_b[c - D] = __float2bfloat16(s);
 }
 
-// The same for the many partial rows of residual_norm_bwd_kernel: 8 columns per block, 64 threads share the rows of each (740 rows of 3072 columns).
+// The same for the many partial rows of residual_norm_bwd_kernel: 8 columns per block, 64 threads share the rows of each.
 __global__ void __launch_bounds__(512) reduce_many_rows_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ out_a, __nv_bfloat16* __restrict__ out_b,
                                                               int R, int C, int D) {
   pdl_trigger();
