@@ -4,6 +4,7 @@
     python bench_kernels.py --op attn_fwd --lens 16384,16384
     python bench_kernels.py --op all
     python bench_kernels.py --op families      # LayerNorm, per-head q/k norm, GeGLU / GELU
+    python bench_kernels.py --op shaped --lens 2726,2184,3282 --tokens 16384   # attention under a rule, norms around a branch, capped head
     (ops: gemm, attn_fwd, attn_bwd, rmsnorm, swiglu, rope, ce, linear_ce, embedding, adamw)
 
 Each op is timed with CUDA events on the launching stream after warm-up, with a synchronize on
@@ -23,6 +24,7 @@ import sys
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from mini_trainer_b200.ops.attention_rule import AttentionRule  # noqa: E402
 from mini_trainer_b200.ops.native import NativeOps  # noqa: E402
 
 
@@ -265,8 +267,36 @@ def main():
         x = bf(T, F)
         report(f"gelu_fwd_{T}x{F}", timeit(lambda: ops.gelu(x), a.iters, a.warmup, flush), bytes_=2.0 * T * F * 2)
         report(f"gelu_bwd_{T}x{F}", timeit(lambda: ops.gelu_bwd(da, x), a.iters, a.warmup, flush), bytes_=3.0 * T * F * 2)
-    for name, fn in (("layernorm", op_layernorm), ("head_rmsnorm", op_head_rmsnorm), ("geglu", op_geglu)):
-        if a.op in (name, "families"):   # kernels of the model families beyond the Llama block; not part of --op all
+    def op_shaped():
+        lens = [int(v) for v in a.lens.split(",")]
+        T, cu = sum(lens), [0]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        qkv, dout = bf(T, (a.hq + 2 * a.hkv) * a.d), bf(T, a.hq * a.d)
+        slopes = torch.tensor([2.0 ** (-8.0 * (h + 1) / a.hq) for h in range(a.hq)], device="cuda")
+        for name, rule in (("causal", None), ("plain", AttentionRule()), ("cap", AttentionRule(cap=50.0)), ("bias", AttentionRule(slopes=slopes)),
+                           ("cap_bias", AttentionRule(cap=50.0, slopes=slopes)), ("window", AttentionRule(window=1024))):
+            seen = [n * (n + 1) / 2 - (max(0, n - 1024) * (n - 1023) / 2 if name == "window" else 0) for n in lens]
+            fl = 4.0 * sum(seen) * a.hq * a.d
+            o, lse = ops.attention(qkv, None, cu, max(lens), a.hq, a.hkv, a.d, rule=rule)
+            report(f"attention_{name}_fwd_T{T}", timeit(lambda: ops.attention(qkv, None, cu, max(lens), a.hq, a.hkv, a.d, rule=rule), a.iters, a.warmup, flush), flops=fl)
+            report(f"attention_{name}_bwd_T{T}", timeit(lambda: ops.attention_bwd(dout, qkv, o, lse, None, cu, max(lens), a.hq, a.hkv, a.d, rule=rule), a.iters, a.warmup,
+                                                        flush), flops=2.5 * fl)
+        T, H = a.tokens, a.hidden
+        x, y, dh, dz, w, g = bf(T, H), bf(T, H), bf(T, H), bf(T, H), bf(H), torch.rand(T, device="cuda")
+        h, _, stats = ops.residual_norm(x, y, w, w, 1e-6, gate=g)
+        dw, dv = torch.empty_like(w), torch.empty_like(w)
+        report(f"residual_norm_fwd_{T}x{H}", timeit(lambda: ops.residual_norm(x, y, w, w, 1e-6, gate=g), a.iters, a.warmup, flush), bytes_=4.0 * T * H * 2)
+        report(f"residual_norm_bwd_{T}x{H}", timeit(lambda: ops.residual_norm_bwd(dh, dz, y, h, stats, w, w, dw, dv, gate=g), a.iters, a.warmup, flush),
+               bytes_=6.0 * T * H * 2)
+        T, V = 4096, a.vocab
+        x, w = bf(T, H), bf(V, H, scale=0.02)
+        tg, dw = torch.randint(0, V, (T,), device="cuda"), torch.empty(V, H, dtype=torch.bfloat16, device="cuda")
+        for cap in (None, 30.0):
+            report(f"linear_ce_{T}x{H}x{V}" + ("_capped" if cap else ""), timeit(lambda: ops.linear_ce(x, w, tg, 1.0, dw, softcap=cap), a.iters, a.warmup, flush),
+                   flops=6.0 * T * H * V)
+    for name, fn in (("shaped", op_shaped), ("layernorm", op_layernorm), ("head_rmsnorm", op_head_rmsnorm), ("geglu", op_geglu)):
+        if a.op == name or a.op == "families" and name != "shaped":   # kernels of the model families beyond the Llama block; not part of --op all
             torch.cuda.empty_cache()
             fn()
     for name, fn in (("rmsnorm", op_rmsnorm), ("swiglu", op_swiglu), ("rope", op_rope), ("ce", op_ce), ("linear_ce", op_linear_ce),

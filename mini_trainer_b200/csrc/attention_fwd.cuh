@@ -15,7 +15,7 @@
 // threads (two threads per row with their maxima exchanged through shared memory measured 1.92 ms below). P is handed over in
 // two halves of 64 keys, so the first half's products run under the second half's exponentials.
 // 1 x 16384 tokens, 32/8 heads, D = 128: 1.65 ms; 41 samples, 12 345 tokens, 16/4 heads, D = 64: 53 us (one tile per CTA, two
-// threads per row: 1.94 ms and 94 us). Launches with few pairs are faster in that other form (attention_fwd_one.cu);
+// threads per row: 1.94 ms and 94 us). Launches with few pairs are faster in that other form (attention_fwd_one.cuh);
 // a long sequence at D = 64 is level (1 x 16384, 32/8 heads: 1.54 ms there, 1.50 here).
 //
 // CTAs are persistent (one per SM): barriers and tensor memory are set up once, K and V of the next item are prefetched

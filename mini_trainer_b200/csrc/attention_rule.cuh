@@ -6,6 +6,12 @@
 // The kernels are instances of the same templates as the plain causal ones; NoRule compiles to what those were. Masks need no parameter of the
 // template: which tiles exist, and which of them are crossed by an edge of the mask, is found per tile.
 // The cap is in cap.cuh.
+//
+// Bound as the plain causal kernels are, by the chain of hand-offs between the softmax warps and the tensor core, and then by what the softmax warps have to do to a
+// score: a cap adds five to seven packed instructions a pair, and the reference's comparisons of absolute values, a bias three. 8192 tokens in three samples, 32/8 heads of 128
+// (188 GFLOP forward, 471 backward): forward 192 us as under a rule without either (the plain causal kernel: 192), 233 capped, 212 biased, 296 both; backward 583, 611, 574, 609.
+// The tensor core is busy for 57, 45, 50 and 34 % of the forward's cycles, issue slots for 44, 42, 48 and 42 %: no pipe is full, a row's instructions depend on each other.
+// Windows and prefixes cost what their tiles do: one sample of 8192 tokens with a window of 1024 takes 0.70 ms both ways, without one 1.8.
 #pragma once
 #include <stdint.h>
 
@@ -39,7 +45,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 
 struct AttTiles {
   int prefix_tiles, skip;
   // The j-th of n. With a bias from the diagonal back: near keys have the larger scores, so the reference maximum is found at once and the accumulator hardly ever
-  // rescaled (the other way round it was in nearly every tile: 280 us where it takes 215, 8192 tokens in three samples, 32/8 heads of 128).
+  // rescaled (the other way round it was in nearly every tile: 280 us where it takes 212, 8192 tokens in three samples, 32/8 heads of 128).
   template <class R>
   __device__ __forceinline__ int tile(int j, int n) const {
     if (R::BIAS) j = n - 1 - j;
@@ -66,14 +72,14 @@ __device__ __forceinline__ uint32_t att_queries_seen(const AttRuleArgs& r, int j
 // the largest capped score; a bias is not, but within 32 keys it changes by 31 slopes: the largest product of each 32, capped, with the bias of the nearer
 // end is a bound that is too high by at most that. Where capped scores are small, up to 2^+-30 as exponentials, their largest absolute value, which has to be known for the cap's
 // polynomial anyhow, is bound enough: 2^60 too high at most, which fp32 has room for. So the scores themselves are only formed on their way into the exponentials, which
-// keeps the FMA pipe and the special-function unit busy at once; formed in place first, capped scores took 286 us where they take 250 (8192 tokens in three samples,
-// 32/8 heads of 128; 194 without a cap). They are formed in place, and their largest taken, where this does not hold (`formed`):
+// keeps the FMA pipe and the special-function unit busy at once; formed in place first, capped scores took 286 us where they take 233 (8192 tokens in three samples,
+// 32/8 heads of 128; 192 without a cap). They are formed in place, and their largest taken, where this does not hold (`formed`):
 // products beyond the cap, slopes so steep that the bound could be 2^40 too high for them alone, and biased keys on the diagonal.
 constexpr float ATT_STEEP = 40.f / 31.f;
 // Rows [first, 128) of a [128, 64 KB] tile in shared memory (128B swizzle: a row's bytes stay together) set to zero by `n` threads, for reads by the tensor core behind
 // the caller's next arrival. A tile at a sample's end holds rows of the next sample, which meet probabilities and gradients of zero; a product
-// with zero is only zero for finite numbers, and one sample's infinities are not another's. (The backward has no such rows zeroed:
-// it took a tenth of its time, and the gradient of the weights is the batch's whatever its samples keep to themselves.)
+// with zero is only zero for finite numbers, and one sample's infinities are not another's. (The forward takes the same time with it. The backward has no such rows zeroed: it took 7 to 15 % of its
+// time, and the gradient of the weights is the batch's whatever its samples keep to themselves.)
 template <int KB>
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int first, int thread, int n) {
 #pragma unroll
@@ -83,7 +89,7 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int first, int thread, 
   fence_proxy_async_smem();
 }
 
-// Which way a tile takes is decided once for all of it: branches for every 32 keys kept the compiler from mixing their instructions (bias 247 -> 279 us).
+// Which way a tile takes is decided once for all of it: branches for every 32 keys kept the compiler from mixing their instructions (a biased forward took 279 us with them and 247 without).
 enum { ATT_RAW = 0, ATT_LOW = 1, ATT_FORMED = 2 };   // from products; the same within half of the cap; scores formed in place
 // EDGE: an edge of the mask crosses the tile. Left for the exponentials: `seen`, `any` (whether one of the warp's rows sees a key of 32), the bias.
 template <class R, bool EDGE, int C>

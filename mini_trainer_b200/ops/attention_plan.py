@@ -50,7 +50,7 @@ def _with_at_least(blocks: list) -> list:
 
 
 def forward_in_pairs(blocks: list, hq: int, hkv: int, d: int, sms: int) -> bool:
-    """Forward: pairs of query tiles (``attention_fwd.cu``) or one tile per CTA (``attention_fwd_one.cu``). A unit with ``n`` key
+    """Forward: pairs of query tiles (``attention_fwd.cuh``) or one tile per CTA (``attention_fwd_one.cuh``). A unit with ``n`` key
     tiles exists once per sequence of at least ``n`` blocks."""
     if not blocks:
         return True
@@ -101,7 +101,7 @@ def _backward_splits(blocks: list, hq: int, hkv: int, sms: int, most: int) -> in
     return splits
 
 
-# Iterations of a CTA, on average, from which the backward is launched behind its predecessor's end and not under its tail (csrc/attention_bwd.cu). 85 batches at head_dim 128
+# Iterations of a CTA, on average, from which the backward is launched behind its predecessor's end and not under its tail (csrc/attention_bwd.cuh). 85 batches at head_dim 128
 # (16/4, 32/8, 12/2, 16/16 and 8/1 heads, one to 148 sequences), early over in order, with the forward and with a product in front of it: from 20 on 0.99 to 1.15, 1.03 on
 # average (8 of 2048 tokens, 16/4: 675 and 586 us; one of 4096, 32/8: 601 and 569), below 12 0.95 to 1.04, 0.99 (37 of 128, 12/2: 53 and 54), between them
 # 0.97 to 1.05. At head_dim 64 early is the faster or level throughout (0.95 to 1.00 in 13 batches).
