@@ -1330,12 +1330,16 @@ __global__ void __launch_bounds__(1024, 1) ce_row_kernel(const __nv_bfloat16* lo
 // Cross-entropy of logits capped by a tanh, l = cap t: loss and dz = (softmax(l) - onehot) (1 - t^2) scale, rounded to bf16, over t [R, V] in fp16, in place. The
 // product that left t has left the softmax's statistics of every 128 columns too, formed before its rounding (gemm_act.cuh, ACT_CAP), and the target's logit is
 // formed again from its rows of x and w: the loss, a difference of numbers many times a rounding apart, sees none. The gradient is that of t as it is
-// rounded (2^-11 of itself, where bf16 logits are off by 2^-8). One block per row; bound by reading and writing it: 3720 x 151936 in 379 us, 6.0 TB/s
-// (0.91 of the copy rate).
+// rounded (2^-11 of itself, where bf16 logits are off by 2^-8). Bound by reading and writing the rows: 3000 x 151936
+// in 304 us, 6.0 TB/s (0.92 of the copy rate). Once the statistics are there the parts of a row need nothing of each other, so a row is divided over blocks where rows alone are not
+// eight blocks to an SM, down to parts of 4096 columns; each part adds up the row's statistics (a hundredth of its bytes at 16 parts), the first has the loss. Blocks are small and
+// five to an SM, so that one's reductions run under another's rows. Rows whole in blocks of 512 and 1024 threads, then like this: 1 x 151936 11.6 -> 4.0 us, 129 x 32000 5.4 -> 4.8,
+// 600 x 32000 22 -> 11.7, 200 x 151936 23.5 -> 16.9, 1500 x 65536 76 -> 74. Over 52 sizes of 1 to 6000 rows by 8192 to 151936 columns it is 5 % off the best of 36 divisions and sizes of block.
+constexpr int CEC_THREADS = 256;
 __device__ __forceinline__ float2 unpack_half(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-__global__ void __launch_bounds__(1024) ce_capped_kernel(__nv_bfloat16* t, const float2* __restrict__ stats, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
-                                                        const long long* __restrict__ targets, float* __restrict__ loss, int V, int H, float alpha, float cap2, float grad_scale,
+__global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16* t, const float2* __restrict__ stats, const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
+                                                        const long long* __restrict__ targets, float* __restrict__ loss, int V, int H, float alpha, float cap2, float grad_scale, int cols,
                                                         long long ignore_index) {
   pdl_trigger();
   pdl_wait();
@@ -1343,10 +1347,11 @@ __global__ void __launch_bounds__(1024) ce_capped_kernel(__nv_bfloat16* t, const
   const long long row = blockIdx.x;
   __nv_bfloat16* tr = t + row * V;
   const long long tgt = targets[row];
-  const int c0 = threadIdx.x * 8, step = blockDim.x * 8;
+  // this block's columns of the row: a multiple of 8 of them
+  const int lo = blockIdx.y * cols, hi = V - lo < cols ? V : lo + cols, c0 = lo + threadIdx.x * 8, step = blockDim.x * 8;
   if (tgt == ignore_index) {
-    for (int c = c0; c < V; c += step) *reinterpret_cast<uint4*>(tr + c) = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x == 0) loss[row] = 0.f;
+    for (int c = c0; c < hi; c += step) *reinterpret_cast<uint4*>(tr + c) = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0 && lo == 0) loss[row] = 0.f;
     return;
   }
   const bool there = tgt >= 0 && tgt < V;
@@ -1357,7 +1362,7 @@ __global__ void __launch_bounds__(1024) ce_capped_kernel(__nv_bfloat16* t, const
     if (q.x > m) { s *= ex2_mufu((m - q.x) * cap2); m = q.x; }
     s += q.y * ex2_mufu((q.x - m) * cap2);
   }
-  for (int c = c0; there && c < H; c += step) {
+  for (int c = threadIdx.x * 8; lo == 0 && there && c < H; c += step) {
     const uint4 a = *reinterpret_cast<const uint4*>(x + row * H + c), b = *reinterpret_cast<const uint4*>(w + tgt * H + c);
     const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -1368,8 +1373,8 @@ __global__ void __launch_bounds__(1024) ce_capped_kernel(__nv_bfloat16* t, const
   }
   const float gm = block_max(m, red);
   const float gs = block_sum(s * ex2_mufu((m - gm) * cap2), red);   // (zero for a thread without columns)
-  dot = block_sum(dot, red) * alpha;
-  if (threadIdx.x == 0) {
+  if (lo == 0) dot = block_sum(dot, red) * alpha;
+  if (threadIdx.x == 0 && lo == 0) {
     const float tt = !there ? NAN : fabsf(dot) <= 1.f ? tanh_pair(splat(dot)).x : tanh_exact(dot);   // NaN of a target that is no column
     loss[row] = 0.6931471805599453f * ((gm - tt) * cap2 + log2f(gs));
   }
@@ -1394,14 +1399,14 @@ __global__ void __launch_bounds__(1024) ce_capped_kernel(__nv_bfloat16* t, const
     *reinterpret_cast<uint4*>(tr + c) = make_uint4(pack_bf16(p[0].x, p[0].y), pack_bf16(p[1].x, p[1].y), pack_bf16(p[2].x, p[2].y), pack_bf16(p[3].x, p[3].y));
   };
   // four vectors are on their way before the first is overwritten
-  for (int c = c0; c < V; c += 4 * step) {
+  for (int c = c0; c < hi; c += 4 * step) {
     uint4 u[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (c + k * step < V) u[k] = *reinterpret_cast<const uint4*>(tr + c + k * step);
+      if (c + k * step < hi) u[k] = *reinterpret_cast<const uint4*>(tr + c + k * step);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (c + k * step < V) gradient(u[k], c + k * step);
+      if (c + k * step < hi) gradient(u[k], c + k * step);
   }
 }
 
@@ -2057,10 +2062,13 @@ int mtb200_ce_capped(void* t, const float2* stats, const void* x, const void* w,
   if (R <= 0) return 0;
   if (V <= 0 || V % 8 || H <= 0 || H % 8) return -10;
   if (!aligned16(t, x, w)) return -11;
-  const int threads = cdiv(V, 8 * 4 * 32) * 32;   // four vectors each, up to the most threads
-  const int most = R >= 6 * num_sms() ? 512 : 1024;   // rows enough: several at a time on an SM hide each other's reductions
-  launch_pdl(ce_capped_kernel, R, threads < most ? threads : most, 0, st, (bf16*)t, stats, (const bf16*)x, (const bf16*)w, targets, loss, V, H, alpha, cap2, grad_scale,
-             ignore_index);
+  int parts = cdiv(8 * num_sms(), R);   // (ce_capped_kernel)
+  parts = parts < V / 4096 ? parts : V / 4096;
+  parts = parts < 1 ? 1 : parts > 16 ? 16 : parts;
+  const int cols = cdiv(V / 8, parts) * 8;
+  const int threads = cdiv(cols, 8 * 4 * 32) * 32;   // four vectors each, up to the most threads
+  launch_pdl(ce_capped_kernel, dim3(R, cdiv(V, cols)), threads < CEC_THREADS ? threads : CEC_THREADS, 0, st, (bf16*)t, stats, (const bf16*)x, (const bf16*)w, targets, loss, V, H, alpha,
+             cap2, grad_scale, cols, ignore_index);
   return launch_ok();
 }
 

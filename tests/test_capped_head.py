@@ -154,6 +154,22 @@ def test_chunks_accumulation_and_ignored_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V", [(1, 4096), (2, 8192), (3, 8200), (7, 20008), (7, 65544), (300, 16392)])
+def test_rows_divided_over_blocks(ops, T, V):
+    """Targets in every part of a row, at the first and last column; ignored rows are zero in all of their parts, and a target that is no column is one row's."""
+    x, w, t = inputs(T, 64, V, seed=V, device="cuda")
+    t.copy_(torch.linspace(V - 1, 0, T).round().long() if T > 1 else torch.tensor([V - 1]))
+    check(ops, x, w, t, 30.0, 1.0, 1.0 / T)
+    t[T // 2] = IGNORE
+    loss, dx, dw = check(ops, x, w, t, 30.0, 1.0, 1.0 / T)
+    assert loss[T // 2] == 0 and not dx[T // 2].any()
+    t[T // 2] = V
+    again = run(ops, x, w, t, 30.0, 1.0, 1.0 / T)[0]
+    assert torch.isnan(again[T // 2]) and torch.equal(torch.isnan(again).nonzero().flatten(), torch.tensor([T // 2], device="cuda"))
+    ops.check_status()
+
+
+@pytest.mark.gpu
 def test_captured_on_two_streams_and_twice(ops):
     x, w, t = inputs(200, 256, 2048, device="cuda")
     a = run(ops, x, w, t, 30.0, 1.0, 0.01)
