@@ -371,7 +371,8 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __nv_bfloat16* __re
 // in one pass: x and y are read once, h and z written once (8 bytes an element; as norm, sum and norm 14, and the first two round n in between). All of it is fp32
 // but for h, which is rounded before its norm: the norm is that of the residual stream that backward and every later block read.
 // Rows are laid out over threads as in norm_fwd_kernel, x and y side by side in a stage; BULK as there.
-// Bound by reading and writing the rows: 16384 x 4096 in 92 us, 5.8 TB/s (0.89 of the copy rate). Half as many vectors a thread as a norm alone has, as a thread holds two rows,
+// Bound by reading and writing the rows: 16384 x 4096 in 92 us, 5.8 TB/s (0.89 of the copy rate; 97 in a row of them
+// when the next launch was let in at the start). Half as many vectors a thread as a norm alone has, as a thread holds two rows,
 // and packed arithmetic: 103 -> 91 us.
 template <int VPT, bool POST, bool PRE, bool BULK>
 __global__ void __launch_bounds__(EW_THREADS, BULK ? (VPT <= 2 ? 3 : 2) : 1) residual_norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ y,
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(EW_THREADS, BULK ? (VPT <= 2 ? 3 : 2) : 1) res
                                                                       const float* __restrict__ gate, __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ z,
                                                                       float* __restrict__ rstd_y, float* __restrict__ rstd_h, float scale, float eps, int T, int H,
                                                                       int lanes, int* status) {
-  pdl_trigger();
+  if (!BULK) pdl_trigger();
   pdl_wait();
   extern __shared__ __align__(128) uint8_t norm_smem[];
   __shared__ uint64_t full[NORM_STAGES];
@@ -485,6 +486,7 @@ __global__ void __launch_bounds__(EW_THREADS, BULK ? (VPT <= 2 ? 3 : 2) : 1) res
       }
     }
   }
+  if (BULK) pdl_trigger();
 }
 
 // Its gradient, from that of h (dh, may be null: zero) and z (dz):
@@ -493,23 +495,22 @@ __global__ void __launch_bounds__(EW_THREADS, BULK ? (VPT <= 2 ? 3 : 2) : 1) res
 //   partial rows of dw_post += b dx yhat and dw_pre += dz hhat, per block, behind each other
 // dx stays in fp32 between its two uses. The second reduction is the gate's gradient and the norm's correction at once. Rows arrive by bulk copies as in
 // norm_bwd_kernel, up to four of them (dh, dz, h, y) to a stage; two barriers a row. Bound by reading them and writing dx and dy, 12 bytes an element:
-// 16384 x 4096 in 131 us, 6.1 TB/s (0.94 of the copy rate), and 6 more for the partial rows; of 5987 x 1536 (22 + 6 us, 17 at that rate) each block has eight rows, whose two
-// reductions one after the other take longer than their bytes. Tried there: the groups of an SM as one block with one partial row (33 -> 31 us, but 16384 x 4096 130 -> 187:
-// registers), a copy's request by each warp in turn (33 -> 35).
-constexpr int RN_VPT = 2;
-template <bool POST, bool PRE>
-__global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloat16* __restrict__ dh, const __nv_bfloat16* __restrict__ dz,
+// 16384 x 4096 in 131 us with the sum of the partial rows, 40000 x 1536 in 119, 6.2 TB/s both (0.95 of the copy rate); 5987 x 1536 in 27 (17 at that rate), as each block has eight rows and
+// the start, the end and the partial rows are a third of it. The next launch is let in when a block's rows are done: let in at the start, the blocks of the sum held their places
+// on SMs from blocks of this kernel (5987 x 1536 34 -> 27 us, 40000 x 1536 161 -> 119, both with the sum's loads under way at once). Tried: the rows of an SM in one block with one partial row (33 -> 31 us
+// then, but 16384 x 4096 130 -> 187: registers), a copy's request by each warp in turn (33 -> 35).
+constexpr int rn_threads(int vpt) { return vpt == 1 ? 768 : 512; }   // an SM's, and a block's at most
+template <int VPT, bool POST, bool PRE>
+__global__ void __launch_bounds__(rn_threads(VPT)) residual_norm_bwd_kernel(const __nv_bfloat16* __restrict__ dh, const __nv_bfloat16* __restrict__ dz,
                                                                const __nv_bfloat16* __restrict__ y, const __nv_bfloat16* __restrict__ h,
                                                                const float* __restrict__ rstd_y, const float* __restrict__ rstd_h,
                                                                const __nv_bfloat16* __restrict__ w_post, const __nv_bfloat16* __restrict__ w_pre,
                                                                const float* __restrict__ gate, __nv_bfloat16* __restrict__ dx, __nv_bfloat16* __restrict__ dy,
                                                                float* __restrict__ dgate, float* __restrict__ part, float scale, int T, int H, int stages, int* status) {
-  pdl_trigger();
   pdl_wait();
-  constexpr int VPT = RN_VPT;
   extern __shared__ __align__(128) uint8_t norm_smem[];
   __shared__ uint64_t full[8];
-  __shared__ __align__(16) float red[2][2][16];
+  __shared__ __align__(16) float red[2][2][rn_threads(VPT) / 32];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int nt = blockDim.x, wid = threadIdx.x >> 5;
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloa
     if (want_c) bulk_load(d + at_y, y + row * H, row_bytes, &full[s]);
     if (have_dh) bulk_load(d + at_dh, dh + row * H, row_bytes, &full[s]);
   };
-  for (int i = threadIdx.x; i < 64; i += nt) red[i >> 5][(i >> 4) & 1][i & 15] = 0.f;   // warps that do not exist add zeros
+  for (int i = threadIdx.x; i < 4 * (rn_threads(VPT) / 32); i += nt) (&red[0][0][0])[i] = 0.f;   // warps that do not exist add zeros
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
     abort_word = 0;
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloa
   uint32_t ph = 0;
   auto load = [&](const uint8_t* p, int c) { return c < H ? *reinterpret_cast<const uint4*>(p + c * 2) : make_uint4(0u, 0u, 0u, 0u); };
   auto two = [&](const uint4& u, int i) { return unpack_bf16(i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w); };
-  auto total = [&](float d, float (&rd)[16]) {   // over the block
+  auto total = [&](float d, float (&rd)[rn_threads(VPT) / 32]) {   // over the block
     d = warp_sum(d);
     if (nt == 32) return d;
     if ((threadIdx.x & 31) == 0) rd[wid] = d;
@@ -642,6 +643,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const __nv_bfloa
     ry = nry; rh = nrh; by = nby;
     if (++s == stages) { s = 0; ph ^= 1; }
   }
+  pdl_trigger();
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int c = c0 + v * nt * 8;
@@ -695,7 +697,9 @@ __global__ void __launch_bounds__(256) reduce_few_rows_kernel(const float* __res
   if (c < D) out_a[c] = __float2bfloat16(s); else out_b[c - D] = __float2bfloat16(s);
 }
 
-// The same for the many partial rows of residual_norm_bwd_kernel: 8 columns per block, 64 threads share the rows of each.
+// The same for the many partial rows of residual_norm_bwd_kernel: 8 columns per block, 64 threads share the rows of each and have AHEAD loads under way, without a remainder that
+// would wait for each of its own.
+template <int AHEAD>
 __global__ void __launch_bounds__(512) reduce_many_rows_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ out_a, __nv_bfloat16* __restrict__ out_b,
                                                               int R, int C, int D) {
   pdl_trigger();
@@ -703,8 +707,13 @@ __global__ void __launch_bounds__(512) reduce_many_rows_kernel(const float* __re
   __shared__ float sm[16][8];
   const int c = blockIdx.x * 8 + (threadIdx.x & 7);   // C is a multiple of 8
   float s = 0.f;
-#pragma unroll 4
-  for (int r = threadIdx.x >> 3; r < R; r += 64) s += part[static_cast<long long>(r) * C + c];
+  for (int r = threadIdx.x >> 3; r < R; r += 64 * AHEAD) {
+    float v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) v[k] = r + 64 * k < R ? part[static_cast<long long>(r + 64 * k) * C + c] : 0.f;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) s += v[k];
+  }
   s += __shfl_xor_sync(0xffffffffu, s, 8);
   s += __shfl_xor_sync(0xffffffffu, s, 16);
   if ((threadIdx.x & 31) < 8) sm[threadIdx.x >> 5][threadIdx.x & 7] = s;
@@ -1762,19 +1771,26 @@ static int launch_residual_norm_fwd(const void* x, const void* y, const void* w_
   return launch_ok();
 }
 
-// Blocks of the backward of norms around a branch, as many as are resident, and the rows of its partials. A thread has two vectors of a row.
-static int residual_norm_threads(int H) { return cdiv(H, 8 * RN_VPT * 32) * 32; }
+// The backward of norms around a branch: rows that an SM works on at once with VPT vectors a thread (0: a row does not fit a block), the vectors chosen, and from them a
+// block's threads and how many blocks there are, all of them resident, one row of partials each. One vector has shorter chains and less waiting in them, two leave more rows their
+// registers: one where it has as many rows under way. 14062 x 640 32.6 us with two and 28.4 with one, 62500 x 640 114 and 96, 8680 x 4608 128 and 113, 14204 x 2816 101 and 93; 5859 x 1536
+// 26.1 and 26.8, 11160 x 3584 89 and 121. Sixteen rows at most: with eight 16384 x 256 took 28 us (25), 20000 x 512 40 (31).
+static int residual_norm_threads(int vpt, int H) { return cdiv(H, 8 * vpt * 32) * 32; }
+static int residual_norm_rows(int vpt, int H) {
+  const int n = rn_threads(vpt) / residual_norm_threads(vpt, H);
+  return n > 16 ? 16 : n;
+}
+static int residual_norm_vpt(int H) { return residual_norm_rows(1, H) >= residual_norm_rows(2, H) ? 1 : 2; }
 extern "C" int mtb200_residual_norm_bwd_blocks(int T, int H) {
-  const int per_sm = 512 / residual_norm_threads(H);
-  const int b = num_sms() * (per_sm < 1 ? 1 : (per_sm > 8 ? 8 : per_sm));
+  const int b = num_sms() * residual_norm_rows(residual_norm_vpt(H), H);
   return T < b ? (T > 0 ? T : 1) : b;
 }
 
-template <bool POST, bool PRE>
+template <int VPT, bool POST, bool PRE>
 static int launch_residual_norm_bwd(const void* dh, const void* dz, const void* y, const void* h, const float* rstd_y, const float* rstd_h, const void* w_post,
                                     const void* w_pre, const float* gate, void* dx, void* dy, float* dgate, float* part, float scale, int T, int H, int* status,
                                     cudaStream_t st) {
-  auto kern = residual_norm_bwd_kernel<POST, PRE>;
+  auto kern = residual_norm_bwd_kernel<VPT, POST, PRE>;
   constexpr int most = 200 * 1024;
   static bool configured = false;
   if (!configured) {
@@ -1786,7 +1802,7 @@ static int launch_residual_norm_bwd(const void* dh, const void* dz, const void* 
   const int stage = H * 2 * ((PRE ? 2 : 0) + (POST || dgate != nullptr ? 1 : 0) + (dh != nullptr ? 1 : 0));
   int stages = most / (per_sm * stage);
   stages = stages > 4 ? 4 : (stages < 2 ? 2 : stages);
-  launch_pdl(kern, blocks, residual_norm_threads(H), stages * stage, st, (const bf16*)dh, (const bf16*)dz, (const bf16*)y, (const bf16*)h, rstd_y, rstd_h,
+  launch_pdl(kern, blocks, residual_norm_threads(VPT, H), stages * stage, st, (const bf16*)dh, (const bf16*)dz, (const bf16*)y, (const bf16*)h, rstd_y, rstd_h,
              (const bf16*)w_post, (const bf16*)w_pre, gate, (bf16*)dx, (bf16*)dy, dgate, part, scale, T, H, stages, status);
   return launch_ok();
 }
@@ -1868,13 +1884,15 @@ int mtb200_residual_norm_bwd(const void* dh, const void* dz, const void* y, cons
   if (T <= 0) return 0;
   if (H <= 0 || H % 8 || H > 4 * 8 * EW_THREADS || (w_post == nullptr && w_pre == nullptr)) return -10;
   if (!aligned16(dh, dz, y) || !aligned16(h, dx, dy) || !aligned16(w_post, w_pre, part)) return -11;
-#define RB(A, B) launch_residual_norm_bwd<A, B>(dh, dz, y, h, rstd_y, rstd_h, w_post, w_pre, gate, dx, dy, dgate, part, scale, T, H, status, st)
+#define RV(V, A, B) launch_residual_norm_bwd<V, A, B>(dh, dz, y, h, rstd_y, rstd_h, w_post, w_pre, gate, dx, dy, dgate, part, scale, T, H, status, st)
+#define RB(A, B) (residual_norm_vpt(H) == 1 ? RV(1, A, B) : RV(2, A, B))
   const int rc = w_post == nullptr ? RB(false, true) : w_pre == nullptr ? RB(true, false) : RB(true, true);
 #undef RB
   if (rc) return rc;
   const int blocks = mtb200_residual_norm_bwd_blocks(T, H), C = w_post != nullptr && w_pre != nullptr ? 2 * H : H;
   void* first = w_post != nullptr ? dw_post : dw_pre;
-  if (blocks > 64) launch_pdl(reduce_many_rows_kernel, C / 8, 512, 0, st, part, (bf16*)first, (bf16*)dw_pre, blocks, C, H);
+  // up to 768 rows in one go; with twelve loads for 100 or 296 rows, registers kept blocks off the SMs: 1.5 us of 8, 2.5 of 131
+  if (blocks > 64) launch_pdl(blocks > 320 ? reduce_many_rows_kernel<12> : blocks > 256 ? reduce_many_rows_kernel<5> : reduce_many_rows_kernel<4>, C / 8, 512, 0, st, part, (bf16*)first, (bf16*)dw_pre, blocks, C, H);
   else reduce_rows(part, first, dw_pre, blocks, C, H, st);
   return launch_ok();
 }

@@ -197,6 +197,15 @@ def test_more_rows_than_resident_blocks(ops, T, H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,H", [(7003, 256), (4501, 640), (2371, 768), (601, 2816), (1201, 5120), (301, 6144), (149, 6152), (2369, 8)])
+def test_both_layouts_of_a_row_over_threads(ops, T, H):
+    """One and two vectors of a row per thread, as many rows under way as an SM holds and one more, several turns of the partial rows' sum."""
+    for post, pre in FORMS:
+        forward_and_backward(ops, inputs(T, H, post, pre, H % 512 == 0, seed=T, device="cuda"), 1.5)
+    ops.check_status()
+
+
+@pytest.mark.gpu
 def test_sizes_of_the_values(ops):
     """Rows of zeros (eps alone holds the root), of tiny and of large values."""
     for size in (0.0, 2.0 ** -40, 2.0 ** 30):
