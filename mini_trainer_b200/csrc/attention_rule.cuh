@@ -9,8 +9,8 @@
 //
 // Bound as the plain causal kernels are, by the chain of hand-offs between the softmax warps and the tensor core, and then by what the softmax warps have to do to a
 // score: a cap adds five to seven packed instructions a pair, and the reference's comparisons of absolute values, a bias three. 8192 tokens in three samples, 32/8 heads of 128
-// (188 GFLOP forward, 471 backward): forward 192 us as under a rule without either (the plain causal kernel: 192), 233 capped, 212 biased, 296 both; backward 583, 611, 574, 609.
-// The tensor core is busy for 57, 45, 50 and 34 % of the forward's cycles, issue slots for 44, 42, 48 and 42 %: no pipe is full, a row's instructions depend on each other.
+// (188 GFLOP forward, 471 backward): forward 192 us under a rule without either as in the plain causal kernel, 232 capped, 210 biased, 269 both; backward 583, 611, 574, 609.
+// The tensor core is busy for 57, 45, 50 and about 37 % of the forward's cycles, issue slots for 44, 42, 48 and 42 %: no pipe is full, a row's instructions depend on each other.
 // Windows and prefixes cost what their tiles do: one sample of 8192 tokens with a window of 1024 takes 0.70 ms both ways, without one 1.8.
 #pragma once
 #include <stdint.h>
@@ -45,7 +45,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 
 struct AttTiles {
   int prefix_tiles, skip;
   // The j-th of n. With a bias from the diagonal back: near keys have the larger scores, so the reference maximum is found at once and the accumulator hardly ever
-  // rescaled (the other way round it was in nearly every tile: 280 us where it takes 212, 8192 tokens in three samples, 32/8 heads of 128).
+  // rescaled (the other way round it was in nearly every tile: 280 us where it takes 210, 8192 tokens in three samples, 32/8 heads of 128).
   template <class R>
   __device__ __forceinline__ int tile(int j, int n) const {
     if (R::BIAS) j = n - 1 - j;
@@ -72,7 +72,7 @@ __device__ __forceinline__ uint32_t att_queries_seen(const AttRuleArgs& r, int j
 // the largest capped score; a bias is not, but within 32 keys it changes by 31 slopes: the largest product of each 32, capped, with the bias of the nearer
 // end is a bound that is too high by at most that. Where capped scores are small, up to 2^+-30 as exponentials, their largest absolute value, which has to be known for the cap's
 // polynomial anyhow, is bound enough: 2^60 too high at most, which fp32 has room for. So the scores themselves are only formed on their way into the exponentials, which
-// keeps the FMA pipe and the special-function unit busy at once; formed in place first, capped scores took 286 us where they take 233 (8192 tokens in three samples,
+// keeps the FMA pipe and the special-function unit busy at once; formed in place first, capped scores took 286 us where they take 232 (8192 tokens in three samples,
 // 32/8 heads of 128; 192 without a cap). They are formed in place, and their largest taken, where this does not hold (`formed`):
 // products beyond the cap, slopes so steep that the bound could be 2^40 too high for them alone, and biased keys on the diagonal.
 constexpr float ATT_STEEP = 40.f / 31.f;
@@ -205,11 +205,18 @@ struct AttScores {
         }
       }
     }
-    if constexpr (R::BIAS) {   // of 32 keys the nearest has the larger bias unless the slope is negative
+    if constexpr (R::BIAS) {
+      if (R::CAP && low) {   // of scores within half of the cap what they are uncapped is bound enough, 2^2.8 too high at most (exactly 284 us where it takes 269)
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
+        for (int c = 0; c < C; ++c) mc[c] *= r.cap.b[0].x;
+      } else if (R::CAP) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) mc[c] = mc[c] > -INFINITY ? cap_exact(r.cap, mc[c]) : mc[c];
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {   // of 32 keys the nearest has the larger bias unless the slope is negative
         const float near = fmaxf(slope2 * (from + (c * 32)), slope2 * (from + (c * 32 + 31)));
-        if (mc[c] > -INFINITY) mc[c] = R::CAP ? cap_exact(r.cap, mc[c]) + near : fmaf(mc[c], sl2, near);
+        mc[c] = R::CAP ? mc[c] + near : fmaf(mc[c], sl2, near);
       }
     }
     float m = fmaxf(mc[0], mc[1]);
