@@ -128,12 +128,23 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
 
   pdl_wait();   // the work table comes first
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int unit = p.splits == 1 ? blockIdx.x : blockIdx.x / p.splits, sub = blockIdx.x - unit * p.splits;
+  int unit = blockIdx.x, sub = 0, splits = p.splits, shared = 0;   // `shared`: the unit's number among those that CTAs share
+  if constexpr (R::ON) {
+    if (unit < p.r.whole) splits = 1;
+    else if (splits > 1) {
+      shared = (unit - p.r.whole) / splits;
+      sub = unit - p.r.whole - shared * splits;
+      unit = p.r.whole + shared;
+    }
+  } else if (splits > 1) {
+    unit = shared = blockIdx.x / splits;
+    sub = blockIdx.x - unit * splits;
+  }
   int item = static_cast<int>(__umulhi(static_cast<unsigned>(unit), p.hkv_inv));   // unit / Hkv, or one less
   if (unit - item * p.Hkv >= p.Hkv) ++item;
   const int hk = unit - item * p.Hkv;
   const int G = p.G;
-  const int h_first = hk * G + (p.splits == 1 ? 0 : G * sub / p.splits), heads = p.splits == 1 ? G : G * (sub + 1) / p.splits - G * sub / p.splits;
+  const int h_first = hk * G + (splits == 1 ? 0 : G * sub / splits), heads = splits == 1 ? G : G * (sub + 1) / splits - G * sub / splits;
   const int seq_start = p.plan[item * R::ROW + 0], seq_len = p.plan[item * R::ROW + 1], k0 = p.plan[item * R::ROW + 2];
   // query blocks [jblk, nq) of the sequence: those at or below the diagonal; under a rule those that see a key of this block
   int prefix = 0, jblk = k0 / AB_B, nq = (seq_len + AB_B - 1) / AB_B;
@@ -554,7 +565,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
         }
       }
     };
-    float* base = p.ws + (static_cast<long long>(unit) * p.splits * 8 + (warp - 4)) * PART + lane * 4;   // split s: + s * 8 * PART
+    float* base = p.ws + (static_cast<long long>(shared) * splits * 8 + (warp - 4)) * PART + lane * 4;   // split s: + s * 8 * PART
 #pragma unroll 1
     for (int x = 0; x < PIECES; ++x) {
       uint32_t v[32];
@@ -563,19 +574,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
       float f[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-      if (p.splits == 1) store(x, f);
+      if (splits == 1) store(x, f);
       else {   // lane-interleaved 16-byte pieces: every access is one contiguous 512 bytes
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           __stcg(reinterpret_cast<float4*>(base + static_cast<long long>(sub) * 8 * PART + x * 1024 + j * 128), make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]));
       }
     }
-    if (p.splits > 1) {   // the warp that arrives last adds the partials, in split order whoever that is; nobody waits
-      unsigned long long* counter = p.counters + unit * 8 + (warp - 4);
+    if (splits > 1) {   // the warp that arrives last adds the partials, in split order whoever that is; nobody waits
+      unsigned long long* counter = p.counters + shared * 8 + (warp - 4);
       __threadfence();
       __syncwarp();
       unsigned last = 0;
-      if (lane == 0) last = last_arrival(counter, p.epoch, p.splits);
+      if (lane == 0) last = last_arrival(counter, p.epoch, splits);
       last = __shfl_sync(0xffffffffu, last, 0);
       if (last) {
         __threadfence();
@@ -585,7 +596,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
 #pragma unroll
           for (int j = 0; j < 32; ++j) f[j] = 0.f;
 #pragma unroll 2
-          for (int s = 0; s < p.splits; ++s) {
+          for (int s = 0; s < splits; ++s) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float4 t = __ldcg(reinterpret_cast<const float4*>(base + static_cast<long long>(s) * 8 * PART + x * 1024 + j * 128));
@@ -675,7 +686,9 @@ static int launch_bwd(const CUtensorMap& a, const CUtensorMap& b, const CUtensor
   // Blocks that come under their predecessor's tail stand on whatever SMs are free first; launched behind its end (in_order), consecutive ones (the kv heads of a
   // key block) go round the chip in order. Where a block has many iterations that decides more than the 3 us of an early launch: the kernel alone, D = 128, 4313 tokens,
   // 32/8 heads, 174 us in order and 195 early with 4 samples, 370 and 406 with one. The rule is attention_plan.backward_in_order.
-  const unsigned grid = n_items * p.Hkv * p.splits;
+  int whole = 0;
+  if constexpr (R::ON) whole = p.r.whole;
+  const unsigned grid = whole + (n_items * p.Hkv - whole) * p.splits;
   if (in_order) kern<<<grid, AB_THREADS, AttBwdSmem<D>::TOTAL, st>>>(a, b, c, d, p);
   else launch_pdl(kern, grid, AB_THREADS, AttBwdSmem<D>::TOTAL, st, a, b, c, d, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
@@ -686,7 +699,11 @@ static int bwd(const void* qkv, long long ld, const void* out, long long ldo, co
                bool in_order, float* delta, const AttBwdParams<R>& p, cudaStream_t st) {
   const int T = p.T, Hq = p.Hq, Hkv = p.Hkv;
   if ((D != 64 && D != 128) || Hkv <= 0 || Hq % Hkv || ld % 8 || ldo % 8 || lddo % 8 || p.ldq % 8 || p.splits < 1 || p.splits > Hq / Hkv) return -10;
-  const long long units = static_cast<long long>(n_items) * Hkv;
+  long long units = static_cast<long long>(n_items) * Hkv;   // that CTAs share
+  if constexpr (R::ON) {
+    if (p.r.whole < 0 || p.r.whole > units) return -10;
+    units -= p.r.whole;
+  }
   if (p.splits > 1 && (p.ws == nullptr || p.counters == nullptr || units * 8 > SPLIT_COUNTERS || p.splits * units * 2 * AB_B * D * 4 > part_bytes)) return -11;
   CUtensorMap tq, tdo, tdq, tdkv;
   int rc = make_tmap_2d_bf16(&tq, qkv, static_cast<uint64_t>(ld), static_cast<uint64_t>(rows), static_cast<uint64_t>(ld), 64, 128);

@@ -23,6 +23,7 @@ namespace mtb {
 struct AttRuleArgs {
   int window;            // keys a query sees, itself among them; 1 << 30 for all
   const float* slopes;   // [Hq]
+  int whole;             // backward: key blocks times kv heads, from the first on, that have one CTA each; only those behind them are shared by p.splits
   CapArgs cap;           // of raw products
 };
 

@@ -180,6 +180,29 @@ def rule_splits(work: list, hq: int, hkv: int, sms: int, most: int) -> int:
     return splits
 
 
+def rule_shares(work: list, hq: int, hkv: int, sms: int, most) -> tuple:
+    """``(CTAs that share a key block, key blocks in front that have one each)`` for these numbers of query blocks, the largest first. ``most(blocks)``: CTAs
+    that so many key blocks may be shared by. Where whole key blocks fill the GPU a few times and a part of a time, only those of the last part are shared, which then takes a part of a
+    block's time: one sample of 8192 tokens through a window of 1024, 32/8 heads of 128, 480 -> 443 us, 16384 through 2048, 16/4 of 64, 478 -> 435, 5000 and 3000 through 512 311 -> 298
+    (four of 4096 through 256 231 -> 233). It does not pay where key blocks differ, as their order evens their sum out: a causal batch of three, 608 -> 611, 40 samples of 300 103 -> 104."""
+    splits = rule_splits(work, hq, hkv, sms, most(len(work)))
+    group, rounds = hq // hkv, len(work) * hkv // sms
+    if group == 1 or rounds == 0 or splits > 1:
+        return splits, 0
+
+    def finish(whole, s):
+        units = [(_BWD_CTA + group * n, c * hkv) for n, c in Counter(work[:whole]).items()]
+        units += [(_BWD_CTA + _BWD_PARTIAL + group / s * n, c * hkv * s) for n, c in Counter(work[whole:]).items()]
+        return finish_time(units, sms)
+    best, choice = finish(len(work), 1) * 0.97, (1, 0)
+    for whole in {rounds * sms // hkv, max(0, rounds - 1) * sms // hkv} - {0}:
+        for s in range(2, min(group, most(len(work) - whole)) + 1) if whole < len(work) else ():
+            t = finish(whole, s)
+            if t < best:
+                best, choice = t, (s, whole)
+    return choice
+
+
 def rule_in_order(work: list, hq: int, hkv: int, d: int, splits: int) -> bool:
     """``backward_in_order`` for key blocks of these numbers of query blocks."""
     return d == 128 and sum(work) * (hq // hkv) >= IN_ORDER_ITERATIONS * splits * len(work) > 0

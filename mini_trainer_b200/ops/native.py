@@ -108,7 +108,7 @@ class _Sig:
     mtb200_attn_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, F, P, P]
     mtb200_attn_rule_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, I, F, F, I, P, P, P]
     mtb200_attn_rule_fwd_one = [P, L, P, L, P, P, I, I, I, I, I, I, F, F, I, P, P, P]
-    mtb200_attn_rule_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, I, P, U, P, L, F, F, I, P, I, P, P]
+    mtb200_attn_rule_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, I, P, U, P, L, F, F, I, P, I, I, P, P]
     mtb200_attn_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, P, U, P, L, F, I, P, P]
 
 
@@ -643,8 +643,8 @@ class NativeOps:
 
     # -- attention under a rule (attention_rule.py) -----------------------------------------
     def _rule_plan(self, cu_host, hq, hkv, d, scale, rule, T, backward):
-        """``(work table, tokens of the samples, entry point, its row_pairs argument)`` of a batch's forward, ``(work table, tokens of the samples, CTAs per key
-        block, bytes of their partials, launched in order)`` of its backward. Checked when it is made and kept like the plans of the causal form, by the values
+        """``(work table, tokens of the samples, entry point, its row_pairs argument)`` of a batch's forward, ``(work table, tokens of the samples, CTAs that
+        share a key block, key blocks times kv heads in front that are not shared, bytes of the partials, launched in order)`` of its backward. Checked when it is made and kept like the plans of the causal form, by the values
         it depends on, and for the stream that fills the table and gives it back. A table that a capture makes is only filled when its graph runs, so it
         serves that launch alone; what a graph reads, the host memory that such a table is copied from or a table made before, lives as long as this backend."""
         what = (backward, hq, hkv, d, scale, rule.key, rule.slopes is None, self._st())
@@ -677,10 +677,10 @@ class NativeOps:
         items = attention_plan.rule_items(cu_host, prefixes, window, 128, backward)
         work = [it[0] for it in items]
         if backward:
-            units = len(items) * hkv
-            most = 1 if units * 8 > _SPLIT_COUNTERS else min(hq // hkv, _SPLIT_FLOATS // max(1, units * 2 * 128 * d))
-            splits = attention_plan.rule_splits(work, hq, hkv, self.sms, most)
-            tail = (splits, splits * units * 2 * 128 * d * 4, int(attention_plan.rule_in_order(work, hq, hkv, d, splits)))
+            def most(blocks):
+                return 1 if blocks * hkv * 8 > _SPLIT_COUNTERS else min(hq // hkv, _SPLIT_FLOATS // max(1, blocks * hkv * 2 * 128 * d))
+            splits, whole = attention_plan.rule_shares(work, hq, hkv, self.sms, most)
+            tail = (splits, whole * hkv, splits * (len(items) - whole) * hkv * 2 * 128 * d * 4, int(attention_plan.rule_in_order(work, hq, hkv, d, 1 if whole else splits)))
         else:
             pairs = attention_plan.rule_items(cu_host, prefixes, window, 256, False) if (hq // hkv) % 2 else []
             if attention_plan.rule_in_pairs(work, lambda: [(it[0], it[3] + 128 < it[2]) for it in pairs], hq, hkv, d, self.sms,
@@ -731,7 +731,7 @@ class NativeOps:
             raise ValueError("attention under a rule runs on the kernels, not on library attention")
         T, width = qkv.shape[0], hq * d
         scale = d ** -0.5 if scale is None else float(scale)
-        table, rows, splits, nbytes, in_order = self._rule_plan(cu_host, hq, hkv, d, scale, rule, T, True)
+        table, rows, splits, whole, nbytes, in_order = self._rule_plan(cu_host, hq, hkv, d, scale, rule, T, True)
         ld, ldo, lddo = self._rule_rows(qkv, T, width + 2 * hkv * d), self._rule_rows(out, T, width), self._rule_rows(dout, T, width)
         rule.check_slopes(hq, qkv)
         if lse.dtype is not torch.float32 or lse.shape != (hq, T) or not lse.is_contiguous() or lse.get_device() != qkv.get_device():
@@ -747,7 +747,7 @@ class NativeOps:
         ws, epoch, part = split or (None, 0, None)
         self._call("mtb200_attn_rule_bwd", qkv.data_ptr(), ld, out.data_ptr(), ldo, dout.data_ptr(), lddo, dqkv.data_ptr(), qkv.shape[1], lse.data_ptr(),
                    dq_acc + 4 * hq * T * d, dq_acc, table.data_ptr(), table.shape[0], T, rows, hq, hkv, d, splits if split else 1, _ptr(ws), epoch, _ptr(part),
-                   4 * part.numel() if split else 0, scale, rule.key[0], rule.key[1], _ptr(rule.slopes), in_order, self.status.data_ptr(), st, n=3, tag="mtb200_attn_bwd")
+                   4 * part.numel() if split else 0, scale, rule.key[0], rule.key[1], _ptr(rule.slopes), in_order, whole, self.status.data_ptr(), st, n=3, tag="mtb200_attn_bwd")
         return dqkv
 
     def attention(self, qkv, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None, rule=None):

@@ -4,6 +4,7 @@ Tolerances count roundings. A rounding to bf16 is off by at most U = 2^-8 of the
 an exponential is off by at most 1.0e-4 (the cubic), a capped score by 5.1e-7 of itself within the cap and 2^-21 of the cap beyond it. dS = p (dP - delta) c is rounded once, its delta is formed
 with the rounded out; dQ, dK and dV are rounded once. ``bounds`` adds these up entry by entry."""
 import math
+import random
 
 import pytest
 import torch
@@ -219,6 +220,24 @@ def test_backward_of_a_rule_without_edges_is_planned_as_the_causal_one():
     assert A.rule_splits([], 4, 1, 148, 4) == 1
 
 
+def test_only_the_last_part_of_a_launch_is_shared():
+    four = lambda blocks: 4
+    assert A.rule_shares([9] * 64, 32, 8, 148, four) == (2, 55)          # 512 key blocks of one length: three times the GPU, and 68 shared by two
+    assert A.rule_shares([9] * 64, 32, 8, 148, lambda blocks: 1) == (1, 0)   # without room for partials
+    assert A.rule_shares([9] * 74, 32, 8, 148, four) == (1, 0)           # four times the GPU exactly
+    assert A.rule_shares([9] * 64, 8, 8, 148, four) == (1, 0)            # a head has nothing to share
+    assert A.rule_shares([], 32, 8, 148, four) == (1, 0)
+    for seed in range(40):
+        r = random.Random(seed)
+        work = sorted((r.randint(1, 40) for _ in range(r.randint(1, 120))), reverse=True)
+        hkv, group = r.choice([1, 2, 4, 8]), r.choice([1, 2, 3, 4, 8])
+        most = r.randint(1, 8)
+        splits, whole = A.rule_shares(work, hkv * group, hkv, 148, lambda blocks: min(group, most))
+        assert 1 <= splits <= min(group, most) and 0 <= whole < len(work) and (splits > 1 or whole == 0)
+        if whole == 0:
+            assert splits == A.rule_splits(work, hkv * group, hkv, 148, min(group, most))
+
+
 def test_forward_of_a_rule_without_edges_takes_the_causal_form():
     for lens, hq, hkv, d in (([2048], 16, 4, 64), ([16384], 2, 1, 128), ([300] * 41, 16, 4, 64), ([128] * 100, 32, 8, 128), ([5000] * 4, 9, 3, 128), ([1024], 14, 2, 128), ([700] * 30, 3, 1, 64)):
         cu = starts(lens)
@@ -334,6 +353,22 @@ def test_every_combination_on_ragged_samples(ops, d, form, monkeypatch):
         want, bound = exact(qkv, starts(case[0]), hq, hkv, d, rule_of(case), dout)
         for g, w, b in zip(run(ops, case, qkv, dout), want, bound):
             within(g, w, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits,whole", [(2, 0), (2, 1), (3, 4), (4, 5), (2, 6)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_key_blocks_shared_from_some_on(ops, d, splits, whole, monkeypatch):
+    """The first key blocks of a table with a CTA each, the others' heads divided over several, with every kind of score."""
+    monkeypatch.setattr(A, "rule_shares", lambda *a: (splits, whole))
+    ops._attn_plan_cache.clear()
+    for cap, window, prefix, bias in ((None, 150, None, False), (30.0, None, [7, 130], False), (None, None, None, True), (30.0, 100, [200, 0], True)):
+        case = ([333, 401], 8, 2, d, cap, window, prefix, bias)   # seven key blocks, two kv heads
+        qkv, dout = make(case[0], 8, 2, d, seed=splits, device="cuda")
+        want, bound = exact(qkv, starts(case[0]), 8, 2, d, rule_of(case), dout)
+        for g, w, b in zip(run(ops, case, qkv, dout), want, bound):
+            within(g, w, b)
+    ops._attn_plan_cache.clear()
 
 
 @pytest.mark.gpu
