@@ -84,7 +84,7 @@ struct AttBwdParams {
   int T, Hq, Hkv;
   int G;                // Hq / Hkv
   unsigned hkv_inv;     // (2^32 - 1) / Hkv
-  int splits;           // CTAs that share a key block's query heads
+  int splits;           // CTAs that share a key block's query heads (under a rule one's behind r.whole)
   float* ws;            // splits > 1: fp32 partials of dK and dV
   unsigned long long* counters;   // splits > 1: one arrival counter per (key block, warp); last_arrival in gemm_epilogue.cuh
   unsigned long long epoch;

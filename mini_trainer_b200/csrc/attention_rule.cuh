@@ -11,7 +11,7 @@
 // score: a cap adds five to seven packed instructions a pair, and the reference's comparisons of absolute values, a bias three. 8192 tokens in three samples, 32/8 heads of 128
 // (188 GFLOP forward, 471 backward): forward 192 us under a rule without either as in the plain causal kernel, 232 capped, 210 biased, 269 both; backward 583, 611, 574, 609.
 // The tensor core is busy for 57, 45, 50 and about 37 % of the forward's cycles, issue slots for 44, 42, 48 and 42 %: no pipe is full, a row's instructions depend on each other.
-// Windows and prefixes cost what their tiles do: one sample of 8192 tokens with a window of 1024 takes 0.70 ms both ways, without one 1.8.
+// Windows and prefixes cost what their tiles do: one sample of 8192 tokens with a window of 1024 takes 0.69 ms both ways, without one 1.8.
 #pragma once
 #include <stdint.h>
 
