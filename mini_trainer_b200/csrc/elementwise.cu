@@ -1337,9 +1337,10 @@ __global__ void __launch_bounds__(1024, 1) ce_row_kernel(const __nv_bfloat16* lo
 }
 
 // Cross-entropy of logits capped by a tanh, l = cap t: loss and dz = (softmax(l) - onehot) (1 - t^2) scale, rounded to bf16, over t [R, V] in fp16, in place. The
-// product that left t has left the softmax's statistics of every 128 columns too, formed before its rounding (gemm_act.cuh, ACT_CAP), and the target's logit is
-// formed again from its rows of x and w: the loss, a difference of numbers many times a rounding apart, sees none. The gradient is that of t as it is
-// rounded (2^-11 of itself, where bf16 logits are off by 2^-8). Bound by reading and writing the rows: 3000 x 151936
+// product that left t has left the softmax's statistics of every 128 columns too, formed before its rounding and without the target's column (gemm_act.cuh, ACT_CAP); the target's
+// logit is formed again from its rows of x and w. With o = the others' sum and e the target's exponential, loss = log(1 + o / e) and the target's p - 1 = -o / (o + e): neither
+// is a difference, so a target that has nearly all of the probability keeps its gradient (formed as a rounded p less one, half of the signs were wrong at a p - 1 of 1e-4). The others'
+// p are those of t as it is rounded (2^-11 of itself, where bf16 logits are off by 2^-8), each off by its own rounding and no more. Bound by reading and writing the rows: 3000 x 151936
 // in 304 us, 6.0 TB/s (0.92 of the copy rate). Once the statistics are there the parts of a row need nothing of each other, so a row is divided over blocks where rows alone are not
 // eight blocks to an SM, down to parts of 4096 columns; each part adds up the row's statistics (a hundredth of its bytes at 16 parts), the first has the loss. Blocks are small and
 // five to an SM, so that one's reductions run under another's rows. Rows whole in blocks of 512 and 1024 threads, then like this: 1 x 151936 11.6 -> 4.0 us, 129 x 32000 5.4 -> 4.8,
@@ -1371,7 +1372,7 @@ __global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16
     if (q.x > m) { s *= ex2_mufu((m - q.x) * cap2); m = q.x; }
     s += q.y * ex2_mufu((q.x - m) * cap2);
   }
-  for (int c = threadIdx.x * 8; lo == 0 && there && c < H; c += step) {
+  for (int c = threadIdx.x * 8; there && c < H; c += step) {   // every part of a row wants it
     const uint4 a = *reinterpret_cast<const uint4*>(x + row * H + c), b = *reinterpret_cast<const uint4*>(w + tgt * H + c);
     const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -1382,12 +1383,14 @@ __global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16
   }
   const float gm = block_max(m, red);
   const float gs = block_sum(s * ex2_mufu((m - gm) * cap2), red);   // (zero for a thread without columns)
-  if (lo == 0) dot = block_sum(dot, red) * alpha;
-  if (threadIdx.x == 0 && lo == 0) {
-    const float tt = !there ? NAN : fabsf(dot) <= 1.f ? tanh_pair(splat(dot)).x : tanh_exact(dot);   // NaN of a target that is no column
-    loss[row] = 0.6931471805599453f * ((gm - tt) * cap2 + log2f(gs));
-  }
-  const float2 inv = splat(grad_scale / gs), nm = splat(-gm * cap2), one = splat(1.f), c2 = splat(cap2);
+  dot = block_sum(dot, red) * alpha;
+  const float tt = fabsf(dot) <= 1.f ? tanh_pair(splat(dot)).x : tanh_exact(dot);
+  // the reference is the larger of the others' largest and the target; a target that is no column counts for nothing, and its loss is NaN
+  const float ref = there ? fmaxf(gm, tt) : gm, others = gs * ex2_mufu((gm - ref) * cap2), self = there ? ex2_mufu((tt - ref) * cap2) : 0.f;
+  if (threadIdx.x == 0 && lo == 0)
+    loss[row] = there ? 0.6931471805599453f * ((ref - tt) * cap2) + (ref == tt ? log1pf(others) : logf(others + self)) : NAN;
+  const float norm = grad_scale / (others + self), minus = -others * norm;   // (p - 1 of the target)
+  const float2 inv = splat(norm), nm = splat(-ref * cap2), one = splat(1.f), c2 = splat(cap2);
   auto gradient = [&](uint4 u, int c) {
     const float2 f[4] = {unpack_half(u.x), unpack_half(u.y), unpack_half(u.z), unpack_half(u.w)};
     float2 p[4];
@@ -1399,8 +1402,8 @@ __global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16
     if (tgt >= c && tgt < c + 8) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (tgt - c == 2 * i) p[i].x -= grad_scale;
-        if (tgt - c == 2 * i + 1) p[i].y -= grad_scale;
+        if (tgt - c == 2 * i) p[i].x = minus;
+        if (tgt - c == 2 * i + 1) p[i].y = minus;
       }
     }
 #pragma unroll

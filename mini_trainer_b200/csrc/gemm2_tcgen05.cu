@@ -578,17 +578,19 @@ int launch_gather(const void* A, long long lda, void* D, long long ldd, const vo
   return launch<false, false, false, true>(ta, tb, td, p, stream, &g);
 }
 
-// Products with an activation or a cap in the epilogue; called by mtb200_gemm_act and mtb200_gemm_capped.
+// Products with an activation in the epilogue, and with a cap; called by mtb200_gemm_act and mtb200_gemm_capped.
 int launch_act(int mode, bool wide, const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_GLU>& m, const EpiParams& e, const ActParams& a, int K,
                int* status, cudaStream_t stream) {
   const Params p{e.M, e.N, K, status, 0, 0, 0, e, a};
   const ActMaps<ACT_PLAIN> plain{m.gate, m.up, m.act};
-  const ActMaps<ACT_CAP> capped{m.gate};
-  if (mode == ACT_CAP) return launch<false, false, false, false, false, false, ACT_CAP>(ta, tb, m.gate, p, stream, nullptr, 0, capped);
   if (wide) return mode == ACT_GLU ? launch<false, false, false, false, false, false, ACT_GLU, true>(ta, tb, m.gate, p, stream, nullptr, 0, m)
                                    : launch<false, false, false, false, false, false, ACT_PLAIN, true>(ta, tb, m.gate, p, stream, nullptr, 0, plain);
   if (mode == ACT_GLU) return launch<false, false, false, false, false, false, ACT_GLU>(ta, tb, m.gate, p, stream, nullptr, 0, m);
   return launch<false, false, false, false, false, false, ACT_PLAIN>(ta, tb, m.gate, p, stream, nullptr, 0, plain);
+}
+int launch_capped(const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_CAP>& m, const EpiParams& e, const ActParams& a, int K, int* status, cudaStream_t stream) {
+  const Params p{e.M, e.N, K, status, 0, 0, 0, e, a};
+  return launch<false, false, false, false, false, false, ACT_CAP>(ta, tb, m.gate, p, stream, nullptr, 0, m);
 }
 
 // Grouped products on wide tiles; called by mtb200_gemm_grouped. `td`, `m`: maps of boxes of 32 rows x 128 bytes.

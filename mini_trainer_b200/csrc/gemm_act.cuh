@@ -4,7 +4,8 @@
 //   ACT_PLAIN  pre = A * B (+ bias), act = f(pre): an MLP without a gate
 //   ACT_CAP    t = tanh(alpha A * B^T) alone, rounded to fp16, and of every row and 128 columns the largest t and the sum of 2^((t - largest) cap2): what
 //              the cross-entropy of capped logits (cap t, cap2 = cap log2 e) reads instead of products in fp32. The statistics are formed before
-//              the rounding. 3720 x 151936 x 1536 1153 us (the product alone 1128), 5000 x 8192 x 512 62 (54), where the exponentials do not hide. Wide tiles, whose one
+//              the rounding, and of every column but the row's target: the gradient of a target that has nearly all of the probability is what
+//              the others have together, which a sum with the target in it does not hold any more. 3720 x 151936 x 1536 1153 us (the product alone 1128), 5000 x 8192 x 512 62 (54), where the exponentials do not hide. Wide tiles, whose one
 //              warp per quarter would form them before it gives the accumulator back, took 1876 us.
 // Eight warps, two per 32-row quarter: with four (one per scheduler) the arithmetic of a tile took longer than short reductions. They work on
 // 32 columns at a time, staged as boxes of 32 rows x 64 bytes (64B-swizzled). Bound by the product. With its activation, in a loop of its own on a B200:
@@ -39,7 +40,7 @@ struct ActParams {
 // Tensor maps of gate (or x), up and act, boxes of 32 rows x 32 columns, 64B-swizzled; nothing in instances without an activation.
 template <int ACT> struct ActMaps { CUtensorMap gate, up, act; };
 template <> struct ActMaps<ACT_NONE> {};
-template <> struct ActMaps<ACT_CAP> { CUtensorMap gate; };
+template <> struct ActMaps<ACT_CAP> { CUtensorMap gate; const long long* targets; };   // targets: [M], a column each or anything else for none
 
 constexpr int ACT_WARPS = 8;
 constexpr int ACT_BOX = 32 * 64;                     // bytes of a box
@@ -74,8 +75,8 @@ __device__ __forceinline__ uint32_t pack_half(float2 v) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 constexpr float CAP_NONE = -2.f;   // below any t: no column yet
-// ACT_CAP: 32 columns of a thread's row, from `col` on, and their part of the row's statistics {largest t, sum}; columns past N count for nothing.
-__device__ __forceinline__ void cap_columns32(const EpiParams& p, float cap2, const uint32_t (&v)[32], int col, uint32_t (&d)[16], float2& st) {
+// ACT_CAP: 32 columns of a thread's row, from `col` on, and their part of the row's statistics {largest t, sum}; the target's column and those past N count for nothing.
+__device__ __forceinline__ void cap_columns32(const EpiParams& p, float cap2, const uint32_t (&v)[32], int col, long long target, uint32_t (&d)[16], float2& st) {
   float2 t[16];
   float big[2] = {0.f, 0.f};
 #pragma unroll
@@ -96,6 +97,14 @@ __device__ __forceinline__ void cap_columns32(const EpiParams& p, float cap2, co
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (col + (i & ~3) * 2 >= p.N) t[i] = f2(-INFINITY);
+  }
+  if (target >= col && target < col + 32) {   // one thread in many
+    const int at = static_cast<int>(target - col);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (at == 2 * i) t[i].x = -INFINITY;
+      if (at == 2 * i + 1) t[i].y = -INFINITY;
+    }
   }
   float mx[2] = {CAP_NONE, CAP_NONE};
 #pragma unroll
@@ -125,6 +134,8 @@ __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams
   const int y0 = row0 + q * 32;
   if (y0 >= p.M) return;
   float2 st = make_float2(CAP_NONE, 0.f);
+  long long target = -1;
+  if constexpr (ACT == ACT_CAP) { if (y0 + lane < p.M) target = maps.targets[y0 + lane]; }
   auto send = [&](const CUtensorMap& map, const uint32_t (&d)[16], int col) {
     if (lane == 0) bulk_wait_read<1>();
     __syncwarp();
@@ -142,7 +153,7 @@ __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams
     tmem_ld_32x32(taddr + at, v);
     tmem_ld_wait();
     if constexpr (ACT == ACT_CAP) {
-      cap_columns32(p, ap.cap2, v, col, g, st);
+      cap_columns32(p, ap.cap2, v, col, target, g, st);
       send(maps.gate, g, col);
       continue;
     }

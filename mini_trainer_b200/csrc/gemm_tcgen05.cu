@@ -415,6 +415,7 @@ static unsigned tune_wait_hint() {
 namespace g2 {
 int launch_act(int mode, bool wide, const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_GLU>& m, const EpiParams& e, const ActParams& a, int K,
                int* status, cudaStream_t stream);
+int launch_capped(const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_CAP>& m, const EpiParams& e, const ActParams& a, int K, int* status, cudaStream_t stream);
 int launch_grouped(int mode, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const ActMaps<ACT_GLU>& m, const EpiParams& e, const ActParams& a,
                    int K, const GroupParams& g, int* status, cudaStream_t stream);
 int launch_gather(const void* A, long long lda, void* D, long long ldd, const void* bias, int M, int N, int K,
@@ -565,15 +566,16 @@ int mtb200_gemm_act(const void* A, long long lda, const void* W, void* out, void
                                                                                      ActMaps<ACT_PLAIN>{m.gate, m.up, m.act});
 }
 
-// t[M, N] = tanh(alpha A[M, K] * W[N, K]^T) in fp16, and stats[M, ceil(N / 128)] = {largest t, sum of 2^((t - largest) cap2)} of its rows (gemm_act.cuh). All row-major,
-// without padding between rows but in A. `form`: FORM_ONE or FORM_PAIR.
-int mtb200_gemm_capped(const void* A, long long lda, const void* W, void* t, float2* stats, int M, int N, int K, float alpha, float cap2, int form, int* status,
+// t[M, N] = tanh(alpha A[M, K] * W[N, K]^T) in fp16, and stats[M, ceil(N / 128)] = {largest t, sum of 2^((t - largest) cap2)} of its rows without the column targets[row]
+// (gemm_act.cuh). All row-major, without padding between rows but in A. `form`: FORM_ONE or FORM_PAIR.
+int mtb200_gemm_capped(const void* A, long long lda, const void* W, void* t, float2* stats, const long long* targets, int M, int N, int K, float alpha, float cap2, int form, int* status,
                        cudaStream_t stream) {
   using namespace mtb;
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if ((form != FORM_ONE && form != FORM_PAIR) || N % 8 || K % 8 || stats == nullptr) return -10;
+  if ((form != FORM_ONE && form != FORM_PAIR) || N % 8 || K % 8 || stats == nullptr || targets == nullptr) return -10;
   CUtensorMap ta, tb;
-  ActMaps<ACT_GLU> m{};
+  ActMaps<ACT_CAP> m{};
+  m.targets = targets;
   int rc = make_tmap_2d_bf16(&ta, A, K, M, lda, 64, 128);
   if (rc) return rc;
   rc = make_tmap_2d_bf16(&tb, W, K, N, K, 64, form != FORM_ONE ? 128 : 256);
@@ -583,9 +585,9 @@ int mtb200_gemm_capped(const void* A, long long lda, const void* W, void* t, flo
   const EpiParams e{M, N, nullptr, 0, nullptr, alpha, 1, nullptr, stats, nullptr, 0};
   ActParams a{N, {}};
   a.cap2 = cap2;
-  if (form != FORM_ONE) return g2::launch_act(ACT_CAP, false, ta, tb, m, e, a, K, status, stream);
+  if (form != FORM_ONE) return g2::launch_capped(ta, tb, m, e, a, K, status, stream);
   const GemmParams p{M, N, K, status, tune_group_m(), tune_wait_hint(), 0u, e, a};
-  return launch<false, false, false, false, false, GROUP_NONE, false, false, ACT_CAP>(ta, tb, m.gate, p, stream, nullptr, 0, nullptr, ActMaps<ACT_CAP>{m.gate});
+  return launch<false, false, false, false, false, GROUP_NONE, false, false, ACT_CAP>(ta, tb, m.gate, p, stream, nullptr, 0, nullptr, m);
 }
 
 enum { GROUPED_WIDE = 4 };

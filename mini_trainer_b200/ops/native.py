@@ -83,7 +83,7 @@ class _Sig:
     mtb200_embedding_bwd_scan = [P, P, P, I, I, I, P, P]
     mtb200_scatter_rows = [P, P, P, P, P, I, I, I, P, P]
     mtb200_ce_fwd_bwd = [P, L, I, P, P, P, P, L, I, I, F, L, P]
-    mtb200_gemm_capped = [P, L, P, P, P, I, I, I, F, F, I, P, P]
+    mtb200_gemm_capped = [P, L, P, P, P, P, I, I, I, F, F, I, P, P]
     mtb200_ce_capped = [P, P, P, P, P, P, I, I, I, F, F, F, L, P]
     mtb200_colsum = [P, L, P, P, I, I, P]
     mtb200_accumulate = [P, P, L, I, I, P]
@@ -991,8 +991,8 @@ class NativeOps:
         return V > 16384 and H >= 1536
 
     def _linear_ce_capped(self, x, w, targets, grad_scale, dw_out, accumulate_dw, ignore_index, logit_scale, softcap):
-        """``linear_ce`` with capped logits. The product leaves them as parts of the cap, in fp16, with the softmax's statistics formed in fp32 before that
-        rounding; the loss kernel writes their gradient over them. Nothing is held between calls."""
+        """``linear_ce`` with capped logits. The product leaves them as parts of the cap, in fp16, with the softmax's statistics, without the targets, formed in fp32
+        before that rounding; the loss kernel writes their gradient over them. Nothing is held between calls."""
         ok = x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1]
         if not ok or any(t.dtype != torch.bfloat16 or t.device != x.device or not t.is_contiguous() or t.data_ptr() % 16 for t in (x, w, dw_out)) or dw_out.shape != w.shape:
             raise ValueError("expected contiguous bf16 rows [T, H], a weight [V, H] and its gradient on one device")
@@ -1019,9 +1019,10 @@ class NativeOps:
             n = min(ck, T - a)
             xc = x[a:a + n]
             form = gemm_plan.capped_form(n, H, self.use_gemm2, 0 if self.pair_max_flops <= 0 and not self.use_gemm2 else self.cta_pairs())
-            self._call("mtb200_gemm_capped", xc.data_ptr(), H, w.data_ptr(), dz.data_ptr(), stats.data_ptr(), n, V, H, alpha, cap2, form, self.status.data_ptr(),
+            tc = targets[a:a + n].data_ptr()
+            self._call("mtb200_gemm_capped", xc.data_ptr(), H, w.data_ptr(), dz.data_ptr(), stats.data_ptr(), tc, n, V, H, alpha, cap2, form, self.status.data_ptr(),
                        self._st(), tag="gemm_nt_capped")
-            self._call("mtb200_ce_capped", dz.data_ptr(), stats.data_ptr(), xc.data_ptr(), w.data_ptr(), targets[a:a + n].data_ptr(), loss[a:a + n].data_ptr(), n, V, H,
+            self._call("mtb200_ce_capped", dz.data_ptr(), stats.data_ptr(), xc.data_ptr(), w.data_ptr(), tc, loss[a:a + n].data_ptr(), n, V, H,
                        alpha, cap2, float(grad_scale), ignore_index, self._st())
             self.gemm(dz, False, w, True, dx[a:a + n], n, H, V, alpha=logit_scale)
             if dw32 is None:
