@@ -81,6 +81,29 @@ __device__ __forceinline__ float tanh_exact(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + ex2_mufu(x * 2.8853900817779268f)));
   return fmaf(-2.f, q, 1.f);
 }
+// tanh in 16 bits from which both t and 1 - t^2 come with 11 bits. A t near to 1 has lost its distance to 1 when it is rounded (5 % of the derivative at x = 3, all of it from 4.5 on). So
+// up to t = tanh(1) the code is t, and beyond it K / sqrt(1 - |t|), which goes on from there: t is off by 2^-11 of itself below and by 2^-10 (1 - |t|) above, the derivative
+// by 2^-11 2 t^2 / (1 - t^2) <= 2^-9.5 below and 2^-10 above, relative, up to |x| = 12.4, whose derivative of 6.4e-11 is all beyond it have.
+constexpr float CAP_BEND = 0.76159416f, CAP_BEND_K = 0.37186221f, CAP_CODE_MOST = 65504.f;
+__device__ __forceinline__ float tanh_coded(float x, float& code) {
+  const float a = fabsf(x);
+  float q, k;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + ex2_mufu(a * 2.8853900817779268f)));
+  const float far = 2.f * q, t = copysignf(1.f - far, x);   // far: 1 - |t|
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(k) : "f"(far));
+  code = a <= 1.f ? t : copysignf(fminf(CAP_BEND_K * k, CAP_CODE_MOST), x);
+  return t;
+}
+__device__ __forceinline__ float tanh_decoded(float code, float& slope) {
+  const float a = fabsf(code);
+  float q;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(a));
+  q *= CAP_BEND_K;
+  const float far = q * q;
+  const bool below = a <= CAP_BEND;
+  slope = below ? fmaf(-code, code, 1.f) : far * (2.f - far);
+  return below ? code : copysignf(1.f - far, code);
+}
 // A warp's numbers in tensor memory, n x 16 columns of its lanes, capped in place by the exact form. A loop of its own, so that the polynomial's code is all that
 // tiles within the cap fetch.
 __device__ __forceinline__ void cap_in_place(const CapArgs& r, uint32_t taddr, int n) {

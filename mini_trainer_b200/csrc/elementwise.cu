@@ -1336,15 +1336,17 @@ __global__ void __launch_bounds__(1024, 1) ce_row_kernel(const __nv_bfloat16* lo
   pdl_trigger();
 }
 
-// Cross-entropy of logits capped by a tanh, l = cap t: loss and dz = (softmax(l) - onehot) (1 - t^2) scale, rounded to bf16, over t [R, V] in fp16, in place. The
+// Cross-entropy of logits capped by a tanh, l = cap t: loss and dz = (softmax(l) - onehot) (1 - t^2) scale, rounded to bf16, over t [R, V] in 16 bits (cap.cuh), in place. The
 // product that left t has left the softmax's statistics of every 128 columns too, formed before its rounding and without the target's column (gemm_act.cuh, ACT_CAP); the target's
 // logit is formed again from its rows of x and w. With o = the others' sum and e the target's exponential, loss = log(1 + o / e) and the target's p - 1 = -o / (o + e): neither
 // is a difference, so a target that has nearly all of the probability keeps its gradient (formed as a rounded p less one, half of the signs were wrong at a p - 1 of 1e-4). The others'
-// p are those of t as it is rounded (2^-11 of itself, where bf16 logits are off by 2^-8), each off by its own rounding and no more. Bound by reading and writing the rows: 3000 x 151936
-// in 304 us, 6.0 TB/s (0.92 of the copy rate). Once the statistics are there the parts of a row need nothing of each other, so a row is divided over blocks where rows alone are not
-// eight blocks to an SM, down to parts of 4096 columns; each part adds up the row's statistics (a hundredth of its bytes at 16 parts), the first has the loss. Blocks are small and
-// five to an SM, so that one's reductions run under another's rows. Rows whole in blocks of 512 and 1024 threads, then like this: 1 x 151936 11.6 -> 4.0 us, 129 x 32000 5.4 -> 4.8,
-// 600 x 32000 22 -> 11.7, 200 x 151936 23.5 -> 16.9, 1500 x 65536 76 -> 74. Over 52 sizes of 1 to 6000 rows by 8192 to 151936 columns it is 5 % off the best of 36 divisions and sizes of block.
+// p are those of t as it is rounded (2^-11 of itself at most, where bf16 logits are off by 2^-8), each off by its own rounding and no more, and 1 - t^2 is off by 2^-9.5 of itself. Bound by reading and writing
+// the rows: 3720 x 151936 behind its product in 394 us, 5.7 TB/s (0.88 of the copy rate); 507 where most logits are beyond the cap and are decoded one by one. What a row is worked on with matters
+// too, as the products in front have lowered the clock: with the tanh formed again from logits in fp16 it took 480, with four vectors on their way at a time instead of two under the arithmetic of
+// two, which spilled, 436. Once the statistics are there the parts of a row need nothing of each other, so a row is divided over blocks where rows alone are not
+// eight blocks to an SM, down to parts of 4096 columns; each part adds up the row's statistics (a hundredth of its bytes at 16 parts) and forms the target's logit, in one reduction, and the first has
+// the loss. Blocks are small and five to an SM, so that one's reduction runs under another's rows. Rows whole in blocks of 512 and 1024 threads, then like this: 1 x 151936 11.6 -> 4.0 us,
+// 600 x 32000 22 -> 11.7. Over 52 sizes of 1 to 6000 rows by 8192 to 151936 columns it is 5 % off the best of 36 divisions and sizes of block.
 constexpr int CEC_THREADS = 256;
 __device__ __forceinline__ float2 unpack_half(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
@@ -1353,7 +1355,7 @@ __global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16
                                                         long long ignore_index) {
   pdl_trigger();
   pdl_wait();
-  __shared__ float red[32];
+  __shared__ float red[3][CEC_THREADS / 32];   // a warp's largest t, its sum, its part of the target's product
   const long long row = blockIdx.x;
   __nv_bfloat16* tr = t + row * V;
   const long long tgt = targets[row];
@@ -1365,6 +1367,12 @@ __global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16
     return;
   }
   const bool there = tgt >= 0 && tgt < V;
+  const int at = there ? static_cast<int>(tgt) : -1;
+  constexpr int AHEAD = 2;   // vectors that are on their way under the arithmetic of as many
+  uint4 u[AHEAD], next[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (c0 + k * step < hi) u[k] = *reinterpret_cast<const uint4*>(tr + c0 + k * step);
   float m = -2.f, s = 0.f, dot = 0.f;
   const int tiles = (V + 127) / 128;
   for (int c = threadIdx.x; c < tiles; c += blockDim.x) {
@@ -1381,9 +1389,17 @@ __global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16
       dot = fmaf(u.x, v.x, fmaf(u.y, v.y, dot));
     }
   }
-  const float gm = block_max(m, red);
-  const float gs = block_sum(s * ex2_mufu((m - gm) * cap2), red);   // (zero for a thread without columns)
-  dot = block_sum(dot, red) * alpha;
+  const int warps = blockDim.x >> 5, wid = threadIdx.x >> 5;
+  const float wm = warp_max(m);
+  s = warp_sum(s * ex2_mufu((m - wm) * cap2));   // (zero for a thread without columns)
+  dot = warp_sum(dot);
+  if ((threadIdx.x & 31) == 0) { red[0][wid] = wm; red[1][wid] = s; red[2][wid] = dot; }
+  __syncthreads();
+  float gm = red[0][0], gs = 0.f;
+  for (int k = 1; k < warps; ++k) gm = fmaxf(gm, red[0][k]);
+  dot = 0.f;
+  for (int k = 0; k < warps; ++k) { gs = fmaf(red[1][k], ex2_mufu((red[0][k] - gm) * cap2), gs); dot += red[2][k]; }
+  dot *= alpha;
   const float tt = fabsf(dot) <= 1.f ? tanh_pair(splat(dot)).x : tanh_exact(dot);
   // the reference is the larger of the others' largest and the target; a target that is no column counts for nothing, and its loss is NaN
   const float ref = there ? fmaxf(gm, tt) : gm, others = gs * ex2_mufu((gm - ref) * cap2), self = there ? ex2_mufu((tt - ref) * cap2) : 0.f;
@@ -1393,32 +1409,42 @@ __global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16
   const float2 inv = splat(norm), nm = splat(-ref * cap2), one = splat(1.f), c2 = splat(cap2);
   auto gradient = [&](uint4 u, int c) {
     const float2 f[4] = {unpack_half(u.x), unpack_half(u.y), unpack_half(u.z), unpack_half(u.w)};
-    float2 p[4];
+    float2 p[4], slope[4];
+    float big = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 e = ffma2(f[i], c2, nm);
+    for (int i = 0; i < 4; ++i) big = fmax3(big, fabsf(f[i].x), fabsf(f[i].y));
+    auto probability = [&](int i, float2 t) {
+      const float2 e = ffma2(t, c2, nm);
       p[i] = fmul2(make_float2(ex2_mufu(e.x), ex2_mufu(e.y)), inv);
+    };
+    if (big <= CAP_BEND) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { probability(i, f[i]); slope[i] = ffma2(make_float2(-f[i].x, -f[i].y), f[i], one); }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) probability(i, make_float2(tanh_decoded(f[i].x, slope[i].x), tanh_decoded(f[i].y, slope[i].y)));
     }
-    if (tgt >= c && tgt < c + 8) {
+    if ((at & ~7) == c) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (tgt - c == 2 * i) p[i].x = minus;
-        if (tgt - c == 2 * i + 1) p[i].y = minus;
+        if ((at & 7) == 2 * i) p[i].x = minus;
+        if ((at & 7) == 2 * i + 1) p[i].y = minus;
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = fmul2(p[i], ffma2(make_float2(-f[i].x, -f[i].y), f[i], one));
+    for (int i = 0; i < 4; ++i) p[i] = fmul2(p[i], slope[i]);
     *reinterpret_cast<uint4*>(tr + c) = make_uint4(pack_bf16(p[0].x, p[0].y), pack_bf16(p[1].x, p[1].y), pack_bf16(p[2].x, p[2].y), pack_bf16(p[3].x, p[3].y));
   };
-  // four vectors are on their way before the first is overwritten
-  for (int c = c0; c < hi; c += 4 * step) {
-    uint4 u[4];
+#pragma unroll 1
+  for (int c = c0; c < hi; c += AHEAD * step) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (c + k * step < hi) u[k] = *reinterpret_cast<const uint4*>(tr + c + k * step);
+    for (int k = 0; k < AHEAD; ++k)
+      if (c + (AHEAD + k) * step < hi) next[k] = *reinterpret_cast<const uint4*>(tr + c + (AHEAD + k) * step);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < AHEAD; ++k)
       if (c + k * step < hi) gradient(u[k], c + k * step);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) u[k] = next[k];
   }
 }
 
@@ -2077,7 +2103,7 @@ int mtb200_ce_fwd_bwd(const void* logits, long long ld, int logits_bf16, const f
   return launch_ok();
 }
 
-// t: fp16 [R, V] and stats [R, ceil(V / 128)], of mtb200_gemm_capped for these x [R, H], w [V, H], alpha and cap2; bf16 gradients of the products come in t's place.
+// t: 16 bits [R, V] and stats [R, ceil(V / 128)], of mtb200_gemm_capped for these x [R, H], w [V, H], alpha and cap2; bf16 gradients of the products come in t's place.
 int mtb200_ce_capped(void* t, const float2* stats, const void* x, const void* w, const long long* targets, float* loss, int R, int V, int H, float alpha, float cap2,
                      float grad_scale, long long ignore_index, cudaStream_t st) {
   if (R <= 0) return 0;

@@ -2,10 +2,11 @@
 // a bandwidth-bound kernel. They are rounded to bf16 before the activation reads them, as if they had been stored in between.
 //   ACT_GLU    pre = A * [Wg; Wu]^T, act = f(g) * u. A tile's 256 columns are 128 of the gate and the same 128 of up, so that one thread has both.
 //   ACT_PLAIN  pre = A * B (+ bias), act = f(pre): an MLP without a gate
-//   ACT_CAP    t = tanh(alpha A * B^T) alone, rounded to fp16, and of every row and 128 columns the largest t and the sum of 2^((t - largest) cap2): what
+//   ACT_CAP    t = tanh(alpha A * B^T) alone, in 16 bits that hold 1 - t^2 too (cap.cuh), and of every row and 128 columns the largest t and the sum of 2^((t - largest) cap2): what
 //              the cross-entropy of capped logits (cap t, cap2 = cap log2 e) reads instead of products in fp32. The statistics are formed before
 //              the rounding, and of every column but the row's target: the gradient of a target that has nearly all of the probability is what
-//              the others have together, which a sum with the target in it does not hold any more. 3720 x 151936 x 1536 1153 us (the product alone 1128), 5000 x 8192 x 512 62 (54), where the exponentials do not hide. Wide tiles, whose one
+//              the others have together, which a sum with the target in it does not hold any more. 3720 x 151936 x 1536 1153 us (the product alone 1128), 5000 x 8192 x 512 62 (54), where the exponentials do not hide; 1399 where most
+//              logits are beyond the cap. Wide tiles, whose one
 //              warp per quarter would form them before it gives the accumulator back, took 1876 us.
 // Eight warps, two per 32-row quarter: with four (one per scheduler) the arithmetic of a tile took longer than short reductions. They work on
 // 32 columns at a time, staged as boxes of 32 rows x 64 bytes (64B-swizzled). Bound by the product. With its activation, in a loop of its own on a B200:
@@ -86,13 +87,15 @@ __device__ __forceinline__ void cap_columns32(const EpiParams& p, float cap2, co
   }
   if (fmaxf(big[0], big[1]) <= 1.f) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] = tanh_pair(t[i]);
+    for (int i = 0; i < 16; ++i) { t[i] = tanh_pair(t[i]); d[i] = pack_half(t[i]); }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] = make_float2(tanh_exact(t[i].x), tanh_exact(t[i].y));
+    for (int i = 0; i < 16; ++i) {
+      float2 code;
+      t[i] = make_float2(tanh_coded(t[i].x, code.x), tanh_coded(t[i].y, code.y));
+      d[i] = pack_half(code);
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) d[i] = pack_half(t[i]);
   if (col + 32 > p.N) {   // N is a multiple of 8
 #pragma unroll
     for (int i = 0; i < 16; ++i)

@@ -566,7 +566,7 @@ int mtb200_gemm_act(const void* A, long long lda, const void* W, void* out, void
                                                                                      ActMaps<ACT_PLAIN>{m.gate, m.up, m.act});
 }
 
-// t[M, N] = tanh(alpha A[M, K] * W[N, K]^T) in fp16, and stats[M, ceil(N / 128)] = {largest t, sum of 2^((t - largest) cap2)} of its rows without the column targets[row]
+// t[M, N] = tanh(alpha A[M, K] * W[N, K]^T) in 16 bits (cap.cuh), and stats[M, ceil(N / 128)] = {largest t, sum of 2^((t - largest) cap2)} of its rows without the column targets[row]
 // (gemm_act.cuh). All row-major, without padding between rows but in A. `form`: FORM_ONE or FORM_PAIR.
 int mtb200_gemm_capped(const void* A, long long lda, const void* W, void* t, float2* stats, const long long* targets, int M, int N, int K, float alpha, float cap2, int form, int* status,
                        cudaStream_t stream) {

@@ -991,7 +991,7 @@ class NativeOps:
         return V > 16384 and H >= 1536
 
     def _linear_ce_capped(self, x, w, targets, grad_scale, dw_out, accumulate_dw, ignore_index, logit_scale, softcap):
-        """``linear_ce`` with capped logits. The product leaves them as parts of the cap, in fp16, with the softmax's statistics, without the targets, formed in fp32
+        """``linear_ce`` with capped logits. The product leaves them as parts of the cap, in 16 bits, with the softmax's statistics, without the targets, formed in fp32
         before that rounding; the loss kernel writes their gradient over them. Nothing is held between calls."""
         ok = x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1]
         if not ok or any(t.dtype != torch.bfloat16 or t.device != x.device or not t.is_contiguous() or t.data_ptr() % 16 for t in (x, w, dw_out)) or dw_out.shape != w.shape:

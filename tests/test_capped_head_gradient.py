@@ -1,8 +1,10 @@
-"""Gradients of the capped head where a difference of rounded numbers would lose them: targets that have nearly all of the probability. Bounds are relative to what is left.
+"""Gradients of the capped head where a difference of rounded numbers would lose them: targets that have nearly all of the probability, and logits far beyond the cap. Bounds are
+relative to what is left.
 
 Tolerances count roundings. A target's p - 1 is minus what the others have, so an error of relative size e in each of the others' p is one of e in it, however small it is.
-The others' p come from l / cap in 16 bits (H = 2^-11 of itself): off by cap |l / cap| H, by their products (2^-17 of sum |x w|) and the tanh's polynomial (6.7e-7), and by the
-normaliser's, which is formed from unrounded logits. The gradient of a logit is p or p - 1 times 1 - (l / cap)^2, rounded to bf16 (U = 2^-8); dx and dw are sums of it in fp32, rounded once."""
+The others' p come from t = tanh(x w / cap) in 16 bits, H = 2^-11: t itself up to tanh(1), and the root of 1 - |t| from there on, so t is off by H of itself or by 2 H of 1 - |t|, and the derivative
+1 - t^2 by 2 t^2 H / (1 - t^2) or 2 H, relative. The product (2^-17 of sum |x w|) is off by as much over the cap times 1 - t^2, and the tanh's polynomial by 6.8e-7; the normaliser is formed from
+unrounded logits. The gradient of a logit is p or p - 1 times the derivative, rounded to bf16 (U = 2^-8); dx and dw are sums of it in fp32, rounded once."""
 import pytest
 import torch
 
@@ -10,7 +12,7 @@ from mini_trainer_b200.ops.torch_ref import TorchOps
 
 U = torch.finfo(torch.bfloat16).eps / 2
 H = torch.finfo(torch.float16).eps / 2
-TANH = 6.7e-7
+TANH = 6.8e-7
 
 
 def rows(levels, width, V, seed=0, gain=0.5, device="cpu"):
@@ -37,15 +39,16 @@ def exact(x, w, t, cap, grad_scale):
     p, left = torch.exp(l - whole), torch.exp(others - whole)
     p1 = p.scatter(1, t, -left)
     dz = p1 * c * grad_scale
-    el = c * 2.0 ** -17 * (x.abs() @ w.abs().t()) + (TANH + 2.0 ** -21) * l.abs() + 2.0 ** -21 * cap * (z.abs() > cap)
+    ez = 2.0 ** -17 * (x.abs() @ w.abs().t())
+    at = (z / cap).abs()
+    below, above = th.abs().clamp_min(2.0 ** -14) * H * (at <= 1.01), (1 - th.abs()) * 2 * H * (at > 1)   # of t; around the bend by either
+    el = c * ez + (TANH + 2.0 ** -21) * l.abs() + 2.0 ** -21 * cap * (z.abs() > cap)
     mine = el.gather(1, t)
     among = ((p.scatter(1, t, 0.0) / left) * el).sum(1, keepdim=True)   # of the others' sum, relative
     norm = left * (among + mine)                                        # of the normaliser
-    rel = el + norm + 2.0 ** -18
-    rel = rel + cap * th.abs().clamp_min(2.0 ** -14) * H
-    rel = rel.scatter(1, t, among + norm + 2.0 ** -18)
-    slope = (2 * th.square() * H + 2 * th.abs() * (el / cap + 2.0 ** -20)) / c + 2.0 ** -18
-    edz = (U + 1.02 * rel + 1.02 * slope) * dz.abs()
+    rel = (el + cap * (below + above) + norm + 2.0 ** -18).scatter(1, t, among + norm + 2.0 ** -18)
+    slope = 2 * th.abs() * (below / c + ez / cap) + 2 * H * (at > 1) + 2 * TANH * th.square() / c * (at <= 1.01) + 2.0 ** -18
+    edz = (U + 1.02 * rel + 1.02 * slope) * dz.abs() + 2.0 ** -124   # what is no normal number of fp32 may be zero
     bl = left[:, 0] * (among + mine + 2.0 ** -18)[:, 0] * 1.02 + 2.0 ** -21 * loss
     dx, dw = dz @ w, dz.t() @ x
     bx, bw = (1.01 * edz + 2.0 ** -17 * dz.abs()) @ w.abs() + U * dx.abs(), (1.01 * edz + 2.0 ** -17 * dz.abs()).t() @ x.abs() + U * dw.abs()
@@ -64,7 +67,7 @@ def check(ops, x, w, t, cap, grad_scale=1.0):
         d = (g.double().cpu() - v).abs()
         assert torch.isfinite(g).all() and (d <= b).all(), (name, int((d > b).sum()), float((d / b).max()))
         if name != "loss":   # the bound says something: a gradient of zero is far outside
-            assert b.norm() <= 0.25 * v.norm(), (name, float(b.norm() / v.norm()))
+            assert b.norm() <= 0.5 * v.norm(), (name, float(b.norm() / v.norm()))
     return got, left
 
 
@@ -115,4 +118,42 @@ def test_a_confident_target_between_ignored_and_missing_ones(ops):
     th = torch.tanh(z / 30.0)
     want = (torch.softmax(30.0 * th, 1) * (1 - th * th) @ w.double())[2::3]
     assert ((dx[2::3].double() - want).norm(dim=1) <= 0.05 * want.norm(dim=1)).all()
+    ops.check_status()
+
+
+def saturated(V, caps, sign, cap, seed=0, device="cpu"):
+    """One row whose logits are ``caps`` caps and more away from zero, on either side; the target's on that of ``sign``. Only the first entry of x is not zero, so dw holds every logit's gradient."""
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(V, 32, generator=g)
+    w[:, 0] = torch.where(torch.rand(V, generator=g) < 0.5, -1.0, 1.0) * cap * (caps + torch.rand(V, generator=g))
+    w[V // 3, 0] = sign * cap * (caps + 0.5)
+    x = torch.zeros(1, 32)
+    x[0, 0] = 1.0
+    return x.bfloat16().to(device), w.bfloat16().to(device), torch.tensor([V // 3], device=device)
+
+
+def test_plain_backend_keeps_the_slope_of_saturated_logits():
+    """1 - t^2 of a t in fp32: off by 2^-23 / (1 - t^2), 1e-5 at three caps."""
+    check(TorchOps(), *saturated(72, 3.0, -1.0, 2.0), 2.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+@pytest.mark.parametrize("cap", [2.0, 30.0])
+@pytest.mark.parametrize("caps", [0.2, 0.9, 2.0, 3.0, 4.5, 6.0, 9.0, 11.3])
+def test_saturated_logits_keep_their_slope(ops, caps, cap, sign):
+    """A target that is certain of the wrong side (sign -1, a p - 1 of one) has the gradient that 1 - tanh^2 leaves it, 2e-10 of it at twelve caps, and so have the others."""
+    for V in (72, 4104):
+        check(ops, *saturated(V, caps, sign, cap, device="cuda"), cap)
+    ops.check_status()
+
+
+@pytest.mark.gpu
+def test_logits_beyond_all_caps_have_hardly_any_gradient(ops):
+    """From 12.4 caps on the derivative stays at what it is there; p and p - 1 are what they are."""
+    least = (4 / (torch.exp(torch.tensor(12.4257)) + torch.exp(torch.tensor(-12.4257))) ** 2).item()
+    for caps, x, w, t in ((k, *saturated(72, k, -1.0, 30.0, device="cuda")) for k in (12.5, 30.0, 1000.0)):
+        loss, dx, dw = run(ops, x, w, t, 30.0)
+        assert abs(float(loss) - float(torch.logsumexp(30.0 * torch.tanh(w.double()[:, 0] / 30.0), 0) + 30.0)) < 1e-4
+        assert torch.isfinite(dx).all() and 0 < -dw[24, 0] <= 1.02 * least and dw.abs().max() <= 1.02 * least
     ops.check_status()
