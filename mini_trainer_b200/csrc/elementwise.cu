@@ -1448,6 +1448,14 @@ __global__ void __launch_bounds__(CEC_THREADS, 5) ce_capped_kernel(__nv_bfloat16
   }
 }
 
+// ------------------------------------------------------------------------------ integers from the launch itself
+struct IntArgs { static constexpr int N = 1008; int v[N]; };   // 4 KB of arguments a launch, with the others
+__global__ void __launch_bounds__(256) write_ints_kernel(int* dst, int n, const __grid_constant__ IntArgs a) {
+  pdl_wait();   // the memory may be an earlier launch's yet
+  for (int i = threadIdx.x; i < n; i += blockDim.x) dst[i] = a.v[i];
+  pdl_trigger();
+}
+
 // ------------------------------------------------------------------------------ column sums (bias grad)
 // part[split, c] = sum over this split's rows of x[r, c]; then reduce_rows_kernel. A lane adds V neighbouring columns of every
 // eighth row: V = 8 (16-byte loads) where rows are 16-byte aligned, V = 2 for any even width, and for few columns and rows, where more
@@ -2143,6 +2151,17 @@ int mtb200_accumulate(float* acc, const void* src, long long n, int src_is_f32, 
   if (n % 8) return -10;
   if (src_is_f32) launch_pdl(accumulate_kernel<float>, cdiv(n / 8, EW_THREADS), EW_THREADS, 0, st, acc, (const float*)src, n, accumulate);
   else launch_pdl(accumulate_kernel<bf16>, cdiv(n / 8, EW_THREADS), EW_THREADS, 0, st, acc, (const bf16*)src, n, accumulate);
+  return launch_ok();
+}
+
+// n integers of host memory written to the device by kernels that carry them as their arguments, so a captured launch needs nothing of the host's any more: read before this returns.
+int mtb200_write_ints(int* dst, const int* src, int n, cudaStream_t st) {
+  for (int i = 0; i < n; i += IntArgs::N) {
+    IntArgs a;
+    const int k = n - i < IntArgs::N ? n - i : IntArgs::N;
+    for (int j = 0; j < k; ++j) a.v[j] = src[i + j];
+    launch_pdl(write_ints_kernel, 1, 256, 0, st, dst + i, k, a);
+  }
   return launch_ok();
 }
 

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import itertools
 import os
+from array import array
 from dataclasses import dataclass
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
 
@@ -88,6 +89,7 @@ class _Sig:
     mtb200_colsum = [P, L, P, P, I, I, P]
     mtb200_accumulate = [P, P, L, I, I, P]
     mtb200_f32_to_bf16 = [P, P, L, I, P]
+    mtb200_write_ints = [P, P, I, P]
     mtb200_sumsq = [P, L, P, P]
     mtb200_adamw = [P, P, P, I, P, P, L, F, F, F, F, F, I, P, P]
     mtb200_sumsq_groups = [P, I, P, P]
@@ -189,7 +191,6 @@ class NativeOps:
         self._gemm_plans = {}   # sizes of a product, or of a grouped one -> entry point and splits, or mode
         self._epoch = itertools.count(1)   # of the launches that may split
         self._attn_plan_cache = {}
-        self._captured = []   # what captured launches under a rule read and copy: a graph may be replayed for as long as there is one
         self._block_specs = {}   # sizes of a block -> its products' plans
         self._pairs = None
         self.sms = torch.cuda.get_device_properties(self._index).multi_processor_count
@@ -644,24 +645,36 @@ class NativeOps:
     # -- attention under a rule (attention_rule.py) -----------------------------------------
     def _rule_plan(self, cu_host, hq, hkv, d, scale, rule, T, backward):
         """``(work table, tokens of the samples, entry point, its row_pairs argument)`` of a batch's forward, ``(work table, tokens of the samples, CTAs that
-        share a key block, key blocks times kv heads in front that are not shared, bytes of the partials, launched in order)`` of its backward. Checked when it is made and kept like the plans of the causal form, by the values
-        it depends on, and for the stream that fills the table and gives it back. A table that a capture makes is only filled when its graph runs, so it
-        serves that launch alone; what a graph reads, the host memory that such a table is copied from or a table made before, lives as long as this backend."""
-        what = (backward, hq, hkv, d, scale, rule.key, rule.slopes is None, self._st())
-        capturing = torch.cuda.is_current_stream_capturing()
-        plan = self._cached(cu_host, what)
+        share a key block, key blocks times kv heads in front that are not shared, bytes of the partials, launched in order)`` of its backward. Checked when it is made and kept like the plans of
+        the causal form, by the values it depends on; the table on the device also for the stream that fills it and gives it back. Under capture each launch fills a table of the graph's own
+        memory, from what the graph itself holds: a graph needs nothing that is kept here."""
+        what = (backward, hq, hkv, d, scale, rule.key, rule.slopes is None)
+        if torch.cuda.is_current_stream_capturing():
+            rows, *rest = self._rule_rows_plan(cu_host, what, hq, hkv, d, scale, rule, T, backward)
+            table = torch.empty(len(rows), 4, dtype=torch.int32, device=self.device)
+            if rows:
+                flat = array("i", itertools.chain.from_iterable(rows))
+                self._call("mtb200_write_ints", table.data_ptr(), flat.buffer_info()[0], len(flat), self._st(), n=-(-len(flat) // 1008))
+            return (table, *rest)
+        there = what + (self._st(),)
+        plan = self._cached(cu_host, there)
         if plan is None:
-            plan = self._make_rule_plan(cu_host, hq, hkv, d, scale, rule, T, backward, capturing)
-            if not capturing:
-                self._keep(cu_host, what, plan)
-            return plan
+            rows, *rest = self._rule_rows_plan(cu_host, what, hq, hkv, d, scale, rule, T, backward)
+            return self._keep(cu_host, there, (self._move_table(rows) if rows else None, *rest))
         if plan[1] > T:
             rule.check_starts(cu_host, T)
-        if capturing:
-            self._captured.append(plan[0])
         return plan
 
-    def _make_rule_plan(self, cu_host, hq, hkv, d, scale, rule, T, backward, capturing):
+    def _rule_rows_plan(self, cu_host, what, hq, hkv, d, scale, rule, T, backward):
+        """``_rule_plan`` with the table's rows on the host."""
+        plan = self._cached(cu_host, what)
+        if plan is None:
+            return self._keep(cu_host, what, self._make_rule_plan(cu_host, hq, hkv, d, scale, rule, T, backward))
+        if plan[1] > T:
+            rule.check_starts(cu_host, T)
+        return plan
+
+    def _make_rule_plan(self, cu_host, hq, hkv, d, scale, rule, T, backward):
         if d not in NATIVE_HEAD_DIMS:
             raise ValueError(f"attention under a rule runs on the kernels for head dimensions {NATIVE_HEAD_DIMS}, not {d}")
         if hkv < 1 or hq < 1 or hq % hkv:
@@ -688,16 +701,7 @@ class NativeOps:
                 items, tail = pairs or items, ("mtb200_attn_rule_fwd", ((hq // hkv) % 2,))
             else:
                 tail = ("mtb200_attn_rule_fwd_one", ())
-        rows = [it[1:] for it in items]
-        if not rows:
-            table = None
-        elif capturing:
-            host = torch.tensor(rows, dtype=torch.int32).pin_memory()
-            self._captured.append(host)
-            table = host.to(self.device, non_blocking=True)
-        else:
-            table = self._move_table(rows)
-        return (table, cu_host[-1], *tail)
+        return ([it[1:] for it in items], cu_host[-1], *tail)
 
     def _rule_rows(self, t, T, width):
         """Leading dimension of bf16 rows ``[T, width]`` on this backend's device, 16 bytes aligned; anything else is refused."""
