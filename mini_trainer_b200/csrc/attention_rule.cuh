@@ -71,8 +71,9 @@ __device__ __forceinline__ uint32_t att_queries_seen(const AttRuleArgs& r, int j
 //
 // The reference of the exponentials does not have to be the largest score, only near it and the same throughout. A cap is monotonic, so the largest product capped is
 // the largest capped score; a bias is not, but within 32 keys it changes by 31 slopes: the largest product of each 32, capped, with the bias of the nearer
-// end is a bound that is too high by at most that. Where capped scores are small, up to 2^+-30 as exponentials, their largest absolute value, which has to be known for the cap's
-// polynomial anyhow, is bound enough: 2^60 too high at most, which fp32 has room for. So the scores themselves are only formed on their way into the exponentials, which
+// end is near it, too high by at most that, or too low by the little that a cap is told by its slope (2^2.3, below). Where capped scores without a bias are small, up to 2^+-30 as exponentials,
+// their largest absolute value, which has to be known for the cap's polynomial anyhow, is bound enough: 2^60 too high at most, which leaves the smallest probability that counts beside the
+// largest, 2^-24 of it, at 2^-84, 42 bits above fp32's last. With a bias the largest product is taken with its sign: 2^60 and the 2^40 of a bias together left nothing. So the scores themselves are only formed on their way into the exponentials, which
 // keeps the FMA pipe and the special-function unit busy at once; formed in place first, capped scores took 286 us where they take 232 (8192 tokens in three samples,
 // 32/8 heads of 128; 192 without a cap). They are formed in place, and their largest taken, where this does not hold (`formed`):
 // products beyond the cap, slopes so steep that the bound could be 2^40 too high for them alone, and biased keys on the diagonal.
@@ -190,7 +191,7 @@ struct AttScores {
           if (!sees(c, i)) sv[c][i] = 0xff800000u;   // -inf
       }
     }
-    if (R::CAP && !EDGE && low) {
+    if (R::CAP && !R::BIAS && !EDGE && low) {
 #pragma unroll
       for (int c = 0; c < C; ++c) mc[c] = big[c];
     } else {
@@ -207,7 +208,7 @@ struct AttScores {
       }
     }
     if constexpr (R::BIAS) {
-      if (R::CAP && low) {   // of scores within half of the cap what they are uncapped is bound enough, 2^2.8 too high at most (exactly 284 us where it takes 269)
+      if (R::CAP && low) {   // of scores within half of the cap what they are uncapped is near enough: 2^2.3 too high at most, or too low where all are negative (exactly 284 us where it takes 269)
 #pragma unroll
         for (int c = 0; c < C; ++c) mc[c] *= r.cap.b[0].x;
       } else if (R::CAP) {
