@@ -27,7 +27,9 @@
 // 128B-swizzled so the staging stores are free of bank conflicts); a small kernel rounds the accumulator to bf16 afterwards.
 // Four warps of their own drain, one more issues the reduces, so the softmax warps see nothing of dQ.
 //
-// Rows past the end of the sequence contribute nothing: a query's lse is staged as +infinity, a key's dS is zero.
+// Rows past the end of the sequence contribute nothing: a query's lse is staged as +infinity, a key's dS is zero. That holds for finite numbers; under a rule also for others, which
+// stay in their sample: the next sample's rows of Q, dO and K in a tile at this one's end, met by zeros, and what this sample's own K adds to the next one's rows of dQ. The first kernel looks
+// for them (AttLook); where there are any, the TMA warp zeroes those rows before the tile counts as landed, and dQ of rows that are not there leaves as zeros.
 //
 // With short samples a CTA has few iterations, and its first loads and its stores count: the loads go out before tensor memory is allocated, and dK and dV
 // leave by tensor stores. 148 samples of 128 tokens, 16/4 heads: 106 -> 102 us at D = 64, 193 -> 182 at 128 (all passes); 37 of 1024 492 -> 482, 879 -> 871.
@@ -125,9 +127,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
   uint64_t* all_done = bars + 19;    // dK and dV complete
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  [[maybe_unused]] uint64_t* tail_full = bars + 21;   // a tile whose last rows are to be zeroed landed
 
   pdl_wait();   // the work table comes first
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  bool careful = false;
+  if constexpr (R::ON) careful = *static_cast<const volatile unsigned long long*>(p.r.odd) >= p.r.number;
   int unit = blockIdx.x, sub = 0, splits = p.splits, shared = 0;   // `shared`: the unit's number among those that CTAs share
   if constexpr (R::ON) {
     if (unit < p.r.whole) splits = 1;
@@ -167,17 +172,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
     mbar_init(stage_full, 4); mbar_init(stage_free, 1); mbar_init(all_done, 1);
     for (int b = 0; b < 2; ++b) { mbar_init(&q_full[b], 1); mbar_init(&q_free[b], 1); mbar_init(&stat_full[b], 1); mbar_init(&stat_free[b], 8); }
     *abort_flag = 0;
+    if constexpr (R::ON) mbar_init(tail_full, 1);
     fence_mbar_init();
-    // the first loads go out before anything else is set up
-    mbar_arrive_expect_tx(kv_full, 2 * L::TILE);
-    mbar_arrive_expect_tx(&q_full[0], L::TILE);
-    mbar_arrive_expect_tx(do_full, L::TILE);
+    if (!careful) {   // the first loads go out before anything else is set up
+      mbar_arrive_expect_tx(kv_full, 2 * L::TILE);
+      mbar_arrive_expect_tx(&q_full[0], L::TILE);
+      mbar_arrive_expect_tx(do_full, L::TILE);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      tma_load_2d(smem + L::OFF_K + kb * 16384, &tm_qkv, kv_full, (p.Hq + hk) * D + kb * 64, seq_start + k0);
-      tma_load_2d(smem + L::OFF_Q + kb * 16384, &tm_qkv, &q_full[0], h_first * D + kb * 64, seq_start + jblk * AB_B);
-      tma_load_2d(smem + L::OFF_V + kb * 16384, &tm_qkv, kv_full, (p.Hq + p.Hkv + hk) * D + kb * 64, seq_start + k0);
-      tma_load_2d(smem + L::OFF_DO + kb * 16384, &tm_do, do_full, h_first * D + kb * 64, seq_start + jblk * AB_B);
+      for (int kb = 0; kb < KB; ++kb) {
+        tma_load_2d(smem + L::OFF_K + kb * 16384, &tm_qkv, kv_full, (p.Hq + hk) * D + kb * 64, seq_start + k0);
+        tma_load_2d(smem + L::OFF_Q + kb * 16384, &tm_qkv, &q_full[0], h_first * D + kb * 64, seq_start + jblk * AB_B);
+        tma_load_2d(smem + L::OFF_V + kb * 16384, &tm_qkv, kv_full, (p.Hq + p.Hkv + hk) * D + kb * 64, seq_start + k0);
+        tma_load_2d(smem + L::OFF_DO + kb * 16384, &tm_do, do_full, h_first * D + kb * 64, seq_start + jblk * AB_B);
+      }
     }
     tma_prefetch_desc(&tm_dq);
     tma_prefetch_desc(&tm_dkv);
@@ -196,7 +203,48 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
     setmaxnreg_dec<AB_REGS_IO>();
     if (warp == 0) {
       // ------------------------------------------------------------------ TMA producer
-      if (elect_one()) {
+      if (R::ON && careful) {
+        if (elect_one()) {
+          uint32_t tails = 0;
+          auto request = [&](uint8_t* tile, const CUtensorMap* map, uint64_t* bar, int column, int first) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) tma_load_2d(tile + kb * 16384, map, bar, column + kb * 64, seq_start + first);
+          };
+          // the tile from row `first` on, landed and the rows behind the sequence zeroed
+          auto tail = [&](uint8_t* tile, const CUtensorMap* map, int column, int first) -> bool {
+            mbar_arrive_expect_tx(tail_full, L::TILE);
+            request(tile, map, tail_full, column, first);
+            if (!mbar_wait(tail_full, tails++ & 1, abort_flag)) return false;
+            zero_rows<KB>(tile, seq_len - first, 0, 1);
+            return true;
+          };
+          auto load = [&](uint8_t* tile, const CUtensorMap* map, uint64_t* full, int column, int first) -> bool {
+            if (first + AB_B > seq_len) {
+              if (!tail(tile, map, column, first)) return false;
+              mbar_arrive(full);
+              return true;
+            }
+            mbar_arrive_expect_tx(full, L::TILE);
+            request(tile, map, full, column, first);
+            return true;
+          };
+          const bool k_tail = k0 + AB_B > seq_len;   // K and V share a barrier: the arrival comes with V's bytes
+          if (k_tail && !tail(smem + L::OFF_K, &tm_qkv, (p.Hq + hk) * D, k0)) { atomicExch(p.status, 21); goto done; }
+          mbar_arrive_expect_tx(kv_full, k_tail ? L::TILE : 2 * L::TILE);
+          if (!k_tail) request(smem + L::OFF_K, &tm_qkv, kv_full, (p.Hq + hk) * D, k0);
+          request(smem + L::OFF_V, &tm_qkv, kv_full, (p.Hq + p.Hkv + hk) * D, k0);
+          int h = h_first, i = jblk;
+          for (int it = 0; it < n_iters; ++it) {
+            const int b = it & 1;
+            if (it > 1 && !mbar_wait(&q_free[b], ((it - 2) >> 1) & 1, abort_flag)) { atomicExch(p.status, 21); goto done; }
+            if (!load(smem + L::OFF_Q + b * L::TILE, &tm_qkv, &q_full[b], h * D, i * AB_B)) { atomicExch(p.status, 21); goto done; }
+            if (it > 0 && !mbar_wait(do_free, (it - 1) & 1, abort_flag)) { atomicExch(p.status, 21); goto done; }
+            if (!load(smem + L::OFF_DO, &tm_do, do_full, h * D, i * AB_B)) { atomicExch(p.status, 21); goto done; }
+            if (++i == nq) { i = jblk; ++h; }
+          }
+          pdl_trigger();
+        }
+      } else if (elect_one()) {
         int h = h_first, i = jblk;
         if (++i == nq) { i = jblk; ++h; }
         for (int it = 1; it < n_iters; ++it) {   // the first iteration's tiles have been asked for above
@@ -347,6 +395,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
     const uint32_t src = t_dq + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     uint8_t* rowp = smem + L::OFF_ST + r * 128;
     int n = 0;
+    [[maybe_unused]] int i = jblk;
     for (int it = 0; it < n_iters; ++it) {
       if (!mbar_wait(dq_full, it & 1, abort_flag)) { atomicExch(p.status, 28); goto done; }
       tc_fence_after();
@@ -361,6 +410,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
           __syncwarp();
           if (lane == 0) mbar_arrive(dq_read);
         }
+        if constexpr (R::ON) {
+          if (careful && i * AB_B + r >= seq_len) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[0][x] = v[1][x] = 0u;
+          }
+        }
         if (n > 0 && !mbar_wait(stage_free, (n - 1) & 1, abort_flag)) { atomicExch(p.status, 31); goto done; }
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -371,6 +426,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(stage_full);
       }
+      if constexpr (R::ON) { if (++i == nq) i = jblk; }
     }
   } else {
     // ------------------------------------------------------------------ softmax (two threads per key row)
@@ -619,17 +675,66 @@ done:
   }
 }
 
+// Under a rule the first kernel also looks for what is not finite where samples share a tile. A row of dO, O, V or Q shows in its delta, as O is not finite with them, but for infinities of Q under
+// a cap, which bounds the scores they make; a row of K need not show (its score may be -infinity). So K is read along, and with a cap the rows of Q behind a sample's end that share a tile with
+// it, by blocks of their own: LOOK_BLOCKS to a row of the work table (a key block of 128), a warp to two rows.
+// 8192 tokens in three samples, 32/8 heads of 128, capped: the first kernel 42.8 -> 47.1 us (of 655), 41 short samples at D = 64 without a cap 17.0 -> 18.5 (of 148), 148 samples of about 100 tokens, 16/4 heads of
+// 128, capped, where those rows are most of Q, 39 -> 49 (of 242); the kernel that works on the tiles is as fast as it was. Zeroing every such row instead took 7 to 15 % of the whole, seeing them in the products 3 to 10 %.
+constexpr int LOOK_BLOCKS = 8;
+struct AttLook {
+  static constexpr bool ON = true;
+  const __nv_bfloat16* qkv;
+  long long ld;
+  const int* plan;
+  int G, blocks;   // blocks: the first of the launch, for Q (none without a cap)
+  unsigned long long *odd, number;
+  __device__ __forceinline__ void report(bool bad) const { if (bad) atomicMax(odd, number); }
+};
+struct AttNoLook { static constexpr bool ON = false; };
+// Zero of a finite 16 bytes, NaN of others.
+__device__ __forceinline__ float2 att_times_zero(const uint4& u, float2 z) {
+  const float2 none = make_float2(0.f, 0.f);
+  z = ffma2(unpack_bf16(u.x), none, z); z = ffma2(unpack_bf16(u.y), none, z); z = ffma2(unpack_bf16(u.z), none, z);
+  return ffma2(unpack_bf16(u.w), none, z);
+}
+__device__ __forceinline__ void att_look_behind(const AttLook& a, int n, int HqD) {
+  const int b = blockIdx.x, item = b / LOOK_BLOCKS;
+  const int seq_start = a.plan[item * 4], seq_len = a.plan[item * 4 + 1], k0 = a.plan[item * 4 + 2];
+  if (seq_start < 0 || seq_len <= 0 || k0 < 0 || k0 >= seq_len || static_cast<long long>(seq_start) + seq_len > n) return;   // reported by the kernel that works on it
+  const int r0 = k0 + (b % LOOK_BLOCKS) * 16 + static_cast<int>(threadIdx.x >> 5) * 2;
+  if (r0 + 1 < seq_len) return;
+  float2 z = make_float2(0.f, 0.f);
+  for (int c = static_cast<int>(threadIdx.x & 31) * 8; c < HqD; c += 2 * 256) {
+    uint4 u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + (k & 1), x = c + (k >> 1) * 256;
+      u[k] = r >= seq_len && seq_start + r < n && x < HqD ? *reinterpret_cast<const uint4*>(a.qkv + static_cast<long long>(seq_start + r) * a.ld + x) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) z = att_times_zero(u[k], z);
+  }
+  a.report(!(z.x + z.y == 0.f));
+}
+
 // delta[h, t] = sum_d dO[t, h, d] * O[t, h, d], and zeros into the dQ accumulator, for the first n of T rows; D / 8 lanes per (t, h), one 16-byte load of each operand per
 // lane and row, two rows in flight. Bound by reading dO and O and writing the accumulator once (as a launch of its own the zeroing
 // took 9 us next to 14 us for 12 345 tokens x 16 heads of 64, forward and backward together 177 us, now 168).
-static __global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloat16* __restrict__ o, long long ldo, const __nv_bfloat16* __restrict__ dout,
-                                                        long long lddo, float* __restrict__ delta, float* __restrict__ dq_acc, int T, int n, int Hq, int D) {
+template <class Look>
+static __global__ void __launch_bounds__(256, Look::ON ? 6 : 0) attn_delta_kernel(const __nv_bfloat16* __restrict__ o, long long ldo, const __nv_bfloat16* __restrict__ dout,
+                                                        long long lddo, float* __restrict__ delta, float* __restrict__ dq_acc, int T, int n, int Hq, int D, [[maybe_unused]] Look look) {
   pdl_trigger();
   pdl_wait();
+  if constexpr (Look::ON) {
+    if (static_cast<int>(blockIdx.x) < look.blocks) { att_look_behind(look, n, Hq * D); return; }
+  }
+  int look_blocks = 0;
+  if constexpr (Look::ON) look_blocks = look.blocks;
   const int lanes = D >> 3;   // 8 or 16: a power of two that divides the warp
   const int per_block = 256 / lanes, sub = threadIdx.x / lanes, c = (threadIdx.x & (lanes - 1)) * 8;
-  const long long rows = static_cast<long long>(n) * Hq, first = static_cast<long long>(blockIdx.x) * 2 * per_block + sub;
+  const long long rows = static_cast<long long>(n) * Hq, first = static_cast<long long>(static_cast<int>(blockIdx.x) - look_blocks) * 2 * per_block + sub;
   uint4 a[2], b[2];
+  [[maybe_unused]] uint4 kv[2];
   int t[2], h[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -640,6 +745,11 @@ static __global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloa
     if (row < rows) {
       a[k] = *reinterpret_cast<const uint4*>(o + static_cast<long long>(t[k]) * ldo + h[k] * D + c);
       b[k] = *reinterpret_cast<const uint4*>(dout + static_cast<long long>(t[k]) * lddo + h[k] * D + c);
+    }
+    if constexpr (Look::ON) {
+      kv[k] = make_uint4(0u, 0u, 0u, 0u);
+      const int head = h[k] / look.G;
+      if (row < rows && head * look.G == h[k]) kv[k] = *reinterpret_cast<const uint4*>(look.qkv + static_cast<long long>(t[k]) * look.ld + (Hq + head) * D + c);
     }
   }
 #pragma unroll
@@ -655,6 +765,10 @@ static __global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloa
     for (int m = lanes >> 1; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
     if (row < rows) {
       if (c == 0) delta[static_cast<long long>(h[k]) * T + t[k]] = s;
+      if constexpr (Look::ON) {
+        const float2 z = att_times_zero(kv[k], make_float2(0.f, 0.f));
+        look.report(!(fabsf(s) <= 3.4e38f && z.x + z.y == 0.f));
+      }
       float4* z = reinterpret_cast<float4*>(dq_acc + row * D + c);
       z[0] = z[1] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -715,8 +829,16 @@ static int bwd(const void* qkv, long long ld, const void* out, long long ldo, co
   rc = make_tmap_2d_bf16(&tdkv, p.dqkv, (static_cast<uint64_t>(Hq) + 2 * Hkv) * D, static_cast<uint64_t>(T), static_cast<uint64_t>(p.ldq), 64, 32);
   if (rc) return rc - 30;
   const int per_block = 2 * 256 / (D / 8);
-  launch_pdl(attn_delta_kernel, static_cast<unsigned>((static_cast<long long>(rows) * Hq + per_block - 1) / per_block), 256, 0, st,
-      reinterpret_cast<const __nv_bfloat16*>(out), ldo, reinterpret_cast<const __nv_bfloat16*>(dout), lddo, delta, p.dq_acc, T, rows, Hq, D);
+  const long long blocks = (static_cast<long long>(rows) * Hq + per_block - 1) / per_block;
+  const __nv_bfloat16 *o = reinterpret_cast<const __nv_bfloat16*>(out), *d_o = reinterpret_cast<const __nv_bfloat16*>(dout);
+  if constexpr (R::ON) {
+    const long long behind = R::CAP ? static_cast<long long>(n_items) * LOOK_BLOCKS : 0;
+    if (blocks + behind >= 1ll << 31) return -10;
+    const AttLook look{reinterpret_cast<const __nv_bfloat16*>(qkv), ld, p.plan, Hq / Hkv, static_cast<int>(behind), p.r.odd, p.r.number};
+    launch_pdl(attn_delta_kernel<AttLook>, static_cast<unsigned>(blocks + behind), 256, 0, st, o, ldo, d_o, lddo, delta, p.dq_acc, T, rows, Hq, D, look);
+  } else {
+    launch_pdl(attn_delta_kernel<AttNoLook>, static_cast<unsigned>(blocks), 256, 0, st, o, ldo, d_o, lddo, delta, p.dq_acc, T, rows, Hq, D, AttNoLook{});
+  }
   rc = D == 128 ? launch_bwd<128, R>(tq, tdo, tdq, tdkv, p, n_items, in_order, st) : launch_bwd<64, R>(tq, tdo, tdq, tdkv, p, n_items, in_order, st);
   if (rc) return rc;
   launch_pdl(attn_dq_store_kernel, dim3(static_cast<unsigned>(rows), (Hq * D / 8 + 255) / 256), 256, 0, st, p.dq_acc, p.dqkv, p.ldq, rows, Hq * D);

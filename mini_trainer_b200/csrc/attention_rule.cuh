@@ -24,6 +24,10 @@ struct AttRuleArgs {
   int window;            // keys a query sees, itself among them; 1 << 30 for all
   const float* slopes;   // [Hq]
   int whole;             // backward: key blocks times kv heads, from the first on, that have one CTA each; only those behind them are shared by p.splits
+  // Backward: *odd is `number` or more where something of this launch's batch is not finite that samples share a tile with (numbers grow from launch to launch, so nothing has to be reset; a
+  // number that an overlapping launch left there costs time and nothing else).
+  unsigned long long* odd;
+  unsigned long long number;
   CapArgs cap;           // of raw products
 };
 
@@ -80,8 +84,8 @@ __device__ __forceinline__ uint32_t att_queries_seen(const AttRuleArgs& r, int j
 constexpr float ATT_STEEP = 40.f / 31.f;
 // Rows [first, 128) of a [128, 64 KB] tile in shared memory (128B swizzle: a row's bytes stay together) set to zero by `n` threads, for reads by the tensor core behind
 // the caller's next arrival. A tile at a sample's end holds rows of the next sample, which meet probabilities and gradients of zero; a product
-// with zero is only zero for finite numbers, and one sample's infinities are not another's. (The forward takes the same time with it. The backward has no such rows zeroed: it took 7 to 15 % of its
-// time, and the gradient of the weights is the batch's whatever its samples keep to themselves.)
+// with zero is only zero for finite numbers, and one sample's infinities are not another's. The forward takes the same time with it. The backward, which has three such tiles and more to do to them, took
+// 7 to 15 % longer with every one's rows zeroed, so it looks for numbers that are not finite beforehand (AttLook of attention_bwd.cuh) and only takes the trouble when there are any.
 template <int KB>
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int first, int thread, int n) {
 #pragma unroll

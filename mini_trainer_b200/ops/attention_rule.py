@@ -9,7 +9,7 @@
 * ``prefix``  one length per sample: all tokens of the sample see its first ``prefix`` keys, whatever the window and on either side of them
 
 so that ``i`` sees ``j`` of its own sample iff ``(j <= i and i - j < window) or j < prefix``. The diagonal is always seen: no row is empty, whatever the rule.
-What is not finite in one sample stays there in the forward. In the backward it reaches gradients of the samples beside it, in tiles of 128 rows that hold both.
+What is not finite in one sample stays there, in outputs and gradients.
 A window without keys, negative prefixes and ones longer than their sample are refused.
 """
 from __future__ import annotations

@@ -110,7 +110,7 @@ class _Sig:
     mtb200_attn_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, F, P, P]
     mtb200_attn_rule_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, I, F, F, I, P, P, P]
     mtb200_attn_rule_fwd_one = [P, L, P, L, P, P, I, I, I, I, I, I, F, F, I, P, P, P]
-    mtb200_attn_rule_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, I, P, U, P, L, F, F, I, P, I, I, P, P]
+    mtb200_attn_rule_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, I, P, U, P, L, F, F, I, P, I, I, P, U, P, P]
     mtb200_attn_bwd = [P, L, P, L, P, L, P, L, P, P, P, P, I, I, I, I, I, I, P, U, P, L, F, I, P, P]
 
 
@@ -167,6 +167,7 @@ def route_topk(logits, k: int, renorm: bool, call=_launch):
 
 class NativeOps:
     name = "native"
+    _odd = None   # on the device, number of the last backward under a rule that met something not finite
 
     def __init__(self, device, ce_chunk: int = 8192, attention: str | None = None):
         self.device = torch.device(device)
@@ -184,6 +185,7 @@ class NativeOps:
         # less (gemm_plan.wide), or single CTAs. MTB200_GEMM2=0 / 1 forces one kernel for all of them (1: also for the fused gathers).
         self.use_gemm2 = os.environ.get("MTB200_GEMM2") == "1"
         self.pair_max_flops = 0.0 if os.environ.get("MTB200_GEMM2") == "0" else 1e12
+        self._odd = torch.zeros(1, dtype=torch.int64, device=self.device)
         self.launches = 0
         self.profile = [] if os.environ.get("MTB200_PROFILE") else None
         self._scratch = {}
@@ -751,7 +753,7 @@ class NativeOps:
         ws, epoch, part = split or (None, 0, None)
         self._call("mtb200_attn_rule_bwd", qkv.data_ptr(), ld, out.data_ptr(), ldo, dout.data_ptr(), lddo, dqkv.data_ptr(), qkv.shape[1], lse.data_ptr(),
                    dq_acc + 4 * hq * T * d, dq_acc, table.data_ptr(), table.shape[0], T, rows, hq, hkv, d, splits if split else 1, _ptr(ws), epoch, _ptr(part),
-                   4 * part.numel() if split else 0, scale, rule.key[0], rule.key[1], _ptr(rule.slopes), in_order, whole, self.status.data_ptr(), st, n=3, tag="mtb200_attn_bwd")
+                   4 * part.numel() if split else 0, scale, rule.key[0], rule.key[1], _ptr(rule.slopes), in_order, whole, _ptr(self._odd), next(self._epoch), self.status.data_ptr(), st, n=3, tag="mtb200_attn_bwd")
         return dqkv
 
     def attention(self, qkv, cu_seqlens, cu_host, max_seqlen, hq, hkv, d, scale=None, rule=None):
