@@ -133,18 +133,21 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   bool careful = false;
   if constexpr (R::ON) careful = *static_cast<const volatile unsigned long long*>(p.r.odd) >= p.r.number;
-  int unit = blockIdx.x, sub = 0, splits = p.splits, shared = 0;   // `shared`: the unit's number among those that CTAs share
+  // units: the first r.whole have a CTA each, p.splits share those behind them, of which `shared` is the number
+  int unit, sub, shared, own_splits = 1;
   if constexpr (R::ON) {
-    if (unit < p.r.whole) splits = 1;
-    else if (splits > 1) {
-      shared = (unit - p.r.whole) / splits;
-      sub = unit - p.r.whole - shared * splits;
+    unit = blockIdx.x; sub = shared = 0;
+    if (unit >= p.r.whole && p.splits > 1) {
+      own_splits = p.splits;
+      shared = (unit - p.r.whole) / p.splits;
+      sub = unit - p.r.whole - shared * p.splits;
       unit = p.r.whole + shared;
     }
-  } else if (splits > 1) {
-    unit = shared = blockIdx.x / splits;
-    sub = blockIdx.x - unit * splits;
+  } else {
+    unit = shared = p.splits == 1 ? blockIdx.x : blockIdx.x / p.splits;
+    sub = blockIdx.x - unit * p.splits;
   }
+  const int splits = R::ON ? own_splits : p.splits;
   int item = static_cast<int>(__umulhi(static_cast<unsigned>(unit), p.hkv_inv));   // unit / Hkv, or one less
   if (unit - item * p.Hkv >= p.Hkv) ++item;
   const int hk = unit - item * p.Hkv;
