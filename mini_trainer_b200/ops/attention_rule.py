@@ -14,12 +14,20 @@ A window without keys, negative prefixes and ones longer than their sample are r
 """
 from __future__ import annotations
 
+import operator
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import torch
 
 _NO_WINDOW = 1 << 30
+
+
+def _whole(x, what: str) -> int:
+    try:
+        return int(x) if isinstance(x, float) and x.is_integer() else operator.index(x)
+    except TypeError:
+        raise ValueError(f"{what} counts tokens, {x!r} does not") from None
 
 
 @dataclass(frozen=True)
@@ -32,11 +40,12 @@ class AttentionRule:
     def __post_init__(self):
         if self.cap is not None and not 0.0 < float(self.cap) < float("inf"):
             raise ValueError(f"a score cap is a positive number, not {self.cap}")
-        if self.window is not None and int(self.window) < 1:
-            raise ValueError(f"a window has at least the query itself, one key, not {self.window}")
         own = object.__setattr__
-        own(self, "prefix", None if self.prefix is None else tuple(int(x) for x in self.prefix))
-        own(self, "keys", _NO_WINDOW if self.window is None else min(int(self.window), _NO_WINDOW))   # of the window; beyond any sample where there is none
+        own(self, "window", None if self.window is None else _whole(self.window, "a window"))
+        if self.window is not None and self.window < 1:
+            raise ValueError(f"a window has at least the query itself, one key, not {self.window}")
+        own(self, "prefix", None if self.prefix is None else tuple(_whole(x, "a prefix") for x in self.prefix))
+        own(self, "keys", _NO_WINDOW if self.window is None else min(self.window, _NO_WINDOW))   # of the window; beyond any sample where there is none
         own(self, "key", (0.0 if self.cap is None else float(self.cap), 0 if self.window is None else self.keys, self.prefix))   # what a plan depends on
 
     def prefixes(self, cu_host) -> list:

@@ -51,3 +51,21 @@ def test_small_values_under_scores_that_are_all_negative(ops, bias, cap, score, 
         assert torch.equal(l2, l) and torch.equal(o2.double() * 2.0 ** (70 if bias else 40), o.double())
     ops._attn_plan_cache.clear()
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------------ CPU
+@pytest.mark.parametrize("bad", [2.7, float("inf"), "3", torch.tensor(2.5), [4]])
+def test_windows_and_prefixes_count_tokens(bad):
+    """A part of a token was cut off without a word."""
+    with pytest.raises(ValueError, match="counts tokens"):
+        AttentionRule(window=bad)
+    with pytest.raises(ValueError, match="counts tokens"):
+        AttentionRule(prefix=[1, bad])
+
+
+def test_whole_numbers_of_any_kind_are_taken():
+    import numpy
+    for k in (5, 5.0, numpy.int32(5), torch.tensor(5)):
+        rule = AttentionRule(window=k, prefix=torch.tensor([5, 0]) if torch.is_tensor(k) else [k, 0])
+        assert rule.window == rule.keys == 5 and rule.prefix == (5, 0) and rule.key == AttentionRule(window=5, prefix=(5, 0)).key
+    assert AttentionRule(window=1 << 40).keys == 1 << 30
