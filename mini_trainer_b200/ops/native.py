@@ -402,6 +402,8 @@ class NativeOps:
         shape, index, bf = y.shape, y.get_device(), torch.bfloat16
         if len(shape) != 2 or shape[1] < 8 or shape[1] & 7 or shape[1] > 8192:
             raise ValueError(f"rows of a multiple of 8 up to 8192 elements, not {tuple(shape)}")
+        if shape[0] >= 1 << 31:
+            raise ValueError(f"{shape[0]} rows are more than the kernels count")
         if index != self._index and self._index is not None:
             raise ValueError(f"this backend was made for {self.device}, the activations are on {y.device}")
         bits = 0
@@ -452,6 +454,8 @@ class NativeOps:
         T, H = self._residual_norm_check(y, (y, h, dh, dz), (w_post, w_pre, dw_post_out, dw_pre_out), (gate, ry, rh))
         if dh is None and w_pre is None:
             raise ValueError("without a gradient of h or z there is nothing to do")
+        if w_post is not None and w_pre is not None and abs(dw_post_out.data_ptr() - dw_pre_out.data_ptr()) < 2 * H:
+            raise ValueError("the weights' gradients go to memory of their own")
         dx, dy = torch.empty_like(y), torch.empty_like(y)
         dgate = None if gate is None else torch.empty(T, dtype=torch.float32, device=y.device)
         if T == 0:
