@@ -7,7 +7,7 @@ Two shared objects are produced under ``mini_trainer_b200/_native``:
   (``-gencode arch=compute_100a,code=sm_100a``). nvcc cross-compiles without a GPU.
 
 Both expose a plain C ABI and are loaded with ``ctypes``; nothing here needs the torch C++
-headers, so a full rebuild takes seconds rather than minutes.
+headers, so a full rebuild takes about a minute.
 
 Run ``python -m mini_trainer_b200.build`` to (re)build; ``build_all()`` is incremental (it
 compares source and header mtimes with the output's).

@@ -3,15 +3,20 @@
 //   s  -> cap tanh(s / cap)                        (CAP)
 //   s  -> s - slope[head] |i - j|                  (BIAS; i, j: positions of query and key in their sample)
 //   query i sees key j  iff  (j <= i and i - j < window) or j < prefix         (the diagonal is always seen: no row is empty)
-// The kernels are instances of the same templates as the plain causal ones; NoRule compiles to what those were. Masks need no parameter of the
-// template: which tiles exist, and which of them are crossed by an edge of the mask, is found per tile.
-// The cap is in cap.cuh.
+// The kernels are instances of the same templates as the plain causal ones, whose own instances (NoRule) have the registers and, to 1 %, the times they had before. Masks need no parameter of
+// the template: which tiles exist, and which of them are crossed by an edge of the mask, is found per tile. The cap is in cap.cuh.
+//
+// P and, in the backward, dS are rounded to bf16 as operands of their products, as in the causal kernels: operands of 32 bits (tf32) have half the rate and twice the tensor memory, which is
+// full. That is what the gradients are off by (2.8e-3 of their norm against 64 bits, where fp32 rounded once is off by 1.7e-3); statistics, scores and accumulators are fp32.
 //
 // Bound as the plain causal kernels are, by the chain of hand-offs between the softmax warps and the tensor core, and then by what the softmax warps have to do to a
 // score: a cap adds five to seven packed instructions a pair, and the reference's comparisons of absolute values, a bias three. 8192 tokens in three samples, 32/8 heads of 128
-// (188 GFLOP forward, 471 backward): forward 192 us under a rule without either as in the plain causal kernel, 232 capped, 210 biased, 269 both; backward 583, 611, 574, 609.
-// The tensor core is busy for 57, 45, 50 and about 37 % of the forward's cycles, issue slots for 44, 42, 48 and 42 %: no pipe is full, a row's instructions depend on each other.
-// Windows and prefixes cost what their tiles do: one sample of 8192 tokens with a window of 1024 takes 0.69 ms both ways, without one 1.8.
+// (188 GFLOP forward, 471 backward), scores with a standard deviation of 1 and of 3, a cap of 50, us:
+//   forward   causal kernel 183, 204   a rule without either 193, 215   cap 237, 256   bias 213, 225   both 274, 283
+//   backward                583, 586                         588, 591       619, 622        579, 583        614, 618
+// Scores that fill the cap (16; one in five hundred is beyond it, so nearly every tile has some) and that pass it (60): forward capped 458, 420, both 630, 626; backward 695, 695, both 705, 706.
+// At a deviation of 1 the tensor core is busy for 57, 45, 50 and about 37 % of the forward's cycles, issue slots for 44, 42, 48 and 42 %: no pipe is full, a row's instructions depend on each other.
+// Windows and prefixes cost what their tiles do: one sample of 8192 tokens with a window of 1024 takes 0.63 ms both ways, without one 1.9.
 #pragma once
 #include <stdint.h>
 

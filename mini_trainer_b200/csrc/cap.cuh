@@ -1,8 +1,9 @@
 // Numbers capped by a tanh, unit tanh(scale s / cap): attention wants them in units of log2 e, as its exponentials do (unit = cap log2 e), the head as a part of the cap (1).
 //
-// Up to the cap (|scale s| <= cap; bigger ones are rare) an odd polynomial of degree eleven, fitted to the least relative error on [-1, 1] (5.1e-7), with the powers of
-// scale / cap in its coefficients: seven packed instructions for two numbers; up to half of it one of degree seven on [-1/2, 1/2] (5.4e-7), five. Beyond the cap tanh as 1 - 2 / (1 + e^2x), two operations on the special-function
-// unit each, whose error is 2^-22 of the cap: a softmax that is bound by that unit as it is would do three times the work there.
+// Up to the cap (|scale s| <= cap) an odd polynomial of degree eleven on [-1, 1], 6.8e-7 off at most, with the powers of scale / cap in its coefficients: seven packed
+// instructions for two numbers; up to half of it one of degree seven on [-1/2, 1/2] (5.7e-7), five. Beyond the cap tanh as 1 - 2 / (1 + e^2x), two operations on the special-function
+// unit each, whose error is 2^-22 of the cap: a softmax that is bound by that unit as it is would do three times the work there. A tile in which one score is beyond the cap takes that form
+// throughout, so batches whose scores fill the cap take it nearly everywhere (attention_rule.cuh has the times).
 #pragma once
 #include <stdint.h>
 

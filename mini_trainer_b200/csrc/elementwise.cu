@@ -495,10 +495,10 @@ __global__ void __launch_bounds__(EW_THREADS, BULK ? (VPT <= 2 ? 3 : 2) : 1) res
 //   partial rows of dw_post += b dx yhat and dw_pre += dz hhat, per block, behind each other
 // dx stays in fp32 between its two uses. The second reduction is the gate's gradient and the norm's correction at once. Rows arrive by bulk copies as in
 // norm_bwd_kernel, up to four of them (dh, dz, h, y) to a stage; two barriers a row. Bound by reading them and writing dx and dy, 12 bytes an element:
-// 16384 x 4096 in 131 us with the sum of the partial rows, 40000 x 1536 in 119, 6.2 TB/s both (0.95 of the copy rate); 5987 x 1536 in 27 (17 at that rate), as each block has eight rows and
-// the start, the end and the partial rows are a third of it. The next launch is let in when a block's rows are done: let in at the start, the blocks of the sum held their places
-// on SMs from blocks of this kernel (5987 x 1536 34 -> 27 us, 40000 x 1536 161 -> 119, both with the sum's loads under way at once). Tried: the rows of an SM in one block with one partial row (33 -> 31 us
-// then, but 16384 x 4096 130 -> 187: registers), a copy's request by each warp in turn (33 -> 35).
+// 16384 x 4096 in 133 us with the sum of the partial rows, 40000 x 1536 in 120, 6.1 TB/s both (0.93 of the copy rate; in a long row of them, at a lower clock, 134 to 141); 5987 x 1536 in 27 (17
+// at that rate), as each block has eight rows and the start, the end and the partial rows are a third of it. The next launch is let in when a block's rows are done: let in at the start, the
+// blocks of the sum held their places on SMs from blocks of this kernel (5987 x 1536 34 us, 40000 x 1536 161). The rows of an SM in one block with one partial row took 187 us for
+// 16384 x 4096 (registers).
 constexpr int rn_threads(int vpt) { return vpt == 1 ? 768 : 512; }   // an SM's, and a block's at most
 template <int VPT, bool POST, bool PRE>
 __global__ void __launch_bounds__(rn_threads(VPT)) residual_norm_bwd_kernel(const __nv_bfloat16* __restrict__ dh, const __nv_bfloat16* __restrict__ dz,
