@@ -30,7 +30,7 @@ struct AttRuleArgs {
   const float* slopes;   // [Hq]
   int whole;             // backward: key blocks times kv heads, from the first on, that have one CTA each; only those behind them are shared by p.splits
   // Backward: *odd is `number` or more where something of this launch's batch is not finite that samples share a tile with (numbers grow from launch to launch, so nothing has to be reset; a
-  // number that an overlapping launch left there costs time and nothing else).
+  // number that an overlapping launch left there costs time and nothing else; so does that of any launch behind a captured one, whose replays keep the number they were captured with).
   unsigned long long* odd;
   unsigned long long number;
   CapArgs cap;           // of raw products
