@@ -8,6 +8,7 @@ there is no silent fallback to PyTorch on a GPU machine.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import itertools
 import os
@@ -19,7 +20,7 @@ import torch
 
 from .. import build as _build
 from ..utils import nvtx
-from . import attention_plan, block_exec, gemm_plan, step_exec
+from . import attention_plan, block_exec, gemm_plan, router_balance, step_exec
 
 _LIB = None
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
@@ -106,6 +107,9 @@ class _Sig:
     mtb200_moe_glu_bwd = [P, P, P, P, P, I, I, I, I, P, P, P]
     mtb200_moe_combine = [P, P, P, P, P, F, I, I, I, P, P]
     mtb200_moe_route_bwd = [P, P, P, P, I, I, I, I, P, P]
+    mtb200_route_balanced_rows = [I, I]
+    mtb200_route_balanced = [P, I, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, P, P, P]
+    mtb200_route_balanced_bwd = [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, I, P, P]
     mtb200_attn_fwd_one = [P, L, P, L, P, P, I, I, I, I, I, F, P, P]
     mtb200_attn_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, F, P, P]
     mtb200_attn_rule_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, I, F, F, I, P, P, P]
@@ -200,6 +204,14 @@ class NativeOps:
     # -- plumbing ---------------------------------------------------------------------
     def _st(self):
         return _raw_stream(self._index)   # handle of the device's current torch stream, without a Stream object around it
+
+    def on_device(self):
+        """Makes this backend's device the current one, where another is: kernels are launched on the current device."""
+        return contextlib.nullcontext() if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
+
+    def check_device(self, t):
+        if t.get_device() != self._index:
+            raise ValueError(f"this backend was made for {self.device}, the tensors are on {t.device}")
 
     def _call(self, name, *args, n=1, tag=None):
         if self.profile is None and not nvtx.ENABLED:
@@ -974,6 +986,14 @@ class NativeOps:
         self._call("mtb200_moe_route_bwd", probs.data_ptr(), topi.data_ptr(), w.data_ptr(), dw.data_ptr(), int(renorm), T, E, topi.shape[1],
                    out.data_ptr(), self._st())
         return out
+
+    def route_balanced(self, logits, k: int, renorm: bool, cu_seqlens=None, counted=None):
+        """``(probs, topi, w, RouterBalance)``: the router's choice with its balance loss, z-loss and the experts' counts (router_balance.py)."""
+        return router_balance.native(self, logits, k, renorm, cu_seqlens, counted)
+
+    def route_balanced_bwd(self, probs, topi, w, dw, renorm: bool, balance, dloss=None, dz=None, dtype=torch.bfloat16):
+        """Gradient of the logits ``[T, E]`` through the weights (``dw`` [T, k]) and the losses (``dloss``, ``dz``: [S] fp32); any of the three may be ``None``."""
+        return router_balance.native_bwd(self, probs, topi, w, dw, renorm, balance, dloss, dz, dtype)
 
     # -- plain GELU (tanh approximation) of a not gated MLP ----------------------------------
     def gelu(self, x):

@@ -1,0 +1,170 @@
+"""A router's choice of experts with the losses that keep all of them in use.
+
+``route_balanced`` of either backend takes the logits ``[T, E]`` of a layer's router and returns what ``moe.route`` does, ``(probs, topi, w)``: the fp32
+softmax, the ``k`` largest logits of each token (the lower expert of equal ones; what is not a number counts as the largest) and their probabilities, renormalised
+over the chosen ones where ``renorm``; and with them a ``RouterBalance``. For every packed sample of ``n`` counted tokens, ``c_e`` of whose (token, slot) pairs
+chose expert ``e``, and with ``P_e`` the sum of its probabilities over them:
+
+* ``loss``    ``E / n^2 sum_e c_e P_e``: ``k`` where all experts are used alike, more where they are not (the load-balancing loss of transformers'
+              ``load_balancing_loss_func``, modeling_mixtral.py, for one layer; there over the whole batch, which is one sample here)
+* ``z_loss``  the mean of ``logsumexp(logits)^2``, which keeps the logits small
+
+``route_balanced_bwd`` is the gradient of the logits through the weights and both losses, in one pass. Counts are constants of it. Tokens that are not counted, and
+those outside all samples, are routed like the others and get their weights' gradient, but have no part in a sample's losses and counts, whatever their
+logits are; a sample without counted tokens has losses of zero. The factors of the losses' gradients are tensors, one number per sample, so they can stay on the device.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+MOST_EXPERTS, MOST_CHOSEN = 512, 32   # of csrc/route_balance.cu
+
+
+@dataclass
+class RouterBalance:
+    loss: torch.Tensor      # [S] fp32
+    z_loss: torch.Tensor    # [S] fp32
+    counts: torch.Tensor    # [S, E] int32 pairs that chose an expert
+    tokens: torch.Tensor    # [S] int32 counted tokens
+    lse: torch.Tensor       # [T] fp32 logsumexp of every token's logits
+    cu_seqlens: Optional[torch.Tensor]   # as given
+    counted: Optional[torch.Tensor]      # as given
+
+
+def _refuse(what, t, dtype, shape, device):
+    raise ValueError(f"{what}: expected contiguous {dtype} {tuple(shape)} on {device}, not {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
+
+
+def _expect(what, t, dtype, shape, device):
+    if t is not None and (t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous()):
+        _refuse(what, t, dtype, shape, device)
+
+
+def check(logits, k, cu_seqlens, counted):
+    """``(T, E, S)`` of a call's arguments, which are refused where they have no right answer. Starts of samples are read by the kernels: ascending, from 0 to T at most."""
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or not logits.is_contiguous():
+        raise ValueError(f"router logits are contiguous bf16 or fp32 rows, not {tuple(logits.shape)} {logits.dtype} with strides {logits.stride()}")
+    T, E = logits.shape
+    if not 0 < E <= MOST_EXPERTS or T >= 1 << 30:
+        raise ValueError(f"{T} tokens and {E} experts: the kernels take up to 2^30 and {MOST_EXPERTS}")
+    if isinstance(k, bool) or not isinstance(k, int) or not 0 < k <= min(E, MOST_CHOSEN):
+        raise ValueError(f"a token chooses 1 to {min(E, MOST_CHOSEN)} of {E} experts, not {k}")
+    if cu_seqlens is not None:
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+            raise ValueError(f"starts of samples are a list of at least two, not {tuple(cu_seqlens.shape)}")
+        _expect("cu_seqlens", cu_seqlens, torch.int32, cu_seqlens.shape, logits.device)
+    if counted is not None:
+        _expect("counted", counted, torch.bool, (T,), logits.device)
+    return T, E, 1 if cu_seqlens is None else cu_seqlens.shape[0] - 1
+
+
+def check_bwd(probs, topi, w, dw, bal, dloss, dz, dtype):
+    """``(T, E, k, S)`` of a gradient's arguments."""
+    if probs.dim() != 2 or topi.dim() != 2:
+        raise ValueError("probs [T, E] and topi [T, k] are what the forward returned")
+    (T, E), k, S, device = probs.shape, topi.shape[1], bal.loss.shape[0], probs.device
+    if not 0 < E <= MOST_EXPERTS or not 0 < k <= min(E, MOST_CHOSEN) or T >= 1 << 30:
+        raise ValueError(f"{T} tokens, {k} of {E} experts: not what the forward returned")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"the gradient of the logits is bf16 or fp32, not {dtype}")
+    if dw is None and dloss is None and dz is None:
+        raise ValueError("without a gradient of the weights or of a loss there is nothing to do")
+    for what, t, ty, shape in (("probs", probs, torch.float32, (T, E)), ("topi", topi, torch.int64, (T, k)), ("w", w, torch.float32, (T, k)), ("dw", dw, torch.float32, (T, k)),
+                               ("dloss", dloss, torch.float32, (S,)), ("dz", dz, torch.float32, (S,)), ("counts", bal.counts, torch.int32, (S, E)),
+                               ("tokens", bal.tokens, torch.int32, (S,)), ("lse", bal.lse, torch.float32, (T,)), ("counted", bal.counted, torch.bool, (T,))):
+        _expect(what, t, ty, shape, device)
+    if bal.cu_seqlens is not None:
+        _expect("cu_seqlens", bal.cu_seqlens, torch.int32, (S + 1,), device)
+    elif S != 1:
+        raise ValueError(f"{S} samples without their starts")
+    return T, E, k, S
+
+
+# -- plain forms ----------------------------------------------------------------------------
+def _samples(T, bal):
+    """``[T]`` sample of each token, and whether it is in that sample's losses."""
+    cu, device = bal.cu_seqlens, bal.lse.device
+    at = torch.arange(T, device=device)
+    if cu is None:
+        sample, inside = torch.zeros_like(at), torch.ones(T, dtype=torch.bool, device=device)
+    else:
+        sample = torch.searchsorted(cu[1:].long().contiguous(), at, right=True)
+        inside = (sample < cu.shape[0] - 1) & (at >= cu[0])
+        sample = sample.clamp_max(cu.shape[0] - 2)
+    return sample, inside if bal.counted is None else inside & bal.counted
+
+
+def plain(logits, k, renorm, cu_seqlens=None, counted=None):
+    T, E, S = check(logits, k, cu_seqlens, counted)
+    l = logits.float()
+    probs, lse = torch.softmax(l, -1), torch.logsumexp(l, -1)
+    topi = torch.argsort(l, dim=-1, descending=True, stable=True)[:, :k].contiguous()
+    top = probs.gather(1, topi)
+    w = top / top.sum(-1, keepdim=True) if renorm else top
+    bal = RouterBalance(None, None, None, None, lse, cu_seqlens, counted)
+    sample, ok = _samples(T, bal)
+    sums = torch.zeros(S, E, dtype=torch.float64, device=l.device).index_add_(0, sample[ok], probs[ok].double())
+    counts = torch.zeros(S * E, dtype=torch.int64, device=l.device)
+    chosen = (sample[ok, None] * E + topi[ok]).reshape(-1)
+    counts = counts.index_add_(0, chosen, torch.ones_like(chosen)).view(S, E)
+    tokens = torch.zeros(S, dtype=torch.int64, device=l.device).index_add_(0, sample[ok], torch.ones_like(sample[ok]))
+    n = tokens.clamp_min(1).double()
+    z = torch.zeros(S, dtype=torch.float64, device=l.device).index_add_(0, sample[ok], lse[ok].double().square())
+    bal.loss, bal.z_loss = (E * (counts * sums).sum(1) / n.square()).float(), (z / n).float()
+    bal.counts, bal.tokens = counts.to(torch.int32), tokens.to(torch.int32)
+    return probs, topi, w, bal
+
+
+def plain_bwd(probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.bfloat16):
+    T, E, k, S = check_bwd(probs, topi, w, dw, bal, dloss, dz, dtype)
+    sample, ok = _samples(T, bal)
+    n = bal.tokens.clamp_min(1).float()
+    g = torch.zeros_like(probs)
+    if dw is not None:
+        d = (dw - (dw * w).sum(-1, keepdim=True)) / probs.gather(1, topi).sum(-1, keepdim=True) if renorm else dw
+        g.scatter_add_(1, topi, d)
+    if dloss is not None:
+        g[ok] += ((dloss * E / n / n)[:, None] * bal.counts)[sample[ok]]
+    g = g - (g * probs).sum(-1, keepdim=True)
+    if dz is not None:
+        g[ok] += (2.0 * bal.lse[ok] * (dz / n)[sample[ok]])[:, None]
+    return (probs * g).to(dtype)
+
+
+# -- kernels --------------------------------------------------------------------------------
+def native(ops, logits, k, renorm, cu_seqlens=None, counted=None):
+    T, E, S = check(logits, k, cu_seqlens, counted)
+    ops.check_device(logits)
+    dev, f32, i32 = logits.device, torch.float32, torch.int32
+    with ops.on_device():
+        sums = torch.empty(S, 2, dtype=f32, device=dev)
+        whole = torch.empty(S * (E + 1), dtype=i32, device=dev)
+        bal = RouterBalance(sums.view(-1)[:S], sums.view(-1)[S:], whole[:S * E].view(S, E), whole[S * E:], torch.empty(T, dtype=f32, device=dev), cu_seqlens, counted)
+        probs, topi, w = torch.empty(T, E, dtype=f32, device=dev), torch.empty(T, k, dtype=torch.int64, device=dev), torch.empty(T, k, dtype=f32, device=dev)
+        if T == 0:
+            sums.zero_()
+            whole.zero_()
+            return probs, topi, w, bal
+        rows = ops.lib.mtb200_route_balanced_rows(T, S)
+        part = torch.empty(rows * (E + 1), dtype=torch.int64, device=dev)
+        ops._call("mtb200_route_balanced", logits.data_ptr(), int(logits.dtype is f32), None if cu_seqlens is None else cu_seqlens.data_ptr(),
+                  None if counted is None else counted.data_ptr(), T, E, k, S, int(bool(renorm)), probs.data_ptr(), topi.data_ptr(), w.data_ptr(), bal.lse.data_ptr(),
+                  part.data_ptr(), part.data_ptr() + 8 * rows * E, bal.loss.data_ptr(), bal.z_loss.data_ptr(), bal.counts.data_ptr(), bal.tokens.data_ptr(),
+                  ops._st(), n=2)
+    return probs, topi, w, bal
+
+
+def native_bwd(ops, probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.bfloat16):
+    T, E, k, S = check_bwd(probs, topi, w, dw, bal, dloss, dz, dtype)
+    ops.check_device(probs)
+    with ops.on_device():
+        out = torch.empty(T, E, dtype=dtype, device=probs.device)
+        if T:
+            ptr = lambda t: None if t is None else t.data_ptr()
+            ops._call("mtb200_route_balanced_bwd", probs.data_ptr(), topi.data_ptr(), w.data_ptr(), ptr(dw), bal.lse.data_ptr(), ptr(bal.cu_seqlens), ptr(bal.counted),
+                      bal.counts.data_ptr(), bal.tokens.data_ptr(), ptr(dloss), ptr(dz), T, E, k, S, int(bool(renorm)), out.data_ptr(), int(dtype is torch.float32),
+                      ops.status.data_ptr(), ops._st())
+    return out

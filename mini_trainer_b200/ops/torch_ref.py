@@ -18,6 +18,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from . import router_balance
+
 
 class TorchOps:
     name = "torch"
@@ -330,6 +332,13 @@ class TorchOps:
     def gelu_bwd_act(self, dy, x):
         """``(dx, act)``: the gradient and the forward output a backward that did not keep it needs."""
         return self.gelu_bwd(dy, x), self.gelu(x)
+
+    # -- router with its balance losses (router_balance.py) ----------------------------------
+    def route_balanced(self, logits, k, renorm, cu_seqlens=None, counted=None):
+        return router_balance.plain(logits, k, renorm, cu_seqlens, counted)
+
+    def route_balanced_bwd(self, probs, topi, w, dw, renorm, balance, dloss=None, dz=None, dtype=torch.bfloat16):
+        return router_balance.plain_bwd(probs, topi, w, dw, renorm, balance, dloss, dz, dtype)
 
     # -- fused linear + cross-entropy ---------------------------------------------------
     def linear_ce(self, x, w, targets, grad_scale, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0, softcap=None):
