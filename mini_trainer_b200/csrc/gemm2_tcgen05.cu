@@ -365,7 +365,7 @@ gemm2_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__
         __syncwarp();
         if (lane == 0) mbar_arrive_cta0(&tempty_bar[h]);
       };
-      if constexpr (ACT == ACT_CAP) drained();   // (never wide)
+      if constexpr (ACT >= ACT_CAP) drained();   // (never wide)
       else if constexpr (ACT != ACT_NONE) epilogue_act_wide<ACT>(p.e, p.act, maps, out, taddr, row0, row_end, col0 / BN + h, q, lane, drained);
       else epilogue_wide<OUT_F32, !GROUP, STATS, EXTRA>(p.e, out, taddr, row0, row_end, col0 + h * BN, q, lane, 2 * (tm * tiles_n + col0 / BN + h) + static_cast<int>(rank),
                                                 splits > 1 ? w / wide_tiles : 0, GROUP == GROUP_REDUCE && kb1 == 0, drained);
@@ -591,6 +591,14 @@ int launch_act(int mode, bool wide, const CUtensorMap& ta, const CUtensorMap& tb
 int launch_capped(const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_CAP>& m, const EpiParams& e, const ActParams& a, int K, int* status, cudaStream_t stream) {
   const Params p{e.M, e.N, K, status, 0, 0, 0, e, a};
   return launch<false, false, false, false, false, false, ACT_CAP>(ta, tb, m.gate, p, stream, nullptr, 0, m);
+}
+int launch_lse(const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_LSE>& m, const EpiParams& e, const ActParams& a, int K, int* status, cudaStream_t stream) {
+  const Params p{e.M, e.N, K, status, 0, 0, 0, e, a};
+  return launch<false, false, false, false, false, false, ACT_LSE>(ta, tb, ta, p, stream, nullptr, 0, m);
+}
+int launch_nll(const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_NLL>& m, const EpiParams& e, const ActParams& a, int K, int* status, cudaStream_t stream) {
+  const Params p{e.M, e.N, K, status, 0, 0, 0, e, a};
+  return launch<false, false, false, false, false, false, ACT_NLL>(ta, tb, m.gate, p, stream, nullptr, 0, m);
 }
 
 // Grouped products on wide tiles; called by mtb200_gemm_grouped. `td`, `m`: maps of boxes of 32 rows x 128 bytes.

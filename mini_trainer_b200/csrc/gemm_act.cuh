@@ -8,6 +8,12 @@
 //              the others have together, which a sum with the target in it does not hold any more. 3720 x 151936 x 1536 1153 us (the product alone 1128), 5000 x 8192 x 512 62 (54), where the exponentials do not hide; 1399 where most
 //              logits are beyond the cap. Wide tiles, whose one
 //              warp per quarter would form them before it gives the accumulator back, took 1876 us.
+//   ACT_LSE    of every row and 128 columns of z = alpha A * B^T the largest z log2 e and the sum of 2^(z log2 e - largest), without the row's target, and the target's z: all that a
+//              likelihood wants of the logits, which are not stored.
+//   ACT_NLL    the gradient of a row's loss and log-partition in the place of its logits, from what the forward has left: g = (dloss + dlse) e^(z - lse), and of the target
+//              dloss expm1(-loss) + dlse e^-loss, which is no difference of numbers near one another however likely the target is. Rounded to bf16 once, as an operand of the two products that
+//              follow (operands of 16 bits are what the tensor cores take at this rate; the sum over them is fp32).
+//              Both in fp32 from the accumulator on.
 // Eight warps, two per 32-row quarter: with four (one per scheduler) the arithmetic of a tile took longer than short reductions. They work on
 // 32 columns at a time, staged as boxes of 32 rows x 64 bytes (64B-swizzled). Bound by the product. With its activation, in a loop of its own on a B200:
 // 5987 x 17920 x 1536 272 -> 231 us (product alone 220), 4099 x 12288 x 2048 167 -> 153, 16384 x 28672 x 4096 3.16 -> 2.8 ms, 7001 x 12288 x 3072 without
@@ -29,19 +35,23 @@
 
 namespace mtb {
 
-enum { ACT_NONE = 0, ACT_GLU = 1, ACT_PLAIN = 2, ACT_CAP = 3 };
+enum { ACT_NONE = 0, ACT_GLU = 1, ACT_PLAIN = 2, ACT_CAP = 3, ACT_LSE = 4, ACT_NLL = 5 };
 
 struct ActParams {
   int F;          // width of the activation
   union {
     int gelu;     // 0: SiLU, 1: tanh-approximated GELU
     float cap2;   // ACT_CAP
+    float k2;     // ACT_LSE, ACT_NLL: alpha log2 e
   };
 };
 // Tensor maps of gate (or x), up and act, boxes of 32 rows x 32 columns, 64B-swizzled; nothing in instances without an activation.
 template <int ACT> struct ActMaps { CUtensorMap gate, up, act; };
 template <> struct ActMaps<ACT_NONE> {};
 template <> struct ActMaps<ACT_CAP> { CUtensorMap gate; const long long* targets; };   // targets: [M], a column each or anything else for none
+template <> struct ActMaps<ACT_LSE> { const long long* targets; float* at_target; };
+struct NllRows { const long long* targets; const float *loss, *lse, *dloss, *dlse; long long ignore; long long first; int columns; };   // [M] each, dlse may be null; column 0 of the product is number `first` of `columns`
+template <> struct ActMaps<ACT_NLL> { CUtensorMap gate; NllRows rows; };
 
 constexpr int ACT_WARPS = 8;
 constexpr int ACT_BOX = 32 * 64;                     // bytes of a box
@@ -129,6 +139,74 @@ __device__ __forceinline__ void cap_stats(const EpiParams& p, int row, int row_e
   if (row < row_end && col < p.N) p.stats[static_cast<long long>(row) * ((p.N + 127) / 128) + col / 128] = st;
 }
 
+// ACT_LSE: 32 columns of a thread's row, from `col` on; `st` {largest, sum} so far. The target's column and those past N count for nothing.
+__device__ __forceinline__ void lse_columns32(const EpiParams& p, float k2, const uint32_t (&v)[32], int col, long long target, float* at_target, float2& st) {
+  float2 t[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t[i] = fmul2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f2(k2));
+  if (col + 32 > p.N) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (col + 2 * i >= p.N) t[i].x = -INFINITY;
+      if (col + 2 * i + 1 >= p.N) t[i].y = -INFINITY;
+    }
+  }
+  if (target >= col && target < col + 32) {   // one thread in many
+    const int at = static_cast<int>(target - col);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (at == 2 * i) { *at_target = __uint_as_float(v[2 * i]) * p.alpha; t[i].x = -INFINITY; }
+      if (at == 2 * i + 1) { *at_target = __uint_as_float(v[2 * i + 1]) * p.alpha; t[i].y = -INFINITY; }
+    }
+  }
+  float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mx[i & 1] = fmax3(mx[i & 1], t[i].x, t[i].y);
+  const float m = fmax3(st.x, mx[0], mx[1]), base = m == -INFINITY ? 0.f : m;   // (nothing but -infinity so far)
+  st.y *= ex2_mufu(st.x - base);
+  st.x = m;
+  const float2 nm = f2(-base);
+  float2 s[2] = {f2(0.f), f2(0.f)};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 x = fadd2(t[i], nm);
+    s[i & 1] = fadd2(s[i & 1], make_float2(ex2_mufu(x.x), ex2_mufu(x.y)));
+  }
+  const float2 q = fadd2(s[0], s[1]);
+  st.y += q.x + q.y;
+}
+// ACT_NLL: what a row's gradient is made of.
+struct NllRow {
+  float lse2 = 0.f, both = 0.f, at_target = 0.f;
+  int target = -1;      // column of the product, where it has it
+  bool live = false;
+};
+__device__ __forceinline__ NllRow nll_row(const NllRows& r, int row, int M) {
+  NllRow o;
+  if (row >= M) return o;
+  const long long t = r.targets[row];
+  if (t == r.ignore || t < 0 || t >= r.columns) return o;
+  const float dl = r.dloss[row], dz = r.dlse != nullptr ? r.dlse[row] : 0.f, loss = r.loss[row];
+  o.live = true;
+  o.lse2 = r.lse[row] * 1.4426950408889634f;
+  o.both = dl + dz;
+  o.at_target = fmaf(dl, expm1f(-loss), dz * expf(-loss));
+  const long long c = t - r.first;
+  o.target = c >= 0 && c < 0x7fffffff ? static_cast<int>(c) : -1;
+  return o;
+}
+__device__ __forceinline__ void nll_columns32(const NllRow& r, float k2, const uint32_t (&v)[32], int col, uint32_t (&d)[16]) {
+  const float2 k = f2(k2), nl = f2(-r.lse2), b = f2(r.both);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 x = ffma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), k, nl);
+    float2 g = fmul2(make_float2(ex2_mufu(x.x), ex2_mufu(x.y)), b);
+    if (r.target == col + 2 * i) g.x = r.at_target;
+    if (r.target == col + 2 * i + 1) g.y = r.at_target;
+    d[i] = r.live ? pack2(g) : 0u;   // a row that is not counted has no gradient, whatever its logits are
+  }
+}
+
 // One warp's part of a tile, `half` of its columns (gated: 64 of the gate and the same of up, else 128). `out`: this warp's two boxes.
 template <int ACT>
 __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams& ap, const ActMaps<ACT>& maps, EpiOut& out, uint32_t taddr, int row0,
@@ -138,7 +216,10 @@ __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams
   if (y0 >= p.M) return;
   float2 st = make_float2(CAP_NONE, 0.f);
   long long target = -1;
-  if constexpr (ACT == ACT_CAP) { if (y0 + lane < p.M) target = maps.targets[y0 + lane]; }
+  if constexpr (ACT == ACT_CAP || ACT == ACT_LSE) { if (y0 + lane < p.M) target = maps.targets[y0 + lane]; }
+  if constexpr (ACT == ACT_LSE) st.x = -INFINITY;
+  NllRow nll;
+  if constexpr (ACT == ACT_NLL) nll = nll_row(maps.rows, y0 + lane, p.M);
   auto send = [&](const CUtensorMap& map, const uint32_t (&d)[16], int col) {
     if (lane == 0) bulk_wait_read<1>();
     __syncwarp();
@@ -160,6 +241,16 @@ __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams
       send(maps.gate, g, col);
       continue;
     }
+    if constexpr (ACT == ACT_LSE) {
+      lse_columns32(p, ap.k2, v, col, target, maps.at_target + y0 + lane, st);
+      continue;
+    }
+    if constexpr (ACT == ACT_NLL) {
+      nll_columns32(nll, ap.k2, v, col, g);
+      send(maps.gate, g, col);
+      continue;
+    }
+    if constexpr (ACT == ACT_GLU || ACT == ACT_PLAIN || ACT == ACT_CAP) {
     if (ACT == ACT_PLAIN && p.bias != nullptr) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -195,8 +286,9 @@ __device__ __forceinline__ void epilogue_act(const EpiParams& p, const ActParams
       }
       send(maps.act, g, col);
     }
+    }
   }
-  if constexpr (ACT == ACT_CAP) cap_stats(p, y0 + lane, p.M, tn * 256 + half * 128, st);
+  if constexpr (ACT == ACT_CAP || ACT == ACT_LSE) cap_stats(p, y0 + lane, p.M, tn * 256 + half * 128, st);
 }
 
 // The same for wide tiles: one warp has all 256 columns of its quarter and reads them before it works on any; boxes of 32 rows x 128 bytes, one per

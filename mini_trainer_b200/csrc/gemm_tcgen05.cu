@@ -416,6 +416,8 @@ namespace g2 {
 int launch_act(int mode, bool wide, const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_GLU>& m, const EpiParams& e, const ActParams& a, int K,
                int* status, cudaStream_t stream);
 int launch_capped(const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_CAP>& m, const EpiParams& e, const ActParams& a, int K, int* status, cudaStream_t stream);
+int launch_lse(const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_LSE>& m, const EpiParams& e, const ActParams& a, int K, int* status, cudaStream_t stream);
+int launch_nll(const CUtensorMap& ta, const CUtensorMap& tb, const ActMaps<ACT_NLL>& m, const EpiParams& e, const ActParams& a, int K, int* status, cudaStream_t stream);
 int launch_grouped(int mode, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const ActMaps<ACT_GLU>& m, const EpiParams& e, const ActParams& a,
                    int K, const GroupParams& g, int* status, cudaStream_t stream);
 int launch_gather(const void* A, long long lda, void* D, long long ldd, const void* bias, int M, int N, int K,
@@ -588,6 +590,49 @@ int mtb200_gemm_capped(const void* A, long long lda, const void* W, void* t, flo
   if (form != FORM_ONE) return g2::launch_capped(ta, tb, m, e, a, K, status, stream);
   const GemmParams p{M, N, K, status, tune_group_m(), tune_wait_hint(), 0u, e, a};
   return launch<false, false, false, false, false, GROUP_NONE, false, false, ACT_CAP>(ta, tb, m.gate, p, stream, nullptr, 0, nullptr, m);
+}
+
+// Products z = alpha A[M, K] * W[N, K]^T whose values are not stored (gemm_act.cuh, ACT_LSE and ACT_NLL); row-major, W without padding between rows, any N. `form`: FORM_ONE or FORM_PAIR.
+// stats[M, ceil(N / 128)] = {largest z log2 e, sum of 2^(z log2 e - largest)} of the columns but the row's target, at_target[row] = the target's z where it has one.
+int mtb200_gemm_lse(const void* A, long long lda, const void* W, float2* stats, float* at_target, const long long* targets, int M, int N, int K, float alpha, int form, int* status,
+                    cudaStream_t stream) {
+  using namespace mtb;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if ((form != FORM_ONE && form != FORM_PAIR) || K % 8 || stats == nullptr || at_target == nullptr || targets == nullptr) return -10;
+  CUtensorMap ta, tb;
+  int rc = make_tmap_2d_bf16(&ta, A, K, M, lda, 64, 128);
+  if (rc) return rc;
+  rc = make_tmap_2d_bf16(&tb, W, K, N, K, 64, form != FORM_ONE ? 128 : 256);
+  if (rc) return rc - 10;
+  const ActMaps<ACT_LSE> m{targets, at_target};
+  const EpiParams e{M, N, nullptr, 0, nullptr, alpha, 1, nullptr, stats, nullptr, 0};
+  ActParams a{N, {}};
+  a.k2 = alpha * 1.4426950408889634f;
+  if (form != FORM_ONE) return g2::launch_lse(ta, tb, m, e, a, K, status, stream);
+  const GemmParams p{M, N, K, status, tune_group_m(), tune_wait_hint(), 0u, e, a};
+  return launch<false, false, false, false, false, GROUP_NONE, false, false, ACT_LSE>(ta, tb, ta, p, stream, nullptr, 0, nullptr, m);
+}
+// dz[M, N] (leading dimension ldz, a multiple of 8) = gradient of the losses by z, where W is rows [first, first + N) of a matrix with `columns` of them.
+int mtb200_gemm_nll(const void* A, long long lda, const void* W, void* dz, long long ldz, const long long* targets, const float* loss, const float* lse, const float* dloss,
+                    const float* dlse, int M, int N, int K, float alpha, long long ignore, long long first, int columns, int form, int* status, cudaStream_t stream) {
+  using namespace mtb;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if ((form != FORM_ONE && form != FORM_PAIR) || K % 8 || ldz % 8 || ldz < N || first < 0 || first + N > columns) return -10;
+  CUtensorMap ta, tb;
+  ActMaps<ACT_NLL> m{};
+  int rc = make_tmap_2d_bf16(&ta, A, K, M, lda, 64, 128);
+  if (rc) return rc;
+  rc = make_tmap_2d_bf16(&tb, W, K, N, K, 64, form != FORM_ONE ? 128 : 256);
+  if (rc) return rc - 10;
+  rc = make_tmap_act(&m.gate, dz, N, M, ldz, false);
+  if (rc) return rc - 20;
+  m.rows = NllRows{targets, loss, lse, dloss, dlse, ignore, first, columns};
+  const EpiParams e{M, N, nullptr, 0, nullptr, alpha, 1, nullptr, nullptr, nullptr, 0};
+  ActParams a{N, {}};
+  a.k2 = alpha * 1.4426950408889634f;
+  if (form != FORM_ONE) return g2::launch_nll(ta, tb, m, e, a, K, status, stream);
+  const GemmParams p{M, N, K, status, tune_group_m(), tune_wait_hint(), 0u, e, a};
+  return launch<false, false, false, false, false, GROUP_NONE, false, false, ACT_NLL>(ta, tb, m.gate, p, stream, nullptr, 0, nullptr, m);
 }
 
 enum { GROUPED_WIDE = 4 };

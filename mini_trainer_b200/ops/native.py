@@ -20,7 +20,7 @@ import torch
 
 from .. import build as _build
 from ..utils import nvtx
-from . import attention_plan, block_exec, gemm_plan, router_balance, step_exec
+from . import attention_plan, block_exec, gemm_plan, linear_nll, router_balance, step_exec
 
 _LIB = None
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
@@ -107,6 +107,9 @@ class _Sig:
     mtb200_moe_glu_bwd = [P, P, P, P, P, I, I, I, I, P, P, P]
     mtb200_moe_combine = [P, P, P, P, P, F, I, I, I, P, P]
     mtb200_moe_route_bwd = [P, P, P, P, I, I, I, I, P, P]
+    mtb200_gemm_lse = [P, L, P, P, P, P, I, I, I, F, I, P, P]
+    mtb200_gemm_nll = [P, L, P, P, L, P, P, P, P, P, I, I, I, F, L, L, I, I, P, P]
+    mtb200_nll = [P, P, P, I, I, L, L, P, P, P, P]
     mtb200_route_balanced_rows = [I, I]
     mtb200_route_balanced = [P, I, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, P, P, P]
     mtb200_route_balanced_bwd = [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, I, P, P]
@@ -270,7 +273,7 @@ class NativeOps:
         if code:
             self.status.zero_()
             what = {60: "a token id outside the embedding table", 61: "an attention work item outside the packed batch",
-                    62: "a chosen expert outside the model's experts"}.get(
+                    62: "a chosen expert outside the model's experts", 63: "a target outside the vocabulary"}.get(
                 code, "a device-side bounded wait expired")
             raise RuntimeError(f"{what} (status code {code})")
 
@@ -1098,6 +1101,15 @@ class NativeOps:
         if not whole:
             self._call("mtb200_f32_to_bf16", dw_out.data_ptr(), dw32.data_ptr(), V * H, int(accumulate_dw), self._st())
         return loss, dx
+
+    # -- likelihoods without logits (linear_nll.py) ----------------------------------------
+    def linear_nll(self, x, w, targets, ignore_index=-100, logit_scale=1.0):
+        """``(loss, lse)`` per token of ``logit_scale * x @ w.T``, whose values are not stored."""
+        return linear_nll.native(self, x, w, targets, ignore_index, logit_scale)
+
+    def linear_nll_bwd(self, dloss, x, w, targets, loss, lse, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0, dlse=None):
+        """``dx`` from the gradients of ``loss`` and ``lse`` (as ``linear_nll`` returned them), one number per token; ``dw_out`` receives (or accumulates) the weight's."""
+        return linear_nll.native_bwd(self, dloss, x, w, targets, loss, lse, dw_out, accumulate_dw, ignore_index, logit_scale, dlse)
 
     # -- optimizer --------------------------------------------------------------------
     def sumsq(self, g):

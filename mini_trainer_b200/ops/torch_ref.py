@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from . import router_balance
+from . import linear_nll, router_balance
 
 
 class TorchOps:
@@ -380,6 +380,13 @@ class TorchOps:
         else:
             dw_out.copy_(dw.to(dw_out.dtype))
         return loss, dx
+
+    # -- likelihoods without logits (linear_nll.py) ----------------------------------------
+    def linear_nll(self, x, w, targets, ignore_index=-100, logit_scale=1.0):
+        return linear_nll.plain(x, w, targets, ignore_index, logit_scale, self.ce_chunk)
+
+    def linear_nll_bwd(self, dloss, x, w, targets, loss, lse, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0, dlse=None):
+        return linear_nll.plain_bwd(dloss, x, w, targets, loss, lse, dw_out, accumulate_dw, ignore_index, logit_scale, dlse, self.ce_chunk)
 
     # -- optimizer --------------------------------------------------------------------
     def sumsq(self, g):
