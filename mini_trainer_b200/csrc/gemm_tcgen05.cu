@@ -377,6 +377,21 @@ int make_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t inner, uint64
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
+// 3-D map over `n` matrices [outer, inner] of 16-bit elements, rows `ld` and matrices `stride` elements apart; boxes 128B-swizzled, or as they are.
+int make_tmap_3d_16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t n, uint64_t ld, uint64_t stride, uint32_t box_inner, uint32_t box_outer, bool swizzle) {
+  EncodeTiledFn enc = get_encode();
+  if (enc == nullptr) return -1;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || ld % 8 || stride % 8) return -2;
+  cuuint64_t dims[3] = {inner, outer, n};
+  cuuint64_t strides[2] = {ld * 2, stride * 2};
+  cuuint32_t box[3] = {box_inner, box_outer, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -3;
+}
+
 // bf16 map for the boxes of the activation epilogues: 32 rows x 32 columns, 64B-swizzled; with wide tiles 32 rows x 64 columns, 128B-swizzled.
 int make_tmap_act(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t ld, bool wide) {
   if (wide) return make_tmap_2d_bf16(out, base, inner, outer, ld, 64, 32);

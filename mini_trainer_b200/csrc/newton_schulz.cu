@@ -1,0 +1,690 @@
+// Matrices orthogonalised by Newton-Schulz products, one or a stack of them, and the update of a parameter by its orthogonalised momentum.
+//
+//   X0 = G / (|G| + 1e-7)  (Frobenius norm)        X <- (a I + b A + c A^2) X,  A = X X^T        steps times
+// takes every singular value x of X to a x + b x^3 + c x^5, so those above 1e-3 of the norm or so end near one. A matrix with more rows than columns is multiplied from the right
+// instead, X (a I + b A + c A^2) with A = X^T X: operands of the tensor cores may have either dimension innermost, so nothing is ever transposed. With r the shorter side
+// and n the longer a step is the products r r n, r r r and r r n; the first two are symmetric: only the tiles on and below the diagonal are computed, and the epilogue stores a tile
+// and its transpose. 3 r^2 n + r^3 operations a step instead of 4 r^2 n + 2 r^3.
+//
+// Two identities keep the epilogues free of operands: with s = b / 2c the gram product's epilogue adds s to the diagonal, M = A + s I, and then
+//   a I + b A + c A^2 = c M^2 + (a - b^2 / 4c) I
+// is one square with a constant on the diagonal, and the step's last product has the linear term in it.
+//
+// Numbers. Operands are fp16, X 2^p with 2^p about the root of the longer side, and M and the polynomial about 2^12: entries of all three then lie in the middle of the type's
+// range (|X| <= 1.3 and |M|, |polynomial| <= 3.5 in norm, whatever G is). Its 11 bits are eight times finer than bf16's 8. That alone is not enough: a rounding of X is noise
+// in all directions, and a direction in which X has next to nothing grows by a = 3.44 in each step, 485 times in five. So X is held as two numbers, hi and lo = 2^11 (X - hi), and the
+// last product's epilogue adds a lo to the polynomial times hi: what is left of the rounding is what b A and c A^2 would have made of it, which is small
+// in just those directions. The last step's X goes without. Error of the result, relative, simulated with the roundings: normal 512 x 1376 1.7e-3 (bf16 throughout: 1.1e-2), features of different
+// size 1.4e-3 (9e-2), rank 8 and a hundredth of noise 2.2e-3 (0.26), rank 1 2.7e-3 (0.76); half of bf16's step, to which the result is rounded, is 1.7e-3 in the mean. Sums are fp32 in tensor memory.
+//
+// The products: persistent, warp-specialised, 3-D TMA maps over the stack, tcgen05.mma of fp16 into two accumulators in tensor memory, by single CTAs (tiles of 128 x 128, for few tiles) or CTA pairs
+// (256 x 256). All launches of a call are queued by one host call, each under its predecessor's tail.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "ptx.cuh"
+
+namespace mtb {
+
+int make_tmap_3d_16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t n, uint64_t ld, uint64_t stride, uint32_t box_inner, uint32_t box_outer, bool swizzle);
+
+namespace ns {
+
+constexpr double NS_A = 3.4445, NS_B = -4.7750, NS_C = 2.0315;
+// Factors of M and of the polynomial in fp16, about 2^12, such that what M has on its diagonal where A is next to nothing, s, and the polynomial's value there, a, are numbers of the type.
+constexpr double NS_S = NS_B / (2.0 * NS_C), NS_D = NS_A - static_cast<double>(NS_B) * NS_B / (4.0 * NS_C);
+constexpr double SCALE_M = 4816.0 / -NS_S, SCALE_P = 14112.0 / NS_A;
+constexpr int LO_BITS = 11;
+constexpr int BM = 128, BK = 64, STAGES = 6;
+constexpr int OP_BYTES = BM * BK * 2;                    // an operand's part of a stage: 128 rows (or columns) of 64
+constexpr int STAGE_BYTES = 2 * OP_BYTES;
+constexpr int EPI_WARPS = 8;                             // two to a quarter of the rows
+constexpr int BOX = 32 * 128;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * BOX + 1024 + 256;
+constexpr int GROUP_M = 8;
+constexpr uint32_t PEER_MASK = 0xFEFFFFFFu;              // of a shared::cluster address: the same place in CTA 0
+static_assert(SMEM <= 227 * 1024, "shared memory");
+
+// SYM: a symmetric product. APPLY: the step's last one, its result hi (and lo).
+enum { SYM = 0, APPLY = 1 };
+
+struct Params {
+  int M, N, K, stack;
+  int workers, group_m;
+  float alpha, diag;             // D = alpha product (SYM: + diag on the diagonal)
+  const __half* lo;              // APPLY: D += beta lo, laid out like D's hi
+  float beta;
+  long long ld, stride;          // of lo
+  int write_lo, bf16_out;        // APPLY
+  int* status;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void load_box(void* dst, const void* map, uint32_t bar, int c0, int c1, int c2) {
+  if constexpr (CTAS == 2)
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+// 128 rows (from `row`) x 64 of the reduction (from `k`) of an operand whose innermost dimension is the reduction, or (MN) the rows.
+template <int CTAS, bool MN>
+__device__ __forceinline__ void load_operand(uint8_t* dst, const void* map, uint32_t bar, int row, int k, int z) {
+  if constexpr (MN) {
+    load_box<CTAS>(dst, map, bar, row, k, z);
+    load_box<CTAS>(dst + OP_BYTES / 2, map, bar, row + 64, k, z);
+  } else {
+    load_box<CTAS>(dst, map, bar, k, row, z);
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CTAS == 2)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CTAS == 2) {
+    const uint16_t mask = 3;
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(mask) : "memory");
+  } else {
+    umma_commit(bar);
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  if constexpr (CTAS == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(smem_u32(bar) & PEER_MASK) : "memory");
+  else mbar_arrive(bar);
+}
+// fp16 x fp16 -> fp32
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
+  return make_idesc_bf16(m, n, a_mn, b_mn) & ~((1u << 7) | (1u << 10));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+// Tile `t` of a matrix: on and below the diagonal row by row, or in bands of group_m row-tiles.
+template <int KIND>
+__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int group_m, int& tm, int& tn) {
+  if constexpr (KIND == SYM) {
+    int i = static_cast<int>((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while (i * (i + 1) / 2 > t) --i;
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    tm = i;
+    tn = t - i * (i + 1) / 2;
+  } else {
+    const int band = t / (group_m * tiles_n), first = band * group_m, rows = min(group_m, tiles_m - first), local = t - first * tiles_n;
+    tm = first + local % rows;
+    tn = local / rows;
+  }
+}
+
+template <int CTAS, bool A_MN, bool B_MN, int KIND>
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1)
+product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
+               const __grid_constant__ CUtensorMap map_t, const Params p) {   // map_t: SYM: the transposed boxes of D; APPLY: lo of D
+  constexpr int TILE = BM * CTAS;      // rows and columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + EPI_WARPS * BOX);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
+  const int worker = blockIdx.x / CTAS;
+  const int tiles_m = (p.M + TILE - 1) / TILE, tiles_n = (p.N + TILE - 1) / TILE;
+  const int tiles = KIND == SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
+  const int items = tiles * p.stack, kblocks = (p.K + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull_bar[a], 1); mbar_init(&tempty_bar[a], CTAS * EPI_WARPS); }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+    tma_prefetch_desc(&map_d);
+  }
+  if (warp == 1) {
+    if constexpr (CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * TILE) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(tmem_slot, 2 * TILE);
+      tmem_relinquish();
+    }
+  }
+  pdl_wait();   // nothing so far has touched global memory
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CTAS == 2) cluster_barrier();   // the partner's barriers are there before anything is sent to them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t it = 0;
+      for (int w = worker; w < items; w += p.workers) {
+        int tm, tn;
+        const int z = w / tiles;
+        tile_at<KIND>(w - z * tiles, tiles_m, tiles_n, p.group_m, tm, tn);
+        const int row = tm * TILE + static_cast<int>(rank) * BM, col = tn * TILE + static_cast<int>(rank) * BM;
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 71); goto done; }
+          uint8_t* sa = smem + s * STAGE_BYTES;
+          const uint32_t bar = CTAS == 2 ? smem_u32(&full_bar[s]) & PEER_MASK : smem_u32(&full_bar[s]);
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * STAGE_BYTES);
+          load_operand<CTAS, A_MN>(sa, &map_a, bar, row, kb * BK, z);
+          load_operand<CTAS, B_MN>(sa + OP_BYTES, &map_b, bar, col, kb * BK, z);
+        }
+      }
+      pdl_trigger();
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = idesc_f16(TILE, TILE, A_MN, B_MN);
+      uint32_t it = 0, n = 0;
+      for (int w = worker; w < items; w += p.workers, ++n) {
+        if (!mbar_wait(&tempty_bar[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 72); goto done; }
+        tc_fence_after();
+        const uint32_t d = tmem_base + (n & 1) * TILE;
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag)) { atomicExch(p.status, 73); goto done; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * STAGE_BYTES), sb = sa + OP_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            const uint64_t da = A_MN ? make_smem_desc(sa + k * 2048, 8192, 1024) : make_smem_desc(sa + k * 32, 16, 1024);
+            const uint64_t db = B_MN ? make_smem_desc(sb + k * 2048, 8192, 1024) : make_smem_desc(sb + k * 32, 16, 1024);
+            mma<CTAS>(d, da, db, idesc, kb != 0 || k != 0);
+          }
+          commit<CTAS>(&empty_bar[s]);
+        }
+        commit<CTAS>(&tfull_bar[n & 1]);
+      }
+    }
+  } else {
+    // epilogue: quarter q of the rows, half of the columns, 64 at a time
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* box = smem + STAGES * STAGE_BYTES + (warp - 2) * BOX;
+    uint32_t n = 0;
+    for (int w = worker; w < items; w += p.workers, ++n) {
+      int tm, tn;
+      const int z = w / tiles;
+      tile_at<KIND>(w - z * tiles, tiles_m, tiles_n, p.group_m, tm, tn);
+      if (!mbar_wait(&tfull_bar[n & 1], (n >> 1) & 1, abort_flag)) { atomicExch(p.status, 74); goto done; }
+      tc_fence_after();
+      const int y0 = tm * TILE + static_cast<int>(rank) * BM + q * 32, row = y0 + lane;
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (n & 1) * TILE;
+#pragma unroll 1
+      for (int c = half * (TILE / 2); c < (half + 1) * (TILE / 2); c += 64) {
+        const int col = tn * TILE + c;
+        if (y0 >= p.M || col >= p.N) break;
+        uint32_t v[2][32];
+        tmem_ld_32x32(taddr + c, v[0]);
+        tmem_ld_32x32(taddr + c + 32, v[1]);
+        tmem_ld_wait();
+        float* f = reinterpret_cast<float*>(&v[0][0]);
+#pragma unroll
+        for (int j = 0; j < 64; ++j) f[j] *= p.alpha;
+        auto free_box = [&]() {
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+        };
+        auto send = [&](const CUtensorMap& map, int x, int y) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) { tma_store_3d(&map, box, x, y, z); bulk_commit(); }
+        };
+        auto stage = [&](const uint32_t (&h)[32]) {   // this thread's row of the box, 128B-swizzled
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+        };
+        uint32_t h[32];
+        if constexpr (KIND == SYM) {
+          if (tm == tn) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) if (col + j == row) f[j] += p.diag;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) h[j] = pack_f16(f[2 * j], f[2 * j + 1]);
+          free_box();
+          stage(h);
+          send(map_d, col, y0);
+          if (tm != tn) {
+            // The transpose: box of 64 rows (this tile's columns) x 32 (its rows). Neighbouring lanes exchange a word, so that each writes two rows' entries of one column.
+            free_box();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const uint32_t o = __shfl_xor_sync(0xffffffffu, h[j], 1);
+              const uint32_t word = lane & 1 ? __byte_perm(o, h[j], 0x7632) : __byte_perm(h[j], o, 0x5410);
+              *reinterpret_cast<uint32_t*>(box + (2 * j + (lane & 1)) * 64 + (lane >> 1) * 4) = word;
+            }
+            send(map_t, y0, col);
+          }
+        } else {
+          if (p.lo != nullptr && row < p.M) {
+            const __half* src = p.lo + z * p.stride + static_cast<long long>(row) * p.ld + col;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (col + 8 * i < p.N) {   // (rows are padded to whole pieces)
+                const uint4 u = *reinterpret_cast<const uint4*>(src + 8 * i);
+                const float2 a = unpack_f16(u.x), b = unpack_f16(u.y), d = unpack_f16(u.z), e = unpack_f16(u.w);
+                f[8 * i] += p.beta * a.x; f[8 * i + 1] += p.beta * a.y; f[8 * i + 2] += p.beta * b.x; f[8 * i + 3] += p.beta * b.y;
+                f[8 * i + 4] += p.beta * d.x; f[8 * i + 5] += p.beta * d.y; f[8 * i + 6] += p.beta * e.x; f[8 * i + 7] += p.beta * e.y;
+              }
+            }
+          }
+          if (p.bf16_out) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) h[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) h[j] = pack_f16(f[2 * j], f[2 * j + 1]);
+          }
+          free_box();
+          stage(h);
+          send(map_d, col, y0);
+          if (p.write_lo) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float2 hi = unpack_f16(h[j]);
+              h[j] = pack_f16((f[2 * j] - hi.x) * (1 << LO_BITS), (f[2 * j + 1] - hi.y) * (1 << LO_BITS));
+            }
+            free_box();
+            stage(h);
+            send(map_t, col, y0);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_leader<CTAS>(&tempty_bar[n & 1]);
+    }
+  }
+done:
+  if (warp >= 2 && lane == 0) bulk_wait_read<0>();
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CTAS == 2) cluster_barrier();   // nobody tears down while the partner may still signal or read
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * TILE) : "memory");
+    else tmem_dealloc(tmem_base, 2 * TILE);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ in front of the products, and behind them
+constexpr int LIN_THREADS = 256;
+constexpr int MOST_CHUNKS = 1024;   // of a matrix, in the sums of squares
+
+// What is orthogonalised: a gradient, or a momentum that takes the gradient in first.
+struct Source {
+  const void* g; int g_bf16;
+  void* m; int m_bf16;             // null: g itself
+  const float* coef;               // factor of the gradient, on the device, or null
+  float mu; int nesterov;
+};
+__device__ __forceinline__ float load16or32(const void* p, int is16, long long i) {
+  return is16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]) : reinterpret_cast<const float*>(p)[i];
+}
+// Eight elements; those past `n` are zero.
+__device__ __forceinline__ void load8(const void* p, int is16, long long i, int n, bool vec, float (&x)[8]) {
+  if (vec) {
+    if (is16) {
+      const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
+      const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), d = unpack_bf16(u.w);
+      x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i), b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i + 4);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < n ? load16or32(p, is16, i + j) : 0.f;
+  }
+}
+__device__ __forceinline__ void store8(void* p, int is16, long long i, int n, bool vec, const float (&x)[8]) {
+  if (vec) {
+    if (is16) {
+      *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p) + i) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    } else {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) {
+        if (is16) reinterpret_cast<__nv_bfloat16*>(p)[i + j] = __float2bfloat16(x[j]);
+        else reinterpret_cast<float*>(p)[i + j] = x[j];
+      }
+  }
+}
+// Eight elements of what is orthogonalised. `update`: the momentum takes the gradient in; else it has. The momentum counts as it is stored.
+__device__ __forceinline__ void source8(const Source& s, float coef, long long i, int n, bool vec, bool update, float (&u)[8]) {
+  load8(s.g, s.g_bf16, i, n, vec, u);
+  if (s.m == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) u[j] *= coef;
+  float m[8];
+  load8(s.m, s.m_bf16, i, n, vec, m);
+  if (update) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = fmaf(s.mu, m[j], u[j]);
+      if (s.m_bf16) m[j] = __bfloat162float(__float2bfloat16(m[j]));
+    }
+    store8(s.m, s.m_bf16, i, n, vec, m);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) u[j] = s.nesterov ? fmaf(s.mu, m[j], u[j]) : m[j];
+}
+
+// Sums of squares of the chunks of each matrix, [stack, chunks]; the momentum's update on the way.
+__global__ void __launch_bounds__(LIN_THREADS) squares_kernel(Source s, long long numel, int chunks, long long per_chunk, int vec, double* __restrict__ sums) {
+  __shared__ double sh[LIN_THREADS / 32];
+  pdl_wait();
+  const int z = blockIdx.x / chunks, c = blockIdx.x - z * chunks;
+  const long long lo = c * per_chunk, hi = min(numel, lo + per_chunk), base = z * numel;
+  const float coef = s.coef != nullptr ? *s.coef : 1.f;
+  double total = 0.0;
+  for (long long i = lo + threadIdx.x * 8; i < hi; i += LIN_THREADS * 8) {
+    float u[8];
+    source8(s, coef, base + i, static_cast<int>(min(8ll, hi - i)), vec != 0, true, u);
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q = fmaf(u[j], u[j], q);
+    total += q;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < LIN_THREADS / 32; ++i) total += sh[i];
+    sums[blockIdx.x] = total;
+  }
+  pdl_trigger();
+}
+
+// X0 2^p as hi and lo, rows padded to ld. `lo` null: hi alone.
+__global__ void __launch_bounds__(LIN_THREADS) scale_kernel(Source s, int rows, int cols, int ld, int chunks, int blocks_per, int vec, int p2, const double* __restrict__ sums,
+                                                           __half* __restrict__ hi, __half* __restrict__ lo) {
+  __shared__ double sh[LIN_THREADS / 32];
+  __shared__ float factor_sh;
+  pdl_wait();
+  const int z = blockIdx.x / blocks_per, blk = blockIdx.x - z * blocks_per;
+  double total = 0.0;
+  for (int i = threadIdx.x; i < chunks; i += LIN_THREADS) total += sums[static_cast<long long>(z) * chunks + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < LIN_THREADS / 32; ++i) total += sh[i];
+    factor_sh = static_cast<float>(ldexp(1.0, p2) / (sqrt(total) + 1e-7));
+  }
+  __syncthreads();
+  const float factor = factor_sh, coef = s.coef != nullptr ? *s.coef : 1.f;
+  const int per_row = ld / 8;
+  const long long units = static_cast<long long>(rows) * per_row, base = static_cast<long long>(z) * rows * cols, out = static_cast<long long>(z) * rows * ld;
+  for (long long u = static_cast<long long>(blk) * LIN_THREADS + threadIdx.x; u < units; u += static_cast<long long>(blocks_per) * LIN_THREADS) {
+    const long long row = u / per_row;
+    const int col = static_cast<int>(u - row * per_row) * 8;
+    float x[8];
+    source8(s, coef, base + row * cols + col, min(8, cols - col), vec != 0, false, x);
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = x[2 * j] * factor, b = x[2 * j + 1] * factor;
+      h[j] = pack_f16(a, b);
+      const float2 r = unpack_f16(h[j]);
+      l[j] = pack_f16((a - r.x) * (1 << LO_BITS), (b - r.y) * (1 << LO_BITS));
+    }
+    *reinterpret_cast<uint4*>(hi + out + row * ld + col) = make_uint4(h[0], h[1], h[2], h[3]);
+    if (lo != nullptr) *reinterpret_cast<uint4*>(lo + out + row * ld + col) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+  pdl_trigger();
+}
+
+// bf16 rows without their padding.
+__global__ void __launch_bounds__(LIN_THREADS) unpad_kernel(const __nv_bfloat16* __restrict__ x, int ld, long long rows, int cols, __nv_bfloat16* __restrict__ out) {
+  pdl_wait();
+  const long long n = rows * cols;
+  for (long long i = static_cast<long long>(blockIdx.x) * LIN_THREADS + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * LIN_THREADS) {
+    const long long row = i / cols;
+    out[i] = x[row * ld + (i - row * cols)];
+  }
+  pdl_trigger();
+}
+
+// w <- keep w - step o 2^-p of the padded fp16 rows o, and the working copy.
+__global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ param, const __half* __restrict__ o, int ld, long long rows,
+                                                            int cols, int vec, float keep, float step) {
+  pdl_wait();
+  const int per_row = ld / 8;
+  const long long units = rows * per_row;
+  for (long long u = static_cast<long long>(blockIdx.x) * LIN_THREADS + threadIdx.x; u < units; u += static_cast<long long>(gridDim.x) * LIN_THREADS) {
+    const long long row = u / per_row, at = row * cols;
+    const int col = static_cast<int>(u - row * per_row) * 8, n = min(8, cols - col);
+    const uint4 q = *reinterpret_cast<const uint4*>(o + row * ld + col);
+    const float2 a = unpack_f16(q.x), b = unpack_f16(q.y), c = unpack_f16(q.z), d = unpack_f16(q.w);
+    const float x[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+    float w[8];
+    load8(master, 0, at + col, n, vec != 0, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = fmaf(-step, x[j], keep * w[j]);
+    store8(master, 0, at + col, n, vec != 0, w);
+    if (param != nullptr) store8(param, 1, at + col, n, vec != 0, w);
+  }
+  pdl_trigger();
+}
+
+// ------------------------------------------------------------------------------------------ host
+struct Matrix {            // stack of fp16 matrices with padded rows
+  const void* p;
+  long long rows, cols, ld, stack;
+  CUtensorMap k, mn, d, t;   // loads with the columns as the reduction, or with the rows; stores, and of transposed boxes
+  int make(bool transposed) {
+    const uint64_t stride = static_cast<uint64_t>(rows) * ld;
+    int rc = make_tmap_3d_16(&k, p, cols, rows, stack, ld, stride, BK, BM, true);
+    if (!rc) rc = make_tmap_3d_16(&mn, p, cols, rows, stack, ld, stride, 64, 64, true);
+    if (!rc) rc = make_tmap_3d_16(&d, p, cols, rows, stack, ld, stride, 64, 32, true);
+    if (!rc && transposed) rc = make_tmap_3d_16(&t, p, cols, rows, stack, ld, stride, 32, 64, false);
+    return rc;
+  }
+};
+
+static int sm_count() {
+  static int n = 0;
+  if (n == 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); n = 148; }
+  }
+  return n;
+}
+template <int CTAS, bool A_MN, bool B_MN, int KIND>
+static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const CUtensorMap& t, Params p, int workers, cudaStream_t st) {
+  auto kern = product_kernel<CTAS, A_MN, B_MN, KIND>;
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -4;
+    configured = true;
+  }
+  const long long tile = BM * CTAS, tm = (p.M + tile - 1) / tile, tn = (p.N + tile - 1) / tile;
+  const long long items = (KIND == SYM ? tm * (tm + 1) / 2 : tm * tn) * p.stack;
+  if (items >= 1ll << 30) return -10;
+  p.workers = static_cast<int>(items < workers ? items : workers);
+  p.group_m = GROUP_M;
+  launch_pdl(kern, p.workers * CTAS, THREADS, SMEM, st, a, b, d, t, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -5;
+}
+// Rounds of single CTAs and of pairs over a product's tiles, by how long a round takes.
+static bool prefers_pairs(long long M, long long N, long long stack, bool sym, int pairs, int sms) {
+  if (pairs <= 0) return false;
+  auto rounds = [&](long long tile, long long workers) {
+    const long long tm = (M + tile - 1) / tile, tn = (N + tile - 1) / tile;
+    return ((sym ? tm * (tm + 1) / 2 : tm * tn) * stack + workers - 1) / workers;
+  };
+  return rounds(256, pairs) * 2.0 <= rounds(128, sms) * 1.2;
+}
+
+static long long up(long long x, long long to) { return (x + to - 1) / to * to; }
+struct Layout { long long ld, r, ldr, xbytes, gbytes, chunks, total; };
+static Layout layout(long long rows, long long cols, long long stack) {
+  Layout l;
+  l.ld = up(cols, 8);
+  l.r = rows < cols ? rows : cols;
+  l.ldr = up(l.r, 8);
+  l.xbytes = up(stack * rows * l.ld * 2, 256);
+  l.gbytes = up(stack * l.r * l.ldr * 2, 256);
+  const long long numel = rows * cols;
+  long long most = MOST_CHUNKS / stack;
+  if (most < 1) most = 1;
+  l.chunks = (numel + 16383) / 16384;
+  if (l.chunks > most) l.chunks = most;
+  l.total = 4 * l.xbytes + 2 * l.gbytes + up(stack * l.chunks * 8, 256);
+  return l;
+}
+
+// Everything up to the last product, which leaves hi 2^p in *result (fp16, padded), or bf16 in `out` (padded rows of out_ld).
+static int orthogonalise(const Source& src, long long rows, long long cols, long long stack, int steps, void* out, long long out_ld, int p2, uint8_t* ws, int pairs, int* status, cudaStream_t st) {
+  const Layout l = layout(rows, cols, stack);
+  const bool right = rows > cols;
+  __half* x[2][2] = {{(__half*)ws, (__half*)(ws + l.xbytes)}, {(__half*)(ws + 2 * l.xbytes), (__half*)(ws + 3 * l.xbytes)}};
+  uint8_t* g = ws + 4 * l.xbytes;
+  double* sums = (double*)(g + 2 * l.gbytes);
+  const long long numel = rows * cols;
+  const bool plain = ((reinterpret_cast<uintptr_t>(src.g) | reinterpret_cast<uintptr_t>(src.m)) & 15) == 0;
+  const int vec_flat = plain && numel % 8 == 0, vec_rows = plain && cols % 8 == 0;
+  const long long per_chunk = up((numel + l.chunks - 1) / l.chunks, 8 * LIN_THREADS);
+  if (stack * l.chunks >= 1ll << 31) return -10;
+  launch_pdl(squares_kernel, static_cast<unsigned>(stack * l.chunks), LIN_THREADS, 0, st, src, numel, static_cast<int>(l.chunks), per_chunk, vec_flat, sums);
+  long long blocks = (rows * l.ld / 8 + LIN_THREADS - 1) / LIN_THREADS, most = (sm_count() * 8 + stack - 1) / stack;
+  if (blocks > most) blocks = most;
+  launch_pdl(scale_kernel, static_cast<unsigned>(stack * blocks), LIN_THREADS, 0, st, src, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(l.ld), static_cast<int>(l.chunks),
+             static_cast<int>(blocks), vec_rows, p2, sums, x[0][0], steps > 1 ? x[0][1] : nullptr);
+  if (cudaGetLastError() != cudaSuccess) return -5;
+
+  Matrix xh[2], xl[2], gram{g, l.r, l.r, l.ldr, stack}, poly{g + l.gbytes, l.r, l.r, l.ldr, stack}, last{out, rows, cols, out_ld, stack};
+  for (int i = 0; i < 2; ++i) {
+    xh[i] = Matrix{x[i][0], rows, cols, l.ld, stack};
+    xl[i] = Matrix{x[i][1], rows, cols, l.ld, stack};
+    int rc = xh[i].make(false);
+    if (!rc) rc = xl[i].make(false);
+    if (rc) return rc - 20;
+  }
+  int rc = gram.make(true);
+  if (!rc) rc = poly.make(true);
+  if (!rc && out != nullptr) rc = last.make(false);
+  if (rc) return rc - 30;
+
+  const int sms = sm_count();
+  const bool sym2 = prefers_pairs(l.r, l.r, stack, true, pairs, sms), app2 = prefers_pairs(rows, cols, stack, false, pairs, sms);
+  const int r = static_cast<int>(l.r), K = static_cast<int>(right ? rows : cols);
+  for (int i = 0; i < steps; ++i) {
+    const Matrix& X = xh[i & 1];
+    Params p{r, r, K, static_cast<int>(stack), 0, 0, static_cast<float>(ldexp(SCALE_M, -2 * p2)), static_cast<float>(SCALE_M * NS_S), nullptr, 0.f, 0, 0, 0, 0, status};
+    if (right) rc = sym2 ? launch<2, true, true, SYM>(X.mn, X.mn, gram.d, gram.t, p, pairs, st) : launch<1, true, true, SYM>(X.mn, X.mn, gram.d, gram.t, p, sms, st);
+    else rc = sym2 ? launch<2, false, false, SYM>(X.k, X.k, gram.d, gram.t, p, pairs, st) : launch<1, false, false, SYM>(X.k, X.k, gram.d, gram.t, p, sms, st);
+    if (rc) return rc;
+    p.K = r;
+    p.alpha = static_cast<float>(SCALE_P * NS_C / (SCALE_M * SCALE_M));
+    p.diag = static_cast<float>(SCALE_P * NS_D);
+    rc = sym2 ? launch<2, false, false, SYM>(gram.k, gram.k, poly.d, poly.t, p, pairs, st) : launch<1, false, false, SYM>(gram.k, gram.k, poly.d, poly.t, p, sms, st);
+    if (rc) return rc;
+    const bool end = i + 1 == steps, to_out = end && out != nullptr;
+    Params a{static_cast<int>(rows), static_cast<int>(cols), r, static_cast<int>(stack), 0, 0, static_cast<float>(ldexp(1.0 / SCALE_P, to_out ? -p2 : 0)), 0.f,
+             end ? nullptr : x[i & 1][1], static_cast<float>(ldexp(NS_A, -LO_BITS)), l.ld, rows * l.ld, i + 2 < steps, to_out, status};
+    const CUtensorMap& to = to_out ? last.d : xh[(i + 1) & 1].d;
+    const CUtensorMap& lo = xl[(i + 1) & 1].d;
+    if (right) rc = app2 ? launch<2, false, false, APPLY>(X.k, poly.k, to, lo, a, pairs, st) : launch<1, false, false, APPLY>(X.k, poly.k, to, lo, a, sms, st);
+    else rc = app2 ? launch<2, false, true, APPLY>(poly.k, X.mn, to, lo, a, pairs, st) : launch<1, false, true, APPLY>(poly.k, X.mn, to, lo, a, sms, st);
+    if (rc) return rc;
+  }
+  return 0;
+}
+static int exponent(long long rows, long long cols) { return static_cast<int>(lround(0.5 * log2(static_cast<double>(rows > cols ? rows : cols)))); }
+static bool sizes_ok(long long rows, long long cols, long long stack, int steps) {
+  return rows > 0 && cols > 0 && stack > 0 && rows < 1 << 24 && cols < 1 << 24 && stack < 1 << 24 && steps >= 1 && steps <= 64 && (rows < cols ? rows : cols) <= 1 << 16;
+}
+
+}  // namespace ns
+}  // namespace mtb
+
+extern "C" {
+
+int mtb200_gemm2_pairs();
+
+// Bytes of the workspace of the two calls below, which starts on 256 bytes.
+long long mtb200_newton_schulz_workspace(long long rows, long long cols, long long stack) {
+  const mtb::ns::Layout l = mtb::ns::layout(rows, cols, stack);
+  return l.total;
+}
+// Launches of a call: sums and scaling, three products a step, one behind them.
+// out [stack, rows, cols] bf16 = g [stack, rows, cols] (bf16 or fp32) orthogonalised.
+int mtb200_newton_schulz(const void* g, int g_bf16, void* out, long long rows, long long cols, long long stack, int steps, void* ws, long long ws_bytes, int* status, cudaStream_t st) {
+  using namespace mtb::ns;
+  if (!sizes_ok(rows, cols, stack, steps)) return -10;
+  const Layout l = layout(rows, cols, stack);
+  if (ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 255)) return -11;
+  const Source src{g, g_bf16, nullptr, 0, nullptr, 0.f, 0};
+  const bool direct = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  uint8_t* w = reinterpret_cast<uint8_t*>(ws);
+  void* to = direct ? out : w + 2 * (steps & 1) * l.xbytes;   // the buffer that the last step writes
+  int rc = orthogonalise(src, rows, cols, stack, steps, to, direct ? cols : l.ld, exponent(rows, cols), w, mtb200_gemm2_pairs(), status, st);
+  if (rc || direct) return rc;
+  const long long n = stack * rows * cols;
+  long long blocks = (n + LIN_THREADS - 1) / LIN_THREADS;
+  if (blocks > sm_count() * 16) blocks = sm_count() * 16;
+  mtb::launch_pdl(unpad_kernel, static_cast<unsigned>(blocks), LIN_THREADS, 0, st, (const __nv_bfloat16*)to, static_cast<int>(l.ld), stack * rows, static_cast<int>(cols), (__nv_bfloat16*)out);
+  return cudaGetLastError() == cudaSuccess ? 0 : -5;
+}
+// m <- mu m + coef g;  master <- keep master - step O(nesterov ? coef g + mu m : m);  param <- master. g bf16 or fp32, m fp32 or bf16, master fp32, param bf16 or null, coef on the device or null.
+int mtb200_muon_step(float* master, void* m, int m_bf16, const void* g, int g_bf16, void* param, const float* coef, long long rows, long long cols, long long stack, int steps, float mu,
+                     int nesterov, float keep, float step, void* ws, long long ws_bytes, int* status, cudaStream_t st) {
+  using namespace mtb::ns;
+  if (!sizes_ok(rows, cols, stack, steps) || m == nullptr) return -10;
+  const Layout l = layout(rows, cols, stack);
+  if (ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 255)) return -11;
+  const Source src{g, g_bf16, m, m_bf16, coef, mu, nesterov};
+  uint8_t* w = reinterpret_cast<uint8_t*>(ws);
+  const int p2 = exponent(rows, cols);
+  int rc = orthogonalise(src, rows, cols, stack, steps, nullptr, 0, p2, w, mtb200_gemm2_pairs(), status, st);
+  if (rc) return rc;
+  const __half* o = reinterpret_cast<const __half*>(w + 2 * (steps & 1) * l.xbytes);
+  const int vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(master) | reinterpret_cast<uintptr_t>(param)) & 15) == 0;
+  long long blocks = (stack * rows * l.ld / 8 + LIN_THREADS - 1) / LIN_THREADS;
+  if (blocks > sm_count() * 8) blocks = sm_count() * 8;
+  mtb::launch_pdl(update_kernel, static_cast<unsigned>(blocks), LIN_THREADS, 0, st, master, (__nv_bfloat16*)param, o, static_cast<int>(l.ld), stack * rows, static_cast<int>(cols), vec, keep,
+                  static_cast<float>(ldexp(step, -p2)));
+  return cudaGetLastError() == cudaSuccess ? 0 : -5;
+}
+
+}  // extern "C"

@@ -20,7 +20,7 @@ import torch
 
 from .. import build as _build
 from ..utils import nvtx
-from . import attention_plan, block_exec, gemm_plan, linear_nll, router_balance, step_exec
+from . import attention_plan, block_exec, gemm_plan, linear_nll, newton_schulz, router_balance, step_exec
 
 _LIB = None
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
@@ -44,6 +44,7 @@ def load_library():
             fn.argtypes = getattr(_Sig, name)
     lib.mtb200_block_workspace.restype = c_longlong
     lib.mtb200_step_workspace.restype = c_longlong
+    lib.mtb200_newton_schulz_workspace.restype = c_longlong
     block_exec.check_layout(lib)
     step_exec.check_layout(lib)
     _LIB = lib
@@ -107,6 +108,9 @@ class _Sig:
     mtb200_moe_glu_bwd = [P, P, P, P, P, I, I, I, I, P, P, P]
     mtb200_moe_combine = [P, P, P, P, P, F, I, I, I, P, P]
     mtb200_moe_route_bwd = [P, P, P, P, I, I, I, I, P, P]
+    mtb200_newton_schulz_workspace = [L, L, L]
+    mtb200_newton_schulz = [P, I, P, L, L, L, I, P, L, P, P]
+    mtb200_muon_step = [P, P, I, P, I, P, P, L, L, L, I, F, I, F, F, P, L, P, P]
     mtb200_gemm_lse = [P, L, P, P, P, P, I, I, I, F, I, P, P]
     mtb200_gemm_nll = [P, L, P, P, L, P, P, P, P, P, I, I, I, F, L, L, I, I, P, P]
     mtb200_nll = [P, P, P, I, I, L, L, P, P, P, P]
@@ -1152,3 +1156,11 @@ class NativeOps:
         self._call("mtb200_adamw", master.data_ptr(), m.data_ptr(), v.data_ptr(), int(m.dtype == torch.float32),
                    grad.data_ptr(), param_out.data_ptr(), master.numel(), lr, beta1, beta2, eps, weight_decay, step,
                    grad_coef.data_ptr(), self._st())
+
+    def orthogonalise(self, g, steps=5):
+        """Matrices ``[..., m, n]`` orthogonalised by Newton-Schulz products, in bf16 (newton_schulz.py)."""
+        return newton_schulz.native(self, g, steps)
+
+    def muon_step(self, master, moment, grad, param_out, lr, momentum, weight_decay, grad_coef=1.0, nesterov=True, steps=5, scale=None):
+        """One step of a parameter ``[..., m, n]`` by its orthogonalised momentum, in place; ``grad_coef``: a number or a one-element tensor on the device."""
+        newton_schulz.native_muon(self, master, moment, grad, param_out, lr, momentum, weight_decay, grad_coef, nesterov, steps, scale)

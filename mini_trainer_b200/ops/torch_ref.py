@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from . import linear_nll, router_balance
+from . import linear_nll, newton_schulz, router_balance
 
 
 class TorchOps:
@@ -410,3 +410,10 @@ class TorchOps:
         denom = (vf.sqrt() / (bc2 ** 0.5)).add_(eps)
         master.addcdiv_(mf, denom, value=-lr / bc1)
         param_out.copy_(master.to(param_out.dtype))
+
+    # -- updates by an orthogonalised momentum (newton_schulz.py) ---------------------------
+    def orthogonalise(self, g, steps=5):
+        return newton_schulz.plain(g, steps)
+
+    def muon_step(self, master, moment, grad, param_out, lr, momentum, weight_decay, grad_coef=1.0, nesterov=True, steps=5, scale=None):
+        newton_schulz.plain_muon(master, moment, grad, param_out, lr, momentum, weight_decay, grad_coef, nesterov, steps, scale)
