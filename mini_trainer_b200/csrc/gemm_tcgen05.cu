@@ -377,8 +377,8 @@ int make_tmap_3d_bf16(CUtensorMap* out, const void* base, uint64_t inner, uint64
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
-// 3-D map over `n` matrices [outer, inner] of 16-bit elements, rows `ld` and matrices `stride` elements apart; boxes 128B-swizzled, or as they are.
-int make_tmap_3d_16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t n, uint64_t ld, uint64_t stride, uint32_t box_inner, uint32_t box_outer, bool swizzle) {
+// 3-D map over `n` matrices [outer, inner] of 16-bit elements, rows `ld` and matrices `stride` elements apart; boxes 128B-swizzled.
+int make_tmap_3d_16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t n, uint64_t ld, uint64_t stride, uint32_t box_inner, uint32_t box_outer) {
   EncodeTiledFn enc = get_encode();
   if (enc == nullptr) return -1;
   if ((reinterpret_cast<uintptr_t>(base) & 15) || ld % 8 || stride % 8) return -2;
@@ -387,7 +387,7 @@ int make_tmap_3d_16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t
   cuuint32_t box[3] = {box_inner, box_outer, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -3;
 }

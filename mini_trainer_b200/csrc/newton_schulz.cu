@@ -6,15 +6,13 @@
 // and n the longer a step is the products r r n, r r r and r r n; the first two are symmetric: only the tiles on and below the diagonal are computed, and the epilogue stores a tile
 // and its transpose. 3 r^2 n + r^3 operations a step instead of 4 r^2 n + 2 r^3.
 //
-// Two identities keep the epilogues free of operands: with s = b / 2c the gram product's epilogue adds s to the diagonal, M = A + s I, and then
-//   a I + b A + c A^2 = c M^2 + (a - b^2 / 4c) I
-// is one square with a constant on the diagonal, and the step's last product has the linear term in it.
+// The second product's epilogue adds b A and a I to c A^2, so that the third has the linear term in it.
 //
-// Numbers. Operands are fp16, X 2^p with 2^p about the root of the longer side, and M and the polynomial about 2^12: entries of all three then lie in the middle of the type's
-// range (|X| <= 1.3 and |M|, |polynomial| <= 3.5 in norm, whatever G is). Its 11 bits are eight times finer than bf16's 8. That alone is not enough: a rounding of X is noise
+// Numbers. Operands are fp16, X 2^p with 2^p about the root of the longer side, and A and the polynomial about 2^12: entries of all three then lie in the middle of the type's
+// range (|X| <= 1.3, |A| <= 1.6 and |polynomial| <= 3.5 in norm, whatever G is). Its 11 bits are eight times finer than bf16's 8. That alone is not enough: a rounding of X is noise
 // in all directions, and a direction in which X has next to nothing grows by a = 3.44 in each step, 485 times in five. So X is held as two numbers, hi and lo = 2^11 (X - hi), and the
 // last product's epilogue adds a lo to the polynomial times hi: what is left of the rounding is what b A and c A^2 would have made of it, which is small
-// in just those directions. The last step's X goes without. Error of the result, relative, simulated with the roundings: normal 512 x 1376 1.7e-3 (bf16 throughout: 1.1e-2), features of different
+// in just those directions. What is rounded in the last two steps grows little more; their X goes without. Error of the result, relative, simulated with the roundings: normal 512 x 1376 1.7e-3 (bf16 throughout: 1.1e-2), features of different
 // size 1.4e-3 (9e-2), rank 8 and a hundredth of noise 2.2e-3 (0.26), rank 1 2.7e-3 (0.76); half of bf16's step, to which the result is rounded, is 1.7e-3 in the mean. Sums are fp32 in tensor memory.
 //
 // The products: persistent, warp-specialised, 3-D TMA maps over the stack, tcgen05.mma of fp16 into two accumulators in tensor memory, by single CTAs (tiles of 128 x 128, for few tiles) or CTA pairs
@@ -30,22 +28,21 @@
 
 namespace mtb {
 
-int make_tmap_3d_16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t n, uint64_t ld, uint64_t stride, uint32_t box_inner, uint32_t box_outer, bool swizzle);
+int make_tmap_3d_16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t n, uint64_t ld, uint64_t stride, uint32_t box_inner, uint32_t box_outer);
 
 namespace ns {
 
 constexpr double NS_A = 3.4445, NS_B = -4.7750, NS_C = 2.0315;
-// Factors of M and of the polynomial in fp16, about 2^12, such that what M has on its diagonal where A is next to nothing, s, and the polynomial's value there, a, are numbers of the type.
-constexpr double NS_S = NS_B / (2.0 * NS_C), NS_D = NS_A - static_cast<double>(NS_B) * NS_B / (4.0 * NS_C);
-constexpr double SCALE_M = 4816.0 / -NS_S, SCALE_P = 14112.0 / NS_A;
+// Factors of A and of the polynomial in fp16, about 2^12; the second such that the polynomial's value where A is next to nothing, a, is a number of the type.
+constexpr double SCALE_A = 4096.0, SCALE_P = 14112.0 / NS_A;
 constexpr int LO_BITS = 11;
-constexpr int BM = 128, BK = 64, STAGES = 6;
+constexpr int BM = 128, BK = 64, STAGES = 5;
 constexpr int OP_BYTES = BM * BK * 2;                    // an operand's part of a stage: 128 rows (or columns) of 64
 constexpr int STAGE_BYTES = 2 * OP_BYTES;
 constexpr int EPI_WARPS = 8;                             // two to a quarter of the rows
-constexpr int BOX = 32 * 128;
+constexpr int BOX = 32 * 128;                            // a warp's staging: 32 rows of 128 bytes, or 64 of 64; and as much for what is added
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
-constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * BOX + 1024 + 256;
+constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * 2 * BOX + 1024 + 256;
 constexpr int GROUP_M = 8;
 constexpr uint32_t PEER_MASK = 0xFEFFFFFFu;              // of a shared::cluster address: the same place in CTA 0
 static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -56,11 +53,13 @@ enum { SYM = 0, APPLY = 1 };
 struct Params {
   int M, N, K, stack;
   int workers, group_m;
-  float alpha, diag;             // D = alpha product (SYM: + diag on the diagonal)
-  const __half* lo;              // APPLY: D += beta lo, laid out like D's hi
+  float alpha, diag;             // D = alpha product + beta res (SYM: + diag on the diagonal)
+  uint16_t* d;                   // fp16, or (bf16_out) bf16; rows padded to whole 16 bytes
+  uint16_t* lo;                  // APPLY: 2^11 of what D's rounding has left, or null
+  const __half* res;             // or null
   float beta;
-  long long ld, stride;          // of lo
-  int write_lo, bf16_out;        // APPLY
+  long long ld, stride;          // of d, lo and res
+  int bf16_out;                  // APPLY
   int* status;
 };
 
@@ -100,9 +99,9 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 template <int CTAS>
-__device__ __forceinline__ void commit(uint64_t* bar) {
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader = 0) {   // `leader`: number of the pair's first CTA in its cluster
   if constexpr (CTAS == 2) {
-    const uint16_t mask = 3;
+    const uint16_t mask = static_cast<uint16_t>(3u << leader);
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(mask) : "memory");
   } else {
     umma_commit(bar);
@@ -123,6 +122,12 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
+// A producer that gave up: until the last of its `issued` loads have landed, or a while has passed.
+__device__ __forceinline__ void settle_loads(uint64_t* full_bar, uint32_t issued) {
+  for (uint32_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+    for (uint32_t n = 0; n < (1u << 22) && !mbar_try_wait(&full_bar[i % STAGES], (i / STAGES) & 1); ++n) {}
+}
+
 // Tile `t` of a matrix: on and below the diagonal row by row, or in bands of group_m row-tiles.
 template <int KIND>
 __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int group_m, int& tm, int& tn) {
@@ -139,14 +144,100 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int gro
   }
 }
 
+// A warp's 32 rows of 64 columns between memory and registers go by its staging in shared memory: eight lanes to a row there, a lane to a row here. (TMA stores of the staged boxes queue
+// behind the operands' loads, up to six stages of them, and a tile has four to wait for: 64 x 2048 x 1024 3.2 ms, APPLY_TIMES.)
+__device__ __forceinline__ uint4* staged(uint8_t* box, int row, int piece) { return reinterpret_cast<uint4*>(box + row * 128 + ((piece ^ (row & 7)) << 4)); }
+// What is added to the sums, into the second box, asked for ahead of them, so that it arrives under their wait.
+__device__ __forceinline__ void ask(const Params& p, uint8_t* box, int y0, int col, int z, int lane) {
+  if (p.res == nullptr) return;
+  const __half* src = p.res + z * p.stride + static_cast<long long>(y0 + (lane >> 3)) * p.ld + col + (lane & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)   // (what is past the matrix stays as it was, and what it is added to is not stored)
+    if (y0 + (lane >> 3) + 4 * i < p.M && col + (lane & 7) * 8 < p.N)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(staged(box + BOX, (lane >> 3) + 4 * i, lane & 7))), "l"(src + 4 * i * p.ld) : "memory");
+}
+__device__ __forceinline__ void arrived() { asm volatile("cp.async.wait_all;" ::: "memory"); __syncwarp(); }
+// `h`: this lane's row, to rows [y0, y0 + 32) and columns [col, col + 64) of a matrix of which [rows, cols] exist.
+__device__ __forceinline__ void put(uint16_t* to, long long ld, int rows, int cols, int y0, int col, uint8_t* box, const uint32_t (&h)[32], int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) *staged(box, lane, i) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+  __syncwarp();
+  uint16_t* dst = to + static_cast<long long>(y0 + (lane >> 3)) * ld + col + (lane & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (y0 + (lane >> 3) + 4 * i < rows && col + (lane & 7) * 8 < cols) *reinterpret_cast<uint4*>(dst + 4 * i * ld) = *staged(box, (lane >> 3) + 4 * i, lane & 7);
+}
+// 64 columns of a warp's 32 rows (a lane has a row), from the product's sums `f` to the stores.
+template <int KIND>
+__device__ __forceinline__ void finish64(const Params& p, float* f, uint8_t* box, bool diagonal, int y0, int col, int z, int lane, bool more = false) {   // `more`: the next 64 columns come after these
+#pragma unroll
+  for (int j = 0; j < 64; ++j) f[j] *= p.alpha;
+  if (p.res != nullptr) {
+    arrived();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 u = *staged(box + BOX, lane, i);
+      const float2 a = unpack_f16(u.x), b = unpack_f16(u.y), d = unpack_f16(u.z), e = unpack_f16(u.w);
+      f[8 * i] += p.beta * a.x; f[8 * i + 1] += p.beta * a.y; f[8 * i + 2] += p.beta * b.x; f[8 * i + 3] += p.beta * b.y;
+      f[8 * i + 4] += p.beta * d.x; f[8 * i + 5] += p.beta * d.y; f[8 * i + 6] += p.beta * e.x; f[8 * i + 7] += p.beta * e.y;
+    }
+    __syncwarp();
+    if (more) ask(p, box, y0, col + 64, z, lane);
+  }
+  uint32_t h[32];
+  uint16_t* d = p.d + z * p.stride;
+  if constexpr (KIND == SYM) {
+    if (diagonal) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) if (col + j == y0 + lane) f[j] += p.diag;
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) h[j] = pack_f16(f[2 * j], f[2 * j + 1]);
+    put(d, p.ld, p.M, p.N, y0, col, box, h, lane);
+    if (!diagonal) {
+      // The transpose: 64 rows (this tile's columns) of 32 (its rows). Neighbouring lanes exchange a word, so that each writes two rows' entries of one column.
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, h[j], 1);
+        const uint32_t word = lane & 1 ? __byte_perm(o, h[j], 0x7632) : __byte_perm(h[j], o, 0x5410);
+        *reinterpret_cast<uint32_t*>(box + (2 * j + (lane & 1)) * 64 + (lane >> 1) * 4) = word;
+      }
+      __syncwarp();
+      uint16_t* dst = d + static_cast<long long>(col + (lane >> 2)) * p.ld + y0 + (lane & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + (lane >> 2) + 8 * i < p.N && y0 + (lane & 3) * 8 < p.M)
+          *reinterpret_cast<uint4*>(dst + 8 * i * p.ld) = *reinterpret_cast<const uint4*>(box + ((lane >> 2) + 8 * i) * 64 + (lane & 3) * 16);
+    }
+  } else {
+    if (p.bf16_out) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) h[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) h[j] = pack_f16(f[2 * j], f[2 * j + 1]);
+    }
+    put(d, p.ld, p.M, p.N, y0, col, box, h, lane);
+    if (p.lo != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float2 hi = unpack_f16(h[j]);
+        h[j] = pack_f16((f[2 * j] - hi.x) * (1 << LO_BITS), (f[2 * j + 1] - hi.y) * (1 << LO_BITS));
+      }
+      put(p.lo + z * p.stride, p.ld, p.M, p.N, y0, col, box, h, lane);
+    }
+  }
+}
+
 template <int CTAS, bool A_MN, bool B_MN, int KIND>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1)
-product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_d,
-               const __grid_constant__ CUtensorMap map_t, const Params p) {   // map_t: SYM: the transposed boxes of D; APPLY: lo of D
+product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
   constexpr int TILE = BM * CTAS;      // rows and columns of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + EPI_WARPS * BOX);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + EPI_WARPS * 2 * BOX);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
@@ -166,7 +257,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     fence_mbar_init();
     tma_prefetch_desc(&map_a);
     tma_prefetch_desc(&map_b);
-    tma_prefetch_desc(&map_d);
   }
   if (warp == 1) {
     if constexpr (CTAS == 2) {
@@ -194,7 +284,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const int row = tm * TILE + static_cast<int>(rank) * BM, col = tn * TILE + static_cast<int>(rank) * BM;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % STAGES;
-          if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 71); goto done; }
+          if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 71); if (rank == 0) settle_loads(full_bar, it); goto done; }
           uint8_t* sa = smem + s * STAGE_BYTES;
           const uint32_t bar = CTAS == 2 ? smem_u32(&full_bar[s]) & PEER_MASK : smem_u32(&full_bar[s]);
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * STAGE_BYTES);
@@ -231,96 +321,26 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   } else {
     // epilogue: quarter q of the rows, half of the columns, 64 at a time
     const int q = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* box = smem + STAGES * STAGE_BYTES + (warp - 2) * BOX;
+    uint8_t* box = smem + STAGES * STAGE_BYTES + (warp - 2) * 2 * BOX;
     uint32_t n = 0;
     for (int w = worker; w < items; w += p.workers, ++n) {
       int tm, tn;
       const int z = w / tiles;
       tile_at<KIND>(w - z * tiles, tiles_m, tiles_n, p.group_m, tm, tn);
+      const int y0 = tm * TILE + static_cast<int>(rank) * BM + q * 32, c0 = half * (TILE / 2);
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (n & 1) * TILE;
+      ask(p, box, y0, tn * TILE + c0, z, lane);
       if (!mbar_wait(&tfull_bar[n & 1], (n >> 1) & 1, abort_flag)) { atomicExch(p.status, 74); goto done; }
       tc_fence_after();
-      const int y0 = tm * TILE + static_cast<int>(rank) * BM + q * 32, row = y0 + lane;
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (n & 1) * TILE;
 #pragma unroll 1
-      for (int c = half * (TILE / 2); c < (half + 1) * (TILE / 2); c += 64) {
+      for (int c = c0; c < c0 + TILE / 2; c += 64) {
         const int col = tn * TILE + c;
         if (y0 >= p.M || col >= p.N) break;
         uint32_t v[2][32];
         tmem_ld_32x32(taddr + c, v[0]);
         tmem_ld_32x32(taddr + c + 32, v[1]);
         tmem_ld_wait();
-        float* f = reinterpret_cast<float*>(&v[0][0]);
-#pragma unroll
-        for (int j = 0; j < 64; ++j) f[j] *= p.alpha;
-        auto free_box = [&]() {
-          if (lane == 0) bulk_wait_read<0>();
-          __syncwarp();
-        };
-        auto send = [&](const CUtensorMap& map, int x, int y) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) { tma_store_3d(&map, box, x, y, z); bulk_commit(); }
-        };
-        auto stage = [&](const uint32_t (&h)[32]) {   // this thread's row of the box, 128B-swizzled
-#pragma unroll
-          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-        };
-        uint32_t h[32];
-        if constexpr (KIND == SYM) {
-          if (tm == tn) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) if (col + j == row) f[j] += p.diag;
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) h[j] = pack_f16(f[2 * j], f[2 * j + 1]);
-          free_box();
-          stage(h);
-          send(map_d, col, y0);
-          if (tm != tn) {
-            // The transpose: box of 64 rows (this tile's columns) x 32 (its rows). Neighbouring lanes exchange a word, so that each writes two rows' entries of one column.
-            free_box();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const uint32_t o = __shfl_xor_sync(0xffffffffu, h[j], 1);
-              const uint32_t word = lane & 1 ? __byte_perm(o, h[j], 0x7632) : __byte_perm(h[j], o, 0x5410);
-              *reinterpret_cast<uint32_t*>(box + (2 * j + (lane & 1)) * 64 + (lane >> 1) * 4) = word;
-            }
-            send(map_t, y0, col);
-          }
-        } else {
-          if (p.lo != nullptr && row < p.M) {
-            const __half* src = p.lo + z * p.stride + static_cast<long long>(row) * p.ld + col;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (col + 8 * i < p.N) {   // (rows are padded to whole pieces)
-                const uint4 u = *reinterpret_cast<const uint4*>(src + 8 * i);
-                const float2 a = unpack_f16(u.x), b = unpack_f16(u.y), d = unpack_f16(u.z), e = unpack_f16(u.w);
-                f[8 * i] += p.beta * a.x; f[8 * i + 1] += p.beta * a.y; f[8 * i + 2] += p.beta * b.x; f[8 * i + 3] += p.beta * b.y;
-                f[8 * i + 4] += p.beta * d.x; f[8 * i + 5] += p.beta * d.y; f[8 * i + 6] += p.beta * e.x; f[8 * i + 7] += p.beta * e.y;
-              }
-            }
-          }
-          if (p.bf16_out) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) h[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) h[j] = pack_f16(f[2 * j], f[2 * j + 1]);
-          }
-          free_box();
-          stage(h);
-          send(map_d, col, y0);
-          if (p.write_lo) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float2 hi = unpack_f16(h[j]);
-              h[j] = pack_f16((f[2 * j] - hi.x) * (1 << LO_BITS), (f[2 * j + 1] - hi.y) * (1 << LO_BITS));
-            }
-            free_box();
-            stage(h);
-            send(map_t, col, y0);
-          }
-        }
+        finish64<KIND>(p, reinterpret_cast<float*>(&v[0][0]), box, tm == tn, y0, col, z, lane, c + 64 < c0 + TILE / 2 && col + 64 < p.N);
       }
       tc_fence_before();
       __syncwarp();
@@ -328,7 +348,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
   }
 done:
-  if (warp >= 2 && lane == 0) bulk_wait_read<0>();
   tc_fence_before();
   __syncthreads();
   if constexpr (CTAS == 2) cluster_barrier();   // nobody tears down while the partner may still signal or read
@@ -339,9 +358,151 @@ done:
   }
 }
 
+// The same product with its reduction divided over the CTAs (or pairs) of a cluster, for launches of few tiles: one tile to a cluster. An SM takes a tile's operands from L2 at 64 bytes a clock, 512 clocks for
+// 64 of the reduction, which is what a launch of one round lasts for; `splits` SMs take it in parts. When all have multiplied, each sends every other the sums of the rows that one finishes, fp32 through
+// the cluster's shared memory (over the operands' stages), and finishes its own: 128 / splits rows, added in the order of the parts.
+constexpr int MOST_SPLITS = 4;
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, float a, float b, float c, float d) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(r), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+template <int CTAS, bool A_MN, bool B_MN, int KIND>
+__global__ void __launch_bounds__(THREADS, 1)
+split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p, const int splits) {
+  constexpr int TILE = BM * CTAS;
+  static_assert(STAGES * STAGE_BYTES >= TILE * 128 * 4, "the sums of a tile's rows fit over the stages");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + EPI_WARPS * 2 * BOX);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t in_cluster = cluster_rank(), rank = in_cluster % CTAS;
+  const int split = in_cluster / CTAS, item = blockIdx.x / (CTAS * splits);
+  const int tiles_m = (p.M + TILE - 1) / TILE, tiles_n = (p.N + TILE - 1) / TILE;
+  const int tiles = KIND == SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * tiles_n;
+  const int kblocks = (p.K + BK - 1) / BK, kb0 = kblocks * split / splits, n = kblocks * (split + 1) / splits - kb0;
+  const int z = item / tiles;
+  int tm, tn;
+  tile_at<KIND>(item - z * tiles, tiles_m, tiles_n, p.group_m, tm, tn);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+    mbar_init(tfull_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    if constexpr (CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TILE) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(tmem_slot, TILE);
+      tmem_relinquish();
+    }
+  }
+  pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const int row = tm * TILE + static_cast<int>(rank) * BM, col = tn * TILE + static_cast<int>(rank) * BM;
+      for (int it = 0; it < n; ++it) {
+        const int s = it % STAGES;
+        if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 71); if (rank == 0) settle_loads(full_bar, it); break; }
+        uint8_t* sa = smem + s * STAGE_BYTES;
+        const uint32_t bar = CTAS == 2 ? smem_u32(&full_bar[s]) & PEER_MASK : smem_u32(&full_bar[s]);
+        if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * STAGE_BYTES);
+        load_operand<CTAS, A_MN>(sa, &map_a, bar, row, (kb0 + it) * BK, z);
+        load_operand<CTAS, B_MN>(sa + OP_BYTES, &map_b, bar, col, (kb0 + it) * BK, z);
+      }
+      pdl_trigger();
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = idesc_f16(TILE, TILE, A_MN, B_MN);
+      for (int it = 0; it < n; ++it) {
+        const int s = it % STAGES;
+        if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag)) { atomicExch(p.status, 73); break; }
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + s * STAGE_BYTES), sb = sa + OP_BYTES;
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k) {
+          const uint64_t da = A_MN ? make_smem_desc(sa + k * 2048, 8192, 1024) : make_smem_desc(sa + k * 32, 16, 1024);
+          const uint64_t db = B_MN ? make_smem_desc(sb + k * 2048, 8192, 1024) : make_smem_desc(sb + k * 32, 16, 1024);
+          mma<CTAS>(tmem_base, da, db, idesc, it != 0 || k != 0);
+        }
+        commit<CTAS>(&empty_bar[s], in_cluster);
+      }
+      commit<CTAS>(tfull_bar, in_cluster);
+    }
+  } else if (!mbar_wait(tfull_bar, 0, abort_flag)) {
+    if (lane == 0) atomicExch(p.status, 74);
+  }
+  __syncthreads();
+  cluster_barrier();   // every CTA has multiplied: nothing reads the stages any more
+  tc_fence_after();
+  // quarter q of the rows is finished by part q / (4 / splits); [part][quarter of those][4 columns][row] of 16 bytes
+  const int q = warp & 3, half = (warp - 2) >> 2, per_owner = 4 / splits;
+  if (warp >= 2) {
+    const uint32_t owner = static_cast<uint32_t>(q / per_owner) * CTAS + rank;
+    const uint32_t at = smem_u32(smem) + (split * per_owner + q % per_owner) * (TILE * 128) + lane * 16;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+#pragma unroll 1
+    for (int c = half * (TILE / 2); c < (half + 1) * (TILE / 2); c += 32) {
+      uint32_t v[32];
+      tmem_ld_32x32(taddr + c, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; j += 4)
+        store_remote(at + (c + j) / 4 * 512, owner, __uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();   // ... and every part has arrived
+  if (warp >= 2) {
+    uint8_t* box = smem + STAGES * STAGE_BYTES + (warp - 2) * 2 * BOX;
+    for (int u = warp - 2; u < per_owner * (TILE / 64); u += EPI_WARPS) {
+      const int mine = u % per_owner, c = u / per_owner * 64;
+      const int y0 = tm * TILE + static_cast<int>(rank) * BM + (split * per_owner + mine) * 32, col = tn * TILE + c;
+      if (y0 >= p.M || col >= p.N) continue;
+      ask(p, box, y0, col, z, lane);
+      float f[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) f[j] = 0.f;
+      for (int s = 0; s < splits; ++s) {
+        const uint8_t* src = smem + (s * per_owner + mine) * (TILE * 128) + c / 4 * 512 + lane * 16;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float4 v = *reinterpret_cast<const float4*>(src + j * 512);
+          f[4 * j] += v.x; f[4 * j + 1] += v.y; f[4 * j + 2] += v.z; f[4 * j + 3] += v.w;
+        }
+      }
+      finish64<KIND>(p, f, box, tm == tn, y0, col, z, lane);
+    }
+  }
+  __syncthreads();
+  if constexpr (CTAS == 2) cluster_barrier();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TILE) : "memory");
+    else tmem_dealloc(tmem_base, TILE);
+  }
+}
+
 // ------------------------------------------------------------------------------------------ in front of the products, and behind them
 constexpr int LIN_THREADS = 256;
-constexpr int MOST_CHUNKS = 1024;   // of a matrix, in the sums of squares
+constexpr int MOST_CHUNKS = 2048;   // of a stack, in the sums of squares
 
 // What is orthogonalised: a gradient, or a momentum that takes the gradient in first.
 struct Source {
@@ -414,13 +575,25 @@ __global__ void __launch_bounds__(LIN_THREADS) squares_kernel(Source s, long lon
   const long long lo = c * per_chunk, hi = min(numel, lo + per_chunk), base = z * numel;
   const float coef = s.coef != nullptr ? *s.coef : 1.f;
   double total = 0.0;
-  for (long long i = lo + threadIdx.x * 8; i < hi; i += LIN_THREADS * 8) {
-    float u[8];
-    source8(s, coef, base + i, static_cast<int>(min(8ll, hi - i)), vec != 0, true, u);
+  auto add = [&](const float (&u)[8]) {
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) q = fmaf(u[j], u[j], q);
     total += q;
+  };
+  constexpr int STEP = LIN_THREADS * 8, AHEAD = 4;
+  long long i = lo + threadIdx.x * 8;
+  for (; i + (AHEAD - 1) * STEP + 8 <= hi; i += AHEAD * STEP) {   // several loads under way
+    float u[AHEAD][8];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) source8(s, coef, base + i + a * STEP, 8, vec != 0, true, u[a]);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) add(u[a]);
+  }
+  for (; i < hi; i += STEP) {
+    float u[8];
+    source8(s, coef, base + i, static_cast<int>(min(8ll, hi - i)), vec != 0, true, u);
+    add(u);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -508,16 +681,13 @@ __global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__
 
 // ------------------------------------------------------------------------------------------ host
 struct Matrix {            // stack of fp16 matrices with padded rows
-  const void* p;
+  uint16_t* p;
   long long rows, cols, ld, stack;
-  CUtensorMap k, mn, d, t;   // loads with the columns as the reduction, or with the rows; stores, and of transposed boxes
-  int make(bool transposed) {
+  CUtensorMap k, mn;       // loads with the columns as the reduction, or with the rows
+  int make() {
     const uint64_t stride = static_cast<uint64_t>(rows) * ld;
-    int rc = make_tmap_3d_16(&k, p, cols, rows, stack, ld, stride, BK, BM, true);
-    if (!rc) rc = make_tmap_3d_16(&mn, p, cols, rows, stack, ld, stride, 64, 64, true);
-    if (!rc) rc = make_tmap_3d_16(&d, p, cols, rows, stack, ld, stride, 64, 32, true);
-    if (!rc && transposed) rc = make_tmap_3d_16(&t, p, cols, rows, stack, ld, stride, 32, 64, false);
-    return rc;
+    const int rc = make_tmap_3d_16(&k, p, cols, rows, stack, ld, stride, BK, BM);
+    return rc ? rc : make_tmap_3d_16(&mn, p, cols, rows, stack, ld, stride, 64, 64);
   }
 };
 
@@ -529,30 +699,86 @@ static int sm_count() {
   }
   return n;
 }
+// Clusters of a split product that can be resident at once; 0 where the device has none of that size.
+template <int CTAS>
+static int resident_clusters(int splits) {
+  static int known[MOST_SPLITS + 1] = {-1, -1, -1, -1, -1};
+  if (known[splits] < 0) {
+    auto kern = split_kernel<CTAS, false, false, SYM>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(CTAS * splits);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = CTAS * splits; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+    known[splits] = n;
+  }
+  return known[splits];
+}
+struct Form { int ctas, splits; };
+// The form of a product by what its rounds of tiles take, in us: 64 of the reduction 0.28 on a single CTA (its operands from L2 at 64 bytes a clock) and 0.30 on a pair, up to 0.36 and 0.43
+// where all SMs multiply at once; and what stands in front of and behind them. Fitted to stacks of 1 to 64 matrices of 64 to 4096: 1024 x 1024 122 us in single CTAs and 201 in pairs, 4096 x 4096 1370 and 1114, 512 x 512 95 and 163, in
+// parts of a half 116 and 157; 1001 x 4097 299 and 327, 239 with the gram product on pairs in four parts; 1536 x 8960 466 and 520, 422 with it on single CTAs in two.
+static Form choose(long long M, long long N, long long K, long long stack, bool sym, int pairs, int sms) {
+  constexpr double base[2][3] = {{3.0, 6.0, 6.8}, {8.0, 8.7, 9.1}};
+  auto tiles = [&](long long tile) {
+    const long long tm = (M + tile - 1) / tile, tn = (N + tile - 1) / tile;
+    return (sym ? tm * (tm + 1) / 2 : tm * tn) * stack;
+  };
+  const long long kb = (K + BK - 1) / BK;
+  Form best{1, 1};
+  double least = 1e30;
+  for (int ctas = 1; ctas <= 2; ++ctas)
+    for (int s = 0; 1 << s <= MOST_SPLITS; ++s) {
+      const int splits = 1 << s;
+      if ((ctas == 2 && pairs <= 0) || (s && kb < 2 * splits)) continue;
+      const int room = s == 0 ? (ctas == 2 ? pairs : sms) : ctas == 2 ? resident_clusters<2>(splits) : resident_clusters<1>(splits);
+      if (room <= 0) continue;
+      const long long n = tiles(BM * ctas), whole = n / room, rest = n % room;   // rounds of all workers, and what is left
+      const double parts = static_cast<double>((kb + splits - 1) / splits);
+      auto part = [&](long long at_once) {
+        const double busy = at_once * splits * ctas >= sms ? 1.0 : static_cast<double>(at_once * splits * ctas) / sms;
+        return parts * (ctas == 2 ? 0.30 + 0.13 * busy : 0.28 + 0.08 * busy);
+      };
+      const double each = s == 0 ? 0.0 : base[ctas - 1][s];   // a split product has nothing of the next round under its epilogue
+      const double t = whole * (part(room) + each) + (rest ? part(rest) + each : 0.0) + (s == 0 ? base[ctas - 1][0] : 0.0);
+      if (t < least) { least = t; best = Form{ctas, splits}; }
+    }
+  return best;
+}
 template <int CTAS, bool A_MN, bool B_MN, int KIND>
-static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& d, const CUtensorMap& t, Params p, int workers, cudaStream_t st) {
+static int launch(const CUtensorMap& a, const CUtensorMap& b, Params p, int splits, int workers, cudaStream_t st) {
   auto kern = product_kernel<CTAS, A_MN, B_MN, KIND>;
+  auto split = split_kernel<CTAS, A_MN, B_MN, KIND>;
   static bool configured = false;
   if (!configured) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -4;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -4;
     configured = true;
   }
   const long long tile = BM * CTAS, tm = (p.M + tile - 1) / tile, tn = (p.N + tile - 1) / tile;
   const long long items = (KIND == SYM ? tm * (tm + 1) / 2 : tm * tn) * p.stack;
-  if (items >= 1ll << 30) return -10;
-  p.workers = static_cast<int>(items < workers ? items : workers);
+  if (items >= 1ll << 27) return -10;
   p.group_m = GROUP_M;
-  launch_pdl(kern, p.workers * CTAS, THREADS, SMEM, st, a, b, d, t, p);
+  if (splits > 1) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CTAS * splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(items * CTAS * splits)); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM; cfg.stream = st;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, split, a, b, p, splits) == cudaSuccess ? 0 : -5;
+  }
+  p.workers = static_cast<int>(items < workers ? items : workers);
+  launch_pdl(kern, p.workers * CTAS, THREADS, SMEM, st, a, b, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
-}
-// Rounds of single CTAs and of pairs over a product's tiles, by how long a round takes.
-static bool prefers_pairs(long long M, long long N, long long stack, bool sym, int pairs, int sms) {
-  if (pairs <= 0) return false;
-  auto rounds = [&](long long tile, long long workers) {
-    const long long tm = (M + tile - 1) / tile, tn = (N + tile - 1) / tile;
-    return ((sym ? tm * (tm + 1) / 2 : tm * tn) * stack + workers - 1) / workers;
-  };
-  return rounds(256, pairs) * 2.0 <= rounds(128, sms) * 1.2;
 }
 
 static long long up(long long x, long long to) { return (x + to - 1) / to * to; }
@@ -586,48 +812,48 @@ static int orthogonalise(const Source& src, long long rows, long long cols, long
   const long long per_chunk = up((numel + l.chunks - 1) / l.chunks, 8 * LIN_THREADS);
   if (stack * l.chunks >= 1ll << 31) return -10;
   launch_pdl(squares_kernel, static_cast<unsigned>(stack * l.chunks), LIN_THREADS, 0, st, src, numel, static_cast<int>(l.chunks), per_chunk, vec_flat, sums);
+  const int kept = steps > 2 ? steps - 2 : steps - 1;   // steps whose X is held as two numbers
   long long blocks = (rows * l.ld / 8 + LIN_THREADS - 1) / LIN_THREADS, most = (sm_count() * 8 + stack - 1) / stack;
   if (blocks > most) blocks = most;
   launch_pdl(scale_kernel, static_cast<unsigned>(stack * blocks), LIN_THREADS, 0, st, src, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(l.ld), static_cast<int>(l.chunks),
-             static_cast<int>(blocks), vec_rows, p2, sums, x[0][0], steps > 1 ? x[0][1] : nullptr);
+             static_cast<int>(blocks), vec_rows, p2, sums, x[0][0], kept > 0 ? x[0][1] : nullptr);
   if (cudaGetLastError() != cudaSuccess) return -5;
 
-  Matrix xh[2], xl[2], gram{g, l.r, l.r, l.ldr, stack}, poly{g + l.gbytes, l.r, l.r, l.ldr, stack}, last{out, rows, cols, out_ld, stack};
+  Matrix xh[2], gram{(uint16_t*)g, l.r, l.r, l.ldr, stack}, poly{(uint16_t*)(g + l.gbytes), l.r, l.r, l.ldr, stack};
   for (int i = 0; i < 2; ++i) {
-    xh[i] = Matrix{x[i][0], rows, cols, l.ld, stack};
-    xl[i] = Matrix{x[i][1], rows, cols, l.ld, stack};
-    int rc = xh[i].make(false);
-    if (!rc) rc = xl[i].make(false);
-    if (rc) return rc - 20;
+    xh[i] = Matrix{(uint16_t*)x[i][0], rows, cols, l.ld, stack};
+    if (const int rc = xh[i].make()) return rc - 20;
   }
-  int rc = gram.make(true);
-  if (!rc) rc = poly.make(true);
-  if (!rc && out != nullptr) rc = last.make(false);
+  int rc = gram.make();
+  if (!rc) rc = poly.make();
   if (rc) return rc - 30;
 
   const int sms = sm_count();
-  const bool sym2 = prefers_pairs(l.r, l.r, stack, true, pairs, sms), app2 = prefers_pairs(rows, cols, stack, false, pairs, sms);
   const int r = static_cast<int>(l.r), K = static_cast<int>(right ? rows : cols);
+  const Form fg = choose(r, r, K, stack, true, pairs, sms), fp = choose(r, r, r, stack, true, pairs, sms), fa = choose(rows, cols, r, stack, false, pairs, sms);
+#define PRODUCT(F, A_MN, B_MN, KIND, ...) (F.ctas == 2 ? launch<2, A_MN, B_MN, KIND>(__VA_ARGS__, F.splits, pairs, st) : launch<1, A_MN, B_MN, KIND>(__VA_ARGS__, F.splits, sms, st))
   for (int i = 0; i < steps; ++i) {
     const Matrix& X = xh[i & 1];
-    Params p{r, r, K, static_cast<int>(stack), 0, 0, static_cast<float>(ldexp(SCALE_M, -2 * p2)), static_cast<float>(SCALE_M * NS_S), nullptr, 0.f, 0, 0, 0, 0, status};
-    if (right) rc = sym2 ? launch<2, true, true, SYM>(X.mn, X.mn, gram.d, gram.t, p, pairs, st) : launch<1, true, true, SYM>(X.mn, X.mn, gram.d, gram.t, p, sms, st);
-    else rc = sym2 ? launch<2, false, false, SYM>(X.k, X.k, gram.d, gram.t, p, pairs, st) : launch<1, false, false, SYM>(X.k, X.k, gram.d, gram.t, p, sms, st);
+    Params p{r, r, K, static_cast<int>(stack), 0, 0, static_cast<float>(ldexp(SCALE_A, -2 * p2)), 0.f, gram.p, nullptr, nullptr, 0.f, l.ldr, l.r * l.ldr, 0, status};
+    rc = right ? PRODUCT(fg, true, true, SYM, X.mn, X.mn, p) : PRODUCT(fg, false, false, SYM, X.k, X.k, p);
     if (rc) return rc;
     p.K = r;
-    p.alpha = static_cast<float>(SCALE_P * NS_C / (SCALE_M * SCALE_M));
-    p.diag = static_cast<float>(SCALE_P * NS_D);
-    rc = sym2 ? launch<2, false, false, SYM>(gram.k, gram.k, poly.d, poly.t, p, pairs, st) : launch<1, false, false, SYM>(gram.k, gram.k, poly.d, poly.t, p, sms, st);
+    p.alpha = static_cast<float>(SCALE_P * NS_C / (SCALE_A * SCALE_A));
+    p.diag = static_cast<float>(SCALE_P * NS_A);
+    p.d = poly.p;
+    p.res = reinterpret_cast<const __half*>(gram.p);
+    p.beta = static_cast<float>(SCALE_P * NS_B / SCALE_A);
+    rc = PRODUCT(fp, false, false, SYM, gram.k, gram.k, p);
     if (rc) return rc;
-    const bool end = i + 1 == steps, to_out = end && out != nullptr;
+    const bool to_out = i + 1 == steps && out != nullptr;
+    const long long ld = to_out ? out_ld : l.ld;   // (the last step has no residual, whose rows would be another matrix's)
     Params a{static_cast<int>(rows), static_cast<int>(cols), r, static_cast<int>(stack), 0, 0, static_cast<float>(ldexp(1.0 / SCALE_P, to_out ? -p2 : 0)), 0.f,
-             end ? nullptr : x[i & 1][1], static_cast<float>(ldexp(NS_A, -LO_BITS)), l.ld, rows * l.ld, i + 2 < steps, to_out, status};
-    const CUtensorMap& to = to_out ? last.d : xh[(i + 1) & 1].d;
-    const CUtensorMap& lo = xl[(i + 1) & 1].d;
-    if (right) rc = app2 ? launch<2, false, false, APPLY>(X.k, poly.k, to, lo, a, pairs, st) : launch<1, false, false, APPLY>(X.k, poly.k, to, lo, a, sms, st);
-    else rc = app2 ? launch<2, false, true, APPLY>(poly.k, X.mn, to, lo, a, pairs, st) : launch<1, false, true, APPLY>(poly.k, X.mn, to, lo, a, sms, st);
+             to_out ? (uint16_t*)out : xh[(i + 1) & 1].p, i + 1 < kept ? (uint16_t*)x[(i + 1) & 1][1] : nullptr, i < kept ? x[i & 1][1] : nullptr, static_cast<float>(ldexp(NS_A, -LO_BITS)),
+             ld, rows * ld, to_out, status};
+    rc = right ? PRODUCT(fa, false, false, APPLY, X.k, poly.k, a) : PRODUCT(fa, false, true, APPLY, poly.k, X.mn, a);
     if (rc) return rc;
   }
+#undef PRODUCT
   return 0;
 }
 static int exponent(long long rows, long long cols) { return static_cast<int>(lround(0.5 * log2(static_cast<double>(rows > cols ? rows : cols)))); }

@@ -4,7 +4,8 @@ The plain form is fp32: a rounding of X (2^-24 of its entries) grows by at most 
 is far above it. The kernels hold X to 22 bits up to the last step, and M and the polynomial to 11: a rounding of those, 2^-12 of their entries, of uniform and independent sign, moves X by
 at most 2^-12 * 2 * 4.8 * |X| in a step through b (their spectral norm is at most that of a random matrix with such entries, and |M|, |polynomial| <= 3.5), and what a step has moved is carried on by at most the polynomial's slope
 at values near one, 1.5 on either side, and 3.9 at the largest (1.2): five steps add up to less than 2^-12 * 9.6 * (1 + 1.5 + 1.5^2 + 1.5^3 + 1.5^4) / sqrt(3) < 0.018 were all of it in
-one direction. It is spread over as many as the matrix has: TOL below is a third of that. The result is rounded by U = 2^-8 of an entry at most."""
+one direction. It is spread over as many as the matrix has: TOL below is a third of that. Where the few entries that are not zero meet in no row or column, each of them is a singular
+value and the products are diagonal: every rounding is in one direction, and the whole 0.018 = 3 TOL is what holds. The result is rounded by U = 2^-8 of an entry at most."""
 import math
 
 import pytest
@@ -161,7 +162,7 @@ def native():
 def test_kernels(native, shape, kind):
     g = matrices(kind, *shape, device="cuda")
     got = native.orthogonalise(g)
-    check(got, g, TOL)
+    check(got, g, 3 * TOL if kind in ("sparse", "one") else TOL)
     assert torch.equal(got, native.orthogonalise(g))
     native.check_status()
 
