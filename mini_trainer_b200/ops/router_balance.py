@@ -16,11 +16,10 @@ logits are; a sample without counted tokens has losses of zero. The factors of t
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
 
 import torch
 
-MOST_EXPERTS, MOST_CHOSEN = 512, 32   # of csrc/route_balance.cu
+MOST_EXPERTS, MOST_CHOSEN, _BLOCKS_PER_SM = 512, 32, 2   # of csrc/route_balance.cu
 
 
 @dataclass
@@ -30,8 +29,7 @@ class RouterBalance:
     counts: torch.Tensor    # [S, E] int32 pairs that chose an expert
     tokens: torch.Tensor    # [S] int32 counted tokens
     lse: torch.Tensor       # [T] fp32 logsumexp of every token's logits
-    cu_seqlens: Optional[torch.Tensor]   # as given
-    counted: Optional[torch.Tensor]      # as given
+    sample: torch.Tensor    # [T] int32 sample whose losses a token is in, -1 for none
 
 
 def _refuse(what, t, dtype, shape, device):
@@ -74,27 +72,19 @@ def check_bwd(probs, topi, w, dw, bal, dloss, dz, dtype):
         raise ValueError("without a gradient of the weights or of a loss there is nothing to do")
     for what, t, ty, shape in (("probs", probs, torch.float32, (T, E)), ("topi", topi, torch.int64, (T, k)), ("w", w, torch.float32, (T, k)), ("dw", dw, torch.float32, (T, k)),
                                ("dloss", dloss, torch.float32, (S,)), ("dz", dz, torch.float32, (S,)), ("counts", bal.counts, torch.int32, (S, E)),
-                               ("tokens", bal.tokens, torch.int32, (S,)), ("lse", bal.lse, torch.float32, (T,)), ("counted", bal.counted, torch.bool, (T,))):
+                               ("tokens", bal.tokens, torch.int32, (S,)), ("lse", bal.lse, torch.float32, (T,)), ("sample", bal.sample, torch.int32, (T,))):
         _expect(what, t, ty, shape, device)
-    if bal.cu_seqlens is not None:
-        _expect("cu_seqlens", bal.cu_seqlens, torch.int32, (S + 1,), device)
-    elif S != 1:
-        raise ValueError(f"{S} samples without their starts")
     return T, E, k, S
 
 
 # -- plain forms ----------------------------------------------------------------------------
-def _samples(T, bal):
-    """``[T]`` sample of each token, and whether it is in that sample's losses."""
-    cu, device = bal.cu_seqlens, bal.lse.device
+def _samples(T, cu, counted, device):
+    """``[T]`` int64: the sample whose losses a token is in, or -1."""
     at = torch.arange(T, device=device)
-    if cu is None:
-        sample, inside = torch.zeros_like(at), torch.ones(T, dtype=torch.bool, device=device)
-    else:
-        sample = torch.searchsorted(cu[1:].long().contiguous(), at, right=True)
-        inside = (sample < cu.shape[0] - 1) & (at >= cu[0])
-        sample = sample.clamp_max(cu.shape[0] - 2)
-    return sample, inside if bal.counted is None else inside & bal.counted
+    sample = torch.zeros_like(at) if cu is None else torch.searchsorted(cu[1:].long().contiguous(), at, right=True)
+    if cu is not None:
+        sample = torch.where((sample < cu.shape[0] - 1) & (at >= cu[0]), sample, -1)
+    return sample if counted is None else torch.where(counted, sample, -1)
 
 
 def plain(logits, k, renorm, cu_seqlens=None, counted=None):
@@ -104,8 +94,8 @@ def plain(logits, k, renorm, cu_seqlens=None, counted=None):
     topi = torch.argsort(l, dim=-1, descending=True, stable=True)[:, :k].contiguous()
     top = probs.gather(1, topi)
     w = top / top.sum(-1, keepdim=True) if renorm else top
-    bal = RouterBalance(None, None, None, None, lse, cu_seqlens, counted)
-    sample, ok = _samples(T, bal)
+    sample = _samples(T, cu_seqlens, counted, l.device)
+    ok = sample >= 0
     sums = torch.zeros(S, E, dtype=torch.float64, device=l.device).index_add_(0, sample[ok], probs[ok].double())
     counts = torch.zeros(S * E, dtype=torch.int64, device=l.device)
     chosen = (sample[ok, None] * E + topi[ok]).reshape(-1)
@@ -113,14 +103,14 @@ def plain(logits, k, renorm, cu_seqlens=None, counted=None):
     tokens = torch.zeros(S, dtype=torch.int64, device=l.device).index_add_(0, sample[ok], torch.ones_like(sample[ok]))
     n = tokens.clamp_min(1).double()
     z = torch.zeros(S, dtype=torch.float64, device=l.device).index_add_(0, sample[ok], lse[ok].double().square())
-    bal.loss, bal.z_loss = (E * (counts * sums).sum(1) / n.square()).float(), (z / n).float()
-    bal.counts, bal.tokens = counts.to(torch.int32), tokens.to(torch.int32)
-    return probs, topi, w, bal
+    loss, z = (E * (counts * sums).sum(1) / n.square()).float(), (z / n).float()
+    return probs, topi, w, RouterBalance(loss, z, counts.to(torch.int32), tokens.to(torch.int32), lse, sample.to(torch.int32))
 
 
 def plain_bwd(probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.bfloat16):
     T, E, k, S = check_bwd(probs, topi, w, dw, bal, dloss, dz, dtype)
-    sample, ok = _samples(T, bal)
+    ok = bal.sample >= 0
+    sample = bal.sample.long()
     n = bal.tokens.clamp_min(1).float()
     g = torch.zeros_like(probs)
     if dw is not None:
@@ -140,21 +130,20 @@ def native(ops, logits, k, renorm, cu_seqlens=None, counted=None):
     ops.check_device(logits)
     dev, f32, i32 = logits.device, torch.float32, torch.int32
     with ops.on_device():
-        sums = torch.empty(S, 2, dtype=f32, device=dev)
-        whole = torch.empty(S * (E + 1), dtype=i32, device=dev)
-        bal = RouterBalance(sums.view(-1)[:S], sums.view(-1)[S:], whole[:S * E].view(S, E), whole[S * E:], torch.empty(T, dtype=f32, device=dev), cu_seqlens, counted)
-        probs, topi, w = torch.empty(T, E, dtype=f32, device=dev), torch.empty(T, k, dtype=torch.int64, device=dev), torch.empty(T, k, dtype=f32, device=dev)
+        loss, z, lse, w = torch.empty(2 * S + T * (k + 1), dtype=f32, device=dev).split([S, S, T, T * k])
+        counts, tokens, sample = torch.empty(S * (E + 1) + T, dtype=i32, device=dev).split([S * E, S, T])
+        probs, topi = torch.empty(T, E, dtype=f32, device=dev), torch.empty(T, k, dtype=torch.int64, device=dev)
+        counts, w = counts.view(S, E), w.view(T, k)
         if T == 0:
-            sums.zero_()
-            whole.zero_()
-            return probs, topi, w, bal
-        rows = ops.lib.mtb200_route_balanced_rows(T, S)
-        part = torch.empty(rows * (E + 1), dtype=torch.int64, device=dev)
-        ops._call("mtb200_route_balanced", logits.data_ptr(), int(logits.dtype is f32), None if cu_seqlens is None else cu_seqlens.data_ptr(),
-                  None if counted is None else counted.data_ptr(), T, E, k, S, int(bool(renorm)), probs.data_ptr(), topi.data_ptr(), w.data_ptr(), bal.lse.data_ptr(),
-                  part.data_ptr(), part.data_ptr() + 8 * rows * E, bal.loss.data_ptr(), bal.z_loss.data_ptr(), bal.counts.data_ptr(), bal.tokens.data_ptr(),
-                  ops._st(), n=2)
-    return probs, topi, w, bal
+            for t in (loss, z, counts, tokens):
+                t.zero_()
+        else:
+            rows = _BLOCKS_PER_SM * ops.sms + S
+            part = torch.empty(rows * (E + 1), dtype=torch.int64, device=dev).data_ptr()
+            ops._call("mtb200_route_balanced", logits.data_ptr(), int(logits.dtype is f32), None if cu_seqlens is None else cu_seqlens.data_ptr(),
+                      None if counted is None else counted.data_ptr(), T, E, k, S, int(bool(renorm)), probs.data_ptr(), topi.data_ptr(), w.data_ptr(), lse.data_ptr(), sample.data_ptr(),
+                      part, part + 8 * rows * E, rows, loss.data_ptr(), z.data_ptr(), counts.data_ptr(), tokens.data_ptr(), ops._st(), n=2)
+    return probs, topi, w, RouterBalance(loss, z, counts, tokens, lse, sample)
 
 
 def native_bwd(ops, probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.bfloat16):
@@ -164,7 +153,7 @@ def native_bwd(ops, probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=
         out = torch.empty(T, E, dtype=dtype, device=probs.device)
         if T:
             ptr = lambda t: None if t is None else t.data_ptr()
-            ops._call("mtb200_route_balanced_bwd", probs.data_ptr(), topi.data_ptr(), w.data_ptr(), ptr(dw), bal.lse.data_ptr(), ptr(bal.cu_seqlens), ptr(bal.counted),
+            ops._call("mtb200_route_balanced_bwd", probs.data_ptr(), topi.data_ptr(), w.data_ptr(), ptr(dw), bal.lse.data_ptr(), bal.sample.data_ptr(),
                       bal.counts.data_ptr(), bal.tokens.data_ptr(), ptr(dloss), ptr(dz), T, E, k, S, int(bool(renorm)), out.data_ptr(), int(dtype is torch.float32),
                       ops.status.data_ptr(), ops._st())
     return out
