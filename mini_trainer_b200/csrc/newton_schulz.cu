@@ -287,9 +287,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 71); if (rank == 0) settle_loads(full_bar, it); goto done; }
           uint8_t* sa = smem + s * STAGE_BYTES;
           const uint32_t bar = CTAS == 2 ? smem_u32(&full_bar[s]) & PEER_MASK : smem_u32(&full_bar[s]);
-          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * STAGE_BYTES);
+          const bool once = KIND == SYM && tm == tn;   // the same rows twice
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * (once ? OP_BYTES : STAGE_BYTES));
           load_operand<CTAS, A_MN>(sa, &map_a, bar, row, kb * BK, z);
-          load_operand<CTAS, B_MN>(sa + OP_BYTES, &map_b, bar, col, kb * BK, z);
+          if (!once) load_operand<CTAS, B_MN>(sa + OP_BYTES, &map_b, bar, col, kb * BK, z);
         }
       }
       pdl_trigger();
@@ -299,6 +300,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       constexpr uint32_t idesc = idesc_f16(TILE, TILE, A_MN, B_MN);
       uint32_t it = 0, n = 0;
       for (int w = worker; w < items; w += p.workers, ++n) {
+        bool once = false;
+        if constexpr (KIND == SYM) {
+          int tm, tn;
+          tile_at<KIND>(w % tiles, tiles_m, tiles_n, p.group_m, tm, tn);
+          once = tm == tn;
+        }
         if (!mbar_wait(&tempty_bar[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 72); goto done; }
         tc_fence_after();
         const uint32_t d = tmem_base + (n & 1) * TILE;
@@ -306,7 +313,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const int s = it % STAGES;
           if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag)) { atomicExch(p.status, 73); goto done; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * STAGE_BYTES), sb = sa + OP_BYTES;
+          const uint32_t sa = smem_u32(smem + s * STAGE_BYTES), sb = once ? sa : sa + OP_BYTES;
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t da = A_MN ? make_smem_desc(sa + k * 2048, 8192, 1024) : make_smem_desc(sa + k * 32, 16, 1024);
@@ -362,10 +369,14 @@ done:
 // 64 of the reduction, which is what a launch of one round lasts for; `splits` SMs take it in parts. When all have multiplied, each sends every other the sums of the rows that one finishes, fp32 through
 // the cluster's shared memory (over the operands' stages), and finishes its own: 128 / splits rows, added in the order of the parts.
 constexpr int MOST_SPLITS = 4;
-__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, float a, float b, float c, float d) {
+// The place of this CTA's shared memory at `addr` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t remote_address(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(r), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+  return r;
+}
+__device__ __forceinline__ void store_cluster4(uint32_t to, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 template <int CTAS, bool A_MN, bool B_MN, int KIND>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -388,6 +399,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   const int z = item / tiles;
   int tm, tn;
   tile_at<KIND>(item - z * tiles, tiles_m, tiles_n, p.group_m, tm, tn);
+  const bool once = KIND == SYM && tm == tn;   // the same rows twice
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
@@ -421,9 +433,9 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 71); if (rank == 0) settle_loads(full_bar, it); break; }
         uint8_t* sa = smem + s * STAGE_BYTES;
         const uint32_t bar = CTAS == 2 ? smem_u32(&full_bar[s]) & PEER_MASK : smem_u32(&full_bar[s]);
-        if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * STAGE_BYTES);
+        if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * (once ? OP_BYTES : STAGE_BYTES));
         load_operand<CTAS, A_MN>(sa, &map_a, bar, row, (kb0 + it) * BK, z);
-        load_operand<CTAS, B_MN>(sa + OP_BYTES, &map_b, bar, col, (kb0 + it) * BK, z);
+        if (!once) load_operand<CTAS, B_MN>(sa + OP_BYTES, &map_b, bar, col, (kb0 + it) * BK, z);
       }
       pdl_trigger();
     }
@@ -434,7 +446,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
         const int s = it % STAGES;
         if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag)) { atomicExch(p.status, 73); break; }
         tc_fence_after();
-        const uint32_t sa = smem_u32(smem + s * STAGE_BYTES), sb = sa + OP_BYTES;
+        const uint32_t sa = smem_u32(smem + s * STAGE_BYTES), sb = once ? sa : sa + OP_BYTES;
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
           const uint64_t da = A_MN ? make_smem_desc(sa + k * 2048, 8192, 1024) : make_smem_desc(sa + k * 32, 16, 1024);
@@ -455,7 +467,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   const int q = warp & 3, half = (warp - 2) >> 2, per_owner = 4 / splits;
   if (warp >= 2) {
     const uint32_t owner = static_cast<uint32_t>(q / per_owner) * CTAS + rank;
-    const uint32_t at = smem_u32(smem) + (split * per_owner + q % per_owner) * (TILE * 128) + lane * 16;
+    const uint32_t at = remote_address(smem_u32(smem) + (split * per_owner + q % per_owner) * (TILE * 128) + lane * 16, owner);
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll 1
     for (int c = half * (TILE / 2); c < (half + 1) * (TILE / 2); c += 32) {
@@ -464,7 +476,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 32; j += 4)
-        store_remote(at + (c + j) / 4 * 512, owner, __uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
+        store_cluster4(at + (c + j) / 4 * 512, __uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
     }
   }
   tc_fence_before();
@@ -679,6 +691,381 @@ __global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__
   pdl_trigger();
 }
 
+// ------------------------------------------------------------------------------------------ a whole call in one launch
+// Where the shorter side is at most 128 and the longer one at most 2048 a call is one launch: a cluster of up to eight CTAs has a matrix, each a slab of the longer side, which stays in shared memory as hi and
+// lo from the first step to the last. In a slab's 64 columns rows are 128 bytes apart, which is an operand with the columns as the reduction (the gram product) and with the rows as the reduction (the last
+// product) alike; a matrix with more rows than columns is turned when it is read. Per step: the gram product of the slab; its sums to the CTA that finishes those rows and columns (shared memory of the cluster), which adds them
+// in the order of the slabs and gives A to all; its square, every CTA for itself; the polynomial over A; the last product and the slab's new hi and lo. What bounds it is the chain of those,
+// about 4 us a step; the launches of the other form take 11 to 16. SMALL_TIMES
+constexpr int SMALL_R = 128, SMALL_W = 256, SMALL_PARTS = 8, SMALL_THREADS = 512;
+constexpr int SMALL_A = 2 * SMALL_R * 128, SMALL_RECV = 16 * 4096;
+constexpr int small_smem(int w) { return 2 * w * 2 * SMALL_R + SMALL_A + SMALL_RECV + 1024 + 256; }
+static_assert(small_smem(SMALL_W) <= 227 * 1024, "shared memory");
+
+struct Small {
+  int rows, cols, r, n, tall;    // r: the shorter side, n: the longer one; tall: it is the rows
+  int w, parts;                  // columns of a slab, slabs
+  int steps, kept, p2, vec;
+  __nv_bfloat16* out;            // what is orthogonalised, or null: the update
+  float* master;
+  __nv_bfloat16* param;
+  float keep, step;              // master <- keep master - step (O 2^p2)
+  int* status;
+};
+// Eight entries of row `row` of the (turned) matrix from column `col` on; `at`: where its stack entry starts.
+__device__ __forceinline__ void gather8(const Source& s, const Small& p, float coef, long long at, int row, int col, bool update, float (&u)[8]) {
+  const int n = row < p.r ? max(0, min(8, p.n - col)) : 0;
+  if (n == 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = 0.f;
+  } else if (!p.tall) {
+    source8(s, coef, at + static_cast<long long>(row) * p.cols + col, n, p.vec != 0, update, u);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u[j] = 0.f;
+      if (j < n) {
+        const long long i = at + static_cast<long long>(col + j) * p.cols + row;
+        u[j] = load16or32(s.g, s.g_bf16, i);
+        if (s.m != nullptr) {
+          u[j] *= coef;
+          float m = load16or32(s.m, s.m_bf16, i);
+          if (update) {
+            m = fmaf(s.mu, m, u[j]);
+            if (s.m_bf16) { const __nv_bfloat16 b = __float2bfloat16(m); reinterpret_cast<__nv_bfloat16*>(s.m)[i] = b; m = __bfloat162float(b); }
+            else reinterpret_cast<float*>(s.m)[i] = m;
+          }
+          u[j] = s.nesterov ? fmaf(s.mu, m, u[j]) : m;
+        }
+      }
+    }
+  }
+}
+__device__ __forceinline__ uint4* piece_at(uint8_t* x, int row, int piece) { return reinterpret_cast<uint4*>(x + (piece >> 3) * (SMALL_R * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4)); }
+// Bounded, as mbar_wait, for what other CTAs of the cluster have sent.
+__device__ __forceinline__ bool wait_sent(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((i & 1023u) == 1023u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+// To another CTA of the cluster, whose barrier counts the bytes.
+__device__ __forceinline__ void send8(uint32_t to, uint2 v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(to), "r"(v.x), "r"(v.y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void send16(uint32_t to, uint4 v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(bar) : "memory");
+}
+
+__global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source src, const Small p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* hi = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* lo = hi + p.w * 2 * SMALL_R;
+  uint8_t* a = lo + p.w * 2 * SMALL_R;         // A, then the polynomial in its place: 128 x 128, two blocks of 64 columns
+  uint8_t* recv = a + SMALL_A;                 // sums from the other slabs
+  double* norm = reinterpret_cast<double*>(recv + SMALL_RECV);
+  uint64_t* done_bar = reinterpret_cast<uint64_t*>(norm + SMALL_PARTS);
+  uint64_t *sums_bar = done_bar + 1, *a_bar = done_bar + 2;   // of the sums that are finished here, and of A from the others
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 3);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* factor = reinterpret_cast<float*>(tmem_slot + 2);
+  __shared__ double warp_sums[SMALL_THREADS / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, sub = warp >> 2;   // a quarter of the rows, a quarter of the columns
+  const int parts = p.parts, rank = parts > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int z = blockIdx.x / parts, n0 = rank * p.w;
+  const long long at = static_cast<long long>(z) * p.rows * p.cols;
+  const int pieces = p.w / 8, tasks = SMALL_R * pieces;
+  auto task = [&](int i, int& row, int& piece) {   // neighbouring threads have neighbours in memory
+    if (p.tall) { row = i % SMALL_R; piece = i / SMALL_R; }
+    else { row = i / pieces; piece = i - row * pieces; }
+  };
+
+  if (threadIdx.x == 0) {
+    mbar_init(done_bar, 1);
+    mbar_init(sums_bar, 1);
+    mbar_init(a_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  pdl_wait();
+  const float coef = src.coef != nullptr ? *src.coef : 1.f;
+  double total = 0.0;
+  for (int i0 = threadIdx.x; i0 < tasks; i0 += 2 * SMALL_THREADS) {   // as they are, fp32, over where hi and lo will be; two pieces under way (tasks are a multiple of 1024)
+    float u[2][8];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      int row, piece;
+      task(i0 + b * SMALL_THREADS, row, piece);
+      gather8(src, p, coef, at, row, n0 + piece * 8, true, u[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      int row, piece;
+      task(i0 + b * SMALL_THREADS, row, piece);
+      float sq = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sq = fmaf(u[b][j], u[b][j], sq);
+      total += sq;
+      *piece_at(hi, row, piece) = make_uint4(__float_as_uint(u[b][0]), __float_as_uint(u[b][1]), __float_as_uint(u[b][2]), __float_as_uint(u[b][3]));
+      *piece_at(lo, row, piece) = make_uint4(__float_as_uint(u[b][4]), __float_as_uint(u[b][5]), __float_as_uint(u[b][6]), __float_as_uint(u[b][7]));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) warp_sums[warp] = total;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (threadIdx.x == 0) {
+    total = 0.0;
+    for (int i = 0; i < SMALL_THREADS / 32; ++i) total += warp_sums[i];
+    norm[rank] = total;
+  }
+  if (parts > 1) {
+    cluster_barrier();   // every CTA of the cluster is there
+    if (threadIdx.x == 0) for (int t = 0; t < parts; ++t) if (t != rank) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote_address(smem_u32(norm + rank), t)), "d"(total) : "memory");
+    __syncwarp();
+    cluster_barrier();
+  }
+  if (threadIdx.x == 0) {
+    total = 0.0;
+    for (int t = 0; t < parts; ++t) total += norm[t];
+    *factor = static_cast<float>(ldexp(1.0, p.p2) / (sqrt(total) + 1e-7));
+  }
+  __syncthreads();
+  const float f0 = *factor;
+  for (int i = threadIdx.x; i < tasks; i += SMALL_THREADS) {
+    int row, piece;
+    task(i, row, piece);
+    const uint4 x = *piece_at(hi, row, piece), y = *piece_at(lo, row, piece);
+    const uint32_t u[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float c = __uint_as_float(u[2 * j]) * f0, d = __uint_as_float(u[2 * j + 1]) * f0;
+      h[j] = pack_f16(c, d);
+      const float2 b = unpack_f16(h[j]);
+      l[j] = pack_f16((c - b.x) * (1 << LO_BITS), (d - b.y) * (1 << LO_BITS));
+    }
+    *piece_at(hi, row, piece) = make_uint4(h[0], h[1], h[2], h[3]);
+    *piece_at(lo, row, piece) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+
+  const float alpha_a = static_cast<float>(ldexp(SCALE_A, -2 * p.p2)), alpha_p = static_cast<float>(SCALE_P * NS_C / (SCALE_A * SCALE_A)), beta_p = static_cast<float>(SCALE_P * NS_B / SCALE_A);
+  constexpr float diag_p = static_cast<float>(SCALE_P * NS_A), beta_x = static_cast<float>(NS_A / (1 << LO_BITS));
+  constexpr uint32_t idesc_sq = idesc_f16(SMALL_R, SMALL_R, false, false);
+  const uint32_t idesc_last = idesc_f16(SMALL_R, p.w, false, true);
+  const uint32_t quarter = tmem + (static_cast<uint32_t>(q * 32) << 16), d3 = SMALL_R;   // D3 behind the square's columns
+  const int row = q * 32 + lane;
+  const bool there = q * 32 < p.r && sub * 32 < p.r;   // whether this warp's part of the square matrices is; the others stay zero
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *piece_at(a, row, sub * 4 + i) = make_uint4(0, 0, 0, 0);
+  uint32_t sums_bytes = 0, a_bytes = 0;   // what comes from other CTAs in a step
+  for (int u = 0; u < 16; ++u)
+    if ((u >> 2) * 32 < p.r && (u & 3) * 32 < p.r) {
+      if (u % parts == rank) sums_bytes += (parts - 1) * 4096;
+      else a_bytes += 2048;
+    }
+  uint32_t phase = 0;
+  // What all have written to shared memory is multiplied by one thread; all wait for the sums.
+  auto multiply = [&](auto issue) {
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0 && elect_one()) {
+      tc_fence_after();
+      issue();
+      umma_commit(done_bar);
+    }
+    __syncwarp();   // (lanes that wait would hold up the one that issues)
+    if (!mbar_wait(done_bar, phase, abort_flag) && lane == 0) atomicExch(p.status, 75);
+    phase ^= 1;
+    __syncwarp();
+    tc_fence_after();
+  };
+  for (int step = 0; step < p.steps; ++step) {
+    multiply([&]() {
+      for (int k = 0; k < p.w / 16; ++k) {
+        const uint64_t d = make_smem_desc(smem_u32(hi) + (k >> 2) * (SMALL_R * 128) + (k & 3) * 32, 16, 1024);
+        umma_bf16(tmem, d, d, idesc_sq, k != 0);
+      }
+    });
+    if (parts == 1) {
+      if (there) {
+        uint32_t v[32];
+        tmem_ld_32x32(quarter + sub * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t h[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) h[j] = pack_f16(__uint_as_float(v[8 * i + 2 * j]) * alpha_a, __uint_as_float(v[8 * i + 2 * j + 1]) * alpha_a);
+          *piece_at(a, row, sub * 4 + i) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+      }
+    } else {
+      // unit (quarter, quarter) is finished by CTA unit % parts, as its unit / parts-th; [unit there][slab][4 columns][row] of 16 bytes
+      if (there) {
+        const int unit = q * 4 + sub, owner = unit % parts, place = ((unit / parts) * parts + rank) * 4096 + lane * 16;
+        uint32_t v[32];
+        tmem_ld_32x32(quarter + sub * 32, v);
+        tmem_ld_wait();
+        // Nothing that is sent overtakes: sums of the next step come from a CTA that has all of this step's A, and A from one that has all of its sums.
+        if (owner == rank) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(recv + place + i * 512) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+          const uint32_t to = remote_address(smem_u32(recv) + place, owner), bar = remote_address(smem_u32(sums_bar), owner);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) send16(to + i * 512, make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]), bar);
+        }
+      }
+      if (threadIdx.x == 0) {
+        mbar_arrive_expect_tx(sums_bar, sums_bytes);
+        mbar_arrive_expect_tx(a_bar, a_bytes);
+      }
+      __syncthreads();   // this CTA's own sums
+      if (!wait_sent(sums_bar, step & 1, abort_flag) && lane == 0) atomicExch(p.status, 76);
+      __syncwarp();
+      // sixteen warps share what is finished here: 32 / parts columns of a unit each
+      const int mine = warp / parts, u = rank + mine * parts, per = 8 / parts;
+      if ((u >> 2) * 32 < p.r && (u & 3) * 32 < p.r) {
+        for (int c = 0; c < per; ++c) {
+          const int four = (warp % parts) * per + c;   // columns 4 four .. of the unit
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+          for (int t = 0; t < parts; ++t) {
+            const float4 x = *reinterpret_cast<const float4*>(recv + (mine * parts + t) * 4096 + four * 512 + lane * 16);
+            s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+          }
+          const uint2 h = make_uint2(pack_f16(s[0] * alpha_a, s[1] * alpha_a), pack_f16(s[2] * alpha_a, s[3] * alpha_a));
+          uint8_t* dst = reinterpret_cast<uint8_t*>(piece_at(a, (u >> 2) * 32 + lane, (u & 3) * 4 + four / 2)) + (four & 1) * 8;
+          *reinterpret_cast<uint2*>(dst) = h;
+          for (int t = 1; t < parts; ++t) send8(remote_address(smem_u32(dst), (rank + t) % parts), h, remote_address(smem_u32(a_bar), (rank + t) % parts));
+        }
+      }
+      if (!wait_sent(a_bar, step & 1, abort_flag) && lane == 0) atomicExch(p.status, 77);
+      __syncwarp();
+    }
+    multiply([&]() {
+      for (int k = 0; k < SMALL_R / 16; ++k) {
+        const uint64_t d = make_smem_desc(smem_u32(a) + (k >> 2) * (SMALL_R * 128) + (k & 3) * 32, 16, 1024);
+        umma_bf16(tmem, d, d, idesc_sq, k != 0);
+      }
+    });
+    if (there) {
+      uint32_t v[32];
+      tmem_ld_32x32(quarter + sub * 32, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4* place = piece_at(a, row, sub * 4 + i);
+        const uint4 old = *place;
+        const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 b = unpack_f16(o[j]);
+          const int col = sub * 32 + 8 * i + 2 * j;
+          float x = fmaf(__uint_as_float(v[8 * i + 2 * j]), alpha_p, beta_p * b.x), y = fmaf(__uint_as_float(v[8 * i + 2 * j + 1]), alpha_p, beta_p * b.y);
+          if (col == row) x += diag_p;
+          if (col + 1 == row) y += diag_p;
+          h[j] = pack_f16(x, y);
+        }
+        *place = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    }
+    multiply([&]() {
+      for (int k = 0; k < SMALL_R / 16; ++k) {
+        const uint64_t da = make_smem_desc(smem_u32(a) + (k >> 2) * (SMALL_R * 128) + (k & 3) * 32, 16, 1024);
+        const uint64_t db = make_smem_desc(smem_u32(hi) + k * 2048, SMALL_R * 128, 1024);
+        umma_bf16(tmem + d3, da, db, idesc_last, k != 0);
+      }
+    });
+    const bool end = step + 1 == p.steps, to_out = end && p.out != nullptr;
+    const float alpha_x = static_cast<float>(ldexp(1.0 / SCALE_P, to_out ? -p.p2 : 0));
+#pragma unroll 2
+    for (int c = sub * (p.w / 4); c < (sub + 1) * (p.w / 4); c += 16) {
+      uint32_t v[16];
+      tmem_ld_32x16(quarter + d3 + c, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int piece = c / 8 + i;
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[8 * i + j]) * alpha_x;
+        if (step < p.kept) {
+          const uint4 old = *piece_at(lo, row, piece);
+          const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { const float2 b = unpack_f16(o[j]); f[2 * j] += beta_x * b.x; f[2 * j + 1] += beta_x * b.y; }
+        }
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = to_out ? pack_bf16(f[2 * j], f[2 * j + 1]) : pack_f16(f[2 * j], f[2 * j + 1]);
+        *piece_at(hi, row, piece) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (step + 1 < p.kept) {
+          uint32_t l[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { const float2 b = unpack_f16(h[j]); l[j] = pack_f16((f[2 * j] - b.x) * (1 << LO_BITS), (f[2 * j + 1] - b.y) * (1 << LO_BITS)); }
+          *piece_at(lo, row, piece) = make_uint4(l[0], l[1], l[2], l[3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  pdl_trigger();
+  for (int i = threadIdx.x; i < tasks; i += SMALL_THREADS) {
+    int row, piece;
+    task(i, row, piece);
+    const int col = n0 + piece * 8, n = row < p.r ? max(0, min(8, p.n - col)) : 0;
+    if (n == 0) continue;
+    const uint4 x = *piece_at(hi, row, piece);
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { const float2 b = p.out != nullptr ? unpack_bf16(u[j]) : unpack_f16(u[j]); f[2 * j] = b.x; f[2 * j + 1] = b.y; }
+    const long long first = at + (p.tall ? static_cast<long long>(col) * p.cols + row : static_cast<long long>(row) * p.cols + col);
+    if (p.out != nullptr) {
+      if (!p.tall) { store8(p.out, 1, first, n, p.vec != 0, f); continue; }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) if (j < n) p.out[first + static_cast<long long>(j) * p.cols] = __float2bfloat16(f[j]);
+      continue;
+    }
+    if (!p.tall) {
+      float w[8];
+      load8(p.master, 0, first, n, p.vec != 0, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = fmaf(-p.step, f[j], p.keep * w[j]);
+      store8(p.master, 0, first, n, p.vec != 0, w);
+      if (p.param != nullptr) store8(p.param, 1, first, n, p.vec != 0, w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) {
+          const long long e = first + static_cast<long long>(j) * p.cols;
+          const float w = fmaf(-p.step, f[j], p.keep * p.master[e]);
+          p.master[e] = w;
+          if (p.param != nullptr) p.param[e] = __float2bfloat16(w);
+        }
+    }
+  }
+  __syncthreads();
+  if (parts > 1) cluster_barrier();   // nobody leaves while another may still write to it
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // ------------------------------------------------------------------------------------------ host
 struct Matrix {            // stack of fp16 matrices with padded rows
   uint16_t* p;
@@ -799,6 +1186,46 @@ static Layout layout(long long rows, long long cols, long long stack) {
   return l;
 }
 
+// The call in one launch; 1 where it does not fit one.
+static int small_call(const Source& src, Small p, long long stack, cudaStream_t st) {
+  p.tall = p.rows > p.cols;
+  p.r = p.tall ? p.cols : p.rows;
+  p.n = p.tall ? p.rows : p.cols;
+  if (p.r > SMALL_R || p.n > SMALL_W * SMALL_PARTS || stack > 1 << 20) return 1;
+  p.parts = 1;   // as few slabs as hold the matrix: what they exchange takes longer than what they save (128 x 128 27 us as one, 38 as two)
+  while (p.parts < SMALL_PARTS && p.n > SMALL_W * p.parts) p.parts *= 2;
+  p.w = static_cast<int>(up((p.n + p.parts - 1) / p.parts, 64));
+  p.kept = p.steps > 2 ? p.steps - 2 : p.steps - 1;
+  static int known[SMALL_PARTS + 1] = {-1, -1, -1, -1, -1, -1, -1, -1, -1};   // clusters of that size at once, 0 where the device takes none
+  int& room = known[p.parts];
+  if (room < 0) {
+    if (cudaFuncSetAttribute(small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_W)) != cudaSuccess) return -4;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(p.parts); cfg.blockDim = dim3(SMALL_THREADS); cfg.dynamicSmemBytes = small_smem(SMALL_W);
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, small_kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+    room = n;
+  }
+  if (room <= 0) return 1;
+  // Rounds of clusters against fifteen launches that pass over the matrices six times a step, in us (five steps): 64 x 128 x 1024, two rounds of clusters of four, 157 as one launch and 130 so; 64 x 128 x 256 37 and 80.
+  const double here = ((stack + room - 1) / room) * (18.0 + 6.5 * (p.w / 64 - 1) + (p.parts > 1 ? 16.0 + 1.5 * p.parts : 0.0));
+  const double there = 60.0 + static_cast<double>(stack) * p.r * p.n * (60.0 / 6.5e6);
+  if (here > there) return 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(stack * p.parts)); cfg.blockDim = dim3(SMALL_THREADS); cfg.dynamicSmemBytes = small_smem(p.w); cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, small_kernel, src, p) == cudaSuccess ? 0 : -5;
+}
+
 // Everything up to the last product, which leaves hi 2^p in *result (fp16, padded), or bf16 in `out` (padded rows of out_ld).
 static int orthogonalise(const Source& src, long long rows, long long cols, long long stack, int steps, void* out, long long out_ld, int p2, uint8_t* ws, int pairs, int* status, cudaStream_t st) {
   const Layout l = layout(rows, cols, stack);
@@ -881,6 +1308,10 @@ int mtb200_newton_schulz(const void* g, int g_bf16, void* out, long long rows, l
   const Layout l = layout(rows, cols, stack);
   if (ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 255)) return -11;
   const Source src{g, g_bf16, nullptr, 0, nullptr, 0.f, 0};
+  Small one{static_cast<int>(rows), static_cast<int>(cols)};
+  one.steps = steps; one.p2 = exponent(rows, cols); one.out = (__nv_bfloat16*)out; one.status = status;
+  one.vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  if (const int did = small_call(src, one, stack, st); did <= 0) return did;
   const bool direct = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   uint8_t* w = reinterpret_cast<uint8_t*>(ws);
   void* to = direct ? out : w + 2 * (steps & 1) * l.xbytes;   // the buffer that the last step writes
@@ -900,6 +1331,10 @@ int mtb200_muon_step(float* master, void* m, int m_bf16, const void* g, int g_bf
   const Layout l = layout(rows, cols, stack);
   if (ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 255)) return -11;
   const Source src{g, g_bf16, m, m_bf16, coef, mu, nesterov};
+  Small one{static_cast<int>(rows), static_cast<int>(cols)};
+  one.steps = steps; one.p2 = exponent(rows, cols); one.master = master; one.param = (__nv_bfloat16*)param; one.keep = keep; one.step = static_cast<float>(ldexp(step, -one.p2)); one.status = status;
+  one.vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(master) | reinterpret_cast<uintptr_t>(param)) & 15) == 0;
+  if (const int did = small_call(src, one, stack, st); did <= 0) return did;
   uint8_t* w = reinterpret_cast<uint8_t*>(ws);
   const int p2 = exponent(rows, cols);
   int rc = orthogonalise(src, rows, cols, stack, steps, nullptr, 0, p2, w, mtb200_gemm2_pairs(), status, st);

@@ -92,6 +92,11 @@ def plain_muon(master, moment, grad, param_out, lr, momentum, weight_decay, grad
 
 
 # -- kernels --------------------------------------------------------------------------------
+def _launches(m, n, steps):
+    """One where ``small_kernel`` of csrc/newton_schulz.cu takes the matrix, else two in front of the products and three of these a step."""
+    return 1 if min(m, n) <= 128 and max(m, n) <= 2048 else 2 + 3 * steps
+
+
 def _workspace(ops, m, n, stack, device):
     ws = torch.empty(ops.lib.mtb200_newton_schulz_workspace(m, n, stack), dtype=torch.uint8, device=device)
     return ws, ws.data_ptr(), ws.numel()
@@ -105,7 +110,7 @@ def native(ops, g, steps=5):
         if out.numel():
             ws, ptr, size = _workspace(ops, m, n, stack, g.device)
             ops._call("mtb200_newton_schulz", g.data_ptr(), int(g.dtype is torch.bfloat16), out.data_ptr(), m, n, stack, steps, ptr, size, ops.status.data_ptr(), ops._st(),
-                      n=2 + 3 * steps + (n % 8 != 0))
+                      n=_launches(m, n, steps) + (n % 8 != 0 and _launches(m, n, steps) > 1))
     return out
 
 
@@ -124,4 +129,4 @@ def native_muon(ops, master, moment, grad, param_out, lr, momentum, weight_decay
         ws, ptr, size = _workspace(ops, m, n, stack, grad.device)
         ops._call("mtb200_muon_step", master.data_ptr(), moment.data_ptr(), int(moment.dtype is torch.bfloat16), grad.data_ptr(), int(grad.dtype is torch.bfloat16),
                   None if param_out is None else param_out.data_ptr(), None if coef is None else coef.data_ptr(), m, n, stack, steps, float(momentum), int(bool(nesterov)), keep, step,
-                  ptr, size, ops.status.data_ptr(), ops._st(), n=3 + 3 * steps)
+                  ptr, size, ops.status.data_ptr(), ops._st(), n=_launches(m, n, steps) + (_launches(m, n, steps) > 1))

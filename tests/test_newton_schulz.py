@@ -157,7 +157,8 @@ def native():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", SHAPES + [(256, 688), (688, 256), (512, 512), (300, 1001), (1001, 300), (1100, 1300), (1300, 1032), (5, 260, 520), (20, 136, 64), (70, 264, 264)])
+@pytest.mark.parametrize("shape", SHAPES + [(256, 688), (688, 256), (512, 512), (300, 1001), (1001, 300), (1100, 1300), (1300, 1032), (5, 260, 520), (20, 136, 64), (70, 264, 264),
+                                            (128, 2048), (2048, 128), (100, 2049), (2100, 40), (128, 300), (33, 1030), (90, 64, 700), (40, 700, 128), (160, 24, 24), (9, 128, 1025)])
 @pytest.mark.parametrize("kind", KINDS)
 def test_kernels(native, shape, kind):
     g = matrices(kind, *shape, device="cuda")
@@ -206,7 +207,8 @@ def test_a_matrix_that_is_not_finite_is_alone(native):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape,moment,grad,nesterov,wd,coef,scale", MUON + [((520, 1032), torch.float32, torch.float32, True, 0.1, 0.9, None), ((4, 264, 129), torch.bfloat16, torch.float32, True, 0.1, 1.0, None)])
+@pytest.mark.parametrize("shape,moment,grad,nesterov,wd,coef,scale", MUON + [((520, 1032), torch.float32, torch.float32, True, 0.1, 0.9, None), ((4, 264, 129), torch.bfloat16, torch.float32, True, 0.1, 1.0, None),
+                                                                                   ((2, 100, 600), torch.bfloat16, torch.bfloat16, False, 0.1, 0.7, None), ((700, 72), torch.float32, torch.bfloat16, True, 0.1, 0.9, None)])
 @pytest.mark.parametrize("unaligned", [False, True])
 def test_muon_kernels(native, shape, moment, grad, nesterov, wd, coef, scale, unaligned):
     check_muon(native, shape, moment, grad, nesterov, wd, coef, scale, TOL, "cuda", unaligned)
@@ -244,6 +246,12 @@ def test_under_capture_and_on_another_stream(native):
 @pytest.mark.gpu
 def test_stacks_behind_2_31_elements(native):
     """A stack of more than 2^31 elements: its last matrices as a stack of their own."""
+    small = torch.zeros((1 << 31) // (128 * 1024) + 5, 1024, 128, dtype=torch.bfloat16, device="cuda")
+    small[-3:] = matrices("normal", 3, 1024, 128, dtype=torch.bfloat16, device="cuda")
+    got = native.orthogonalise(small)   # (how many slabs a matrix has goes by the stack, and with it the order of sums)
+    alone = native.orthogonalise(small[-3:].contiguous())
+    assert (got[:-3] == 0).all() and ((got[-3:].double() - alone.double()).norm() <= TOL * alone.double().norm())
+    del small, got
     g = torch.zeros((1 << 31) // (2048 * 1024) + 3, 2048, 1024, dtype=torch.bfloat16, device="cuda")
     g[-4:] = matrices("normal", 4, 2048, 1024, dtype=torch.bfloat16, device="cuda")
     got = native.orthogonalise(g)
