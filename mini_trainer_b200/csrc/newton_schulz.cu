@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(LIN_THREADS) scale_kernel(Source s, int rows, 
   }
   __syncthreads();
   const float factor = factor_sh, coef = s.coef != nullptr ? *s.coef : 1.f;
-  const int per_row = ld / 8;
+  const int per_row = (cols + 7) / 8;   // (what pads a row is never read)
   const long long units = static_cast<long long>(rows) * per_row, base = static_cast<long long>(z) * rows * cols, out = static_cast<long long>(z) * rows * ld;
   for (long long u = static_cast<long long>(blk) * LIN_THREADS + threadIdx.x; u < units; u += static_cast<long long>(blocks_per) * LIN_THREADS) {
     const long long row = u / per_row;
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(LIN_THREADS) unpad_kernel(const __nv_bfloat16*
 __global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ param, const __half* __restrict__ o, int ld, long long rows,
                                                             int cols, int vec, float keep, float step) {
   pdl_wait();
-  const int per_row = ld / 8;
+  const int per_row = (cols + 7) / 8;   // (what pads a row is never read)
   const long long units = rows * per_row;
   for (long long u = static_cast<long long>(blockIdx.x) * LIN_THREADS + threadIdx.x; u < units; u += static_cast<long long>(gridDim.x) * LIN_THREADS) {
     const long long row = u / per_row, at = row * cols;
@@ -692,12 +692,12 @@ __global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------ a whole call in one launch
-// Where the shorter side is at most 128 and the longer one at most 2048 a call is one launch: a cluster of up to eight CTAs has a matrix, each a slab of the longer side, which stays in shared memory as hi and
+// Where the shorter side is at most 128 and the longer one at most 4096 a call is one launch: a cluster of up to sixteen CTAs has a matrix, each a slab of the longer side, which stays in shared memory as hi and
 // lo from the first step to the last. In a slab's 64 columns rows are 128 bytes apart, which is an operand with the columns as the reduction (the gram product) and with the rows as the reduction (the last
 // product) alike; a matrix with more rows than columns is turned when it is read. Per step: the gram product of the slab; its sums to the CTA that finishes those rows and columns (shared memory of the cluster), which adds them
 // in the order of the slabs and gives A to all; its square, every CTA for itself; the polynomial over A; the last product and the slab's new hi and lo. What bounds it is the chain of those,
 // about 4 us a step; the launches of the other form take 11 to 16. SMALL_TIMES
-constexpr int SMALL_R = 128, SMALL_W = 256, SMALL_PARTS = 8, SMALL_THREADS = 512;
+constexpr int SMALL_R = 128, SMALL_W = 256, SMALL_PARTS = 16, SMALL_THREADS = 512;
 constexpr int SMALL_A = 2 * SMALL_R * 128, SMALL_RECV = 16 * 4096;
 constexpr int small_smem(int w) { return 2 * w * 2 * SMALL_R + SMALL_A + SMALL_RECV + 1024 + 256; }
 static_assert(small_smem(SMALL_W) <= 227 * 1024, "shared memory");
@@ -778,10 +778,16 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
   const int parts = p.parts, rank = parts > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int z = blockIdx.x / parts, n0 = rank * p.w;
   const long long at = static_cast<long long>(z) * p.rows * p.cols;
-  const int pieces = p.w / 8, tasks = SMALL_R * pieces;
+  const int pieces = p.w / 8, tasks = p.r * pieces;
+  const float per = 1.f / (p.tall ? p.r : pieces);
   auto task = [&](int i, int& row, int& piece) {   // neighbouring threads have neighbours in memory
-    if (p.tall) { row = i % SMALL_R; piece = i / SMALL_R; }
-    else { row = i / pieces; piece = i - row * pieces; }
+    const int d = p.tall ? p.r : pieces;
+    int a = __float2int_rz(static_cast<float>(i) * per);   // i below 2^12: off by one at most
+    int b = i - a * d;
+    if (b >= d) { ++a; b -= d; }
+    if (b < 0) { --a; b += d; }
+    row = p.tall ? b : a;
+    piece = p.tall ? a : b;
   };
 
   if (threadIdx.x == 0) {
@@ -795,25 +801,29 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
   pdl_wait();
   const float coef = src.coef != nullptr ? *src.coef : 1.f;
   double total = 0.0;
-  for (int i0 = threadIdx.x; i0 < tasks; i0 += 2 * SMALL_THREADS) {   // as they are, fp32, over where hi and lo will be; two pieces under way (tasks are a multiple of 1024)
+  for (int i0 = threadIdx.x; i0 < tasks; i0 += 2 * SMALL_THREADS) {   // as they are, fp32, over where hi and lo will be; two pieces under way
     float u[2][8];
+    int row[2], piece[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      int row, piece;
-      task(i0 + b * SMALL_THREADS, row, piece);
-      gather8(src, p, coef, at, row, n0 + piece * 8, true, u[b]);
+      task(min(i0 + b * SMALL_THREADS, tasks - 1), row[b], piece[b]);
+      if (b == 0 || i0 + SMALL_THREADS < tasks) gather8(src, p, coef, at, row[b], n0 + piece[b] * 8, true, u[b]);
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      int row, piece;
-      task(i0 + b * SMALL_THREADS, row, piece);
+      if (b == 1 && i0 + SMALL_THREADS >= tasks) break;
       float sq = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) sq = fmaf(u[b][j], u[b][j], sq);
       total += sq;
-      *piece_at(hi, row, piece) = make_uint4(__float_as_uint(u[b][0]), __float_as_uint(u[b][1]), __float_as_uint(u[b][2]), __float_as_uint(u[b][3]));
-      *piece_at(lo, row, piece) = make_uint4(__float_as_uint(u[b][4]), __float_as_uint(u[b][5]), __float_as_uint(u[b][6]), __float_as_uint(u[b][7]));
+      *piece_at(hi, row[b], piece[b]) = make_uint4(__float_as_uint(u[b][0]), __float_as_uint(u[b][1]), __float_as_uint(u[b][2]), __float_as_uint(u[b][3]));
+      *piece_at(lo, row[b], piece[b]) = make_uint4(__float_as_uint(u[b][4]), __float_as_uint(u[b][5]), __float_as_uint(u[b][6]), __float_as_uint(u[b][7]));
     }
+  }
+  for (int i = threadIdx.x; i < (SMALL_R - p.r) * pieces; i += SMALL_THREADS) {   // rows that are not there
+    const int row = p.r + i / pieces;
+    uint4* x = piece_at(hi, row, i - (row - p.r) * pieces);
+    *x = *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(x) + (lo - hi)) = make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -859,7 +869,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
 
   const float alpha_a = static_cast<float>(ldexp(SCALE_A, -2 * p.p2)), alpha_p = static_cast<float>(SCALE_P * NS_C / (SCALE_A * SCALE_A)), beta_p = static_cast<float>(SCALE_P * NS_B / SCALE_A);
   constexpr float diag_p = static_cast<float>(SCALE_P * NS_A), beta_x = static_cast<float>(NS_A / (1 << LO_BITS));
-  constexpr uint32_t idesc_sq = idesc_f16(SMALL_R, SMALL_R, false, false);
+  const uint32_t idesc_sq = idesc_f16(SMALL_R, (p.r + 31) / 32 * 32, false, false);   // columns of the warps' parts that are there
+  const int ksteps = (p.r + 15) / 16;
   const uint32_t idesc_last = idesc_f16(SMALL_R, p.w, false, true);
   const uint32_t quarter = tmem + (static_cast<uint32_t>(q * 32) << 16), d3 = SMALL_R;   // D3 behind the square's columns
   const int row = q * 32 + lane;
@@ -933,11 +944,11 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
       __syncthreads();   // this CTA's own sums
       if (!wait_sent(sums_bar, step & 1, abort_flag) && lane == 0) atomicExch(p.status, 76);
       __syncwarp();
-      // sixteen warps share what is finished here: 32 / parts columns of a unit each
-      const int mine = warp / parts, u = rank + mine * parts, per = 8 / parts;
-      if ((u >> 2) * 32 < p.r && (u & 3) * 32 < p.r) {
+      // sixteen warps share what is finished here: 32 / parts columns of a unit each, four at least
+      const int share = min(parts, 8), mine = warp / share, u = rank + mine * parts, per = 8 / share;
+      if (u < 16 && (u >> 2) * 32 < p.r && (u & 3) * 32 < p.r) {
         for (int c = 0; c < per; ++c) {
-          const int four = (warp % parts) * per + c;   // columns 4 four .. of the unit
+          const int four = (warp % share) * per + c;   // columns 4 four .. of the unit
           float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
           for (int t = 0; t < parts; ++t) {
@@ -954,7 +965,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
       __syncwarp();
     }
     multiply([&]() {
-      for (int k = 0; k < SMALL_R / 16; ++k) {
+      for (int k = 0; k < ksteps; ++k) {
         const uint64_t d = make_smem_desc(smem_u32(a) + (k >> 2) * (SMALL_R * 128) + (k & 3) * 32, 16, 1024);
         umma_bf16(tmem, d, d, idesc_sq, k != 0);
       }
@@ -982,7 +993,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
       }
     }
     multiply([&]() {
-      for (int k = 0; k < SMALL_R / 16; ++k) {
+      for (int k = 0; k < ksteps; ++k) {
         const uint64_t da = make_smem_desc(smem_u32(a) + (k >> 2) * (SMALL_R * 128) + (k & 3) * 32, 16, 1024);
         const uint64_t db = make_smem_desc(smem_u32(hi) + k * 2048, SMALL_R * 128, 1024);
         umma_bf16(tmem + d3, da, db, idesc_last, k != 0);
@@ -990,32 +1001,36 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
     });
     const bool end = step + 1 == p.steps, to_out = end && p.out != nullptr;
     const float alpha_x = static_cast<float>(ldexp(1.0 / SCALE_P, to_out ? -p.p2 : 0));
-#pragma unroll 2
-    for (int c = sub * (p.w / 4); c < (sub + 1) * (p.w / 4); c += 16) {
-      uint32_t v[16];
-      tmem_ld_32x16(quarter + d3 + c, v);
-      tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int piece = c / 8 + i;
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[8 * i + j]) * alpha_x;
+    if (q * 32 < p.r) {
+      const float2 alpha2 = make_float2(alpha_x, alpha_x), beta2 = make_float2(beta_x, beta_x), up2 = make_float2(1 << LO_BITS, 1 << LO_BITS);
+#pragma unroll 1
+      for (int c = sub * (p.w / 4); c < (sub + 1) * (p.w / 4); c += 16) {
+        uint32_t v[16];
+        tmem_ld_32x16(quarter + d3 + c, v);
+        uint8_t *hp = reinterpret_cast<uint8_t*>(piece_at(hi, row, c / 8)), *lp = lo + (hp - hi);
+        const int second = row & 1 ? -16 : 16;   // c is a multiple of 16: its second piece differs in the lowest bit
+        uint32_t o[8];
         if (step < p.kept) {
-          const uint4 old = *piece_at(lo, row, piece);
-          const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+          const uint4 x = *reinterpret_cast<const uint4*>(lp), y = *reinterpret_cast<const uint4*>(lp + second);
+          o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w; o[4] = y.x; o[5] = y.y; o[6] = y.z; o[7] = y.w;
+        } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) { const float2 b = unpack_f16(o[j]); f[2 * j] += beta_x * b.x; f[2 * j + 1] += beta_x * b.y; }
+          for (int j = 0; j < 8; ++j) o[j] = 0u;
         }
-        uint32_t h[4];
+        tmem_ld_wait();
+        uint32_t h[8], l[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = to_out ? pack_bf16(f[2 * j], f[2 * j + 1]) : pack_f16(f[2 * j], f[2 * j + 1]);
-        *piece_at(hi, row, piece) = make_uint4(h[0], h[1], h[2], h[3]);
+        for (int j = 0; j < 8; ++j) {
+          const float2 f = ffma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), alpha2, fmul2(unpack_f16(o[j]), beta2));
+          h[j] = to_out ? pack_bf16(f.x, f.y) : pack_f16(f.x, f.y);
+          const float2 b = unpack_f16(h[j]), d = fmul2(fadd2(f, make_float2(-b.x, -b.y)), up2);
+          l[j] = pack_f16(d.x, d.y);
+        }
+        *reinterpret_cast<uint4*>(hp) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(hp + second) = make_uint4(h[4], h[5], h[6], h[7]);
         if (step + 1 < p.kept) {
-          uint32_t l[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) { const float2 b = unpack_f16(h[j]); l[j] = pack_f16((f[2 * j] - b.x) * (1 << LO_BITS), (f[2 * j + 1] - b.y) * (1 << LO_BITS)); }
-          *piece_at(lo, row, piece) = make_uint4(l[0], l[1], l[2], l[3]);
+          *reinterpret_cast<uint4*>(lp) = make_uint4(l[0], l[1], l[2], l[3]);
+          *reinterpret_cast<uint4*>(lp + second) = make_uint4(l[4], l[5], l[6], l[7]);
         }
       }
     }
@@ -1172,9 +1187,9 @@ static long long up(long long x, long long to) { return (x + to - 1) / to * to; 
 struct Layout { long long ld, r, ldr, xbytes, gbytes, chunks, total; };
 static Layout layout(long long rows, long long cols, long long stack) {
   Layout l;
-  l.ld = up(cols, 8);
+  l.ld = up(cols, 64);   // rows of whole 128 bytes: ones that start off 32 cost a TMA load up to twice the requests
   l.r = rows < cols ? rows : cols;
-  l.ldr = up(l.r, 8);
+  l.ldr = up(l.r, 64);
   l.xbytes = up(stack * rows * l.ld * 2, 256);
   l.gbytes = up(stack * l.r * l.ldr * 2, 256);
   const long long numel = rows * cols;
@@ -1196,10 +1211,11 @@ static int small_call(const Source& src, Small p, long long stack, cudaStream_t 
   while (p.parts < SMALL_PARTS && p.n > SMALL_W * p.parts) p.parts *= 2;
   p.w = static_cast<int>(up((p.n + p.parts - 1) / p.parts, 64));
   p.kept = p.steps > 2 ? p.steps - 2 : p.steps - 1;
-  static int known[SMALL_PARTS + 1] = {-1, -1, -1, -1, -1, -1, -1, -1, -1};   // clusters of that size at once, 0 where the device takes none
+  static int known[SMALL_PARTS + 1] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};   // clusters of that size at once, 0 where the device takes none
   int& room = known[p.parts];
   if (room < 0) {
-    if (cudaFuncSetAttribute(small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_W)) != cudaSuccess) return -4;
+    if (cudaFuncSetAttribute(small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_W)) != cudaSuccess ||
+        cudaFuncSetAttribute(small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return -4;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -1212,8 +1228,8 @@ static int small_call(const Source& src, Small p, long long stack, cudaStream_t 
   }
   if (room <= 0) return 1;
   // Rounds of clusters against fifteen launches that pass over the matrices six times a step, in us (five steps): 64 x 128 x 1024, two rounds of clusters of four, 157 as one launch and 130 so; 64 x 128 x 256 37 and 80.
-  const double here = ((stack + room - 1) / room) * (18.0 + 6.5 * (p.w / 64 - 1) + (p.parts > 1 ? 16.0 + 1.5 * p.parts : 0.0));
-  const double there = 60.0 + static_cast<double>(stack) * p.r * p.n * (60.0 / 6.5e6);
+  const double here = (stack > room ? 1.3 : 1.0) * ((stack + room - 1) / room) * (18.0 + 6.5 * (p.w / 64 - 1) + (p.parts > 1 ? (p.r > 64 ? 16.0 : 8.0) + 1.5 * p.parts : 0.0));
+  const double there = 75.0 + static_cast<double>(stack) * p.r * p.n * 6.5e-6;
   if (here > there) return 1;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1240,7 +1256,7 @@ static int orthogonalise(const Source& src, long long rows, long long cols, long
   if (stack * l.chunks >= 1ll << 31) return -10;
   launch_pdl(squares_kernel, static_cast<unsigned>(stack * l.chunks), LIN_THREADS, 0, st, src, numel, static_cast<int>(l.chunks), per_chunk, vec_flat, sums);
   const int kept = steps > 2 ? steps - 2 : steps - 1;   // steps whose X is held as two numbers
-  long long blocks = (rows * l.ld / 8 + LIN_THREADS - 1) / LIN_THREADS, most = (sm_count() * 8 + stack - 1) / stack;
+  long long blocks = (rows * ((cols + 7) / 8) + LIN_THREADS - 1) / LIN_THREADS, most = (sm_count() * 8 + stack - 1) / stack;
   if (blocks > most) blocks = most;
   launch_pdl(scale_kernel, static_cast<unsigned>(stack * blocks), LIN_THREADS, 0, st, src, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(l.ld), static_cast<int>(l.chunks),
              static_cast<int>(blocks), vec_rows, p2, sums, x[0][0], kept > 0 ? x[0][1] : nullptr);
@@ -1341,7 +1357,7 @@ int mtb200_muon_step(float* master, void* m, int m_bf16, const void* g, int g_bf
   if (rc) return rc;
   const __half* o = reinterpret_cast<const __half*>(w + 2 * (steps & 1) * l.xbytes);
   const int vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(master) | reinterpret_cast<uintptr_t>(param)) & 15) == 0;
-  long long blocks = (stack * rows * l.ld / 8 + LIN_THREADS - 1) / LIN_THREADS;
+  long long blocks = (stack * rows * ((cols + 7) / 8) + LIN_THREADS - 1) / LIN_THREADS;
   if (blocks > sm_count() * 8) blocks = sm_count() * 8;
   mtb::launch_pdl(update_kernel, static_cast<unsigned>(blocks), LIN_THREADS, 0, st, master, (__nv_bfloat16*)param, o, static_cast<int>(l.ld), stack * rows, static_cast<int>(cols), vec, keep,
                   static_cast<float>(ldexp(step, -p2)));

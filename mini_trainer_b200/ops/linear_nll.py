@@ -133,7 +133,7 @@ def native_bwd(ops, dloss, x, w, targets, loss, lse, dw_out, accumulate_dw=False
                 dw_out.zero_()
             return dx
         n = piece_columns(T, V)
-        ldz = -(-n // 8) * 8
+        ldz = -(-n // 64) * 64   # rows of whole 128 bytes
         dz = torch.empty(T, ldz, dtype=torch.bfloat16, device=x.device)
         dx32 = torch.empty(T, H, dtype=torch.float32, device=x.device) if n < V else None
         form, scale = _form(ops, T, H), float(logit_scale)

@@ -94,7 +94,7 @@ def plain_muon(master, moment, grad, param_out, lr, momentum, weight_decay, grad
 # -- kernels --------------------------------------------------------------------------------
 def _launches(m, n, steps):
     """One where ``small_kernel`` of csrc/newton_schulz.cu takes the matrix, else two in front of the products and three of these a step."""
-    return 1 if min(m, n) <= 128 and max(m, n) <= 2048 else 2 + 3 * steps
+    return 1 if min(m, n) <= 128 and max(m, n) <= 4096 else 2 + 3 * steps
 
 
 def _workspace(ops, m, n, stack, device):
