@@ -15,6 +15,7 @@ from __future__ import annotations
 import torch
 
 PIECE_BYTES = 512 << 20   # of a piece's gradient, about
+STATS_BYTES = 512 << 20   # of the forward's statistics at a time, about: 8 bytes per token and 128 columns
 
 
 def check(x, w, targets, logit_scale):
@@ -43,6 +44,8 @@ def check_bwd(dloss, x, w, targets, loss, lse, dw_out, logit_scale, dlse):
             raise ValueError(f"{what}: expected {T} contiguous fp32 numbers on {x.device}")
         _per_token(what, t, T, x.device)
     _per_token("dlse", dlse, T, x.device)
+    if dw_out.device.type != "meta" and dw_out.numel() and dw_out.data_ptr() in (w.data_ptr(), x.data_ptr()):
+        raise ValueError("the weight's gradient goes to memory of its own")
     if dw_out.dtype != w.dtype or dw_out.shape != w.shape or dw_out.device != w.device:
         raise ValueError(f"the weight's gradient is {w.dtype} {tuple(w.shape)} on {w.device}, not {dw_out.dtype} {tuple(dw_out.shape)} on {dw_out.device}")
     return T, H, V
@@ -106,11 +109,13 @@ def native(ops, x, w, targets, ignore_index=-100, logit_scale=1.0):
         if T == 0:
             return loss, lse
         pieces = -(-V // 128)
-        scratch = torch.empty(T * (2 * pieces + 1), dtype=torch.float32, device=x.device)   # statistics, and the targets' logits
-        stats, at = scratch.data_ptr(), scratch.data_ptr() + 8 * T * pieces
-        ops._call("mtb200_gemm_lse", x.data_ptr(), H, w.data_ptr(), stats, at, targets.data_ptr(), T, V, H, float(logit_scale), _form(ops, T, H), ops.status.data_ptr(),
-                  ops._st(), tag="gemm_nt_lse")
-        ops._call("mtb200_nll", stats, at, targets.data_ptr(), T, pieces, V, ignore_index, loss.data_ptr(), lse.data_ptr(), ops.status.data_ptr(), ops._st())
+        rows = min(T, max(256, STATS_BYTES // (8 * pieces) // 256 * 256))
+        scratch = torch.empty(rows * (2 * pieces + 1), dtype=torch.float32, device=x.device)   # statistics, and the targets' logits
+        stats, at, form, st, status = scratch.data_ptr(), scratch.data_ptr() + 8 * rows * pieces, _form(ops, rows, H), ops._st(), ops.status.data_ptr()
+        for a in range(0, T, rows):
+            n, t = min(rows, T - a), targets.data_ptr() + 8 * a
+            ops._call("mtb200_gemm_lse", x.data_ptr() + 2 * a * H, H, w.data_ptr(), stats, at, t, n, V, H, float(logit_scale), form, status, st, tag="gemm_nt_lse")
+            ops._call("mtb200_nll", stats, at, t, n, pieces, V, ignore_index, loss.data_ptr() + 4 * a, lse.data_ptr() + 4 * a, status, st)
     return loss, lse
 
 

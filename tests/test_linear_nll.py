@@ -136,6 +136,8 @@ def test_refusals(backend):
         with pytest.raises(ValueError):
             ops.linear_nll_bwd(**{**good, "dw_out": torch.empty(16, 24, dtype=torch.bfloat16).t()})
         assert not ops.calls
+    with pytest.raises(ValueError, match="memory of its own"):
+        ops.linear_nll_bwd(**{**good, "dw_out": w})
 
 
 # ------------------------------------------------------------------------------------------ kernels
@@ -165,6 +167,7 @@ def test_kernels_in_pieces(native, monkeypatch, T, H, V):
     v = inputs(T, H, V, device="cuda", seed=1)
     whole = check(native, v)
     monkeypatch.setattr(LN, "PIECE_BYTES", 1)
+    monkeypatch.setattr(LN, "STATS_BYTES", 1)   # and the forward 256 tokens at a time
     assert LN.piece_columns(T, V) in (512, 256 * -(-V // (256 * -(-V // 512))))
     parts = check(native, v)
     assert torch.equal(whole[0], parts[0]) and torch.equal(whole[3], parts[3])

@@ -177,6 +177,15 @@ def test_kernels_by_steps(native, shape, steps):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(40, 72), (72, 40), (264, 520), (520, 264), (140, 301)])
+def test_matrices_that_start_off_16_bytes(native, shape):
+    for dtype in (torch.float32, torch.bfloat16):
+        g = matrices("features", *shape, dtype=dtype, device="cuda")
+        b = torch.empty(g.numel() + 3, dtype=dtype, device="cuda")[3:].view(shape).copy_(g)
+        assert torch.equal(native.orthogonalise(b), native.orthogonalise(g))
+
+
+@pytest.mark.gpu
 def test_large_matrices(native):
     """Tiles by single CTAs and by pairs, either side the longer, against products in 64 bits."""
     for shape in ((2048, 2048), (4096, 1040), (1040, 4096), (2500, 6000)):

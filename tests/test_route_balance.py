@@ -149,6 +149,27 @@ def test_special_rows():
     special(TorchOps(), "cpu")
 
 
+def outside(ops, device):
+    """Tokens in front of the first sample and behind the last one are routed, and have no part in a loss."""
+    v = inputs(50, 12, 3, device=device)
+    cu = torch.tensor([7, 20, 20, 44], dtype=torch.int32, device=device)
+    probs, topi, w, bal = ops.route_balanced(v["logits"], 3, True, cu)
+    inner = v["logits"][7:44].contiguous()
+    p2, t2, w2, b2 = ops.route_balanced(inner, 3, True, (cu - 7).to(torch.int32))
+    assert torch.equal(topi[7:44], t2) and torch.equal(probs[7:44], p2) and torch.equal(bal.counts, b2.counts) and torch.allclose(bal.loss, b2.loss, rtol=1e-6)
+    assert bal.tokens.tolist() == [13, 0, 24] and bal.sample.tolist() == [-1] * 7 + [0] * 13 + [2] * 24 + [-1] * 6
+    d, one = v["dw"], torch.ones(3, device=device)
+    g = ops.route_balanced_bwd(probs, topi, w, d, True, bal, one, one, torch.float32)
+    alone = ops.route_balanced_bwd(probs, topi, w, d, True, bal, dtype=torch.float32)
+    assert torch.equal(g[:7], alone[:7]) and torch.equal(g[44:], alone[44:])
+    g2 = ops.route_balanced_bwd(p2, t2, w2, d[7:44].contiguous(), True, b2, one, one, torch.float32)
+    assert torch.allclose(g[7:44], g2, rtol=1e-5, atol=1e-7)
+
+
+def test_tokens_outside_all_samples():
+    outside(TorchOps(), "cpu")
+
+
 def test_no_tokens():
     probs, topi, w, bal = TorchOps().route_balanced(torch.empty(0, 4), 2, True, torch.zeros(3, dtype=torch.int32))
     assert probs.shape == (0, 4) and bal.loss.tolist() == [0.0, 0.0] and bal.counts.tolist() == [[0] * 4] * 2
@@ -201,6 +222,7 @@ def test_kernels(native, T, E, k, lens, counted, renorm, dtype):
 @pytest.mark.gpu
 def test_kernels_on_special_rows(native):
     special(native, "cuda")
+    outside(native, "cuda")
     probs, topi, w, bal = native.route_balanced(torch.empty(0, 4, device="cuda"), 2, True, torch.zeros(3, dtype=torch.int32, device="cuda"))
     assert bal.loss.tolist() == [0.0, 0.0] and bal.counts.tolist() == [[0] * 4] * 2
     assert native.route_balanced_bwd(probs, topi, w, None, True, bal, torch.ones(2, device="cuda")).shape == (0, 4)
