@@ -15,21 +15,43 @@ logits are; a sample without counted tokens has losses of zero. The factors of t
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
 
 MOST_EXPERTS, MOST_CHOSEN, _BLOCKS_PER_SM = 512, 32, 2   # of csrc/route_balance.cu
 
 
-@dataclass
 class RouterBalance:
-    loss: torch.Tensor      # [S] fp32
-    z_loss: torch.Tensor    # [S] fp32
-    counts: torch.Tensor    # [S, E] int32 pairs that chose an expert
-    tokens: torch.Tensor    # [S] int32 counted tokens
-    lse: torch.Tensor       # [T] fp32 logsumexp of every token's logits
-    sample: torch.Tensor    # [T] int32 sample whose losses a token is in, -1 for none
+    """What the losses of a router are, and what their gradient needs.
+
+    * ``loss``, ``z_loss``  [S] fp32
+    * ``counts``            [S, E] int32 pairs that chose an expert
+    * ``tokens``            [S] int32 counted tokens
+    * ``lse``               [T] fp32 logsumexp of every token's logits
+    * ``sample``            [T] int32 sample whose losses a token is in, -1 for none
+
+    The kernels leave all of them in one buffer of 32-bit words, ``[counts | tokens | sample | loss | z_loss | lse]``; they are tensors when they are asked for, which a layer's step does for few of them.
+    """
+
+    NAMES = ("counts", "tokens", "sample", "loss", "z_loss", "lse")
+
+    def __init__(self, T, E, S, words=None, **tensors):
+        self.T, self.E, self.S, self.words = T, E, S, words
+        self.__dict__.update(tensors)
+
+    def offsets(self):
+        """First word of each of ``NAMES``."""
+        c = self.S * self.E
+        return 0, c, c + self.S, c + self.S + self.T, c + 2 * self.S + self.T, c + 3 * self.S + self.T
+
+    def __getattr__(self, name):   # not there yet
+        words = self.__dict__.get("words")
+        if words is None or name not in self.NAMES:
+            raise AttributeError(name)
+        i = self.NAMES.index(name)
+        t = words.narrow(0, self.offsets()[i], (self.S * self.E, self.S, self.T)[i if i < 3 else (1, 1, 2)[i - 3]])
+        t = t.view(self.S, self.E) if i == 0 else t.view(torch.float32) if i >= 3 else t
+        self.__dict__[name] = t
+        return t
 
 
 def _refuse(what, t, dtype, shape, device):
@@ -63,17 +85,22 @@ def check_bwd(probs, topi, w, dw, bal, dloss, dz, dtype):
     """``(T, E, k, S)`` of a gradient's arguments."""
     if probs.dim() != 2 or topi.dim() != 2:
         raise ValueError("probs [T, E] and topi [T, k] are what the forward returned")
-    (T, E), k, S, device = probs.shape, topi.shape[1], bal.loss.shape[0], probs.device
-    if not 0 < E <= MOST_EXPERTS or not 0 < k <= min(E, MOST_CHOSEN) or T >= 1 << 30:
+    (T, E), k, S, device = probs.shape, topi.shape[1], bal.S, probs.device
+    if (T, E) != (bal.T, bal.E) or not 0 < k <= min(E, MOST_CHOSEN):
         raise ValueError(f"{T} tokens, {k} of {E} experts: not what the forward returned")
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"the gradient of the logits is bf16 or fp32, not {dtype}")
     if dw is None and dloss is None and dz is None:
         raise ValueError("without a gradient of the weights or of a loss there is nothing to do")
-    for what, t, ty, shape in (("probs", probs, torch.float32, (T, E)), ("topi", topi, torch.int64, (T, k)), ("w", w, torch.float32, (T, k)), ("dw", dw, torch.float32, (T, k)),
-                               ("dloss", dloss, torch.float32, (S,)), ("dz", dz, torch.float32, (S,)), ("counts", bal.counts, torch.int32, (S, E)),
-                               ("tokens", bal.tokens, torch.int32, (S,)), ("lse", bal.lse, torch.float32, (T,)), ("sample", bal.sample, torch.int32, (T,))):
-        _expect(what, t, ty, shape, device)
+    f32, pairs = torch.float32, (T, k)
+    _expect("probs", probs, f32, (T, E), device)
+    _expect("topi", topi, torch.int64, pairs, device)
+    _expect("w", w, f32, pairs, device)
+    _expect("dw", dw, f32, pairs, device)
+    _expect("dloss", dloss, f32, (S,), device)
+    _expect("dz", dz, f32, (S,), device)
+    if (bal.lse if bal.words is None else bal.words).device != device:
+        raise ValueError(f"the losses are on another device than the probabilities, {device}")
     return T, E, k, S
 
 
@@ -104,7 +131,7 @@ def plain(logits, k, renorm, cu_seqlens=None, counted=None):
     n = tokens.clamp_min(1).double()
     z = torch.zeros(S, dtype=torch.float64, device=l.device).index_add_(0, sample[ok], lse[ok].double().square())
     loss, z = (E * (counts * sums).sum(1) / n.square()).float(), (z / n).float()
-    return probs, topi, w, RouterBalance(loss, z, counts.to(torch.int32), tokens.to(torch.int32), lse, sample.to(torch.int32))
+    return probs, topi, w, RouterBalance(T, E, S, loss=loss, z_loss=z, counts=counts.to(torch.int32), tokens=tokens.to(torch.int32), lse=lse, sample=sample.to(torch.int32))
 
 
 def plain_bwd(probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.bfloat16):
@@ -128,22 +155,20 @@ def plain_bwd(probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.
 def native(ops, logits, k, renorm, cu_seqlens=None, counted=None):
     T, E, S = check(logits, k, cu_seqlens, counted)
     ops.check_device(logits)
-    dev, f32, i32 = logits.device, torch.float32, torch.int32
+    dev, f32 = logits.device, torch.float32
     with ops.on_device():
-        loss, z, lse, w = torch.empty(2 * S + T * (k + 1), dtype=f32, device=dev).split([S, S, T, T * k])
-        counts, tokens, sample = torch.empty(S * (E + 1) + T, dtype=i32, device=dev).split([S * E, S, T])
-        probs, topi = torch.empty(T, E, dtype=f32, device=dev), torch.empty(T, k, dtype=torch.int64, device=dev)
-        counts, w = counts.view(S, E), w.view(T, k)
+        probs, topi, w = torch.empty(T, E, dtype=f32, device=dev), torch.empty(T, k, dtype=torch.int64, device=dev), torch.empty(T, k, dtype=f32, device=dev)
+        bal = RouterBalance(T, E, S, torch.empty(S * (E + 3) + 2 * T, dtype=torch.int32, device=dev))
         if T == 0:
-            for t in (loss, z, counts, tokens):
-                t.zero_()
-        else:
-            rows = _BLOCKS_PER_SM * ops.sms + S
-            part = torch.empty(rows * (E + 1), dtype=torch.int64, device=dev).data_ptr()
-            ops._call("mtb200_route_balanced", logits.data_ptr(), int(logits.dtype is f32), None if cu_seqlens is None else cu_seqlens.data_ptr(),
-                      None if counted is None else counted.data_ptr(), T, E, k, S, int(bool(renorm)), probs.data_ptr(), topi.data_ptr(), w.data_ptr(), lse.data_ptr(), sample.data_ptr(),
-                      part, part + 8 * rows * E, rows, loss.data_ptr(), z.data_ptr(), counts.data_ptr(), tokens.data_ptr(), ops._st(), n=2)
-    return probs, topi, w, RouterBalance(loss, z, counts, tokens, lse, sample)
+            bal.words.zero_()
+            return probs, topi, w, bal
+        rows, at = _BLOCKS_PER_SM * ops.sms + S, bal.words.data_ptr()
+        part = torch.empty(rows * (E + 1), dtype=torch.int64, device=dev).data_ptr()
+        counts, tokens, sample, loss, z, lse = bal.offsets()
+        ops._call("mtb200_route_balanced", logits.data_ptr(), logits.dtype is f32, None if cu_seqlens is None else cu_seqlens.data_ptr(), None if counted is None else counted.data_ptr(),
+                  T, E, k, S, bool(renorm), probs.data_ptr(), topi.data_ptr(), w.data_ptr(), at + 4 * lse, at + 4 * sample, part, part + 8 * rows * E, rows, at + 4 * loss, at + 4 * z,
+                  at, at + 4 * tokens, ops._st(), n=2)
+    return probs, topi, w, bal
 
 
 def native_bwd(ops, probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.bfloat16):
@@ -152,8 +177,12 @@ def native_bwd(ops, probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=
     with ops.on_device():
         out = torch.empty(T, E, dtype=dtype, device=probs.device)
         if T:
-            ptr = lambda t: None if t is None else t.data_ptr()
-            ops._call("mtb200_route_balanced_bwd", probs.data_ptr(), topi.data_ptr(), w.data_ptr(), ptr(dw), bal.lse.data_ptr(), bal.sample.data_ptr(),
-                      bal.counts.data_ptr(), bal.tokens.data_ptr(), ptr(dloss), ptr(dz), T, E, k, S, int(bool(renorm)), out.data_ptr(), int(dtype is torch.float32),
+            if bal.words is not None:
+                at = bal.words.data_ptr()
+                counts, tokens, sample, _, _, lse = (at + 4 * i for i in bal.offsets())
+            else:
+                counts, tokens, sample, lse = (t.data_ptr() for t in (bal.counts, bal.tokens, bal.sample, bal.lse))
+            ops._call("mtb200_route_balanced_bwd", probs.data_ptr(), topi.data_ptr(), w.data_ptr(), None if dw is None else dw.data_ptr(), lse, sample, counts, tokens,
+                      None if dloss is None else dloss.data_ptr(), None if dz is None else dz.data_ptr(), T, E, k, S, bool(renorm), out.data_ptr(), dtype is torch.float32,
                       ops.status.data_ptr(), ops._st())
     return out
