@@ -147,13 +147,21 @@ __device__ __forceinline__ float log2_mufu(float x) {
   return r;
 }
 
+// Sum over lanes 0 .. k - 1, zero elsewhere, in those lanes.
+__device__ __forceinline__ float sum_first(float v, int k) {
+  if (k > 8) return warp_sum(v);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // {sum of p_e, pairs} of a (block, sample) and expert, and {sum of lse^2, tokens} of a (block, sample)
 struct Part { float p; int c; };
 
 template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(THREADS, PER == 16 ? 1 : BLOCKS_PER_SM) route_kernel(const T* __restrict__ logits, const int* __restrict__ cu, const uint8_t* __restrict__ counted, int tokens, int E,
                                                         int k, int S, int renorm, int run, float* __restrict__ probs, long long* __restrict__ topi,
-                                                        float* __restrict__ w, float* __restrict__ lse, int* __restrict__ sample, Part* __restrict__ part,
+                                                        float* __restrict__ w, float* __restrict__ lse, float* __restrict__ inverse, int* __restrict__ sample, Part* __restrict__ part,
                                                         Part* __restrict__ part_z) {
   __shared__ __align__(16) float row_sh[WARPS][PER * 32];   // a token's probabilities; at the end of a sample's tokens, the warps' sums
   __shared__ int count_sh[PER * 32];
@@ -233,24 +241,23 @@ __global__ void __launch_bounds__(THREADS, PER == 16 ? 1 : BLOCKS_PER_SM) route_
 #pragma unroll 2
       while (true) {   // the lowest of the lanes that have the largest head writes its expert down and goes on to its next
         const bool has = head == top;
-        const uint32_t all = __ballot_sync(0xffffffffu, has);
-        if (has && (all & below) == 0u) {
-          if constexpr (SORTED) {
-            choice_sh[warp][c] = lane * PER + static_cast<int>(places & 3u);
-            places >>= 2;
+        const uint32_t all = __ballot_sync(0xffffffffu, has);   // of every lane, so before the condition
+        const bool own = has && (all & below) == 0u;
+        if constexpr (SORTED) {
+          if (own) choice_sh[warp][c] = lane * PER + static_cast<int>(places & 3u);
+          places = own ? places >> 2 : places;
 #pragma unroll
-            for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
-            key[PER - 1] = 0u;
-            head = key[0];
-          } else {
-            int at_i = 0;
+          for (int i = 0; i + 1 < PER; ++i) key[i] = own ? key[i + 1] : key[i];
+          key[PER - 1] = own ? 0u : key[PER - 1];
+          head = key[0];
+        } else if (own) {
+          int at_i = 0;
 #pragma unroll
-            for (int i = PER - 1; i >= 0; --i) if (key[i] == head) at_i = i;
-            choice_sh[warp][c] = lane * PER + at_i;
-            head = 0u;
+          for (int i = PER - 1; i >= 0; --i) if (key[i] == head) at_i = i;
+          choice_sh[warp][c] = lane * PER + at_i;
+          head = 0u;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) { if (i == at_i) key[i] = 0u; head = max(head, key[i]); }
-          }
+          for (int i = 0; i < PER; ++i) { if (i == at_i) key[i] = 0u; head = max(head, key[i]); }
         }
         if (++c == k) break;
         top = __reduce_max_sync(0xffffffffu, head);
@@ -258,13 +265,14 @@ __global__ void __launch_bounds__(THREADS, PER == 16 ? 1 : BLOCKS_PER_SM) route_
       __syncwarp();
       const int mine_at = lane < k ? choice_sh[warp][lane] : 0;   // lane c has the c-th choice
       const float mine = lane < k ? row_sh[warp][mine_at] : 0.f;
-      float share = mine;
-      if (renorm) share *= reciprocal(warp_sum(mine));
+      float scale = 1.f;
+      if (renorm) scale = reciprocal(sum_first(mine, k));
+      const float share = mine * scale;
       if (lane < k) {
         topi[static_cast<long long>(t) * k + lane] = mine_at;
         w[static_cast<long long>(t) * k + lane] = share;
       }
-      if (lane == 0) { lse[t] = l; sample[t] = in_loss ? s : -1; }
+      if (lane == 0) { lse[t] = l; inverse[t] = scale; sample[t] = in_loss ? s : -1; }
       if (in_loss) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) sum[i] += x[i];
@@ -303,10 +311,11 @@ __global__ void __launch_bounds__(THREADS, PER == 16 ? 1 : BLOCKS_PER_SM) route_
 // One block per sample: sums of its rows, in 64 bits, and the losses.
 __global__ void __launch_bounds__(FINISH_THREADS) finish_kernel(const int* __restrict__ cu, int tokens, int E, int S, int run, const Part* __restrict__ part,
                                                                 const Part* __restrict__ part_z, float* __restrict__ balance, float* __restrict__ zloss,
-                                                                int* __restrict__ counts, int* __restrict__ ns) {
+                                                                int* __restrict__ counts, int* __restrict__ ns, float* __restrict__ usage) {
   __shared__ double p_sh[FINISH_THREADS];
   __shared__ int c_sh[FINISH_THREADS];
   __shared__ double3 total_sh[FINISH_THREADS / 32];
+  __shared__ double per_sh;
   pdl_wait();
   const int s = blockIdx.x, lo = bound(cu, s, S, tokens), hi = bound(cu, s + 1, S, tokens);
   const int row0 = lo / run + s, rows = hi > lo ? (hi - 1) / run - lo / run + 1 : 0;
@@ -354,25 +363,27 @@ __global__ void __launch_bounds__(FINISH_THREADS) finish_kernel(const int* __res
       balance[s] = some ? static_cast<float>(E * v.x / (v.z * v.z)) : 0.f;
       zloss[s] = some ? static_cast<float>(v.y / v.z) : 0.f;
       ns[s] = static_cast<int>(v.z);
+      per_sh = some ? E / (v.z * v.z) : 0.0;
     }
   }
+  __syncthreads();
+  if (g == 0) usage[static_cast<long long>(s) * E + e] = static_cast<float>(c * per_sh);
 }
 static_assert(FINISH_THREADS == 1024 && MOST_EXPERTS <= FINISH_THREADS, "a warp per 32 threads' sums, a thread to an expert at least");
 
 // What a token's gradient is made of; loaded one token ahead.
 template <int PER>
 struct Token {
-  float p[PER], d, w, l;
+  float p[PER], d, w, l, inverse;
   long long e;
   int s;
 };
 template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(BWD_THREADS, bwd_blocks(PER)) route_bwd_kernel(const float* __restrict__ probs, const long long* __restrict__ topi, const float* __restrict__ w,
-                                                                const float* __restrict__ dw, const float* __restrict__ lse, const int* __restrict__ sample,
-                                                                const int* __restrict__ counts, const int* __restrict__ ns, const float* __restrict__ dbalance,
+                                                                const float* __restrict__ dw, const float* __restrict__ lse, const float* __restrict__ inverse, const int* __restrict__ sample,
+                                                                const float* __restrict__ usage, const int* __restrict__ ns, const float* __restrict__ dbalance,
                                                                 const float* __restrict__ dz, int tokens, int E, int k, int S, int renorm, T* __restrict__ dlogits, int* status) {
   __shared__ __align__(16) float top_sh[BWD_WARPS][PER * 32];   // dtop of the token's chosen experts, zero elsewhere
-  __shared__ __align__(16) float row_sh[BWD_WARPS][PER * 32];   // its probabilities
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int i = 0; i < PER; ++i) top_sh[warp][lane * PER + i] = 0.f;
@@ -390,6 +401,7 @@ __global__ void __launch_bounds__(BWD_THREADS, bwd_blocks(PER)) route_bwd_kernel
     }
     o.s = sample[t];
     o.l = dz != nullptr ? lse[t] : 0.f;
+    o.inverse = inverse[t];
   };
   Token<PER> next;
   int t = blockIdx.x * BWD_WARPS + warp;
@@ -403,38 +415,19 @@ __global__ void __launch_bounds__(BWD_THREADS, bwd_blocks(PER)) route_bwd_kernel
     for (int i = 0; i < PER; ++i) g[i] = 0.f;
     float zt = 0.f;
     if (in_loss) {
-      const float n = static_cast<float>(ns[o.s]);
       if (dbalance != nullptr) {
-        const float f = dbalance[o.s] * (static_cast<float>(E) / n) / n;
-        const int* c = counts + static_cast<long long>(o.s) * E + lane * PER;
-        if constexpr (VEC && PER % 4 == 0) {
-          if (lane * PER < E) {
+        const float f = dbalance[o.s];
+        load_row<float, PER, VEC>(usage + static_cast<long long>(o.s) * E, E, lane, g);
 #pragma unroll
-            for (int i = 0; i < PER; i += 4) {
-              const int4 v = *reinterpret_cast<const int4*>(c + i);
-              g[i] = f * v.x; g[i + 1] = f * v.y; g[i + 2] = f * v.z; g[i + 3] = f * v.w;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < PER; ++i) if (lane * PER + i < E) g[i] = f * static_cast<float>(c[i]);
-        }
+        for (int i = 0; i < PER; ++i) g[i] = (VEC ? lane * PER : lane * PER + i) < E ? g[i] * f : 0.f;
       }
-      if (dz != nullptr) zt = 2.f * o.l * dz[o.s] / n;
+      if (dz != nullptr) zt = 2.f * o.l * dz[o.s] * reciprocal(static_cast<float>(ns[o.s]));
     }
     if (dw != nullptr) {
       float d = o.d;
       const bool named = lane < k && o.e >= 0 && o.e < E;
       if (lane < k && !named) atomicExch(status, 62);   // no expert: its pair has no gradient
-      if (renorm) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < PER; ++i) row_sh[warp][lane * PER + i] = o.p[i];
-        __syncwarp();
-        const float pt = named ? row_sh[warp][o.e] : 0.f;
-        const float dot = warp_sum(named ? d * o.w : 0.f), chosen = warp_sum(pt);
-        d = (d - dot) / chosen;
-      }
+      if (renorm) d = (d - sum_first(named ? d * o.w : 0.f, k)) * o.inverse;
       if (named) atomicAdd(&top_sh[warp][o.e], d);   // of an expert that is named twice, both
       __syncwarp();
 #pragma unroll
@@ -445,7 +438,7 @@ __global__ void __launch_bounds__(BWD_THREADS, bwd_blocks(PER)) route_bwd_kernel
     }
     float inner = 0.f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) inner += lane * PER + i < E ? o.p[i] * g[i] : 0.f;
+    for (int i = 0; i < PER; ++i) inner += (VEC ? lane * PER : lane * PER + i) < E ? o.p[i] * g[i] : 0.f;
     inner = warp_sum(inner);
 #pragma unroll
     for (int i = 0; i < PER; ++i) g[i] = o.p[i] * (g[i] - inner + zt);
@@ -480,32 +473,33 @@ using namespace mtb::rb;
   if (E <= 32) { CALL(1); } else if (E <= 64) { CALL(2); } else if (E <= 128) { CALL(4); } else if (E <= 256) { CALL(8); } else { CALL(16); }
 
 // part [rows, E] and part_z [rows] are scratch of 8 bytes an entry, rows at least S and BLOCKS_PER_SM (2) an SM. logits [T, E], bf16 or (fp32) fp32; cu [S + 1] int32 ascending, or null for one sample of all tokens (S = 1); counted [T] bytes, or null. probs [T, E], w [T, k], lse [T],
-// balance [S], zloss [S]: fp32; topi [T, k]: int64; counts [S, E], ns [S], sample [T] (whose losses a token is in, or -1): int32.
+// balance [S], zloss [S]: fp32; topi [T, k]: int64; counts [S, E], ns [S], sample [T] (whose losses a token is in, or -1): int32; inverse [T] (of the sum
+// of a token's chosen probabilities where renorm, else 1), usage [S, E] (E counts / n^2): fp32, for the gradient.
 int mtb200_route_balanced(const void* logits, int fp32, const int* cu, const void* counted, int T, int E, int k, int S, int renorm, float* probs, long long* topi, float* w,
-                          float* lse, int* sample, void* part, void* part_z, int rows, float* balance, float* zloss, int* counts, int* ns, cudaStream_t st) {
+                          float* lse, float* inverse, int* sample, void* part, void* part_z, int rows, float* balance, float* zloss, int* counts, int* ns, float* usage, cudaStream_t st) {
   if (!sizes_ok(T, E, k, S) || (cu == nullptr && S != 1)) return -10;
   const int run = run_of(T, sms_of()), blocks = (T + run - 1) / run;
   if (rows < blocks + S) return -11;
   const int per = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
   const bool vec = E % per == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(probs)) & 15) == 0;
-#define FWD(T_, PER, VEC) mtb::launch_pdl(route_kernel<T_, PER, VEC>, blocks, THREADS, 0, st, (const T_*)logits, cu, (const uint8_t*)counted, T, E, k, S, renorm, run, probs, topi, w, lse, sample, (Part*)part, (Part*)part_z)
+#define FWD(T_, PER, VEC) mtb::launch_pdl(route_kernel<T_, PER, VEC>, blocks, THREADS, 0, st, (const T_*)logits, cu, (const uint8_t*)counted, T, E, k, S, renorm, run, probs, topi, w, lse, inverse, sample, (Part*)part, (Part*)part_z)
 #define FWD_TYPE(PER) if (fp32) { if (vec) FWD(float, PER, true); else FWD(float, PER, false); } else { if (vec) FWD(bf16, PER, true); else FWD(bf16, PER, false); }
   ROUTE_PER(FWD_TYPE)
 #undef FWD_TYPE
 #undef FWD
-  mtb::launch_pdl(finish_kernel, S, FINISH_THREADS, 0, st, cu, T, E, S, run, (const Part*)part, (const Part*)part_z, balance, zloss, counts, ns);
+  mtb::launch_pdl(finish_kernel, S, FINISH_THREADS, 0, st, cu, T, E, S, run, (const Part*)part, (const Part*)part_z, balance, zloss, counts, ns, usage);
   return ok();
 }
 
 // dw [T, k], dbalance [S], dz [S]: fp32, any of them null. dlogits [T, E]: bf16 or (fp32) fp32.
-int mtb200_route_balanced_bwd(const float* probs, const long long* topi, const float* w, const float* dw, const float* lse, const int* sample, const int* counts, const int* ns, const float* dbalance, const float* dz, int T, int E, int k, int S, int renorm, void* dlogits, int fp32,
+int mtb200_route_balanced_bwd(const float* probs, const long long* topi, const float* w, const float* dw, const float* lse, const float* inverse, const int* sample, const float* usage, const int* ns, const float* dbalance, const float* dz, int T, int E, int k, int S, int renorm, void* dlogits, int fp32,
                               int* status, cudaStream_t st) {
   if (!sizes_ok(T, E, k, S)) return -10;
   const int per = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
   int blocks = (T + BWD_WARPS - 1) / BWD_WARPS;
   if (blocks > bwd_blocks(per) * sms_of()) blocks = bwd_blocks(per) * sms_of();
-  const bool vec = E % per == 0 && ((reinterpret_cast<uintptr_t>(dlogits) | reinterpret_cast<uintptr_t>(probs) | reinterpret_cast<uintptr_t>(counts)) & 15) == 0;
-#define BWD(T_, PER, VEC) mtb::launch_pdl(route_bwd_kernel<T_, PER, VEC>, blocks, BWD_THREADS, 0, st, probs, topi, w, dw, lse, sample, counts, ns, dbalance, dz, T, E, k, S, renorm, (T_*)dlogits, status)
+  const bool vec = E % per == 0 && ((reinterpret_cast<uintptr_t>(dlogits) | reinterpret_cast<uintptr_t>(probs) | reinterpret_cast<uintptr_t>(usage)) & 15) == 0;
+#define BWD(T_, PER, VEC) mtb::launch_pdl(route_bwd_kernel<T_, PER, VEC>, blocks, BWD_THREADS, 0, st, probs, topi, w, dw, lse, inverse, sample, usage, ns, dbalance, dz, T, E, k, S, renorm, (T_*)dlogits, status)
 #define BWD_TYPE(PER) if (fp32) { if (vec) BWD(float, PER, true); else BWD(float, PER, false); } else { if (vec) BWD(bf16, PER, true); else BWD(bf16, PER, false); }
   ROUTE_PER(BWD_TYPE)
 #undef BWD_TYPE

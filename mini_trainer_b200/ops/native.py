@@ -114,8 +114,8 @@ class _Sig:
     mtb200_gemm_lse = [P, L, P, P, P, P, I, I, I, F, I, P, P]
     mtb200_gemm_nll = [P, L, P, P, L, P, P, P, P, P, I, I, I, F, L, L, I, I, P, P]
     mtb200_nll = [P, P, P, I, I, L, L, P, P, P, P]
-    mtb200_route_balanced = [P, I, P, P, I, I, I, I, I, P, P, P, P, P, P, P, I, P, P, P, P, P]
-    mtb200_route_balanced_bwd = [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, I, P, P]
+    mtb200_route_balanced = [P, I, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, I, P, P, P, P, P, P]
+    mtb200_route_balanced_bwd = [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, I, P, P]
     mtb200_attn_fwd_one = [P, L, P, L, P, P, I, I, I, I, I, F, P, P]
     mtb200_attn_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, F, P, P]
     mtb200_attn_rule_fwd = [P, L, P, L, P, P, I, I, I, I, I, I, I, F, F, I, P, P, P]

@@ -28,29 +28,33 @@ class RouterBalance:
     * ``tokens``            [S] int32 counted tokens
     * ``lse``               [T] fp32 logsumexp of every token's logits
     * ``sample``            [T] int32 sample whose losses a token is in, -1 for none
+    * ``usage``             [S, E] fp32 ``E counts / tokens^2``, what an expert's probability weighs in its sample's loss
+    * ``inverse``           [T] fp32 one over the sum of a token's chosen probabilities, one where they are not renormalised
 
-    The kernels leave all of them in one buffer of 32-bit words, ``[counts | tokens | sample | loss | z_loss | lse]``; they are tensors when they are asked for, which a layer's step does for few of them.
+    The kernels leave all of them in one buffer of 32-bit words, in the order of ``NAMES``; they are tensors when they are asked for, which a layer's step does for few of them.
     """
 
-    NAMES = ("counts", "tokens", "sample", "loss", "z_loss", "lse")
+    NAMES = ("usage", "counts", "tokens", "sample", "loss", "z_loss", "lse", "inverse")
+    WHOLE = ("counts", "tokens", "sample")
 
     def __init__(self, T, E, S, words=None, **tensors):
         self.T, self.E, self.S, self.words = T, E, S, words
         self.__dict__.update(tensors)
 
     def offsets(self):
-        """First word of each of ``NAMES``."""
-        c = self.S * self.E
-        return 0, c, c + self.S, c + self.S + self.T, c + 2 * self.S + self.T, c + 3 * self.S + self.T
+        """First word of each of ``NAMES``, and the number of words."""
+        T, S, c = self.T, self.S, self.S * self.E
+        d = 2 * c + S + T
+        return 0, c, 2 * c, 2 * c + S, d, d + S, d + 2 * S, d + 2 * S + T, d + 2 * S + 2 * T
 
     def __getattr__(self, name):   # not there yet
         words = self.__dict__.get("words")
         if words is None or name not in self.NAMES:
             raise AttributeError(name)
-        i = self.NAMES.index(name)
-        t = words.narrow(0, self.offsets()[i], (self.S * self.E, self.S, self.T)[i if i < 3 else (1, 1, 2)[i - 3]])
-        t = t.view(self.S, self.E) if i == 0 else t.view(torch.float32) if i >= 3 else t
-        self.__dict__[name] = t
+        i, at = self.NAMES.index(name), self.offsets()
+        t = words[at[i]:at[i + 1]]
+        t = t if name in self.WHOLE else t.view(torch.float32)
+        self.__dict__[name] = t = t.view(self.S, self.E) if i < 2 else t
         return t
 
 
@@ -131,7 +135,9 @@ def plain(logits, k, renorm, cu_seqlens=None, counted=None):
     n = tokens.clamp_min(1).double()
     z = torch.zeros(S, dtype=torch.float64, device=l.device).index_add_(0, sample[ok], lse[ok].double().square())
     loss, z = (E * (counts * sums).sum(1) / n.square()).float(), (z / n).float()
-    return probs, topi, w, RouterBalance(T, E, S, loss=loss, z_loss=z, counts=counts.to(torch.int32), tokens=tokens.to(torch.int32), lse=lse, sample=sample.to(torch.int32))
+    inverse = 1.0 / top.sum(-1) if renorm else torch.ones(T, device=l.device)
+    usage = (E * counts / n.square()[:, None]).float()
+    return probs, topi, w, RouterBalance(T, E, S, usage=usage, inverse=inverse, loss=loss, z_loss=z, counts=counts.to(torch.int32), tokens=tokens.to(torch.int32), lse=lse, sample=sample.to(torch.int32))
 
 
 def plain_bwd(probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.bfloat16):
@@ -141,10 +147,10 @@ def plain_bwd(probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=torch.
     n = bal.tokens.clamp_min(1).float()
     g = torch.zeros_like(probs)
     if dw is not None:
-        d = (dw - (dw * w).sum(-1, keepdim=True)) / probs.gather(1, topi).sum(-1, keepdim=True) if renorm else dw
+        d = (dw - (dw * w).sum(-1, keepdim=True)) * bal.inverse[:, None] if renorm else dw
         g.scatter_add_(1, topi, d)
     if dloss is not None:
-        g[ok] += ((dloss * E / n / n)[:, None] * bal.counts)[sample[ok]]
+        g[ok] += (dloss[:, None] * bal.usage)[sample[ok]]
     g = g - (g * probs).sum(-1, keepdim=True)
     if dz is not None:
         g[ok] += (2.0 * bal.lse[ok] * (dz / n)[sample[ok]])[:, None]
@@ -158,16 +164,17 @@ def native(ops, logits, k, renorm, cu_seqlens=None, counted=None):
     dev, f32 = logits.device, torch.float32
     with ops.on_device():
         probs, topi, w = torch.empty(T, E, dtype=f32, device=dev), torch.empty(T, k, dtype=torch.int64, device=dev), torch.empty(T, k, dtype=f32, device=dev)
-        bal = RouterBalance(T, E, S, torch.empty(S * (E + 3) + 2 * T, dtype=torch.int32, device=dev))
+        bal = RouterBalance(T, E, S)
+        usage, counts, tokens, sample, loss, z, lse, inverse, words = bal.offsets()
+        bal.words = torch.empty(words, dtype=torch.int32, device=dev)
         if T == 0:
             bal.words.zero_()
             return probs, topi, w, bal
         rows, at = _BLOCKS_PER_SM * ops.sms + S, bal.words.data_ptr()
         part = torch.empty(rows * (E + 1), dtype=torch.int64, device=dev).data_ptr()
-        counts, tokens, sample, loss, z, lse = bal.offsets()
         ops._call("mtb200_route_balanced", logits.data_ptr(), logits.dtype is f32, None if cu_seqlens is None else cu_seqlens.data_ptr(), None if counted is None else counted.data_ptr(),
-                  T, E, k, S, bool(renorm), probs.data_ptr(), topi.data_ptr(), w.data_ptr(), at + 4 * lse, at + 4 * sample, part, part + 8 * rows * E, rows, at + 4 * loss, at + 4 * z,
-                  at, at + 4 * tokens, ops._st(), n=2)
+                  T, E, k, S, bool(renorm), probs.data_ptr(), topi.data_ptr(), w.data_ptr(), at + 4 * lse, at + 4 * inverse, at + 4 * sample, part, part + 8 * rows * E, rows,
+                  at + 4 * loss, at + 4 * z, at + 4 * counts, at + 4 * tokens, at + 4 * usage, ops._st(), n=2)
     return probs, topi, w, bal
 
 
@@ -179,10 +186,10 @@ def native_bwd(ops, probs, topi, w, dw, renorm, bal, dloss=None, dz=None, dtype=
         if T:
             if bal.words is not None:
                 at = bal.words.data_ptr()
-                counts, tokens, sample, _, _, lse = (at + 4 * i for i in bal.offsets())
+                usage, _, tokens, sample, _, _, lse, inverse, _ = (at + 4 * i for i in bal.offsets())
             else:
-                counts, tokens, sample, lse = (t.data_ptr() for t in (bal.counts, bal.tokens, bal.sample, bal.lse))
-            ops._call("mtb200_route_balanced_bwd", probs.data_ptr(), topi.data_ptr(), w.data_ptr(), None if dw is None else dw.data_ptr(), lse, sample, counts, tokens,
+                usage, tokens, sample, lse, inverse = (t.data_ptr() for t in (bal.usage, bal.tokens, bal.sample, bal.lse, bal.inverse))
+            ops._call("mtb200_route_balanced_bwd", probs.data_ptr(), topi.data_ptr(), w.data_ptr(), None if dw is None else dw.data_ptr(), lse, inverse, sample, usage, tokens,
                       None if dloss is None else dloss.data_ptr(), None if dz is None else dz.data_ptr(), T, E, k, S, bool(renorm), out.data_ptr(), dtype is torch.float32,
                       ops.status.data_ptr(), ops._st())
     return out
