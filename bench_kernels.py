@@ -5,6 +5,7 @@
     python bench_kernels.py --op all
     python bench_kernels.py --op families      # LayerNorm, per-head q/k norm, GeGLU / GELU
     python bench_kernels.py --op shaped --lens 2726,2184,3282 --tokens 16384   # attention under a rule, norms around a branch, capped head
+    python bench_kernels.py --op routed        # router with its balance losses, likelihoods without logits, orthogonalised updates
     (ops: gemm, attn_fwd, attn_bwd, rmsnorm, swiglu, rope, ce, linear_ce, embedding, adamw)
 
 Each op is timed with CUDA events on the launching stream after warm-up, with a synchronize on
@@ -295,8 +296,32 @@ def main():
         for cap in (None, 30.0):
             report(f"linear_ce_{T}x{H}x{V}" + ("_capped" if cap else ""), timeit(lambda: ops.linear_ce(x, w, tg, 1.0, dw, softcap=cap), a.iters, a.warmup, flush),
                    flops=6.0 * T * H * V)
-    for name, fn in (("shaped", op_shaped), ("layernorm", op_layernorm), ("head_rmsnorm", op_head_rmsnorm), ("geglu", op_geglu)):
-        if a.op == name or a.op == "families" and name != "shaped":   # kernels of the model families beyond the Llama block; not part of --op all
+    def op_routed():
+        for T, E, k, S in ((a.tokens, 8, 2, 1), (a.tokens, 128, 8, 40)):
+            logits, dw = torch.randn(T, E, device="cuda"), torch.randn(T, k, device="cuda")
+            cu = torch.linspace(0, T, S + 1).to(torch.int32).cuda()
+            one = torch.ones(S, device="cuda")
+            probs, topi, w, bal = ops.route_balanced(logits, k, True, cu)
+            report(f"route_balanced_fwd_{T}x{E}", timeit(lambda: ops.route_balanced(logits, k, True, cu), a.iters, a.warmup, flush), bytes_=T * (8.0 * E + 12 * k + 12))
+            report(f"route_balanced_bwd_{T}x{E}", timeit(lambda: ops.route_balanced_bwd(probs, topi, w, dw, True, bal, one, one, torch.float32), a.iters, a.warmup, flush),
+                   bytes_=T * (8.0 * E + 16 * k + 12))
+        T, H, V = 4096, a.hidden, a.vocab
+        x, w = bf(T, H), bf(V, H, scale=0.02)
+        tg, dw, dl = torch.randint(0, V, (T,), device="cuda"), torch.empty(V, H, dtype=torch.bfloat16, device="cuda"), torch.randn(T, device="cuda")
+        loss, lse = ops.linear_nll(x, w, tg)
+        report(f"linear_nll_{T}x{H}x{V}", timeit(lambda: ops.linear_nll(x, w, tg), a.iters, a.warmup, flush), flops=2.0 * T * H * V)
+        report(f"linear_nll_bwd_{T}x{H}x{V}", timeit(lambda: ops.linear_nll_bwd(dl, x, w, tg, loss, lse, dw), a.iters, a.warmup, flush), flops=6.0 * T * H * V)
+        del x, w, dw
+        for shape in ((64, 64), (128, 1024), (256, 688), (1536, 1536), (4096, 4096), (64, 2048, 1024)):
+            g = torch.randn(*shape, device="cuda")
+            m, n = sorted(shape[-2:])
+            report("orthogonalise_" + "x".join(map(str, shape)), timeit(lambda: ops.orthogonalise(g), a.iters, a.warmup, flush),
+                   flops=5.0 * g.numel() / (m * n) * (3.0 * m * m * n + m ** 3))
+        g, m, w = (torch.randn(14336, 4096, device="cuda") for _ in range(3))
+        p = torch.empty(14336, 4096, dtype=torch.bfloat16, device="cuda")
+        report("muon_step_14336x4096", timeit(lambda: ops.muon_step(w, m, g, p, 1e-4, 0.95, 0.1), a.iters, a.warmup, flush), flops=5.0 * (3.0 * 4096 ** 2 * 14336 + 4096.0 ** 3))
+    for name, fn in (("shaped", op_shaped), ("routed", op_routed), ("layernorm", op_layernorm), ("head_rmsnorm", op_head_rmsnorm), ("geglu", op_geglu)):
+        if a.op == name or a.op == "families" and name not in ("shaped", "routed"):   # kernels of the model families beyond the Llama block; not part of --op all
             torch.cuda.empty_cache()
             fn()
     for name, fn in (("rmsnorm", op_rmsnorm), ("swiglu", op_swiglu), ("rope", op_rope), ("ce", op_ce), ("linear_ce", op_linear_ce),

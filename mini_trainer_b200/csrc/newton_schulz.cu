@@ -12,11 +12,15 @@
 // range (|X| <= 1.3, |A| <= 1.6 and |polynomial| <= 3.5 in norm, whatever G is). Its 11 bits are eight times finer than bf16's 8. That alone is not enough: a rounding of X is noise
 // in all directions, and a direction in which X has next to nothing grows by a = 3.44 in each step, 485 times in five. So X is held as two numbers, hi and lo = 2^11 (X - hi), and the
 // last product's epilogue adds a lo to the polynomial times hi: what is left of the rounding is what b A and c A^2 would have made of it, which is small
-// in just those directions. What is rounded in the last two steps grows little more; their X goes without. Error of the result, relative, simulated with the roundings: normal 512 x 1376 1.7e-3 (bf16 throughout: 1.1e-2), features of different
-// size 1.4e-3 (9e-2), rank 8 and a hundredth of noise 2.2e-3 (0.26), rank 1 2.7e-3 (0.76); half of bf16's step, to which the result is rounded, is 1.7e-3 in the mean. Sums are fp32 in tensor memory.
+// in just those directions. What is rounded in the last two steps grows little more; their X goes without. Error of the result, relative, simulated with the roundings (in brackets: X without lo, and
+// bf16 throughout): normal 512 x 1376 1.3e-3 (1.3e-3, 1.1e-2), sums of outer products of features that differ in size 1.3e-3 (2.2e-3, 1.7e-2), rank 8 and a hundredth of noise 2.5e-3 (3.7e-2, 0.3), rank 1 3.4e-3
+// (0.15, 1.2); half of bf16's step, to which the result is rounded, is 1.7e-3 in the mean. Sums are fp32 in tensor memory.
 //
 // The products: persistent, warp-specialised, 3-D TMA maps over the stack, tcgen05.mma of fp16 into two accumulators in tensor memory, by single CTAs (tiles of 128 x 128, for few tiles) or CTA pairs
-// (256 x 256). All launches of a call are queued by one host call, each under its predecessor's tail.
+// (256 x 256). All launches of a call are queued by one host call, each under its predecessor's tail. A large call is bound by its products: 4096 x 4096 (0.38 PFLOP in five steps' tiles) 1.10 ms,
+// its gram product and square 59 us each at 76 % of the tensor pipe (136 tiles on 74 pairs), its last product 100 us at 88 %. A launch of one round is bound by its chain, about 3.9 us beside its reduction (first
+// operands 1.0, sums to stores 1.5, end to the next one's start 1.4), and on single CTAs by L2, from which an SM takes 64 bytes a clock: 0.25 us for 64 of the reduction. More epilogue warps (sixteen of
+// 32 columns) made it longer: 688 x 256 88 -> 95 us, 1024 x 1024 121 -> 127.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -145,7 +149,7 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int gro
 }
 
 // A warp's 32 rows of 64 columns between memory and registers go by its staging in shared memory: eight lanes to a row there, a lane to a row here. (TMA stores of the staged boxes queue
-// behind the operands' loads, up to six stages of them, and a tile has four to wait for: 64 x 2048 x 1024 3.2 ms, APPLY_TIMES.)
+// behind the operands' loads, and a tile has four to wait for: the last product of 64 x 2048 x 1024 with hi and lo 303 us with them, 260 so.)
 __device__ __forceinline__ uint4* staged(uint8_t* box, int row, int piece) { return reinterpret_cast<uint4*>(box + row * 128 + ((piece ^ (row & 7)) << 4)); }
 // What is added to the sums, into the second box, asked for ahead of them, so that it arrives under their wait.
 __device__ __forceinline__ void ask(const Params& p, uint8_t* box, int y0, int col, int z, int lane) {
@@ -695,8 +699,8 @@ __global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__
 // Where the shorter side is at most 128 and the longer one at most 4096 a call is one launch: a cluster of up to sixteen CTAs has a matrix, each a slab of the longer side, which stays in shared memory as hi and
 // lo from the first step to the last. In a slab's 64 columns rows are 128 bytes apart, which is an operand with the columns as the reduction (the gram product) and with the rows as the reduction (the last
 // product) alike; a matrix with more rows than columns is turned when it is read. Per step: the gram product of the slab; its sums to the CTA that finishes those rows and columns (shared memory of the cluster), which adds them
-// in the order of the slabs and gives A to all; its square, every CTA for itself; the polynomial over A; the last product and the slab's new hi and lo. What bounds it is the chain of those,
-// about 4 us a step; the launches of the other form take 11 to 16. SMALL_TIMES
+// in the order of the slabs and gives A to all; its square, every CTA for itself; the polynomial over A; the last product and the slab's new hi and lo. Bound by the chain of those: a step takes 2.0 us for 64 x 64,
+// 4.9 for 128 x 256, 8.2 and 10.4 in two and eight slabs of 256 (the other form's launches 14 to 16): 64 x 64 56 -> 16 us, 128 x 512 88 -> 54, 32 x 2048 74 -> 37, 64 x 4096 84 -> 52.
 constexpr int SMALL_R = 128, SMALL_W = 256, SMALL_PARTS = 16, SMALL_THREADS = 512;
 constexpr int SMALL_A = 2 * SMALL_R * 128, SMALL_RECV = 16 * 4096;
 constexpr int small_smem(int w) { return 2 * w * 2 * SMALL_R + SMALL_A + SMALL_RECV + 1024 + 256; }
