@@ -696,19 +696,21 @@ __global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------ a whole call in one launch
-// Where the shorter side is at most 128 and the longer one at most 4096 a call is one launch: a cluster of up to sixteen CTAs has a matrix, each a slab of the longer side, which stays in shared memory as hi and
-// lo from the first step to the last. In a slab's 64 columns rows are 128 bytes apart, which is an operand with the columns as the reduction (the gram product) and with the rows as the reduction (the last
-// product) alike; a matrix with more rows than columns is turned when it is read. Per step: the gram product of the slab; its sums to the CTA that finishes those rows and columns (shared memory of the cluster), which adds them
-// in the order of the slabs and gives A to all; its square, every CTA for itself; the polynomial over A; the last product and the slab's new hi and lo. Bound by the chain of those: a step takes 2.0 us for 64 x 64,
-// 4.9 for 128 x 256, 8.2 and 10.4 in two and eight slabs of 256 (the other form's launches 14 to 16): 64 x 64 56 -> 16 us, 128 x 512 88 -> 54, 32 x 2048 74 -> 37, 64 x 4096 84 -> 52.
-constexpr int SMALL_R = 128, SMALL_W = 256, SMALL_PARTS = 16, SMALL_THREADS = 512;
+// Where the shorter side is at most 128 a call may be one launch: a cluster of up to sixteen CTAs has a matrix, each a slab of the longer side (256, 512 or 1024 columns where the shorter one is up to 128, 64 or 32),
+// which stays in shared memory as hi and lo from the first step to the last. In a slab's 64 columns rows are 128 bytes apart, which is an operand with the columns as the reduction (the gram product) and with the
+// rows as the reduction (the last product) alike; a matrix with more rows than columns is turned when it is read. Per step: the gram product of the slab; its sums to the CTA that finishes those rows and columns (shared
+// memory of the cluster), which adds them in the order of the slabs and gives A to all; its square, every CTA for itself; the polynomial over A; the last product and the slab's new hi and lo.
+// A slab of at most 64 (32) rows goes through the last product in two (four) parts side by side: the polynomial stands two (four) times on the diagonal of a 128 x 128 operand, the reduction runs over
+// the parts one behind the other, and each part's columns come out in rows of their own, so that all warps have some. Bound by the chain of
+// those, a step takes 2.0 us for 64 x 64, 2.9 for 32 x 256, 5.3 for 128 x 256 and 8.7 in two slabs of it (the other form's launches 14 to 22): 64 x 64 56 -> 15 us, 128 x 512 88 -> 54, 32 x 2048 74 -> 37, 64 x 8192 100 -> 61.
+constexpr int SMALL_R = 128, SMALL_PARTS = 16, SMALL_THREADS = 512, SMALL_ENTRIES = 128 * 256;   // most of a slab
 constexpr int SMALL_A = 2 * SMALL_R * 128, SMALL_RECV = 16 * 4096;
-constexpr int small_smem(int w) { return 2 * w * 2 * SMALL_R + SMALL_A + SMALL_RECV + 1024 + 256; }
-static_assert(small_smem(SMALL_W) <= 227 * 1024, "shared memory");
+constexpr int small_smem(int entries) { return 4 * entries + SMALL_A + SMALL_RECV + 1024 + 256; }
+static_assert(small_smem(SMALL_ENTRIES) <= 227 * 1024, "shared memory");
 
 struct Small {
   int rows, cols, r, n, tall;    // r: the shorter side, n: the longer one; tall: it is the rows
-  int w, parts;                  // columns of a slab, slabs
+  int w, parts, R;               // columns of a slab, slabs; rows of a slab in shared memory, 32, 64 or 128
   int steps, kept, p2, vec;
   __nv_bfloat16* out;            // what is orthogonalised, or null: the update
   float* master;
@@ -745,7 +747,7 @@ __device__ __forceinline__ void gather8(const Source& s, const Small& p, float c
     }
   }
 }
-__device__ __forceinline__ uint4* piece_at(uint8_t* x, int row, int piece) { return reinterpret_cast<uint4*>(x + (piece >> 3) * (SMALL_R * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4)); }
+__device__ __forceinline__ uint4* piece_at(uint8_t* x, int row, int piece, int R = SMALL_R) { return reinterpret_cast<uint4*>(x + (piece >> 3) * (R * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4)); }
 // Bounded, as mbar_wait, for what other CTAs of the cluster have sent.
 __device__ __forceinline__ bool wait_sent(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
@@ -768,8 +770,9 @@ __device__ __forceinline__ void send16(uint32_t to, uint4 v, uint32_t bar) {
 __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source src, const Small p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* hi = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* lo = hi + p.w * 2 * SMALL_R;
-  uint8_t* a = lo + p.w * 2 * SMALL_R;         // A, then the polynomial in its place: 128 x 128, two blocks of 64 columns
+  const int R = p.R, copies = SMALL_R / R, cw = p.w / copies;   // parts of a slab in the last product, and their columns
+  uint8_t* lo = hi + p.w * 2 * R;
+  uint8_t* a = lo + p.w * 2 * R;               // A, then the polynomial in its place: 128 x 128, two blocks of 64 columns
   uint8_t* recv = a + SMALL_A;                 // sums from the other slabs
   double* norm = reinterpret_cast<double*>(recv + SMALL_RECV);
   uint64_t* done_bar = reinterpret_cast<uint64_t*>(norm + SMALL_PARTS);
@@ -820,13 +823,13 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
 #pragma unroll
       for (int j = 0; j < 8; ++j) sq = fmaf(u[b][j], u[b][j], sq);
       total += sq;
-      *piece_at(hi, row[b], piece[b]) = make_uint4(__float_as_uint(u[b][0]), __float_as_uint(u[b][1]), __float_as_uint(u[b][2]), __float_as_uint(u[b][3]));
-      *piece_at(lo, row[b], piece[b]) = make_uint4(__float_as_uint(u[b][4]), __float_as_uint(u[b][5]), __float_as_uint(u[b][6]), __float_as_uint(u[b][7]));
+      *piece_at(hi, row[b], piece[b], R) = make_uint4(__float_as_uint(u[b][0]), __float_as_uint(u[b][1]), __float_as_uint(u[b][2]), __float_as_uint(u[b][3]));
+      *piece_at(lo, row[b], piece[b], R) = make_uint4(__float_as_uint(u[b][4]), __float_as_uint(u[b][5]), __float_as_uint(u[b][6]), __float_as_uint(u[b][7]));
     }
   }
-  for (int i = threadIdx.x; i < (SMALL_R - p.r) * pieces; i += SMALL_THREADS) {   // rows that are not there
+  for (int i = threadIdx.x; i < (R - p.r) * pieces; i += SMALL_THREADS) {   // rows that are not there
     const int row = p.r + i / pieces;
-    uint4* x = piece_at(hi, row, i - (row - p.r) * pieces);
+    uint4* x = piece_at(hi, row, i - (row - p.r) * pieces, R);
     *x = *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(x) + (lo - hi)) = make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
@@ -857,7 +860,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
   for (int i = threadIdx.x; i < tasks; i += SMALL_THREADS) {
     int row, piece;
     task(i, row, piece);
-    const uint4 x = *piece_at(hi, row, piece), y = *piece_at(lo, row, piece);
+    const uint4 x = *piece_at(hi, row, piece, R), y = *piece_at(lo, row, piece, R);
     const uint32_t u[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     uint32_t h[4], l[4];
 #pragma unroll
@@ -867,15 +870,15 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
       const float2 b = unpack_f16(h[j]);
       l[j] = pack_f16((c - b.x) * (1 << LO_BITS), (d - b.y) * (1 << LO_BITS));
     }
-    *piece_at(hi, row, piece) = make_uint4(h[0], h[1], h[2], h[3]);
-    *piece_at(lo, row, piece) = make_uint4(l[0], l[1], l[2], l[3]);
+    *piece_at(hi, row, piece, R) = make_uint4(h[0], h[1], h[2], h[3]);
+    *piece_at(lo, row, piece, R) = make_uint4(l[0], l[1], l[2], l[3]);
   }
 
   const float alpha_a = static_cast<float>(ldexp(SCALE_A, -2 * p.p2)), alpha_p = static_cast<float>(SCALE_P * NS_C / (SCALE_A * SCALE_A)), beta_p = static_cast<float>(SCALE_P * NS_B / SCALE_A);
   constexpr float diag_p = static_cast<float>(SCALE_P * NS_A), beta_x = static_cast<float>(NS_A / (1 << LO_BITS));
   const uint32_t idesc_sq = idesc_f16(SMALL_R, (p.r + 31) / 32 * 32, false, false);   // columns of the warps' parts that are there
   const int ksteps = (p.r + 15) / 16;
-  const uint32_t idesc_last = idesc_f16(SMALL_R, p.w, false, true);
+  const uint32_t idesc_last = idesc_f16(SMALL_R, cw, false, true);
   const uint32_t quarter = tmem + (static_cast<uint32_t>(q * 32) << 16), d3 = SMALL_R;   // D3 behind the square's columns
   const int row = q * 32 + lane;
   const bool there = q * 32 < p.r && sub * 32 < p.r;   // whether this warp's part of the square matrices is; the others stay zero
@@ -907,7 +910,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
   for (int step = 0; step < p.steps; ++step) {
     multiply([&]() {
       for (int k = 0; k < p.w / 16; ++k) {
-        const uint64_t d = make_smem_desc(smem_u32(hi) + (k >> 2) * (SMALL_R * 128) + (k & 3) * 32, 16, 1024);
+        const uint64_t d = make_smem_desc(smem_u32(hi) + (k >> 2) * (R * 128) + (k & 3) * 32, 16, 1024);   // (rows past R are the next columns', and what they give is not read)
         umma_bf16(tmem, d, d, idesc_sq, k != 0);
       }
     });
@@ -980,8 +983,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
       tmem_ld_wait();
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint4* place = piece_at(a, row, sub * 4 + i);
-        const uint4 old = *place;
+        const uint4 old = *piece_at(a, row, sub * 4 + i);
         const uint32_t o[4] = {old.x, old.y, old.z, old.w};
         uint32_t h[4];
 #pragma unroll
@@ -993,26 +995,29 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
           if (col + 1 == row) y += diag_p;
           h[j] = pack_f16(x, y);
         }
-        *place = make_uint4(h[0], h[1], h[2], h[3]);
+        for (int c = 0; c < copies; ++c) *piece_at(a, row + c * R, sub * 4 + i + c * (R / 8)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
     }
     multiply([&]() {
-      for (int k = 0; k < ksteps; ++k) {
-        const uint64_t da = make_smem_desc(smem_u32(a) + (k >> 2) * (SMALL_R * 128) + (k & 3) * 32, 16, 1024);
-        const uint64_t db = make_smem_desc(smem_u32(hi) + k * 2048, SMALL_R * 128, 1024);
-        umma_bf16(tmem + d3, da, db, idesc_last, k != 0);
-      }
+      for (int c = 0; c < copies; ++c)
+        for (int k = 0; k < ksteps; ++k) {
+          const int at_k = c * R + k * 16;
+          const uint64_t da = make_smem_desc(smem_u32(a) + (at_k >> 6) * (SMALL_R * 128) + (at_k & 63) * 2, 16, 1024);
+          const uint64_t db = make_smem_desc(smem_u32(hi) + c * (cw / 64) * (R * 128) + k * 2048, R * 128, 1024);
+          umma_bf16(tmem + d3, da, db, idesc_last, (c | k) != 0);
+        }
     });
     const bool end = step + 1 == p.steps, to_out = end && p.out != nullptr;
     const float alpha_x = static_cast<float>(ldexp(1.0 / SCALE_P, to_out ? -p.p2 : 0));
-    if (q * 32 < p.r) {
+    const int xrow = (q * 32) % R + lane, xcol = q * 32 / R * cw;   // of the slab: this lane's row, the first column of its part
+    if (xrow - lane < p.r) {
       const float2 alpha2 = make_float2(alpha_x, alpha_x), beta2 = make_float2(beta_x, beta_x), up2 = make_float2(1 << LO_BITS, 1 << LO_BITS);
 #pragma unroll 1
-      for (int c = sub * (p.w / 4); c < (sub + 1) * (p.w / 4); c += 16) {
+      for (int c = sub * (cw / 4); c < (sub + 1) * (cw / 4); c += 16) {
         uint32_t v[16];
         tmem_ld_32x16(quarter + d3 + c, v);
-        uint8_t *hp = reinterpret_cast<uint8_t*>(piece_at(hi, row, c / 8)), *lp = lo + (hp - hi);
-        const int second = row & 1 ? -16 : 16;   // c is a multiple of 16: its second piece differs in the lowest bit
+        uint8_t *hp = reinterpret_cast<uint8_t*>(piece_at(hi, xrow, (xcol + c) / 8, R)), *lp = lo + (hp - hi);
+        const int second = xrow & 1 ? -16 : 16;   // c is a multiple of 16: its second piece differs in the lowest bit
         uint32_t o[8];
         if (step < p.kept) {
           const uint4 x = *reinterpret_cast<const uint4*>(lp), y = *reinterpret_cast<const uint4*>(lp + second);
@@ -1047,7 +1052,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
     task(i, row, piece);
     const int col = n0 + piece * 8, n = row < p.r ? max(0, min(8, p.n - col)) : 0;
     if (n == 0) continue;
-    const uint4 x = *piece_at(hi, row, piece);
+    const uint4 x = *piece_at(hi, row, piece, R);
     const uint32_t u[4] = {x.x, x.y, x.z, x.w};
     float f[8];
 #pragma unroll
@@ -1205,43 +1210,54 @@ static Layout layout(long long rows, long long cols, long long stack) {
   return l;
 }
 
-// The call in one launch; 1 where it does not fit one.
+// Clusters of `parts` CTAs that can be resident at once, 0 where the device takes none of that size.
+static int small_room(int parts) {
+  static int known[SMALL_PARTS + 1] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
+  if (known[parts] < 0) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(parts); cfg.blockDim = dim3(SMALL_THREADS); cfg.dynamicSmemBytes = small_smem(SMALL_ENTRIES);
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_ENTRIES)) != cudaSuccess ||
+        cudaFuncSetAttribute(small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, small_kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+    known[parts] = n;
+  }
+  return known[parts];
+}
+// The call in one launch; 1 where it does not fit one, or would take longer so.
 static int small_call(const Source& src, Small p, long long stack, cudaStream_t st) {
   p.tall = p.rows > p.cols;
   p.r = p.tall ? p.cols : p.rows;
   p.n = p.tall ? p.rows : p.cols;
-  if (p.r > SMALL_R || p.n > SMALL_W * SMALL_PARTS || stack > 1 << 20) return 1;
-  p.parts = 1;   // as few slabs as hold the matrix: what they exchange takes longer than what they save (128 x 128 27 us as one, 38 as two)
-  while (p.parts < SMALL_PARTS && p.n > SMALL_W * p.parts) p.parts *= 2;
-  p.w = static_cast<int>(up((p.n + p.parts - 1) / p.parts, 64));
+  if (p.r > SMALL_R || stack > 1 << 20) return 1;
+  p.R = p.r <= 32 && p.n > 128 ? 32 : p.r <= 64 && p.n > 64 ? 64 : 128;   // a slab's parts have 64 columns at least
   p.kept = p.steps > 2 ? p.steps - 2 : p.steps - 1;
-  static int known[SMALL_PARTS + 1] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};   // clusters of that size at once, 0 where the device takes none
-  int& room = known[p.parts];
-  if (room < 0) {
-    if (cudaFuncSetAttribute(small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_W)) != cudaSuccess ||
-        cudaFuncSetAttribute(small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return -4;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = p.parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(p.parts); cfg.blockDim = dim3(SMALL_THREADS); cfg.dynamicSmemBytes = small_smem(SMALL_W);
-    cfg.attrs = &attr; cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, small_kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
-    room = n;
+  const int most = SMALL_ENTRIES / p.R, step = 64 * (SMALL_R / p.R);
+  // Rounds of clusters, of what a slab's size takes and what its exchange does, in us, against fifteen launches that pass over the matrices six times a step: 32 x 2048 47 as two slabs and 37 as eight, 128 x 128 27 as
+  // one and 38 as two, 64 x 128 x 1024 (two rounds of clusters of four) 157 and 130 in the other form.
+  double least = 75.0 + static_cast<double>(stack) * p.r * p.n * 6.5e-6;
+  p.parts = 0;
+  for (int parts = 1; parts <= SMALL_PARTS; parts *= 2) {
+    const int w = static_cast<int>(up((p.n + parts - 1) / parts, step));
+    if (w > most) continue;
+    const int room = small_room(parts);
+    if (room <= 0) continue;
+    const double e = w * p.R / 8192.0, wide = p.r > 64 ? 1.0 : 0.0;
+    const double t = (stack > room ? 1.3 : 1.0) * ((stack + room - 1) / room) * (3.0 + 2.3 * e + p.steps * (2.1 + 0.5 * wide + 0.78 * e + (parts > 1 ? 1.9 + 2.6 * wide + 0.1 * parts : 0.0)));
+    if (t < least) { least = t; p.parts = parts; p.w = w; }
   }
-  if (room <= 0) return 1;
-  // Rounds of clusters against fifteen launches that pass over the matrices six times a step, in us (five steps): 64 x 128 x 1024, two rounds of clusters of four, 157 as one launch and 130 so; 64 x 128 x 256 37 and 80.
-  const double here = (stack > room ? 1.3 : 1.0) * ((stack + room - 1) / room) * (18.0 + 6.5 * (p.w / 64 - 1) + (p.parts > 1 ? (p.r > 64 ? 16.0 : 8.0) + 1.5 * p.parts : 0.0));
-  const double there = 75.0 + static_cast<double>(stack) * p.r * p.n * 6.5e-6;
-  if (here > there) return 1;
+  if (p.parts == 0) return 1;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = p.parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(stack * p.parts)); cfg.blockDim = dim3(SMALL_THREADS); cfg.dynamicSmemBytes = small_smem(p.w); cfg.stream = st;
+  cfg.gridDim = dim3(static_cast<unsigned>(stack * p.parts)); cfg.blockDim = dim3(SMALL_THREADS); cfg.dynamicSmemBytes = small_smem(p.w * p.R); cfg.stream = st;
   cfg.attrs = attr; cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, small_kernel, src, p) == cudaSuccess ? 0 : -5;
 }

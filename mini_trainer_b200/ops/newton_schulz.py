@@ -94,7 +94,8 @@ def plain_muon(master, moment, grad, param_out, lr, momentum, weight_decay, grad
 # -- kernels --------------------------------------------------------------------------------
 def _launches(m, n, steps):
     """One where ``small_kernel`` of csrc/newton_schulz.cu takes the matrix, else two in front of the products and three of these a step."""
-    return 1 if min(m, n) <= 128 and max(m, n) <= 4096 else 2 + 3 * steps
+    r = min(m, n)
+    return 1 if r <= 128 and max(m, n) <= 16 * 32768 // (32 if r <= 32 else 64 if r <= 64 else 128) else 2 + 3 * steps
 
 
 def _workspace(ops, m, n, stack, device):

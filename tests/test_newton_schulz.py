@@ -158,7 +158,7 @@ def native():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", SHAPES + [(256, 688), (688, 256), (512, 512), (300, 1001), (1001, 300), (1100, 1300), (1300, 1032), (5, 260, 520), (20, 136, 64), (70, 264, 264),
-                                            (128, 2048), (2048, 128), (100, 2049), (2100, 40), (128, 4096), (3, 3001, 70), (100, 4100), (128, 300), (33, 1030), (90, 64, 700), (40, 700, 128), (160, 24, 24), (9, 128, 1025)])
+                                            (128, 2048), (2048, 128), (100, 2049), (2100, 40), (128, 4096), (3, 3001, 70), (100, 4100), (64, 128), (32, 129), (20, 257), (257, 64), (50, 513), (33, 8192), (8192, 64), (32, 16384), (17, 9000), (16385, 30), (8193, 48), (5, 31, 3000), (128, 300), (33, 1030), (90, 64, 700), (40, 700, 128), (160, 24, 24), (9, 128, 1025)])
 @pytest.mark.parametrize("kind", KINDS)
 def test_kernels(native, shape, kind):
     g = matrices(kind, *shape, device="cuda")
