@@ -5,8 +5,8 @@ softmax, the ``k`` largest logits of each token (the lower expert of equal ones;
 over the chosen ones where ``renorm``; and with them a ``RouterBalance``. For every packed sample of ``n`` counted tokens, ``c_e`` of whose (token, slot) pairs
 chose expert ``e``, and with ``P_e`` the sum of its probabilities over them:
 
-* ``loss``    ``E / n^2 sum_e c_e P_e``: ``k`` where all experts are used alike, more where they are not (the load-balancing loss of transformers'
-              ``load_balancing_loss_func``, modeling_mixtral.py, for one layer; there over the whole batch, which is one sample here)
+* ``loss``    ``E / n^2 sum_e c_e P_e``: ``k`` where all experts are used alike, more where they are not (the load-balancing loss that Mixtral's configuration
+              weighs by ``router_aux_loss_coef``, for one layer; there over the whole batch, which is one sample here)
 * ``z_loss``  the mean of ``logsumexp(logits)^2``, which keeps the logits small
 
 ``route_balanced_bwd`` is the gradient of the logits through the weights and both losses, in one pass. Counts are constants of it. Tokens that are not counted, and

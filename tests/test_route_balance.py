@@ -118,16 +118,16 @@ def test_gradient_against_differences():
 
 
 def test_balanced_use_has_the_least_loss():
-    """``k`` for experts that are used alike, and the loss of transformers' function for one layer."""
+    """``k`` for experts that are used alike, and else the experts' number times the sum of the products of two means: pairs per token and probabilities."""
     ops = TorchOps()
     assert abs(float(ops.route_balanced(torch.eye(8).repeat(5, 1) * 1e-3, 8, True)[3].loss) - 8.0) < 1e-4
-    from transformers.models.mixtral.modeling_mixtral import load_balancing_loss_func
     logits = torch.randn(64, 8, generator=torch.Generator().manual_seed(1))
-    ref = load_balancing_loss_func((logits,), 8, 2)
-    assert abs(float(ops.route_balanced(logits, 2, True)[3].loss) - float(ref)) < 1e-5
-    mask = (torch.arange(64).view(2, 32) % 32) < torch.tensor([[20], [32]])
-    ref = load_balancing_loss_func((logits,), 8, 2, mask.long())
-    assert abs(float(ops.route_balanced(logits, 2, True, counted=mask.reshape(-1))[3].loss) - float(ref)) < 1e-5
+    mask = ((torch.arange(64).view(2, 32) % 32) < torch.tensor([[20], [32]])).reshape(-1)
+    for counted in (None, mask):
+        p = logits.double().softmax(1)[slice(None) if counted is None else counted]
+        pairs = torch.zeros_like(p).scatter_(1, p.topk(2, dim=1).indices, 1.0)
+        want = 8 * float((pairs.mean(0) * p.mean(0)).sum())
+        assert abs(float(ops.route_balanced(logits, 2, True, counted=counted)[3].loss) - want) < 1e-5
 
 
 def special(ops, device):
