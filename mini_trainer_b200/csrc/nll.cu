@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(THREADS) nll_kernel(const float2* __restrict__
     for (int i = 1; i < THREADS / 32; ++i) add(sh[i]);
     const long long t = targets[row];
     const float others = (m + log2f(s)) * 0.69314718055994531f;   // natural again; -infinity where there are none
-    const bool has = t != ignore && t >= 0 && t < columns;
+    const bool has = t >= 0 && t < columns;   // a column's number may be what is ignored, too: the partition is of all columns then as well
     if (t != ignore && !has) atomicExch(status, 63);
     float l = 0.f, z = others;
     if (has) {
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(THREADS) nll_kernel(const float2* __restrict__
       if (d != d) l = d;
       z = at + l;
     }
-    loss[row] = l;
+    loss[row] = t != ignore ? l : 0.f;
     lse[row] = z;
   }
   pdl_trigger();

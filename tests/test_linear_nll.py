@@ -231,6 +231,33 @@ def test_rows_that_are_not_counted_or_not_numbers(native):
         native.check_status()
 
 
+def ignored_column(ops, device):
+    """``ignore_index`` may be the number of a column (a padding token's): the column stays in every partition, its rows' too, which have no loss and no gradient."""
+    v = inputs(60, 64, 300, 0.0, device=device)
+    x, w, t = v["x"], v["w"], v["t"]
+    t[::5] = 7
+    ok = t != 7
+    loss, lse = ops.linear_nll(x, w, t, ignore_index=7)
+    every, same = ops.linear_nll(x, w, t)
+    assert torch.equal(lse, same) and torch.equal(loss[ok], every[ok]) and (loss[~ok] == 0).all() and (every > 0).all()
+    assert ((lse - torch.logsumexp(x.double() @ w.double().t(), 1)).abs() <= 1e-4).all()
+    dw, dw2 = torch.empty_like(w), torch.empty_like(w)
+    dx = ops.linear_nll_bwd(v["dloss"], x, w, t, loss, lse, dw, ignore_index=7, dlse=v["dlse"])
+    weigh = torch.where(ok, v["dloss"], 0.0), torch.where(ok, v["dlse"], 0.0)
+    want = ops.linear_nll_bwd(weigh[0], x, w, t, every, same, dw2, dlse=weigh[1])
+    assert (dx[~ok] == 0).all() and torch.equal(dx, want) and torch.equal(dw, dw2)
+
+
+def test_a_column_that_is_ignored():
+    ignored_column(TorchOps(), "cpu")
+
+
+@pytest.mark.gpu
+def test_a_column_that_is_ignored_by_the_kernels(native):
+    ignored_column(native, "cuda")
+    native.check_status()
+
+
 @pytest.mark.gpu
 def test_no_tokens(native):
     w = torch.randn(24, 16, device="cuda").bfloat16()
