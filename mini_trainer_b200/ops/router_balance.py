@@ -171,7 +171,8 @@ def native(ops, logits, k, renorm, cu_seqlens=None, counted=None):
             bal.words.zero_()
             return probs, topi, w, bal
         rows, at = _BLOCKS_PER_SM * ops.sms + S, bal.words.data_ptr()
-        part = torch.empty(rows * (E + 1), dtype=torch.int64, device=dev).data_ptr()
+        scratch = torch.empty(rows * (E + 1), dtype=torch.int64, device=dev)   # held until the kernels are queued: nobody else is given it before
+        part = scratch.data_ptr()
         ops._call("mtb200_route_balanced", logits.data_ptr(), logits.dtype is f32, None if cu_seqlens is None else cu_seqlens.data_ptr(), None if counted is None else counted.data_ptr(),
                   T, E, k, S, bool(renorm), probs.data_ptr(), topi.data_ptr(), w.data_ptr(), at + 4 * lse, at + 4 * inverse, at + 4 * sample, part, part + 8 * rows * E, rows,
                   at + 4 * loss, at + 4 * z, at + 4 * counts, at + 4 * tokens, at + 4 * usage, ops._st(), n=2)
