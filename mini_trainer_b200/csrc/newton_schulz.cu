@@ -3,8 +3,8 @@
 //   X0 = G / (|G| + 1e-7)  (Frobenius norm)        X <- (a I + b A + c A^2) X,  A = X X^T        steps times
 // takes every singular value x of X to a x + b x^3 + c x^5, so those above 1e-3 of the norm or so end near one. A matrix with more rows than columns is multiplied from the right
 // instead, X (a I + b A + c A^2) with A = X^T X: operands of the tensor cores may have either dimension innermost, so nothing is ever transposed. With r the shorter side
-// and n the longer a step is the products r r n, r r r and r r n; the first two are symmetric: only the tiles on and below the diagonal are computed, and the epilogue stores a tile
-// and its transpose. 3 r^2 n + r^3 operations a step instead of 4 r^2 n + 2 r^3.
+// and n the longer a step is the products r r n, r r r and r r n; the first two are symmetric: only the tiles on and below the diagonal are computed. Of large ones no others are stored, and who reads a block of 64 columns
+// above it loads the rows below instead, the other dimension innermost: the transposes passed through the shared memory that the operands need (they took 3 to 5 % of a call). 3 r^2 n + r^3 operations a step instead of 4 r^2 n + 2 r^3.
 //
 // The second product's epilogue adds b A and a I to c A^2, so that the third has the linear term in it.
 //
@@ -48,6 +48,7 @@ constexpr int BOX = 32 * 128;                            // a warp's staging: 32
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int SMEM = STAGES * STAGE_BYTES + EPI_WARPS * 2 * BOX + 1024 + 256;
 constexpr int GROUP_M = 8;
+constexpr int WHOLE_BITS = 8;                            // large symmetric matrices are stored in blocks of 256, the largest tile: those on the diagonal whole, none above it
 constexpr uint32_t PEER_MASK = 0xFEFFFFFFu;              // of a shared::cluster address: the same place in CTA 0
 static_assert(SMEM <= 227 * 1024, "shared memory");
 
@@ -64,6 +65,8 @@ struct Params {
   float beta;
   long long ld, stride;          // of d, lo and res
   int bf16_out;                  // APPLY
+  int whole_bits;                // SYM: of D's blocks that are stored whole on the diagonal, and not above it
+  int sym_a, sym_b;              // TURN: whether the operand is a symmetric matrix, of which map_s has the transpose
   int* status;
 };
 
@@ -95,6 +98,13 @@ __device__ __forceinline__ void load_operand(uint8_t* dst, const void* map, uint
     load_box<CTAS>(dst, map, bar, k, row, z);
   }
 }
+// First block of 64 of the reduction in which 128 rows of a symmetric operand, from `row` on, are above what is stored; the same in both CTAs of a pair.
+__device__ __forceinline__ int turn_at(int sym, int row) { return sym ? ((row >> WHOLE_BITS) + 1) << (WHOLE_BITS - 6) : 0x7fffffff; }
+template <int CTAS, bool MN>
+__device__ __forceinline__ void load_side(uint8_t* dst, const void* map, const void* map_s, bool turned, uint32_t bar, int row, int k, int z) {
+  if (!MN && turned) load_operand<CTAS, true>(dst, map_s, bar, row, k, z);
+  else load_operand<CTAS, MN>(dst, map, bar, row, k, z);
+}
 template <int CTAS>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if constexpr (CTAS == 2)
@@ -115,6 +125,16 @@ template <int CTAS>
 __device__ __forceinline__ void arrive_leader(uint64_t* bar) {
   if constexpr (CTAS == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(smem_u32(bar) & PEER_MASK) : "memory");
   else mbar_arrive(bar);
+}
+// One stage, 64 of the reduction.
+template <int CTAS>
+__device__ __forceinline__ void mma_stage(uint32_t d, uint32_t sa, uint32_t sb, uint32_t idesc, bool a_mn, bool b_mn, bool first) {
+#pragma unroll
+  for (int k = 0; k < BK / 16; ++k) {
+    const uint64_t da = a_mn ? make_smem_desc(sa + k * 2048, 8192, 1024) : make_smem_desc(sa + k * 32, 16, 1024);
+    const uint64_t db = b_mn ? make_smem_desc(sb + k * 2048, 8192, 1024) : make_smem_desc(sb + k * 32, 16, 1024);
+    mma<CTAS>(d, da, db, idesc, !first || k != 0);
+  }
 }
 // fp16 x fp16 -> fp32
 __host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
@@ -199,8 +219,8 @@ __device__ __forceinline__ void finish64(const Params& p, float* f, uint8_t* box
 #pragma unroll
     for (int j = 0; j < 32; ++j) h[j] = pack_f16(f[2 * j], f[2 * j + 1]);
     put(d, p.ld, p.M, p.N, y0, col, box, h, lane);
-    if (!diagonal) {
-      // The transpose: 64 rows (this tile's columns) of 32 (its rows). Neighbouring lanes exchange a word, so that each writes two rows' entries of one column.
+    if (!diagonal && (y0 >> p.whole_bits) == (col >> p.whole_bits)) {
+      // In a block on the diagonal, which is stored whole, the transpose: 64 rows (this tile's columns) of 32 (its rows). Neighbouring lanes exchange a word, so that each writes two rows' entries of one column.
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
@@ -235,9 +255,10 @@ __device__ __forceinline__ void finish64(const Params& p, float* f, uint8_t* box
   }
 }
 
-template <int CTAS, bool A_MN, bool B_MN, int KIND>
+// TURN: an operand that is not MN may be symmetric, with more than a block of 256.
+template <int CTAS, bool A_MN, bool B_MN, int KIND, bool TURN>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS, 1)
-product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_s, const Params p) {
   constexpr int TILE = BM * CTAS;      // rows and columns of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -261,6 +282,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     fence_mbar_init();
     tma_prefetch_desc(&map_a);
     tma_prefetch_desc(&map_b);
+    if (TURN) tma_prefetch_desc(&map_s);
   }
   if (warp == 1) {
     if constexpr (CTAS == 2) {
@@ -286,6 +308,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const int z = w / tiles;
         tile_at<KIND>(w - z * tiles, tiles_m, tiles_n, p.group_m, tm, tn);
         const int row = tm * TILE + static_cast<int>(rank) * BM, col = tn * TILE + static_cast<int>(rank) * BM;
+        const int turn_a = turn_at(p.sym_a, row), turn_b = turn_at(p.sym_b, col);
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 71); if (rank == 0) settle_loads(full_bar, it); goto done; }
@@ -293,23 +316,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const uint32_t bar = CTAS == 2 ? smem_u32(&full_bar[s]) & PEER_MASK : smem_u32(&full_bar[s]);
           const bool once = KIND == SYM && tm == tn;   // the same rows twice
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * (once ? OP_BYTES : STAGE_BYTES));
-          load_operand<CTAS, A_MN>(sa, &map_a, bar, row, kb * BK, z);
-          if (!once) load_operand<CTAS, B_MN>(sa + OP_BYTES, &map_b, bar, col, kb * BK, z);
+          load_side<CTAS, A_MN>(sa, &map_a, &map_s, TURN && kb >= turn_a, bar, row, kb * BK, z);
+          if (!once) load_side<CTAS, B_MN>(sa + OP_BYTES, &map_b, &map_s, TURN && kb >= turn_b, bar, col, kb * BK, z);
         }
       }
       pdl_trigger();
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = idesc_f16(TILE, TILE, A_MN, B_MN);
       uint32_t it = 0, n = 0;
       for (int w = worker; w < items; w += p.workers, ++n) {
-        bool once = false;
-        if constexpr (KIND == SYM) {
-          int tm, tn;
-          tile_at<KIND>(w % tiles, tiles_m, tiles_n, p.group_m, tm, tn);
-          once = tm == tn;
-        }
+        int tm = 0, tn = 1;
+        if constexpr (KIND == SYM || TURN) tile_at<KIND>(w % tiles, tiles_m, tiles_n, p.group_m, tm, tn);
+        const bool once = KIND == SYM && tm == tn;
+        const int turn_a = turn_at(p.sym_a, tm * TILE), turn_b = turn_at(p.sym_b, tn * TILE);
         if (!mbar_wait(&tempty_bar[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 72); goto done; }
         tc_fence_after();
         const uint32_t d = tmem_base + (n & 1) * TILE;
@@ -318,12 +338,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag)) { atomicExch(p.status, 73); goto done; }
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + s * STAGE_BYTES), sb = once ? sa : sa + OP_BYTES;
-#pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t da = A_MN ? make_smem_desc(sa + k * 2048, 8192, 1024) : make_smem_desc(sa + k * 32, 16, 1024);
-            const uint64_t db = B_MN ? make_smem_desc(sb + k * 2048, 8192, 1024) : make_smem_desc(sb + k * 32, 16, 1024);
-            mma<CTAS>(d, da, db, idesc, kb != 0 || k != 0);
-          }
+          const bool a_mn = A_MN || (TURN && kb >= turn_a), b_mn = B_MN || (TURN && kb >= turn_b);
+          mma_stage<CTAS>(d, sa, sb, idesc_f16(TILE, TILE, a_mn, b_mn), a_mn, b_mn, kb == 0);
           commit<CTAS>(&empty_bar[s]);
         }
         commit<CTAS>(&tfull_bar[n & 1]);
@@ -382,9 +398,9 @@ __device__ __forceinline__ uint32_t remote_address(uint32_t addr, uint32_t rank)
 __device__ __forceinline__ void store_cluster4(uint32_t to, float a, float b, float c, float d) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
-template <int CTAS, bool A_MN, bool B_MN, int KIND>
+template <int CTAS, bool A_MN, bool B_MN, int KIND, bool TURN>
 __global__ void __launch_bounds__(THREADS, 1)
-split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p, const int splits) {
+split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_s, const Params p, const int splits) {
   constexpr int TILE = BM * CTAS;
   static_assert(STAGES * STAGE_BYTES >= TILE * 128 * 4, "the sums of a tile's rows fit over the stages");
   extern __shared__ uint8_t smem_raw[];
@@ -412,6 +428,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     fence_mbar_init();
     tma_prefetch_desc(&map_a);
     tma_prefetch_desc(&map_b);
+    if (TURN) tma_prefetch_desc(&map_s);
   }
   if (warp == 1) {
     if constexpr (CTAS == 2) {
@@ -432,31 +449,28 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   if (warp == 0) {
     if (elect_one()) {
       const int row = tm * TILE + static_cast<int>(rank) * BM, col = tn * TILE + static_cast<int>(rank) * BM;
+      const int turn_a = turn_at(p.sym_a, row), turn_b = turn_at(p.sym_b, col);
       for (int it = 0; it < n; ++it) {
         const int s = it % STAGES;
         if (!mbar_wait(&empty_bar[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { atomicExch(p.status, 71); if (rank == 0) settle_loads(full_bar, it); break; }
         uint8_t* sa = smem + s * STAGE_BYTES;
         const uint32_t bar = CTAS == 2 ? smem_u32(&full_bar[s]) & PEER_MASK : smem_u32(&full_bar[s]);
         if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * (once ? OP_BYTES : STAGE_BYTES));
-        load_operand<CTAS, A_MN>(sa, &map_a, bar, row, (kb0 + it) * BK, z);
-        if (!once) load_operand<CTAS, B_MN>(sa + OP_BYTES, &map_b, bar, col, (kb0 + it) * BK, z);
+        load_side<CTAS, A_MN>(sa, &map_a, &map_s, TURN && kb0 + it >= turn_a, bar, row, (kb0 + it) * BK, z);
+        if (!once) load_side<CTAS, B_MN>(sa + OP_BYTES, &map_b, &map_s, TURN && kb0 + it >= turn_b, bar, col, (kb0 + it) * BK, z);
       }
       pdl_trigger();
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = idesc_f16(TILE, TILE, A_MN, B_MN);
+      const int turn_a = turn_at(p.sym_a, tm * TILE), turn_b = turn_at(p.sym_b, tn * TILE);
       for (int it = 0; it < n; ++it) {
         const int s = it % STAGES;
         if (!mbar_wait(&full_bar[s], (it / STAGES) & 1, abort_flag)) { atomicExch(p.status, 73); break; }
         tc_fence_after();
         const uint32_t sa = smem_u32(smem + s * STAGE_BYTES), sb = once ? sa : sa + OP_BYTES;
-#pragma unroll
-        for (int k = 0; k < BK / 16; ++k) {
-          const uint64_t da = A_MN ? make_smem_desc(sa + k * 2048, 8192, 1024) : make_smem_desc(sa + k * 32, 16, 1024);
-          const uint64_t db = B_MN ? make_smem_desc(sb + k * 2048, 8192, 1024) : make_smem_desc(sb + k * 32, 16, 1024);
-          mma<CTAS>(tmem_base, da, db, idesc, it != 0 || k != 0);
-        }
+        const bool a_mn = A_MN || (TURN && kb0 + it >= turn_a), b_mn = B_MN || (TURN && kb0 + it >= turn_b);
+        mma_stage<CTAS>(tmem_base, sa, sb, idesc_f16(TILE, TILE, a_mn, b_mn), a_mn, b_mn, it == 0);
         commit<CTAS>(&empty_bar[s], in_cluster);
       }
       commit<CTAS>(tfull_bar, in_cluster);
@@ -1115,7 +1129,7 @@ template <int CTAS>
 static int resident_clusters(int splits) {
   static int known[MOST_SPLITS + 1] = {-1, -1, -1, -1, -1};
   if (known[splits] < 0) {
-    auto kern = split_kernel<CTAS, false, false, SYM>;
+    auto kern = split_kernel<CTAS, false, false, SYM, false>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS * splits);
     cfg.blockDim = dim3(THREADS);
@@ -1162,10 +1176,10 @@ static Form choose(long long M, long long N, long long K, long long stack, bool 
     }
   return best;
 }
-template <int CTAS, bool A_MN, bool B_MN, int KIND>
-static int launch(const CUtensorMap& a, const CUtensorMap& b, Params p, int splits, int workers, cudaStream_t st) {
-  auto kern = product_kernel<CTAS, A_MN, B_MN, KIND>;
-  auto split = split_kernel<CTAS, A_MN, B_MN, KIND>;
+template <int CTAS, bool A_MN, bool B_MN, int KIND, bool TURN>
+static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& s, Params p, int splits, int workers, cudaStream_t st) {
+  auto kern = product_kernel<CTAS, A_MN, B_MN, KIND, TURN>;
+  auto split = split_kernel<CTAS, A_MN, B_MN, KIND, TURN>;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
@@ -1185,10 +1199,10 @@ static int launch(const CUtensorMap& a, const CUtensorMap& b, Params p, int spli
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(items * CTAS * splits)); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM; cfg.stream = st;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, split, a, b, p, splits) == cudaSuccess ? 0 : -5;
+    return cudaLaunchKernelEx(&cfg, split, a, b, s, p, splits) == cudaSuccess ? 0 : -5;
   }
   p.workers = static_cast<int>(items < workers ? items : workers);
-  launch_pdl(kern, p.workers * CTAS, THREADS, SMEM, st, a, b, p);
+  launch_pdl(kern, p.workers * CTAS, THREADS, SMEM, st, a, b, s, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
@@ -1294,11 +1308,15 @@ static int orthogonalise(const Source& src, long long rows, long long cols, long
   const int sms = sm_count();
   const int r = static_cast<int>(l.r), K = static_cast<int>(right ? rows : cols);
   const Form fg = choose(r, r, K, stack, true, pairs, sms), fp = choose(r, r, r, stack, true, pairs, sms), fa = choose(rows, cols, r, stack, false, pairs, sms);
-#define PRODUCT(F, A_MN, B_MN, KIND, ...) (F.ctas == 2 ? launch<2, A_MN, B_MN, KIND>(__VA_ARGS__, F.splits, pairs, st) : launch<1, A_MN, B_MN, KIND>(__VA_ARGS__, F.splits, sms, st))
+#define PRODUCT(F, A_MN, B_MN, KIND, TURN, ...) (F.ctas == 2 ? launch<2, A_MN, B_MN, KIND, TURN>(__VA_ARGS__, F.splits, pairs, st) : launch<1, A_MN, B_MN, KIND, TURN>(__VA_ARGS__, F.splits, sms, st))
+#define PRODUCT_SYM(F, A_MN, B_MN, KIND, ...) (turn ? PRODUCT(F, A_MN, B_MN, KIND, true, __VA_ARGS__) : PRODUCT(F, A_MN, B_MN, KIND, false, __VA_ARGS__))
+  // Where the matrix is two blocks wide the launches are short, and the transposes cost less than what each of them has to think about: 8 x 2048 x 512 178 us and 183, 4 x 512 x 1376 129 and 131; 64 x 2048 x 1024
+  // 2640 and 2500, 4096 x 4096 1270 and 1206.
+  const bool turn = r > 2 << WHOLE_BITS;
   for (int i = 0; i < steps; ++i) {
     const Matrix& X = xh[i & 1];
-    Params p{r, r, K, static_cast<int>(stack), 0, 0, static_cast<float>(ldexp(SCALE_A, -2 * p2)), 0.f, gram.p, nullptr, nullptr, 0.f, l.ldr, l.r * l.ldr, 0, status};
-    rc = right ? PRODUCT(fg, true, true, SYM, X.mn, X.mn, p) : PRODUCT(fg, false, false, SYM, X.k, X.k, p);
+    Params p{r, r, K, static_cast<int>(stack), 0, 0, static_cast<float>(ldexp(SCALE_A, -2 * p2)), 0.f, gram.p, nullptr, nullptr, 0.f, l.ldr, l.r * l.ldr, 0, turn ? WHOLE_BITS : 24, 0, 0, status};
+    rc = right ? PRODUCT(fg, true, true, SYM, false, X.mn, X.mn, gram.mn, p) : PRODUCT(fg, false, false, SYM, false, X.k, X.k, gram.mn, p);
     if (rc) return rc;
     p.K = r;
     p.alpha = static_cast<float>(SCALE_P * NS_C / (SCALE_A * SCALE_A));
@@ -1306,16 +1324,18 @@ static int orthogonalise(const Source& src, long long rows, long long cols, long
     p.d = poly.p;
     p.res = reinterpret_cast<const __half*>(gram.p);
     p.beta = static_cast<float>(SCALE_P * NS_B / SCALE_A);
-    rc = PRODUCT(fp, false, false, SYM, gram.k, gram.k, p);
+    p.sym_a = p.sym_b = 1;
+    rc = PRODUCT_SYM(fp, false, false, SYM, gram.k, gram.k, gram.mn, p);
     if (rc) return rc;
     const bool to_out = i + 1 == steps && out != nullptr;
     const long long ld = to_out ? out_ld : l.ld;   // (the last step has no residual, whose rows would be another matrix's)
     Params a{static_cast<int>(rows), static_cast<int>(cols), r, static_cast<int>(stack), 0, 0, static_cast<float>(ldexp(1.0 / SCALE_P, to_out ? -p2 : 0)), 0.f,
              to_out ? (uint16_t*)out : xh[(i + 1) & 1].p, i + 1 < kept ? (uint16_t*)x[(i + 1) & 1][1] : nullptr, i < kept ? x[i & 1][1] : nullptr, static_cast<float>(ldexp(NS_A, -LO_BITS)),
-             ld, rows * ld, to_out, status};
-    rc = right ? PRODUCT(fa, false, false, APPLY, X.k, poly.k, a) : PRODUCT(fa, false, true, APPLY, poly.k, X.mn, a);
+             ld, rows * ld, to_out, 0, !right, right, status};
+    rc = right ? PRODUCT_SYM(fa, false, false, APPLY, X.k, poly.k, poly.mn, a) : PRODUCT_SYM(fa, false, true, APPLY, poly.k, X.mn, poly.mn, a);
     if (rc) return rc;
   }
+#undef PRODUCT_SYM
 #undef PRODUCT
   return 0;
 }
