@@ -57,13 +57,18 @@ __global__ void __launch_bounds__(THREADS) nll_kernel(const float2* __restrict__
 
 extern "C" {
 
-// stats [T, pieces], at_target [T]: of mtb200_gemm_lse; loss, lse [T] fp32. A target that is neither a column nor `ignore` is recorded and counts as ignored.
-int mtb200_nll(const float2* stats, const float* at_target, const long long* targets, int T, int pieces, long long columns, long long ignore, float* loss, float* lse, int* status,
-               cudaStream_t st) {
+int mtb200_gemm_lse(const void* A, long long lda, const void* W, float2* stats, float* at_target, const long long* targets, int M, int N, int K, float alpha, int form, int* status,
+                    cudaStream_t stream);
+
+// loss, lse [T] fp32 of the logits alpha x[T, H] * w[columns, H]^T, row-major without padding. stats [T, ceil(columns / 128)] and at_target [T] are scratch; `form` as in mtb200_gemm_lse. A target that is
+// neither a column nor `ignore` is recorded and counts as ignored.
+int mtb200_linear_nll(const void* x, const void* w, const long long* targets, float2* stats, float* at_target, int T, int columns, int H, float alpha, long long ignore, int form, float* loss, float* lse,
+                      int* status, cudaStream_t st) {
   using namespace mtb;
   if (T <= 0) return 0;
-  if (pieces <= 0) return -10;
-  launch_pdl(nll::nll_kernel, T, nll::THREADS, 0, st, stats, at_target, targets, pieces, columns, ignore, loss, lse, status);
+  if (columns <= 0) return -10;
+  if (const int rc = mtb200_gemm_lse(x, H, w, stats, at_target, targets, T, columns, H, alpha, form, status, st)) return rc;
+  launch_pdl(nll::nll_kernel, T, nll::THREADS, 0, st, stats, at_target, targets, (columns + 127) / 128, static_cast<long long>(columns), ignore, loss, lse, status);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 

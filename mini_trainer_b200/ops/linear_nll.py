@@ -114,8 +114,7 @@ def native(ops, x, w, targets, ignore_index=-100, logit_scale=1.0):
         stats, at, form, st, status = scratch.data_ptr(), scratch.data_ptr() + 8 * rows * pieces, _form(ops, rows, H), ops._st(), ops.status.data_ptr()
         for a in range(0, T, rows):
             n, t = min(rows, T - a), targets.data_ptr() + 8 * a
-            ops._call("mtb200_gemm_lse", x.data_ptr() + 2 * a * H, H, w.data_ptr(), stats, at, t, n, V, H, float(logit_scale), form, status, st, tag="gemm_nt_lse")
-            ops._call("mtb200_nll", stats, at, t, n, pieces, V, ignore_index, loss.data_ptr() + 4 * a, lse.data_ptr() + 4 * a, status, st)
+            ops._call("mtb200_linear_nll", x.data_ptr() + 2 * a * H, w.data_ptr(), t, stats, at, n, V, H, float(logit_scale), ignore_index, form, loss.data_ptr() + 4 * a, lse.data_ptr() + 4 * a, status, st, n=2)
     return loss, lse
 
 

@@ -111,9 +111,8 @@ class _Sig:
     mtb200_newton_schulz_workspace = [L, L, L]
     mtb200_newton_schulz = [P, I, P, L, L, L, I, P, L, P, P]
     mtb200_muon_step = [P, P, I, P, I, P, P, L, L, L, I, F, I, F, F, P, L, P, P]
-    mtb200_gemm_lse = [P, L, P, P, P, P, I, I, I, F, I, P, P]
     mtb200_gemm_nll = [P, L, P, P, L, P, P, P, P, P, I, I, I, F, L, L, I, I, P, P]
-    mtb200_nll = [P, P, P, I, I, L, L, P, P, P, P]
+    mtb200_linear_nll = [P, P, P, P, P, I, I, I, F, L, I, P, P, P, P]
     mtb200_route_balanced = [P, I, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, I, P, P, P, P, P, P]
     mtb200_route_balanced_bwd = [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, I, P, P]
     mtb200_attn_fwd_one = [P, L, P, L, P, P, I, I, I, I, I, F, P, P]

@@ -52,9 +52,11 @@ class RouterBalance:
         if words is None or name not in self.NAMES:
             raise AttributeError(name)
         i, at = self.NAMES.index(name), self.offsets()
-        t = words[at[i]:at[i + 1]]
-        t = t if name in self.WHOLE else t.view(torch.float32)
-        self.__dict__[name] = t = t.view(self.S, self.E) if i < 2 else t
+        if name not in self.WHOLE:
+            words = self.__dict__.get("numbers")
+            if words is None:
+                words = self.__dict__["numbers"] = self.words.view(torch.float32)
+        self.__dict__[name] = t = words.as_strided((self.S, self.E), (self.E, 1), at[i]) if i < 2 else words.as_strided((at[i + 1] - at[i],), (1,), at[i])
         return t
 
 
