@@ -386,9 +386,9 @@ done:
 }
 
 // The same product with its reduction divided over the CTAs (or pairs) of a cluster, for launches of few tiles: one tile to a cluster. An SM takes a tile's operands from L2 at 64 bytes a clock, 512 clocks for
-// 64 of the reduction, which is what a launch of one round lasts for; `splits` SMs take it in parts. When all have multiplied, each sends every other the sums of the rows that one finishes, fp32 through
-// the cluster's shared memory (over the operands' stages), and finishes its own: 128 / splits rows, added in the order of the parts.
-constexpr int MOST_SPLITS = 4;
+// 64 of the reduction, which is what a launch of one round lasts for; `splits` SMs take it in parts. When all have multiplied, each sends every other the sums that one finishes, fp32 through
+// the cluster's shared memory (over the operands' stages), and finishes its own: units of 32 rows and 64 columns, added in the order of the parts.
+constexpr int MOST_SPLITS = 8;   // of single CTAs; 4 of pairs (a cluster has eight CTAs at most)
 // The place of this CTA's shared memory at `addr` in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t remote_address(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -481,20 +481,22 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   __syncthreads();
   cluster_barrier();   // every CTA has multiplied: nothing reads the stages any more
   tc_fence_after();
-  // quarter q of the rows is finished by part q / (4 / splits); [part][quarter of those][4 columns][row] of 16 bytes
-  const int q = warp & 3, half = (warp - 2) >> 2, per_owner = 4 / splits;
+  // [part][unit of the one that finishes it][4 columns][row] of 16 bytes
+  constexpr int ACROSS = TILE / 64;   // units side by side
+  const int per_owner = 4 * ACROSS / splits;
   if (warp >= 2) {
-    const uint32_t owner = static_cast<uint32_t>(q / per_owner) * CTAS + rank;
-    const uint32_t at = remote_address(smem_u32(smem) + (split * per_owner + q % per_owner) * (TILE * 128) + lane * 16, owner);
+    const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll 1
     for (int c = half * (TILE / 2); c < (half + 1) * (TILE / 2); c += 32) {
+      const int unit = q * ACROSS + c / 64;
+      const uint32_t at = remote_address(smem_u32(smem) + (split * per_owner + unit % per_owner) * 8192 + (c % 64) / 4 * 512 + lane * 16, static_cast<uint32_t>(unit / per_owner) * CTAS + rank);
       uint32_t v[32];
       tmem_ld_32x32(taddr + c, v);
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 32; j += 4)
-        store_cluster4(at + (c + j) / 4 * 512, __uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
+        store_cluster4(at + j / 4 * 512, __uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
     }
   }
   tc_fence_before();
@@ -502,16 +504,15 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
   cluster_barrier();   // ... and every part has arrived
   if (warp >= 2) {
     uint8_t* box = smem + STAGES * STAGE_BYTES + (warp - 2) * 2 * BOX;
-    for (int u = warp - 2; u < per_owner * (TILE / 64); u += EPI_WARPS) {
-      const int mine = u % per_owner, c = u / per_owner * 64;
-      const int y0 = tm * TILE + static_cast<int>(rank) * BM + (split * per_owner + mine) * 32, col = tn * TILE + c;
+    for (int u = warp - 2; u < per_owner; u += EPI_WARPS) {
+      const int unit = split * per_owner + u, y0 = tm * TILE + static_cast<int>(rank) * BM + unit / ACROSS * 32, col = tn * TILE + unit % ACROSS * 64;
       if (y0 >= p.M || col >= p.N) continue;
       ask(p, box, y0, col, z, lane);
       float f[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) f[j] = 0.f;
       for (int s = 0; s < splits; ++s) {
-        const uint8_t* src = smem + (s * per_owner + mine) * (TILE * 128) + c / 4 * 512 + lane * 16;
+        const uint8_t* src = smem + (s * per_owner + u) * 8192 + lane * 16;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const float4 v = *reinterpret_cast<const float4*>(src + j * 512);
@@ -1127,7 +1128,7 @@ static int sm_count() {
 // Clusters of a split product that can be resident at once; 0 where the device has none of that size.
 template <int CTAS>
 static int resident_clusters(int splits) {
-  static int known[MOST_SPLITS + 1] = {-1, -1, -1, -1, -1};
+  static int known[MOST_SPLITS + 1] = {-1, -1, -1, -1, -1, -1, -1, -1, -1};
   if (known[splits] < 0) {
     auto kern = split_kernel<CTAS, false, false, SYM, false>;
     cudaLaunchConfig_t cfg = {};
@@ -1148,9 +1149,10 @@ static int resident_clusters(int splits) {
 struct Form { int ctas, splits; };
 // The form of a product by what its rounds of tiles take, in us: 64 of the reduction 0.28 on a single CTA (its operands from L2 at 64 bytes a clock) and 0.30 on a pair, up to 0.36 and 0.43
 // where all SMs multiply at once; and what stands in front of and behind them. Fitted to stacks of 1 to 64 matrices of 64 to 4096: 1024 x 1024 122 us in single CTAs and 201 in pairs, 4096 x 4096 1370 and 1114, 512 x 512 95 and 163, in
-// parts of a half 116 and 157; 1001 x 4097 299 and 327, 239 with the gram product on pairs in four parts; 1536 x 8960 466 and 520, 422 with it on single CTAs in two.
+// parts of a half 116 and 157; 1001 x 4097 299 and 327, 239 with the gram product on pairs in four parts; 1536 x 8960 466 and 520, 422 with it on single CTAs in two;
+// 64 x 28672 198 with it in four parts and 147 in eight, 256 x 14336 163 and 139.
 static Form choose(long long M, long long N, long long K, long long stack, bool sym, int pairs, int sms) {
-  constexpr double base[2][3] = {{3.0, 6.0, 6.8}, {8.0, 8.7, 9.1}};
+  constexpr double base[2][4] = {{3.0, 6.0, 6.8, 7.6}, {8.0, 8.7, 9.1, 0.0}};
   auto tiles = [&](long long tile) {
     const long long tm = (M + tile - 1) / tile, tn = (N + tile - 1) / tile;
     return (sym ? tm * (tm + 1) / 2 : tm * tn) * stack;
@@ -1161,7 +1163,7 @@ static Form choose(long long M, long long N, long long K, long long stack, bool 
   for (int ctas = 1; ctas <= 2; ++ctas)
     for (int s = 0; 1 << s <= MOST_SPLITS; ++s) {
       const int splits = 1 << s;
-      if ((ctas == 2 && pairs <= 0) || (s && kb < 2 * splits)) continue;
+      if ((ctas == 2 && (pairs <= 0 || splits * 2 > MOST_SPLITS)) || (s && kb < 2 * splits)) continue;
       const int room = s == 0 ? (ctas == 2 ? pairs : sms) : ctas == 2 ? resident_clusters<2>(splits) : resident_clusters<1>(splits);
       if (room <= 0) continue;
       const long long n = tiles(BM * ctas), whole = n / room, rest = n % room;   // rounds of all workers, and what is left

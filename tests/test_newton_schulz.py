@@ -169,6 +169,18 @@ def test_kernels(native, shape, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(40, 12440), (12440, 40), (200, 8201), (8201, 200), (700, 4100), (4100, 700), (3, 600, 1000), (2, 1000, 600), (40, 520, 640), (1281, 1290)])
+@pytest.mark.parametrize("kind", ["features", "rank_one", "one"])
+def test_long_reductions_and_blocks_above_the_diagonal(native, shape, kind):
+    """A reduction in up to eight parts; symmetric operands whose blocks above the diagonal are read from below it."""
+    g = matrices(kind, *shape, device="cuda")
+    got = native.orthogonalise(g)
+    check(got, g, 3 * TOL if kind in ("sparse", "one") else TOL)
+    assert torch.equal(got, native.orthogonalise(g))
+    native.check_status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(130, 250), (250, 130), (520, 512)])
 @pytest.mark.parametrize("steps", [1, 2, 6])
 def test_kernels_by_steps(native, shape, steps):
