@@ -4,7 +4,7 @@
 // takes every singular value x of X to a x + b x^3 + c x^5, so those above 1e-3 of the norm or so end near one. A matrix with more rows than columns is multiplied from the right
 // instead, X (a I + b A + c A^2) with A = X^T X: operands of the tensor cores may have either dimension innermost, so nothing is ever transposed. With r the shorter side
 // and n the longer a step is the products r r n, r r r and r r n; the first two are symmetric: only the tiles on and below the diagonal are computed. Of large ones no others are stored, and who reads a block of 64 columns
-// above it loads the rows below instead, the other dimension innermost: the transposes passed through the shared memory that the operands need (they took 3 to 5 % of a call). 3 r^2 n + r^3 operations a step instead of 4 r^2 n + 2 r^3.
+// above it loads the rows below instead, the other dimension innermost: the transposes passed through the shared memory that the operands need (they took 4 to 5 % of a call). 3 r^2 n + r^3 operations a step instead of 4 r^2 n + 2 r^3.
 //
 // The second product's epilogue adds b A and a I to c A^2, so that the third has the linear term in it.
 //
@@ -17,8 +17,8 @@
 // (0.15, 1.2); half of bf16's step, to which the result is rounded, is 1.7e-3 in the mean. Sums are fp32 in tensor memory.
 //
 // The products: persistent, warp-specialised, 3-D TMA maps over the stack, tcgen05.mma of fp16 into two accumulators in tensor memory, by single CTAs (tiles of 128 x 128, for few tiles) or CTA pairs
-// (256 x 256). All launches of a call are queued by one host call, each under its predecessor's tail. A large call is bound by its products: 4096 x 4096 (1.37 TFLOP in five steps) 1.10 ms of kernels one by one, 1.4 in a row under the power cap:
-// its gram product and square 59 us each at 76 % of the tensor pipe (136 tiles on 74 pairs), its last product 100 us at 88 %. A launch of one round is bound by its chain, about 3.9 us beside its reduction (first
+// (256 x 256). All launches of a call are queued by one host call, each under its predecessor's tail. A large call is bound by its products: 4096 x 4096 (1.37 TFLOP in five steps) 1.21 ms in a row under the power cap:
+// its gram product and square 57 us each at 80 % of the tensor pipe (136 tiles on 74 pairs), its last product 103 us at 88 %. A launch of one round is bound by its chain, about 3.9 us beside its reduction (first
 // operands 1.0, sums to stores 1.5, end to the next one's start 1.4), and on single CTAs by L2, from which an SM takes 64 bytes a clock: 0.25 us for 64 of the reduction. More epilogue warps (sixteen of
 // 32 columns) made it longer: 688 x 256 88 -> 95 us, 1024 x 1024 121 -> 127.
 #include <cuda.h>
