@@ -143,7 +143,7 @@ def native_bwd(ops, dloss, x, w, targets, loss, lse, dw_out, accumulate_dw=False
         form, scale = _form(ops, T, H), float(logit_scale)
         for a in range(0, V, n):
             c = min(n, V - a)
-            wc, dwc = w[a:a + c], dw_out[a:a + c]
+            wc, dwc = (w, dw_out) if c == V else (w[a:a + c], dw_out[a:a + c])
             ops._call("mtb200_gemm_nll", x.data_ptr(), H, wc.data_ptr(), dz.data_ptr(), ldz, targets.data_ptr(), loss.data_ptr(), lse.data_ptr(), dloss.data_ptr(),
                       None if dlse is None else dlse.data_ptr(), T, c, H, scale, ignore_index, a, V, form, ops.status.data_ptr(), ops._st(), tag="gemm_nt_nll")
             ops.gemm(dz, True, x, True, dwc, c, H, T, residual=dwc if accumulate_dw else None, alpha=scale)
