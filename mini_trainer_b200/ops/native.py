@@ -301,11 +301,15 @@ class NativeOps:
             self._gemm_ws[stream] = ws
         return ws
 
-    def _split(self, stream, nbytes):
+    def own_counters(self):
+        """Arrival counters for the ``gemm`` calls of an operator that is being captured, so that they may split as outside of a graph: the graph's own, set to zero by every replay. ``None`` without a capture."""
+        return torch.zeros(_SPLIT_COUNTERS, dtype=torch.int64, device=self.device) if torch.cuda.is_current_stream_capturing() else None
+
+    def _split(self, stream, nbytes, counters=None):
         """``(counters, epoch, partials)`` of a split launch, or ``None`` where it has to run whole. The partials are scratch of this call:
         taken from the allocator (in powers of two, at most 128 MB) and given back behind the launch, so nothing is held
         between calls, and without memory for them the launch simply does not split."""
-        ws = self._split_workspace(stream)
+        ws = self._split_workspace(stream) if counters is None else counters
         if ws is None:
             return None
         try:
@@ -346,18 +350,18 @@ class NativeOps:
         ragged = pitches & 15 != 0
         return self._gemm_plans.get((M, N, K, None, ragged, act)) or self._plan_gemm(M, N, K, None, ragged, act)
 
-    def gemm(self, a, a_mn, b, b_mn, out, M, N, K, residual=None, bias=None, tag=None, two_cta=None, alpha=1.0, stats=None):
+    def gemm(self, a, a_mn, b, b_mn, out, M, N, K, residual=None, bias=None, tag=None, two_cta=None, alpha=1.0, stats=None, counters=None):
         """out[M,N] = alpha*A*B (+bias) (+residual). ``a_mn``/``b_mn``: operand stored [K, rows].
         ``stats`` [M, ceil(N / 256), 2] fp32 receives the softmax statistics of the (bf16) output rows per 256 columns.
         ``two_cta``: force (True) or forbid (False) the cta_group::2 kernel; default by problem size. Without CTA pairs on the
-        device the one-CTA kernel runs in any case."""
+        device the one-CTA kernel runs in any case. ``counters``: of the caller's own, for a product that is split (``own_counters``)."""
         out_f32 = out.dtype == torch.float32
         assert a.dtype == torch.bfloat16 and b.dtype == torch.bfloat16
         assert residual is None or residual.dtype == out.dtype
         ragged, act = (a.stride(0) | b.stride(0)) & 15 != 0, stats is not None
         name, splits, nbytes = self._gemm_plans.get((M, N, K, two_cta, ragged, act)) or self._plan_gemm(M, N, K, two_cta, ragged, act)
         st = self._st()
-        split = self._split(st, nbytes) if splits > 1 else None
+        split = self._split(st, nbytes, counters) if splits > 1 else None
         ws, epoch, part = split or (None, 0, None)
         self._call(name, a.data_ptr(), a.stride(0), int(a_mn), b.data_ptr(), b.stride(0), int(b_mn),
                    out.data_ptr(), out.stride(0), int(out_f32), _ptr(residual),

@@ -259,6 +259,43 @@ def test_a_column_that_is_ignored_by_the_kernels(native):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("piece", [None, 8192])
+def test_captured_gradients_are_those_outside_of_a_graph(native, monkeypatch, piece):
+    """Few tokens and many columns, whose sums over the vocabulary are divided: the same bits from every replay, whatever else runs beside it."""
+    T, H, V = 64, 256, 30011
+    if piece:
+        monkeypatch.setattr(LN, "PIECE_BYTES", 2 * T * piece)
+    v = inputs(T, H, V, device="cuda")
+    dw = torch.empty_like(v["w"])
+
+    def run(w):
+        loss, lse = native.linear_nll(v["x"], v["w"], v["t"])
+        return loss, lse, native.linear_nll_bwd(v["dloss"], v["x"], v["w"], v["t"], loss, lse, w, dlse=v["dlse"])
+    want = run(dw)
+    torch.cuda.synchronize()
+    graph, captured = torch.cuda.CUDAGraph(), torch.empty_like(dw)
+    with torch.cuda.graph(graph):
+        got = run(captured)
+    side, beside = torch.cuda.Stream(), torch.empty_like(dw)
+    for _ in range(3):
+        for t in (*got, captured):
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            other = run(beside)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(captured, dw)
+        assert all(torch.equal(a, b) for a, b in zip(other, want)) and torch.equal(beside, dw)
+    v["dloss"].mul_(0.5), v["dlse"].mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    halves = run(dw)
+    assert torch.equal(got[2], halves[2]) and torch.equal(captured, dw)
+    native.check_status()
+
+
+@pytest.mark.gpu
 def test_no_tokens(native):
     w = torch.randn(24, 16, device="cuda").bfloat16()
     x, t, f = torch.empty(0, 16, dtype=torch.bfloat16, device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda"), torch.empty(0, device="cuda")
