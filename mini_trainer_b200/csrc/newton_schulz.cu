@@ -293,8 +293,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       tmem_relinquish();
     }
   }
-  pdl_wait();   // nothing so far has touched global memory
-  tc_fence_before();
+  tc_fence_before();   // (who touches global memory waits for the launch in front before it does: all this passes under that one's tail)
   __syncthreads();
   if constexpr (CTAS == 2) cluster_barrier();   // the partner's barriers are there before anything is sent to them
   tc_fence_after();
@@ -316,6 +315,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           const uint32_t bar = CTAS == 2 ? smem_u32(&full_bar[s]) & PEER_MASK : smem_u32(&full_bar[s]);
           const bool once = KIND == SYM && tm == tn;   // the same rows twice
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], CTAS * (once ? OP_BYTES : STAGE_BYTES));
+          if (it == 0) pdl_wait();
           load_side<CTAS, A_MN>(sa, &map_a, &map_s, TURN && kb >= turn_a, bar, row, kb * BK, z);
           if (!once) load_side<CTAS, B_MN>(sa + OP_BYTES, &map_b, &map_s, TURN && kb >= turn_b, bar, col, kb * BK, z);
         }
@@ -324,6 +324,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
+      pdl_wait();   // (so that its bounded waits are for this launch's loads alone)
       uint32_t it = 0, n = 0;
       for (int w = worker; w < items; w += p.workers, ++n) {
         int tm = 0, tn = 1;
@@ -356,6 +357,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       tile_at<KIND>(w - z * tiles, tiles_m, tiles_n, p.group_m, tm, tn);
       const int y0 = tm * TILE + static_cast<int>(rank) * BM + q * 32, c0 = half * (TILE / 2);
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (n & 1) * TILE;
+      if (n == 0) pdl_wait();
       ask(p, box, y0, tn * TILE + c0, z, lane);
       if (!mbar_wait(&tfull_bar[n & 1], (n >> 1) & 1, abort_flag)) { atomicExch(p.status, 74); goto done; }
       tc_fence_after();
@@ -439,7 +441,6 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
       tmem_relinquish();
     }
   }
-  pdl_wait();
   tc_fence_before();
   __syncthreads();
   cluster_barrier();
@@ -448,6 +449,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
 
   if (warp == 0) {
     if (elect_one()) {
+      pdl_wait();
       const int row = tm * TILE + static_cast<int>(rank) * BM, col = tn * TILE + static_cast<int>(rank) * BM;
       const int turn_a = turn_at(p.sym_a, row), turn_b = turn_at(p.sym_b, col);
       for (int it = 0; it < n; ++it) {
@@ -463,6 +465,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
+      pdl_wait();
       const int turn_a = turn_at(p.sym_a, tm * TILE), turn_b = turn_at(p.sym_b, tn * TILE);
       for (int it = 0; it < n; ++it) {
         const int s = it % STAGES;
@@ -475,8 +478,9 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
       }
       commit<CTAS>(tfull_bar, in_cluster);
     }
-  } else if (!mbar_wait(tfull_bar, 0, abort_flag)) {
-    if (lane == 0) atomicExch(p.status, 74);
+  } else {
+    pdl_wait();
+    if (!mbar_wait(tfull_bar, 0, abort_flag) && lane == 0) atomicExch(p.status, 74);
   }
   __syncthreads();
   cluster_barrier();   // every CTA has multiplied: nothing reads the stages any more
