@@ -18,7 +18,7 @@
 //
 // The products: persistent, warp-specialised, 3-D TMA maps over the stack, tcgen05.mma of fp16 into two accumulators in tensor memory, by single CTAs (tiles of 128 x 128, for few tiles) or CTA pairs
 // (256 x 256). All launches of a call are queued by one host call, each under its predecessor's tail. A large call is bound by its products: 4096 x 4096 (1.37 TFLOP in five steps) 1.21 ms in a row under the power cap:
-// its gram product and square 57 us each at 80 % of the tensor pipe (136 tiles on 74 pairs), its last product 103 us at 88 %. A launch of one round is bound by its chain, about 3.9 us beside its reduction (first
+// its gram product and square 57 us each at 80 % of the tensor pipe (136 tiles on 74 pairs), its last product 103 us at 88 %. A launch of one round is bound by its chain, about 3.4 us beside its reduction (first
 // operands 1.0, sums to stores 1.5, end to the next one's start 1.4), and on single CTAs by L2, from which an SM takes 64 bytes a clock: 0.25 us for 64 of the reduction. More epilogue warps (sixteen of
 // 32 columns) made it longer: 688 x 256 88 -> 95 us, 1024 x 1024 121 -> 127.
 #include <cuda.h>
