@@ -284,6 +284,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     tma_prefetch_desc(&map_b);
     if (TURN) tma_prefetch_desc(&map_s);
   }
+  __syncwarp();   // (whatever is .aligned is for whole warps: here and below they come together again behind what one thread, or each for itself, has done)
   if (warp == 1) {
     if constexpr (CTAS == 2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * TILE) : "memory");
@@ -359,12 +360,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (n & 1) * TILE;
       if (n == 0) pdl_wait();
       ask(p, box, y0, tn * TILE + c0, z, lane);
-      if (!mbar_wait(&tfull_bar[n & 1], (n >> 1) & 1, abort_flag)) { atomicExch(p.status, 74); goto done; }
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull_bar[n & 1], (n >> 1) & 1, abort_flag))) { atomicExch(p.status, 74); goto done; }
       tc_fence_after();
 #pragma unroll 1
       for (int c = c0; c < c0 + TILE / 2; c += 64) {
         const int col = tn * TILE + c;
         if (y0 >= p.M || col >= p.N) break;
+        __syncwarp();
         uint32_t v[2][32];
         tmem_ld_32x32(taddr + c, v[0]);
         tmem_ld_32x32(taddr + c + 32, v[1]);
@@ -432,6 +434,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ 
     tma_prefetch_desc(&map_b);
     if (TURN) tma_prefetch_desc(&map_s);
   }
+  __syncwarp();   // (whatever is .aligned is for whole warps: here and below they come together again behind what one thread, or each for itself, has done)
   if (warp == 1) {
     if constexpr (CTAS == 2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TILE) : "memory");
@@ -823,6 +826,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
     *abort_flag = 0;
     fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 0) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
   pdl_wait();
   const float coef = src.coef != nullptr ? *src.coef : 1.f;
@@ -863,6 +867,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
     for (int i = 0; i < SMALL_THREADS / 32; ++i) total += warp_sums[i];
     norm[rank] = total;
   }
+  __syncwarp();
   if (parts > 1) {
     cluster_barrier();   // every CTA of the cluster is there
     if (threadIdx.x == 0) for (int t = 0; t < parts; ++t) if (t != rank) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote_address(smem_u32(norm + rank), t)), "d"(total) : "memory");
