@@ -37,6 +37,17 @@ def _per_token(what, t, T, device):
         raise ValueError(f"{what}: expected {T} contiguous fp32 numbers on {device}, not {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
+def _shares(out, others):
+    """Whether ``out`` holds bytes of another tensor; of views with gaps, which the kernels do not take, whether both start at the same one."""
+    if out.device.type == "meta":
+        return False
+    a, n = out.data_ptr(), out.nbytes
+    for t in others:
+        if t is not None and a < (b := t.data_ptr()) + t.nbytes and b < a + n and (a == b or out.is_contiguous() and t.is_contiguous()):
+            return True
+    return False
+
+
 def check_bwd(dloss, x, w, targets, loss, lse, dw_out, logit_scale, dlse):
     T, H, V = check(x, w, targets, logit_scale)
     for what, t in (("dloss", dloss), ("loss", loss), ("lse", lse)):
@@ -44,7 +55,7 @@ def check_bwd(dloss, x, w, targets, loss, lse, dw_out, logit_scale, dlse):
             raise ValueError(f"{what}: expected {T} contiguous fp32 numbers on {x.device}")
         _per_token(what, t, T, x.device)
     _per_token("dlse", dlse, T, x.device)
-    if dw_out.device.type != "meta" and dw_out.numel() and dw_out.data_ptr() in (w.data_ptr(), x.data_ptr()):
+    if _shares(dw_out, (w, x, targets, dloss, loss, lse, dlse)):   # all of which the pieces behind the first read again
         raise ValueError("the weight's gradient goes to memory of its own")
     if dw_out.dtype != w.dtype or dw_out.shape != w.shape or dw_out.device != w.device:
         raise ValueError(f"the weight's gradient is {w.dtype} {tuple(w.shape)} on {w.device}, not {dw_out.dtype} {tuple(dw_out.shape)} on {dw_out.device}")

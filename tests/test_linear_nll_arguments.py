@@ -1,0 +1,46 @@
+"""Arguments of ``linear_nll`` and its gradient at the edges of what is documented: memory that is shared, targets outside the vocabulary, what a captured call takes."""
+import pytest
+import torch
+
+from mini_trainer_b200.ops.torch_ref import TorchOps
+
+
+def arguments(T=6, H=16, V=24):
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(T, H, generator=g).bfloat16(), torch.randn(V, H, generator=g).bfloat16()
+    one = torch.ones(T)
+    return dict(dloss=one.clone(), x=x, w=w, targets=torch.randint(0, V, (T,), generator=g), loss=one.clone(), lse=one.clone(), dlse=one.clone(), dw_out=torch.empty_like(w))
+
+
+@pytest.mark.parametrize("backend", ["plain", "native"])
+@pytest.mark.parametrize("name,shift", [("w", 0), ("w", 1), ("w", 23), ("w", -1), ("w", -23), ("x", 1), ("x", -5), ("x", 23), ("dloss", 0), ("loss", 0), ("lse", 0), ("dlse", 0), ("targets", 0)])
+def test_weight_gradient_over_an_operand_is_refused(backend, name, shift):
+    """A part of the weight that is overwritten would be read by the pieces of the vocabulary behind it."""
+    from .test_native_host import make_ops
+    ops = TorchOps() if backend == "plain" else make_ops()
+    if backend == "native":
+        ops.check_device = lambda t: None
+    v = arguments()
+    rows = v["w"].shape[0]
+    memory = torch.zeros(3 * rows, v["w"].shape[1], dtype=torch.bfloat16)
+    dw = memory[rows:2 * rows]
+    if name in ("w", "x"):
+        v[name] = memory[rows + shift:][:v[name].shape[0]].copy_(v[name])
+    else:
+        n = v[name].numel() * v[name].element_size()
+        v[name] = dw.view(-1).view(torch.uint8)[64:64 + n].view(v[name].dtype).copy_(v[name])
+    with pytest.raises(ValueError, match="memory of its own"):
+        ops.linear_nll_bwd(**{**v, "dw_out": dw})
+    if backend == "native":
+        assert not ops.calls
+
+
+@pytest.mark.parametrize("shift", [24, -24])
+def test_weight_gradient_beside_an_operand(shift):
+    """Neighbours in one allocation, as parameters and their gradients are, share nothing."""
+    v = arguments()
+    memory = torch.zeros(72, 16, dtype=torch.bfloat16)
+    v["w"], dw = memory[24 + shift:48 + shift].copy_(v["w"]), memory[24:48]
+    dx = TorchOps().linear_nll_bwd(**{**v, "dw_out": dw})
+    want = torch.empty_like(v["w"])
+    assert torch.equal(dx, TorchOps().linear_nll_bwd(**{**v, "dw_out": want})) and torch.equal(dw, want)
