@@ -8,7 +8,7 @@ vocabulary: a piece's gradient ``[T, columns]`` is all that exists at a time, ``
 pieces in fp32. ``linear_ce`` is the form for one uniform weight known beforehand: it needs the product once less.
 
 A target equal to ``ignore_index`` has a loss of zero and no gradient (of ``lse`` either), whatever its logits are, but ``x`` is to be finite there too: a sum over all tokens
-multiplies it by zero. On a GPU any other target outside the vocabulary counts as ignored and is reported by ``check_status``.
+multiplies it by zero. Any other target outside the vocabulary counts as ignored and is reported by ``check_status``.
 """
 from __future__ import annotations
 
@@ -63,29 +63,36 @@ def check_bwd(dloss, x, w, targets, loss, lse, dw_out, logit_scale, dlse):
 
 
 # -- plain forms ----------------------------------------------------------------------------
+def columns(targets, V, ignore_index):
+    """Which targets are a column that counts, and whether there are others that are not ``ignore_index``."""
+    inside, other = (targets >= 0) & (targets < V), targets != ignore_index
+    return inside & other, (other & ~inside).any()
+
+
 def plain(x, w, targets, ignore_index=-100, logit_scale=1.0, chunk=2048):
     T, H, V = check(x, w, targets, logit_scale)
     loss, lse = (torch.zeros(T, dtype=torch.float32, device=x.device) for _ in range(2))
+    ok, _ = columns(targets, V, ignore_index)
     for a in range(0, T, chunk):
         z = (x[a:a + chunk].float() @ w.float().t()) * logit_scale
         t = targets[a:a + chunk]
         lse[a:a + chunk] = torch.logsumexp(z, -1)
         picked = z.gather(1, t.clamp(0, V - 1).unsqueeze(1)).squeeze(1)
-        loss[a:a + chunk] = torch.where(t != ignore_index, lse[a:a + chunk] - picked, 0.0)
+        loss[a:a + chunk] = torch.where(ok[a:a + chunk], lse[a:a + chunk] - picked, 0.0)
     return loss, lse
 
 
 def plain_bwd(dloss, x, w, targets, loss, lse, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0, dlse=None, chunk=2048):
     T, H, V = check_bwd(dloss, x, w, targets, loss, lse, dw_out, logit_scale, dlse)
     dx, dw, wf = torch.empty_like(x), torch.zeros(w.shape, dtype=torch.float32, device=x.device), w.float()
+    ok, _ = columns(targets, V, ignore_index)
     for a in range(0, T, chunk):
         xc, t = x[a:a + chunk].float(), targets[a:a + chunk]
-        ok = (t != ignore_index).unsqueeze(1)
         d, dz = dloss[a:a + chunk], 0.0 if dlse is None else dlse[a:a + chunk]
         g = torch.exp((xc @ wf.t()) * logit_scale - lse[a:a + chunk, None]) * (d + dz).unsqueeze(1)
         l = loss[a:a + chunk]
         g.scatter_(1, t.clamp(0, V - 1).unsqueeze(1), (d * torch.expm1(-l) + dz * torch.exp(-l)).unsqueeze(1))
-        g = torch.where(ok, g, 0.0) * logit_scale
+        g = torch.where(ok[a:a + chunk, None], g, 0.0) * logit_scale
         dx[a:a + chunk] = (g @ wf).to(x.dtype)
         dw += g.t() @ xc
     if accumulate_dw:

@@ -24,8 +24,16 @@ from . import linear_nll, newton_schulz, router_balance
 class TorchOps:
     name = "torch"
 
+    _outside = None   # on the tensors' device: whether a target was outside the vocabulary
+
     def __init__(self, ce_chunk: int = 2048):
         self.ce_chunk = ce_chunk
+
+    def check_status(self):
+        """Raises where a call met an input it had to skip, as the kernel backend's does."""
+        outside, self._outside = self._outside, None
+        if outside is not None and bool(outside):
+            raise RuntimeError("a target outside the vocabulary (status code 63)")
 
     # -- embedding --------------------------------------------------------------------
     def embedding(self, weight, ids):
@@ -383,7 +391,10 @@ class TorchOps:
 
     # -- likelihoods without logits (linear_nll.py) ----------------------------------------
     def linear_nll(self, x, w, targets, ignore_index=-100, logit_scale=1.0):
-        return linear_nll.plain(x, w, targets, ignore_index, logit_scale, self.ce_chunk)
+        out = linear_nll.plain(x, w, targets, ignore_index, logit_scale, self.ce_chunk)
+        outside = linear_nll.columns(targets, w.shape[0], ignore_index)[1]
+        self._outside = outside if self._outside is None else self._outside | outside.to(self._outside.device)
+        return out
 
     def linear_nll_bwd(self, dloss, x, w, targets, loss, lse, dw_out, accumulate_dw=False, ignore_index=-100, logit_scale=1.0, dlse=None):
         return linear_nll.plain_bwd(dloss, x, w, targets, loss, lse, dw_out, accumulate_dw, ignore_index, logit_scale, dlse, self.ce_chunk)

@@ -44,3 +44,42 @@ def test_weight_gradient_beside_an_operand(shift):
     dx = TorchOps().linear_nll_bwd(**{**v, "dw_out": dw})
     want = torch.empty_like(v["w"])
     assert torch.equal(dx, TorchOps().linear_nll_bwd(**{**v, "dw_out": want})) and torch.equal(dw, want)
+
+
+def targets_outside(ops, device, dtype):
+    """A target that is no column counts as ignored, in the losses and in both gradients, and is reported once."""
+    g = torch.Generator().manual_seed(1)
+    T, H, V = 40, 16, 5
+    x, w = torch.randn(T, H, generator=g).to(dtype).to(device), torch.randn(V, H, generator=g).to(dtype).to(device)
+    t = torch.randint(0, V, (T,), generator=g).to(device)
+    t[3] = -100
+    dloss, dlse = torch.randn(T, generator=g).to(device), torch.randn(T, generator=g).to(device)
+    ignored, outside = t.clone(), t.clone()
+    rows = torch.tensor([0, 7, 8, 30, 39], device=device)
+    ignored[rows] = -100
+    outside[rows] = torch.tensor([V, -1, 1 << 40, -(1 << 62), V + 3], device=device)
+
+    def run(targets):
+        loss, lse = ops.linear_nll(x, w, targets)
+        dw = torch.empty_like(w)
+        return loss, lse, ops.linear_nll_bwd(dloss, x, w, targets, loss, lse, dw, dlse=dlse), dw
+    want = run(ignored)
+    ops.check_status()
+    assert (want[0][rows] == 0).all() and (want[2][rows] == 0).all() and (want[0][[1, 2, 4]] > 0).all()
+    got = run(outside)
+    run(t)   # a call without such targets takes nothing back
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="target outside the vocabulary"):
+        ops.check_status()
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_targets_outside_the_vocabulary(dtype):
+    targets_outside(TorchOps(ce_chunk=11), "cpu", dtype)
+
+
+@pytest.mark.gpu
+def test_targets_outside_the_vocabulary_by_the_kernels():
+    from mini_trainer_b200.ops import get_ops
+    targets_outside(get_ops(torch.device("cuda:0")), "cuda", torch.bfloat16)
