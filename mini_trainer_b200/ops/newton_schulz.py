@@ -52,12 +52,12 @@ def check_muon(master, moment, grad, param_out, lr, momentum, weight_decay, grad
     held = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (master, moment, grad, param_out) if t is not None and t.device.type != "meta"]
     if any(a < d and c < b for i, (a, b) in enumerate(held) for c, d in held[:i]):
         raise ValueError("master, moment, gradient and working copy are memory of their own")
-    for what, v in (("lr", lr), ("momentum", momentum), ("weight_decay", weight_decay)):
+    scale = 0.2 * math.sqrt(max(m, n)) if scale is None else float(scale)
+    for what, v in (("lr", lr), ("momentum", momentum), ("weight_decay", weight_decay), ("scale", scale), ("the gradient's factor", 0.0 if torch.is_tensor(grad_coef) else grad_coef)):
         if not math.isfinite(v):
             raise ValueError(f"{what} is a finite number, not {v}")
     if torch.is_tensor(grad_coef) and grad_coef.numel() != 1:
         raise ValueError(f"the gradient's factor is one number, not {tuple(grad_coef.shape)}")
-    scale = 0.2 * math.sqrt(max(m, n)) if scale is None else float(scale)
     return stack, m, n, 1.0 - lr * weight_decay, lr * scale
 
 

@@ -3,6 +3,9 @@ import re
 from pathlib import Path
 
 import pytest
+import torch
+
+from mini_trainer_b200.ops.torch_ref import TorchOps
 
 CSRC = Path(__file__).resolve().parent.parent / "mini_trainer_b200" / "csrc"
 
@@ -33,3 +36,24 @@ def test_warps_are_whole_before_aligned_instructions(name):
         else:
             whole = m.lastgroup == "together"
     assert seen >= 5
+
+
+def backend(name):
+    from .test_native_host import make_ops
+    if name == "plain":
+        return TorchOps()
+    ops = make_ops()
+    ops.check_device = lambda t: None
+    return ops
+
+
+@pytest.mark.parametrize("name", ["plain", "native"])
+@pytest.mark.parametrize("bad", [dict(scale=float("nan")), dict(scale=float("inf")), dict(grad_coef=float("nan")), dict(grad_coef=-float("inf"))])
+def test_factors_that_are_not_finite_are_refused(name, bad):
+    """They would overwrite the parameter, its momentum and its working copy with what is not finite."""
+    ops, g = backend(name), torch.ones(6, 8)
+    held = dict(master=g.clone(), moment=g.clone(), grad=g, param_out=g.bfloat16())
+    with pytest.raises(ValueError, match="finite"):
+        ops.muon_step(**held, lr=0.1, momentum=0.9, weight_decay=0.0, **bad)
+    assert all((t == 1).all() for t in held.values())
+    assert name == "plain" or not ops.calls
