@@ -35,10 +35,10 @@ def check(g, steps):
     if g.dim() < 2 or g.dtype not in (torch.bfloat16, torch.float32) or not g.is_contiguous():
         raise ValueError(f"expected contiguous bf16 or fp32 matrices [..., m, n], not {tuple(g.shape)} {g.dtype} with strides {g.stride()}")
     _check_steps(steps)
-    m, n = g.shape[-2:]
-    if max(m, n) >= 1 << 24 or min(m, n) > 1 << 16 or g.numel() >= 1 << 40:
-        raise ValueError(f"matrices of {m} x {n} are more than the kernels count")
-    return math.prod(g.shape[:-2]), m, n
+    (m, n), stack = g.shape[-2:], math.prod(g.shape[:-2])
+    if max(m, n, stack) >= 1 << 24 or min(m, n) > 1 << 16 or g.numel() >= 1 << 40:
+        raise ValueError(f"{stack} matrices of {m} x {n} are more than the kernels count")
+    return stack, m, n
 
 
 def check_muon(master, moment, grad, param_out, lr, momentum, weight_decay, grad_coef, scale, steps):

@@ -57,3 +57,11 @@ def test_factors_that_are_not_finite_are_refused(name, bad):
         ops.muon_step(**held, lr=0.1, momentum=0.9, weight_decay=0.0, **bad)
     assert all((t == 1).all() for t in held.values())
     assert name == "plain" or not ops.calls
+
+
+@pytest.mark.parametrize("name", ["plain", "native"])
+def test_stacks_beyond_what_the_kernels_count_are_refused(name):
+    ops = backend(name)
+    for shape in ((1 << 24, 1, 1), (1 << 12, 1 << 12, 2, 3)):
+        with pytest.raises(ValueError, match="more than the kernels count"):
+            ops.orthogonalise(torch.empty(shape, device="meta"))
