@@ -1253,12 +1253,12 @@ static int small_room(int parts) {
   }
   return known[parts];
 }
-// The call in one launch; 1 where it does not fit one, or would take longer so.
-static int small_call(const Source& src, Small p, long long stack, cudaStream_t st) {
+// Whether a call is one launch, and how that divides a matrix: false where it does not fit one, or would take longer so. By sizes and the device alone.
+static bool small_form(Small& p, long long stack) {
   p.tall = p.rows > p.cols;
   p.r = p.tall ? p.cols : p.rows;
   p.n = p.tall ? p.rows : p.cols;
-  if (p.r > SMALL_R || stack > 1 << 20) return 1;
+  if (p.r > SMALL_R || stack > 1 << 20) return false;
   p.R = p.r <= 32 && p.n > 128 ? 32 : p.r <= 64 && p.n > 64 ? 64 : 128;   // a slab's parts have 64 columns at least
   p.kept = p.steps > 2 ? p.steps - 2 : p.steps - 1;
   const int most = SMALL_ENTRIES / p.R, step = 64 * (SMALL_R / p.R);
@@ -1275,7 +1275,9 @@ static int small_call(const Source& src, Small p, long long stack, cudaStream_t 
     const double t = (stack > room ? 1.3 : 1.0) * ((stack + room - 1) / room) * (3.0 + 2.3 * e + p.steps * (2.1 + 0.5 * wide + 0.78 * e + (parts > 1 ? 1.9 + 2.6 * wide + 0.1 * parts : 0.0)));
     if (t < least) { least = t; p.parts = parts; p.w = w; }
   }
-  if (p.parts == 0) return 1;
+  return p.parts != 0;
+}
+static int small_call(const Source& src, const Small& p, long long stack, cudaStream_t st) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1362,23 +1364,26 @@ extern "C" {
 
 int mtb200_gemm2_pairs();
 
-// Bytes of the workspace of the two calls below, which starts on 256 bytes.
-long long mtb200_newton_schulz_workspace(long long rows, long long cols, long long stack) {
-  const mtb::ns::Layout l = mtb::ns::layout(rows, cols, stack);
-  return l.total;
+// Bytes of the workspace of the two calls below, which starts on 256 bytes; 0 where they are one launch on the current device, and take none.
+long long mtb200_newton_schulz_workspace(long long rows, long long cols, long long stack, int steps) {
+  using namespace mtb::ns;
+  if (!sizes_ok(rows, cols, stack, steps)) return -1;
+  Small one{static_cast<int>(rows), static_cast<int>(cols)};
+  one.steps = steps;
+  return small_form(one, stack) ? 0 : layout(rows, cols, stack).total;
 }
 // Launches of a call: sums and scaling, three products a step, one behind them.
 // out [stack, rows, cols] bf16 = g [stack, rows, cols] (bf16 or fp32) orthogonalised.
 int mtb200_newton_schulz(const void* g, int g_bf16, void* out, long long rows, long long cols, long long stack, int steps, void* ws, long long ws_bytes, int* status, cudaStream_t st) {
   using namespace mtb::ns;
   if (!sizes_ok(rows, cols, stack, steps)) return -10;
-  const Layout l = layout(rows, cols, stack);
-  if (ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 255)) return -11;
   const Source src{g, g_bf16, nullptr, 0, nullptr, 0.f, 0};
   Small one{static_cast<int>(rows), static_cast<int>(cols)};
   one.steps = steps; one.p2 = exponent(rows, cols); one.out = (__nv_bfloat16*)out; one.status = status;
   one.vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  if (const int did = small_call(src, one, stack, st); did <= 0) return did;
+  if (small_form(one, stack)) return small_call(src, one, stack, st);
+  const Layout l = layout(rows, cols, stack);
+  if (ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 255)) return -11;
   const bool direct = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   uint8_t* w = reinterpret_cast<uint8_t*>(ws);
   void* to = direct ? out : w + 2 * (steps & 1) * l.xbytes;   // the buffer that the last step writes
@@ -1395,13 +1400,13 @@ int mtb200_muon_step(float* master, void* m, int m_bf16, const void* g, int g_bf
                      int nesterov, float keep, float step, void* ws, long long ws_bytes, int* status, cudaStream_t st) {
   using namespace mtb::ns;
   if (!sizes_ok(rows, cols, stack, steps) || m == nullptr) return -10;
-  const Layout l = layout(rows, cols, stack);
-  if (ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 255)) return -11;
   const Source src{g, g_bf16, m, m_bf16, coef, mu, nesterov};
   Small one{static_cast<int>(rows), static_cast<int>(cols)};
   one.steps = steps; one.p2 = exponent(rows, cols); one.master = master; one.param = (__nv_bfloat16*)param; one.keep = keep; one.step = static_cast<float>(ldexp(step, -one.p2)); one.status = status;
   one.vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(master) | reinterpret_cast<uintptr_t>(param)) & 15) == 0;
-  if (const int did = small_call(src, one, stack, st); did <= 0) return did;
+  if (small_form(one, stack)) return small_call(src, one, stack, st);
+  const Layout l = layout(rows, cols, stack);
+  if (ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 255)) return -11;
   uint8_t* w = reinterpret_cast<uint8_t*>(ws);
   const int p2 = exponent(rows, cols);
   int rc = orthogonalise(src, rows, cols, stack, steps, nullptr, 0, p2, w, mtb200_gemm2_pairs(), status, st);

@@ -108,7 +108,7 @@ class _Sig:
     mtb200_moe_glu_bwd = [P, P, P, P, P, I, I, I, I, P, P, P]
     mtb200_moe_combine = [P, P, P, P, P, F, I, I, I, P, P]
     mtb200_moe_route_bwd = [P, P, P, P, I, I, I, I, P, P]
-    mtb200_newton_schulz_workspace = [L, L, L]
+    mtb200_newton_schulz_workspace = [L, L, L, I]
     mtb200_newton_schulz = [P, I, P, L, L, L, I, P, L, P, P]
     mtb200_muon_step = [P, P, I, P, I, P, P, L, L, L, I, F, I, F, F, P, L, P, P]
     mtb200_gemm_nll = [P, L, P, P, L, P, P, P, P, P, I, I, I, F, L, L, I, I, P, P]

@@ -13,6 +13,9 @@ singular vectors stay, singular values above about a thousandth of the norm end 
 
 ``scale`` defaults to ``0.2 sqrt(max(m, n))``, which gives the update the root mean square of an AdamW step. It is meant for the matrices inside the blocks; embeddings, the head and vectors
 stay with ``adamw_step``. Matrices are whole here: a flat shard that cuts one is gathered first.
+
+Beside the result, a call on the kernels holds a workspace of 8 bytes an element and 4 for each of the square of the shorter side (rows and sides in whole 64s: 1.3 GB for 64 of 2048 x 1024, 1.1 GB for 16384 of 128 x 16)
+while it runs, unless it is one launch (csrc/newton_schulz.cu), which has none. The matrices of a stack have nothing to do with one another, so one that leaves no room for it is called in parts.
 """
 from __future__ import annotations
 
@@ -98,9 +101,13 @@ def _launches(m, n, steps):
     return 1 if r <= 128 and max(m, n) <= 16 * 32768 // (32 if r <= 32 else 64 if r <= 64 else 128) else 2 + 3 * steps
 
 
-def _workspace(ops, m, n, stack, device):
-    ws = torch.empty(ops.lib.mtb200_newton_schulz_workspace(m, n, stack), dtype=torch.uint8, device=device)
-    return ws, ws.data_ptr(), ws.numel()
+def _workspace(ops, m, n, stack, steps, device):
+    """``(tensor, address, bytes)`` of a call's workspace; nothing where the library makes the call one launch, which takes none."""
+    size = ops._fn["mtb200_newton_schulz_workspace"](m, n, stack, steps)
+    if size == 0:
+        return None, None, 0
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), size
 
 
 def native(ops, g, steps=5):
@@ -109,7 +116,7 @@ def native(ops, g, steps=5):
     with ops.on_device():
         out = torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
         if out.numel():
-            ws, ptr, size = _workspace(ops, m, n, stack, g.device)
+            ws, ptr, size = _workspace(ops, m, n, stack, steps, g.device)
             ops._call("mtb200_newton_schulz", g.data_ptr(), int(g.dtype is torch.bfloat16), out.data_ptr(), m, n, stack, steps, ptr, size, ops.status.data_ptr(), ops._st(),
                       n=_launches(m, n, steps) + (n % 8 != 0 and _launches(m, n, steps) > 1))
     return out
@@ -127,7 +134,7 @@ def native_muon(ops, master, moment, grad, param_out, lr, momentum, weight_decay
             coef = None if grad_coef == 1.0 else torch.full((1,), float(grad_coef), dtype=torch.float32, device=grad.device)
         else:
             coef = grad_coef.to(device=grad.device, dtype=torch.float32).reshape(1)
-        ws, ptr, size = _workspace(ops, m, n, stack, grad.device)
+        ws, ptr, size = _workspace(ops, m, n, stack, steps, grad.device)
         ops._call("mtb200_muon_step", master.data_ptr(), moment.data_ptr(), int(moment.dtype is torch.bfloat16), grad.data_ptr(), int(grad.dtype is torch.bfloat16),
                   None if param_out is None else param_out.data_ptr(), None if coef is None else coef.data_ptr(), m, n, stack, steps, float(momentum), int(bool(nesterov)), keep, step,
                   ptr, size, ops.status.data_ptr(), ops._st(), n=_launches(m, n, steps) + (_launches(m, n, steps) > 1))

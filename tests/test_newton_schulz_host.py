@@ -1,4 +1,5 @@
 """Newton-Schulz products on the host: what the kernels' source, the library's own choices and the entry points' arguments have to hold, without a GPU."""
+import math
 import re
 from pathlib import Path
 
@@ -65,3 +66,54 @@ def test_stacks_beyond_what_the_kernels_count_are_refused(name):
     for shape in ((1 << 24, 1, 1), (1 << 12, 1 << 12, 2, 3)):
         with pytest.raises(ValueError, match="more than the kernels count"):
             ops.orthogonalise(torch.empty(shape, device="meta"))
+
+
+def calls(ops, shape, steps=5, muon=False):
+    """Arguments of the library call that one of the entry points makes."""
+    g = torch.ones(shape)
+    if muon:
+        ops.muon_step(g.clone(), g.clone(), g, g.bfloat16(), 0.1, 0.9, 0.0, steps=steps)
+    else:
+        ops.orthogonalise(g, steps)
+    return ops.calls[-1]
+
+
+@pytest.fixture
+def current_device(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+
+
+@pytest.mark.parametrize("muon", [False, True])
+def test_workspace_is_what_the_library_asks_for(current_device, muon):
+    """None where the library makes the call one launch, which depends on the stack, the steps and the device too."""
+    ops, asked = backend("native"), []
+
+    def workspace(*sizes):
+        asked.append(sizes)
+        return 0 if sizes[2] == 3 else 4096 * sizes[3]
+    ops._fn["mtb200_newton_schulz_workspace"] = workspace
+    name, args = calls(ops, (3, 40, 24), 2, muon)
+    assert name == ("mtb200_muon_step" if muon else "mtb200_newton_schulz") and asked == [(40, 24, 3, 2)] and args[-4:-2] == (None, 0)
+    for steps in (2, 7):
+        args = calls(ops, (4, 40, 24), steps, muon)[1]
+        assert asked[-1] == (40, 24, 4, steps) and args[-4] and args[-3] == 4096 * steps
+
+
+@pytest.fixture(scope="module")
+def native():
+    from mini_trainer_b200.ops import get_ops
+    return get_ops(torch.device("cuda:0"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(64, 64), (64, 768, 16), (148, 128, 256), (32, 16384)])
+def test_one_launch_holds_no_workspace(native, shape):
+    assert native._fn["mtb200_newton_schulz_workspace"](*shape[-2:], math.prod(shape[:-2]), 5) == 0
+    g = torch.randn(shape, device="cuda")
+    native.orthogonalise(g)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = native.orthogonalise(g)
+    assert torch.cuda.max_memory_allocated() - before <= out.numel() * 2 + 512   # the result alone, in the allocator's steps
+    native.check_status()
