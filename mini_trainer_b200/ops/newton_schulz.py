@@ -95,10 +95,9 @@ def plain_muon(master, moment, grad, param_out, lr, momentum, weight_decay, grad
 
 
 # -- kernels --------------------------------------------------------------------------------
-def _launches(m, n, steps):
-    """One where ``small_kernel`` of csrc/newton_schulz.cu takes the matrix, else two in front of the products and three of these a step."""
-    r = min(m, n)
-    return 1 if r <= 128 and max(m, n) <= 16 * 32768 // (32 if r <= 32 else 64 if r <= 64 else 128) else 2 + 3 * steps
+def _launches(ptr, steps, more):
+    """One where the library has asked for no workspace, else two in front of the products, three of these a step and ``more`` behind them."""
+    return 1 if ptr is None else 2 + 3 * steps + more
 
 
 def _workspace(ops, m, n, stack, steps, device):
@@ -118,7 +117,7 @@ def native(ops, g, steps=5):
         if out.numel():
             ws, ptr, size = _workspace(ops, m, n, stack, steps, g.device)
             ops._call("mtb200_newton_schulz", g.data_ptr(), int(g.dtype is torch.bfloat16), out.data_ptr(), m, n, stack, steps, ptr, size, ops.status.data_ptr(), ops._st(),
-                      n=_launches(m, n, steps) + (n % 8 != 0 and _launches(m, n, steps) > 1))
+                      n=_launches(ptr, steps, n % 8 != 0))
     return out
 
 
@@ -137,4 +136,4 @@ def native_muon(ops, master, moment, grad, param_out, lr, momentum, weight_decay
         ws, ptr, size = _workspace(ops, m, n, stack, steps, grad.device)
         ops._call("mtb200_muon_step", master.data_ptr(), moment.data_ptr(), int(moment.dtype is torch.bfloat16), grad.data_ptr(), int(grad.dtype is torch.bfloat16),
                   None if param_out is None else param_out.data_ptr(), None if coef is None else coef.data_ptr(), m, n, stack, steps, float(momentum), int(bool(nesterov)), keep, step,
-                  ptr, size, ops.status.data_ptr(), ops._st(), n=_launches(m, n, steps) + (_launches(m, n, steps) > 1))
+                  ptr, size, ops.status.data_ptr(), ops._st(), n=_launches(ptr, steps, 1))

@@ -1,4 +1,5 @@
 """Newton-Schulz products on the host: what the kernels' source, the library's own choices and the entry points' arguments have to hold, without a GPU."""
+import ctypes
 import math
 import re
 from pathlib import Path
@@ -116,4 +117,39 @@ def test_one_launch_holds_no_workspace(native, shape):
     before = torch.cuda.memory_allocated()
     out = native.orthogonalise(g)
     assert torch.cuda.max_memory_allocated() - before <= out.numel() * 2 + 512   # the result alone, in the allocator's steps
+    native.check_status()
+
+
+@pytest.mark.parametrize("muon", [False, True])
+def test_launches_are_counted_by_what_the_library_does(current_device, muon):
+    """The backend's own count, of a stack of small matrices that is one launch and of one that is not."""
+    ops, counted = backend("native"), []
+    call = ops._call
+    ops._call = lambda *a, n=1, tag=None: (counted.append(n), call(*a))
+    ops._fn["mtb200_newton_schulz_workspace"] = lambda m, n, stack, steps: 0 if stack == 3 else 4096
+    for shape, steps, more in (((3, 40, 24), 5, None), ((4, 40, 24), 5, 0), ((4, 40, 24), 2, 0), ((4, 24, 41), 5, 1), ((300, 300), 5, 1)):
+        calls(ops, shape, steps, muon)
+        assert counted.pop() == (1 if more is None else 2 + 3 * steps + (1 if muon else more))
+
+
+def kernels_of(graph):
+    """Number of a captured graph's nodes: all of these calls' are kernels."""
+    n = ctypes.c_size_t()
+    assert ctypes.CDLL("libcuda.so.1").cuGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(64, 64), (64, 128, 1024), (20, 128, 2048), (1000, 128, 256), (100, 601), (300, 301), (688, 256)])
+@pytest.mark.parametrize("steps", [1, 5])
+def test_launches_counted_are_launches_queued(native, shape, steps):
+    g = torch.randn(shape, device="cuda") * 1e-3
+    held = g.clone(), torch.zeros_like(g), g, g.bfloat16()
+    for run in (lambda: native.orthogonalise(g, steps), lambda: native.muon_step(*held, 0.01, 0.9, 0.0, steps=steps)):
+        run()
+        graph, before = torch.cuda.CUDAGraph(keep_graph=True), native.launches
+        with torch.cuda.graph(graph):
+            kept = run()
+        assert native.launches - before == kernels_of(graph)
+        del kept
     native.check_status()
