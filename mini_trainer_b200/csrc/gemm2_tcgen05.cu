@@ -38,6 +38,7 @@
 #include "gather.cuh"
 #include "gemm_act.cuh"
 #include "gemm_epilogue.cuh"
+#include "per_device.h"
 #include "ptx.cuh"
 
 namespace mtb {
@@ -507,12 +508,13 @@ done:
 
 // Clusters of two that can be co-resident (0: unsupported), plain / gather variant. Instances differ in threads and registers (wide tiles: 384 of 168)
 // and in static shared memory (the grouped forms' table), but with tensor memory taken whole and more than half of an SM's shared memory every one
-// of them fits an SM exactly once, so one is asked, once.
+// of them fits an SM exactly once, so one is asked, once a device.
 static_assert(SMEM + sizeof(GroupTable) <= 227 * 1024 && 2 * SMEM > 228 * 1024, "one CTA to an SM, in every instance");
 template <bool GATHER>
 static int co_resident_pairs() {
-  static int pairs = -1;
-  if (pairs < 0) {
+  static PerDevice<int> known;   // one more than them; 0: not asked yet
+  int& here = known.here();
+  if (here == 0) {
     auto kern = gemm2_kernel<false, false, false, GATHER>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2, 1, 1);
@@ -526,9 +528,9 @@ static int co_resident_pairs() {
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
-    pairs = n;
+    here = n + 1;
   }
-  return pairs;
+  return here - 1;
 }
 
 template <bool A_MN, bool B_MN, bool OUT_F32, bool GATHER = false, bool STATS = false, bool EXTRA = true, int ACT = ACT_NONE, bool WIDE = false,
@@ -537,10 +539,10 @@ static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMa
                   long long part_bytes = 0, const ActMaps<ACT>& maps = ActMaps<ACT>{}, const GroupParams* grp = nullptr) {
   auto kern = gemm2_kernel<A_MN, B_MN, OUT_F32, GATHER, STATS, EXTRA, ACT, WIDE, GROUP>;
   constexpr int threads = GATHER ? THREADS + GATHER_EXTRA_THREADS : threads_of(ACT, WIDE);
-  static bool configured = false;
-  if (!configured) {
+  static PerDevice<bool> configured;
+  if (bool& done = configured.here(); !done) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -4;
-    configured = true;
+    done = true;
   }
   const int pairs = co_resident_pairs<GATHER>();
   if (pairs <= 0) return -6;

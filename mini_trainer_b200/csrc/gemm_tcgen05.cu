@@ -31,6 +31,7 @@
 #include "gather.cuh"
 #include "gemm_act.cuh"
 #include "gemm_epilogue.cuh"
+#include "per_device.h"
 #include "ptx.cuh"
 
 namespace mtb {
@@ -413,8 +414,6 @@ int make_tmap_out(CUtensorMap* out, const void* D, int M, int N, long long ldd, 
   return out_f32 ? make_tmap_2d_f32(out, D, N, M, ldd, 32, 32) : make_tmap_2d_bf16(out, D, N, M, ldd, 64, 32);
 }
 
-static int g_num_sms = 0;
-
 // Tuning knobs read once from the environment (experiments; the defaults are what ships).
 static int tune_group_m() {
   static int v = -1;
@@ -443,23 +442,19 @@ template <bool A_MN, bool B_MN, bool OUT_F32, bool GATHER = false, bool REDUCE =
           int ACT = ACT_NONE, int NT = BN>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, GemmParams p, cudaStream_t stream,
                   const GatherParams* gp = nullptr, long long part_bytes = 0, const GroupParams* grp = nullptr, const ActMaps<ACT>& maps = ActMaps<ACT>{}) {
-  static bool configured = false;
+  static PerDevice<bool> configured;
   auto kern = gemm_kernel<A_MN, B_MN, OUT_F32, GATHER, REDUCE, GROUP, STATS, EXTRA, ACT, NT>;
-  if (!configured) {
+  if (bool& done = configured.here(); !done) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM) != cudaSuccess) return -4;
-    configured = true;
+    done = true;
   }
-  if (g_num_sms == 0) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&g_num_sms, cudaDevAttrMultiProcessorCount, dev);
-  }
+  const int sms = sms_here();
   int tiles = ((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT);
   if (GROUP == GROUP_REDUCE) tiles *= grp->E;
   if (p.e.splits > 1 && !split_fits(p.e, tiles, (p.K + BK - 1) / BK, part_bytes, 128 * NT)) return -11;
   // the gathering variant always uses every SM: its extra warps carry the transfer
   const int items = tiles * p.e.splits;
-  const int grid = (GATHER || items >= g_num_sms) ? g_num_sms : items;
+  const int grid = (GATHER || items >= sms) ? sms : items;
   static const GatherParams none{};
   // A gathering launch neither overlaps its predecessor nor lets a successor in: its CTAs are counted on to be resident. A long
   // launch (PDL_MAX_FLOPS) starts behind its predecessor too.

@@ -28,6 +28,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "per_device.h"
 #include "ptx.cuh"
 
 namespace mtb {
@@ -1126,19 +1127,12 @@ struct Matrix {            // stack of fp16 matrices with padded rows
   }
 };
 
-static int sm_count() {
-  static int n = 0;
-  if (n == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); n = 148; }
-  }
-  return n;
-}
 // Clusters of a split product that can be resident at once; 0 where the device has none of that size.
 template <int CTAS>
 static int resident_clusters(int splits) {
-  static int known[MOST_SPLITS + 1] = {-1, -1, -1, -1, -1, -1, -1, -1, -1};
-  if (known[splits] < 0) {
+  static PerDevice<int> known[MOST_SPLITS + 1];   // and one more than them; 0: not asked yet
+  int& here = known[splits].here();
+  if (here == 0) {
     auto kern = split_kernel<CTAS, false, false, SYM, false>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS * splits);
@@ -1151,9 +1145,9 @@ static int resident_clusters(int splits) {
     cfg.numAttrs = 1;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
-    known[splits] = n;
+    here = n + 1;
   }
-  return known[splits];
+  return here - 1;
 }
 struct Form { int ctas, splits; };
 // The form of a product by what its rounds of tiles take, in us: 64 of the reduction 0.28 on a single CTA (its operands from L2 at 64 bytes a clock) and 0.30 on a pair, up to 0.36 and 0.43
@@ -1191,11 +1185,11 @@ template <int CTAS, bool A_MN, bool B_MN, int KIND, bool TURN>
 static int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& s, Params p, int splits, int workers, cudaStream_t st) {
   auto kern = product_kernel<CTAS, A_MN, B_MN, KIND, TURN>;
   auto split = split_kernel<CTAS, A_MN, B_MN, KIND, TURN>;
-  static bool configured = false;
-  if (!configured) {
+  static PerDevice<bool> configured;
+  if (bool& done = configured.here(); !done) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
         cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -4;
-    configured = true;
+    done = true;
   }
   const long long tile = BM * CTAS, tm = (p.M + tile - 1) / tile, tn = (p.N + tile - 1) / tile;
   const long long items = (KIND == SYM ? tm * (tm + 1) / 2 : tm * tn) * p.stack;
@@ -1237,8 +1231,9 @@ static Layout layout(long long rows, long long cols, long long stack) {
 
 // Clusters of `parts` CTAs that can be resident at once, 0 where the device takes none of that size.
 static int small_room(int parts) {
-  static int known[SMALL_PARTS + 1] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
-  if (known[parts] < 0) {
+  static PerDevice<int> known[SMALL_PARTS + 1];   // and one more than them; 0: not asked yet
+  int& here = known[parts].here();
+  if (here == 0) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -1249,9 +1244,9 @@ static int small_room(int parts) {
     if (cudaFuncSetAttribute(small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, small_smem(SMALL_ENTRIES)) != cudaSuccess ||
         cudaFuncSetAttribute(small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, small_kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
-    known[parts] = n;
+    here = n + 1;
   }
-  return known[parts];
+  return here - 1;
 }
 // Whether a call is one launch, and how that divides a matrix: false where it does not fit one, or would take longer so. By sizes and the device alone.
 static bool small_form(Small& p, long long stack) {
@@ -1303,7 +1298,7 @@ static int orthogonalise(const Source& src, long long rows, long long cols, long
   if (stack * l.chunks >= 1ll << 31) return -10;
   launch_pdl(squares_kernel, static_cast<unsigned>(stack * l.chunks), LIN_THREADS, 0, st, src, numel, static_cast<int>(l.chunks), per_chunk, vec_flat, sums);
   const int kept = steps > 2 ? steps - 2 : steps - 1;   // steps whose X is held as two numbers
-  long long blocks = (rows * ((cols + 7) / 8) + LIN_THREADS - 1) / LIN_THREADS, most = (sm_count() * 8 + stack - 1) / stack;
+  long long blocks = (rows * ((cols + 7) / 8) + LIN_THREADS - 1) / LIN_THREADS, most = (sms_here() * 8 + stack - 1) / stack;
   if (blocks > most) blocks = most;
   launch_pdl(scale_kernel, static_cast<unsigned>(stack * blocks), LIN_THREADS, 0, st, src, static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(l.ld), static_cast<int>(l.chunks),
              static_cast<int>(blocks), vec_rows, p2, sums, x[0][0], kept > 0 ? x[0][1] : nullptr);
@@ -1318,7 +1313,7 @@ static int orthogonalise(const Source& src, long long rows, long long cols, long
   if (!rc) rc = poly.make();
   if (rc) return rc - 30;
 
-  const int sms = sm_count();
+  const int sms = sms_here();
   const int r = static_cast<int>(l.r), K = static_cast<int>(right ? rows : cols);
   const Form fg = choose(r, r, K, stack, true, pairs, sms), fp = choose(r, r, r, stack, true, pairs, sms), fa = choose(rows, cols, r, stack, false, pairs, sms);
 #define PRODUCT(F, A_MN, B_MN, KIND, TURN, ...) (F.ctas == 2 ? launch<2, A_MN, B_MN, KIND, TURN>(__VA_ARGS__, F.splits, pairs, st) : launch<1, A_MN, B_MN, KIND, TURN>(__VA_ARGS__, F.splits, sms, st))
@@ -1391,7 +1386,7 @@ int mtb200_newton_schulz(const void* g, int g_bf16, void* out, long long rows, l
   if (rc || direct) return rc;
   const long long n = stack * rows * cols;
   long long blocks = (n + LIN_THREADS - 1) / LIN_THREADS;
-  if (blocks > sm_count() * 16) blocks = sm_count() * 16;
+  if (blocks > mtb::sms_here() * 16) blocks = mtb::sms_here() * 16;
   mtb::launch_pdl(unpad_kernel, static_cast<unsigned>(blocks), LIN_THREADS, 0, st, (const __nv_bfloat16*)to, static_cast<int>(l.ld), stack * rows, static_cast<int>(cols), (__nv_bfloat16*)out);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
@@ -1414,7 +1409,7 @@ int mtb200_muon_step(float* master, void* m, int m_bf16, const void* g, int g_bf
   const __half* o = reinterpret_cast<const __half*>(w + 2 * (steps & 1) * l.xbytes);
   const int vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(master) | reinterpret_cast<uintptr_t>(param)) & 15) == 0;
   long long blocks = (stack * rows * ((cols + 7) / 8) + LIN_THREADS - 1) / LIN_THREADS;
-  if (blocks > sm_count() * 8) blocks = sm_count() * 8;
+  if (blocks > mtb::sms_here() * 8) blocks = mtb::sms_here() * 8;
   mtb::launch_pdl(update_kernel, static_cast<unsigned>(blocks), LIN_THREADS, 0, st, master, (__nv_bfloat16*)param, o, static_cast<int>(l.ld), stack * rows, static_cast<int>(cols), vec, keep,
                   static_cast<float>(ldexp(step, -p2)));
   return cudaGetLastError() == cudaSuccess ? 0 : -5;

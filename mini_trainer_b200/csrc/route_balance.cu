@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "per_device.h"
 #include "ptx.cuh"
 
 namespace mtb {
@@ -457,14 +458,6 @@ inline int run_of(int tokens, int sms) {
 }
 inline bool sizes_ok(int T, int E, int k, int S) { return T > 0 && E > 0 && E <= MOST_EXPERTS && k > 0 && k <= MOST_CHOSEN && k <= E && S > 0; }
 inline int ok() { return cudaGetLastError() == cudaSuccess ? 0 : -5; }
-inline int sms_of() {
-  static int sms = 0;
-  if (sms == 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
-  }
-  return sms;
-}
 
 }  // namespace rb
 }  // namespace mtb
@@ -481,7 +474,7 @@ using namespace mtb::rb;
 int mtb200_route_balanced(const void* logits, int fp32, const int* cu, const void* counted, int T, int E, int k, int S, int renorm, float* probs, long long* topi, float* w,
                           float* lse, float* inverse, int* sample, void* part, void* part_z, int rows, float* balance, float* zloss, int* counts, int* ns, float* usage, cudaStream_t st) {
   if (!sizes_ok(T, E, k, S) || (cu == nullptr && S != 1)) return -10;
-  const int run = run_of(T, sms_of()), blocks = (T + run - 1) / run;
+  const int run = run_of(T, mtb::sms_here()), blocks = (T + run - 1) / run;
   if (rows < blocks + S) return -11;
   const int per = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
   const bool vec = E % per == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(probs)) & 15) == 0;
@@ -500,7 +493,7 @@ int mtb200_route_balanced_bwd(const float* probs, const long long* topi, const f
   if (!sizes_ok(T, E, k, S)) return -10;
   const int per = E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
   int blocks = (T + BWD_WARPS - 1) / BWD_WARPS;
-  if (blocks > bwd_blocks(per) * sms_of()) blocks = bwd_blocks(per) * sms_of();
+  if (blocks > bwd_blocks(per) * mtb::sms_here()) blocks = bwd_blocks(per) * mtb::sms_here();
   const bool vec = E % per == 0 && ((reinterpret_cast<uintptr_t>(dlogits) | reinterpret_cast<uintptr_t>(probs) | reinterpret_cast<uintptr_t>(usage)) & 15) == 0;
 #define BWD(T_, PER, VEC) mtb::launch_pdl(route_bwd_kernel<T_, PER, VEC>, blocks, BWD_THREADS, 0, st, probs, topi, w, dw, lse, inverse, sample, usage, ns, dbalance, dz, T, E, k, S, renorm, (T_*)dlogits, status)
 #define BWD_TYPE(PER) if (fp32) { if (vec) BWD(float, PER, true); else BWD(float, PER, false); } else { if (vec) BWD(bf16, PER, true); else BWD(bf16, PER, false); }
