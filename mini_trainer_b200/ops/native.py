@@ -290,7 +290,7 @@ class NativeOps:
         """Arrival counters of a stream's split launches (32 KB). Launches of one stream run one after the other, those of different
         streams may overlap, so each stream has its own (the last eight streams do; dropped ones go back to their stream's
         pool, behind the launches that use them). ``None`` under capture: a graph may be replayed beside anything, so its
-        launches never split."""
+        launches do not split on a stream's counters, and without some of the graph's own (``own_counters``) not at all."""
         if torch.cuda.is_current_stream_capturing():
             return None
         ws = self._gemm_ws.get(stream)
@@ -302,14 +302,23 @@ class NativeOps:
         return ws
 
     def own_counters(self):
-        """Arrival counters for the ``gemm`` calls of an operator that is being captured, so that they may split as outside of a graph: the graph's own, set to zero by every replay. ``None`` without a capture."""
-        return torch.zeros(_SPLIT_COUNTERS, dtype=torch.int64, device=self.device) if torch.cuda.is_current_stream_capturing() else None
+        """Arrival counters for the ``gemm`` calls of an operator that is being captured, so that they may split as outside of a graph: the graph's own, set to zero by every replay. A function that gives them,
+        and makes them for the first product that splits: 32 KB and a node of the graph. ``None`` without a capture."""
+        if not torch.cuda.is_current_stream_capturing():
+            return None
+        made = []
+
+        def counters():
+            if not made:
+                made.append(torch.zeros(_SPLIT_COUNTERS, dtype=torch.int64, device=self.device))
+            return made[0]
+        return counters
 
     def _split(self, stream, nbytes, counters=None):
         """``(counters, epoch, partials)`` of a split launch, or ``None`` where it has to run whole. The partials are scratch of this call:
         taken from the allocator (in powers of two, at most 128 MB) and given back behind the launch, so nothing is held
         between calls, and without memory for them the launch simply does not split."""
-        ws = self._split_workspace(stream) if counters is None else counters
+        ws = self._split_workspace(stream) if counters is None else counters()
         if ws is None:
             return None
         try:
@@ -354,7 +363,7 @@ class NativeOps:
         """out[M,N] = alpha*A*B (+bias) (+residual). ``a_mn``/``b_mn``: operand stored [K, rows].
         ``stats`` [M, ceil(N / 256), 2] fp32 receives the softmax statistics of the (bf16) output rows per 256 columns.
         ``two_cta``: force (True) or forbid (False) the cta_group::2 kernel; default by problem size. Without CTA pairs on the
-        device the one-CTA kernel runs in any case. ``counters``: of the caller's own, for a product that is split (``own_counters``)."""
+        device the one-CTA kernel runs in any case. ``counters``: the caller's ``own_counters``, for a product that is split."""
         out_f32 = out.dtype == torch.float32
         assert a.dtype == torch.bfloat16 and b.dtype == torch.bfloat16
         assert residual is None or residual.dtype == out.dtype

@@ -1,4 +1,6 @@
 """Arguments of ``linear_nll`` and its gradient at the edges of what is documented: memory that is shared, targets outside the vocabulary, what a captured call takes."""
+import ctypes
+
 import pytest
 import torch
 
@@ -83,3 +85,43 @@ def test_targets_outside_the_vocabulary(dtype):
 def test_targets_outside_the_vocabulary_by_the_kernels():
     from mini_trainer_b200.ops import get_ops
     targets_outside(get_ops(torch.device("cuda:0")), "cuda", torch.bfloat16)
+
+
+@pytest.mark.parametrize("capturing", [False, True])
+def test_arrival_counters_are_made_where_a_product_splits(monkeypatch, capturing):
+    """Under capture a call has counters of its own, one set for all of its products that split and none where none does; outside of a graph a stream's are used."""
+    from .test_native_host import make_ops
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    made, zeros = [], torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, **k: made.append(a) or zeros(*a, **k))
+    ops = make_ops()
+    ops.check_device = lambda t: None
+    stream = zeros(1, dtype=torch.int64)
+    ops._split_workspace = lambda st: stream
+    for T, H, V, splits in ((6, 16, 24, False), (64, 256, 30016, True), (64, 1024, 30016, True)):
+        v = arguments(T, H, V)
+        made.clear(), ops.calls.clear()
+        ops.linear_nll_bwd(**v)
+        products = [a for n, a in ops.calls if n.startswith("mtb200_gemm") and n != "mtb200_gemm_nll"]
+        divided = [a for a in products if a[16] > 1]
+        assert len(products) == 2 and bool(divided) == splits
+        assert len(made) == (capturing and splits)
+        own = {a[17] for a in divided}
+        assert len(own) == splits and all((a == stream.data_ptr()) != capturing for a in own)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,V,splits", [(5, 64, 500, False), (64, 1024, 30016, True)])
+def test_a_captured_gradient_is_its_launches(T, H, V, splits):
+    """Nothing in the graph beside the kernels, and one set of counters where a product splits."""
+    from mini_trainer_b200.ops import get_ops
+    ops = get_ops(torch.device("cuda:0"))
+    v = {k: t.cuda() for k, t in arguments(T, H, V).items()}
+    ops.linear_nll_bwd(**v)
+    graph, before, n = torch.cuda.CUDAGraph(keep_graph=True), ops.launches, ctypes.c_size_t()
+    with torch.cuda.graph(graph):
+        held = ops.linear_nll_bwd(**v)
+    assert ctypes.CDLL("libcuda.so.1").cuGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n)) == 0
+    assert n.value == ops.launches - before + splits and held.shape == v["x"].shape
+    ops.check_status()
