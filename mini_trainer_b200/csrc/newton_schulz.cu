@@ -606,6 +606,27 @@ __device__ __forceinline__ void source8(const Source& s, float coef, long long i
   for (int j = 0; j < 8; ++j) u[j] = s.nesterov ? fmaf(s.mu, m[j], u[j]) : m[j];
 }
 
+// Sum of eight squares. In fp32, but where that is past its range the numbers themselves need not be (from 1.8e19 on): those again in 64 bits.
+__device__ __forceinline__ double squares8(const float (&u)[8]) {
+  float q = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q = fmaf(u[j], u[j], q);
+  double sum = q;
+  if (!(q <= 3.4028234e38f)) {
+    sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { const double x = u[j]; sum = fma(x, x, sum); }
+  }
+  return sum;
+}
+// What takes a matrix with these squares to X0 2^p, as two factors: one alone would be too small a number of the type for the largest matrices.
+struct Factor { float first, second; };
+__device__ __forceinline__ Factor factor_of(double squares, int p2) {
+  const double norm = sqrt(squares) + 1e-7;
+  const bool large = norm > 0x1p100;
+  return Factor{large ? 0x1p-64f : 1.f, static_cast<float>(ldexp(1.0, large ? p2 + 64 : p2) / norm)};
+}
+
 // Sums of squares of the chunks of each matrix, [stack, chunks]; the momentum's update on the way.
 __global__ void __launch_bounds__(LIN_THREADS) squares_kernel(Source s, long long numel, int chunks, long long per_chunk, int vec, double* __restrict__ sums) {
   __shared__ double sh[LIN_THREADS / 32];
@@ -614,12 +635,7 @@ __global__ void __launch_bounds__(LIN_THREADS) squares_kernel(Source s, long lon
   const long long lo = c * per_chunk, hi = min(numel, lo + per_chunk), base = z * numel;
   const float coef = s.coef != nullptr ? *s.coef : 1.f;
   double total = 0.0;
-  auto add = [&](const float (&u)[8]) {
-    float q = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q = fmaf(u[j], u[j], q);
-    total += q;
-  };
+  auto add = [&](const float (&u)[8]) { total += squares8(u); };
   constexpr int STEP = LIN_THREADS * 8, AHEAD = 4;
   long long i = lo + threadIdx.x * 8;
   for (; i + (AHEAD - 1) * STEP + 8 <= hi; i += AHEAD * STEP) {   // several loads under way
@@ -649,7 +665,7 @@ __global__ void __launch_bounds__(LIN_THREADS) squares_kernel(Source s, long lon
 __global__ void __launch_bounds__(LIN_THREADS) scale_kernel(Source s, int rows, int cols, int ld, int chunks, int blocks_per, int vec, int p2, const double* __restrict__ sums,
                                                            __half* __restrict__ hi, __half* __restrict__ lo) {
   __shared__ double sh[LIN_THREADS / 32];
-  __shared__ float factor_sh;
+  __shared__ Factor factor_sh;
   pdl_wait();
   const int z = blockIdx.x / blocks_per, blk = blockIdx.x - z * blocks_per;
   double total = 0.0;
@@ -660,10 +676,11 @@ __global__ void __launch_bounds__(LIN_THREADS) scale_kernel(Source s, int rows, 
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < LIN_THREADS / 32; ++i) total += sh[i];
-    factor_sh = static_cast<float>(ldexp(1.0, p2) / (sqrt(total) + 1e-7));
+    factor_sh = factor_of(total, p2);
   }
   __syncthreads();
-  const float factor = factor_sh, coef = s.coef != nullptr ? *s.coef : 1.f;
+  const Factor f = factor_sh;
+  const float coef = s.coef != nullptr ? *s.coef : 1.f;
   const int per_row = (cols + 7) / 8;   // (what pads a row is never read)
   const long long units = static_cast<long long>(rows) * per_row, base = static_cast<long long>(z) * rows * cols, out = static_cast<long long>(z) * rows * ld;
   for (long long u = static_cast<long long>(blk) * LIN_THREADS + threadIdx.x; u < units; u += static_cast<long long>(blocks_per) * LIN_THREADS) {
@@ -674,7 +691,7 @@ __global__ void __launch_bounds__(LIN_THREADS) scale_kernel(Source s, int rows, 
     uint32_t h[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float a = x[2 * j] * factor, b = x[2 * j + 1] * factor;
+      const float a = x[2 * j] * f.first * f.second, b = x[2 * j + 1] * f.first * f.second;
       h[j] = pack_f16(a, b);
       const float2 r = unpack_f16(h[j]);
       l[j] = pack_f16((a - r.x) * (1 << LO_BITS), (b - r.y) * (1 << LO_BITS));
@@ -802,7 +819,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
   uint64_t *sums_bar = done_bar + 1, *a_bar = done_bar + 2;   // of the sums that are finished here, and of A from the others
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 3);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* factor = reinterpret_cast<float*>(tmem_slot + 2);
+  Factor* factor = reinterpret_cast<Factor*>(tmem_slot + 2);
   __shared__ double warp_sums[SMALL_THREADS / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, sub = warp >> 2;   // a quarter of the rows, a quarter of the columns
   const int parts = p.parts, rank = parts > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -843,10 +860,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       if (b == 1 && i0 + SMALL_THREADS >= tasks) break;
-      float sq = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sq = fmaf(u[b][j], u[b][j], sq);
-      total += sq;
+      total += squares8(u[b]);
       *piece_at(hi, row[b], piece[b], R) = make_uint4(__float_as_uint(u[b][0]), __float_as_uint(u[b][1]), __float_as_uint(u[b][2]), __float_as_uint(u[b][3]));
       *piece_at(lo, row[b], piece[b], R) = make_uint4(__float_as_uint(u[b][4]), __float_as_uint(u[b][5]), __float_as_uint(u[b][6]), __float_as_uint(u[b][7]));
     }
@@ -878,10 +892,10 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
   if (threadIdx.x == 0) {
     total = 0.0;
     for (int t = 0; t < parts; ++t) total += norm[t];
-    *factor = static_cast<float>(ldexp(1.0, p.p2) / (sqrt(total) + 1e-7));
+    *factor = factor_of(total, p.p2);
   }
   __syncthreads();
-  const float f0 = *factor;
+  const Factor f0 = *factor;
   for (int i = threadIdx.x; i < tasks; i += SMALL_THREADS) {
     int row, piece;
     task(i, row, piece);
@@ -890,7 +904,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const Source sr
     uint32_t h[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float c = __uint_as_float(u[2 * j]) * f0, d = __uint_as_float(u[2 * j + 1]) * f0;
+      const float c = __uint_as_float(u[2 * j]) * f0.first * f0.second, d = __uint_as_float(u[2 * j + 1]) * f0.first * f0.second;
       h[j] = pack_f16(c, d);
       const float2 b = unpack_f16(h[j]);
       l[j] = pack_f16((c - b.x) * (1 << LO_BITS), (d - b.y) * (1 << LO_BITS));

@@ -4,7 +4,7 @@
 
     ``X = g / (|g| + 1e-7)``, then ``steps`` times ``X <- (a I + b A + c A^2) X`` with ``A = X X^T``, ``(a, b, c) = (3.4445, -4.7750, 2.0315)``:
 
-singular vectors stay, singular values above about a thousandth of the norm end between 0.7 and 1.2. A zero matrix stays zero; what is not finite stays in its matrix.
+singular vectors stay, singular values above about a thousandth of the norm end between 0.7 and 1.2. A zero matrix stays zero; what is not finite stays in its matrix. Matrices may be as large as their type allows.
 
 ``muon_step`` is one step of a parameter, or of a stack of parameters of one shape, in place:
 
@@ -68,7 +68,9 @@ def check_muon(master, moment, grad, param_out, lr, momentum, weight_decay, grad
 def _iterate(x, steps):
     a, b, c = NS
     x = x.float()
-    x = x / (torch.linalg.matrix_norm(x, keepdim=True) + EPS)
+    norm = torch.linalg.matrix_norm(x, keepdim=True)
+    small = x * 2.0 ** -96   # where the squares are past the type's range, the numbers need not be
+    x = torch.where(torch.isinf(norm), small / torch.linalg.matrix_norm(small, keepdim=True), x / (norm + EPS))
     right = x.shape[-2] > x.shape[-1]
     for _ in range(steps):
         g = x.mT @ x if right else x @ x.mT

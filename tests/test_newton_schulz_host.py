@@ -9,6 +9,8 @@ import torch
 
 from mini_trainer_b200.ops.torch_ref import TorchOps
 
+from . import test_newton_schulz as ns
+
 CSRC = Path(__file__).resolve().parent.parent / "mini_trainer_b200" / "csrc"
 
 
@@ -152,4 +154,43 @@ def test_launches_counted_are_launches_queued(native, shape, steps):
             kept = run()
         assert native.launches - before == kernels_of(graph)
         del kept
+    native.check_status()
+
+
+def scaled(shape, norm, kind="features", device="cpu", dtype=torch.float32):
+    """Matrices of this norm each."""
+    g = ns.matrices(kind, *shape, device=device).double()
+    return (g / torch.linalg.matrix_norm(g, keepdim=True) * norm).to(dtype)
+
+
+def large_matrices(ops, shape, device, tol):
+    """Finite matrices whose squares are past the range of fp32: in a stack beside others, and a momentum of them."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for norm in (1e18, 4e19, 1e25, 1e31, 1e38):
+            g = scaled(shape, norm, device=device, dtype=dtype)
+            ns.check(ops.orthogonalise(g), g, tol)
+    g = torch.full(shape, 3e38, device=device)
+    g[..., 0, ::2] *= -1.0
+    ns.check(ops.orthogonalise(g), g, 3 * tol)   # (of rank two, with its rows alike: roundings in one direction)
+    stack = torch.stack([scaled(shape, n, device=device) for n in (1.0, 1e30, 1e-3)])
+    one = ops.orthogonalise(stack)
+    ns.check(one, stack, tol)
+    stack[1, ..., 0, 0] = float("inf")
+    bad = ops.orthogonalise(stack)
+    assert torch.equal(bad[0], one[0]) and torch.equal(bad[2], one[2]) and torch.isnan(bad[1]).any()
+    g, w = scaled(shape, 1e25, device=device), torch.zeros(shape, device=device)
+    ops.muon_step(w, torch.zeros_like(g), g, None, 1.0, 0.5, 0.0, nesterov=False, scale=1.0)
+    want = -ns.exact(g)
+    assert (torch.linalg.matrix_norm(w.double() - want) <= tol * torch.linalg.matrix_norm(want)).all()
+
+
+@pytest.mark.parametrize("shape", [(13, 30), (40, 24), (2, 17, 9)])
+def test_large_matrices_plain(shape):
+    large_matrices(TorchOps(), shape, "cpu", 2.0 ** -10)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(13, 30), (40, 24), (128, 600), (2100, 100), (300, 520), (2, 264, 130), (301, 143)])
+def test_large_matrices_by_the_kernels(native, shape):
+    large_matrices(native, shape, "cuda", ns.TOL)
     native.check_status()
