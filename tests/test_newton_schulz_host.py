@@ -194,3 +194,16 @@ def test_large_matrices_plain(shape):
 def test_large_matrices_by_the_kernels(native, shape):
     large_matrices(native, shape, "cuda", ns.TOL)
     native.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(13, 30), (128, 600), (2100, 100), (300, 520), (301, 143), (700, 1100)])
+def test_norms_far_below_epsilon(native, shape):
+    """An entry of X 2^p is held to half of fp16's smallest step, 2^-25, in the last two steps, which carry it on by 3.4445 each, and to 2^-36 in the others, by 485 at most: together 2^-25 (11.9 + 3.5 + 0.3) < 2^-21, so
+    the result is off by 2^-21 sqrt(rows columns) / 2^p in norm at most, beside what it is off anyway; 2^p is within a factor of sqrt(2) of the root of the longer side."""
+    for norm in (1e-8, 1e-11, 1e-13, 1e-15, 1e-18, 1e-30):
+        g = scaled(shape, norm, device="cuda")
+        got, want = native.orthogonalise(g).double(), ns.exact(g)
+        off = (ns.TOL + ns.U / math.sqrt(3)) * want.norm() + 2.0 ** -21 * math.sqrt(2 * min(shape))
+        assert float((got - want).norm()) <= float(off), norm
+    native.check_status()
