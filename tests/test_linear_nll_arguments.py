@@ -125,3 +125,28 @@ def test_a_captured_gradient_is_its_launches(T, H, V, splits):
     assert ctypes.CDLL("libcuda.so.1").cuGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n)) == 0
     assert n.value == ops.launches - before + splits and held.shape == v["x"].shape
     ops.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,V", [(300, 256, 5000), (64, 1024, 30016), (700, 512, 9001), (1, 64, 40000)])
+def test_replays_are_the_calls_outside_of_a_graph(T, H, V):
+    """Losses and gradients bit for bit, products that split their reduction among them."""
+    from mini_trainer_b200.ops import get_ops
+    ops = get_ops(torch.device("cuda:0"))
+    v = {k: t.cuda() for k, t in arguments(T, H, V).items()}
+    v["targets"][::5] = -100
+
+    def run():
+        loss, lse = ops.linear_nll(v["x"], v["w"], v["targets"])
+        dw = torch.empty_like(v["w"])
+        return loss, lse, ops.linear_nll_bwd(v["dloss"], v["x"], v["w"], v["targets"], loss, lse, dw, dlse=v["dlse"]), dw
+    want = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for _ in range(2):
+        for t in held:
+            t.fill_(7)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+    ops.check_status()
