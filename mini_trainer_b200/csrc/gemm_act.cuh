@@ -13,8 +13,8 @@
 //   ACT_NLL    the gradient of a row's loss and log-partition in the place of its logits, from what the forward has left: g = (dloss + dlse) e^(z - lse), and of the target
 //              dloss expm1(-loss) + dlse e^-loss, which is no difference of numbers near one another however likely the target is. Rounded to bf16 once, as an operand of the two products that
 //              follow (operands of 16 bits are what the tensor cores take at this rate; the sum over them is fp32).
-//              Both in fp32 from the accumulator on, and bound by the tensor pipe (96 and 95 % active): 1777 x 2048 x 50021 226 and 231 us (1608 and 1575 TFLOP/s, alone), 5987 x 1536 x 151936 ACT_LSE 1.83 ms
-//              in a loop where the plain product, which stores its logits, takes 2.12.
+//              Both in fp32 from the accumulator on, and bound by the tensor pipe (96 and 95 % active): 1777 x 2048 x 50021 226 and 231 us (1608 and 1575 TFLOP/s, alone), in loops, at
+//              the power cap, 273 (with the losses) and 283, and 5987 x 1536 x 151936 2.07 and 2.18 ms where the plain product, which stores its logits, takes 2.10.
 // Eight warps, two per 32-row quarter: with four (one per scheduler) the arithmetic of a tile took longer than short reductions. They work on
 // 32 columns at a time, staged as boxes of 32 rows x 64 bytes (64B-swizzled). Bound by the product. With its activation, in a loop of its own on a B200:
 // 5987 x 17920 x 1536 272 -> 231 us (product alone 220), 4099 x 12288 x 2048 167 -> 153, 16384 x 28672 x 4096 3.16 -> 2.8 ms, 7001 x 12288 x 3072 without

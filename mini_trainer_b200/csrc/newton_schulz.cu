@@ -4,7 +4,7 @@
 // takes every singular value x of X to a x + b x^3 + c x^5, so those above 1e-3 of the norm or so end near one. A matrix with more rows than columns is multiplied from the right
 // instead, X (a I + b A + c A^2) with A = X^T X: operands of the tensor cores may have either dimension innermost, so nothing is ever transposed. With r the shorter side
 // and n the longer a step is the products r r n, r r r and r r n; the first two are symmetric: only the tiles on and below the diagonal are computed. Of large ones no others are stored, and who reads a block of 64 columns
-// above it loads the rows below instead, the other dimension innermost: the transposes passed through the shared memory that the operands need (they took 4 to 5 % of a call). 3 r^2 n + r^3 operations a step instead of 4 r^2 n + 2 r^3.
+// above it loads the rows below instead, the other dimension innermost: the transposes passed through the shared memory that the operands need (they took 3 to 5 % of a call: 64 x 2048 x 1024 3.00 -> 2.88 ms, 4096 x 4096 1.26 -> 1.22, loops at the power cap). 3 r^2 n + r^3 operations a step instead of 4 r^2 n + 2 r^3.
 //
 // The second product's epilogue adds b A and a I to c A^2, so that the third has the linear term in it.
 //
@@ -17,10 +17,10 @@
 // (0.15, 1.2); half of bf16's step, to which the result is rounded, is 1.7e-3 in the mean. Sums are fp32 in tensor memory.
 //
 // The products: persistent, warp-specialised, 3-D TMA maps over the stack, tcgen05.mma of fp16 into two accumulators in tensor memory, by single CTAs (tiles of 128 x 128, for few tiles) or CTA pairs
-// (256 x 256). All launches of a call are queued by one host call, each under its predecessor's tail. A large call is bound by its products: 4096 x 4096 (1.37 TFLOP in five steps) 1.21 ms in a row under the power cap:
+// (256 x 256). All launches of a call are queued by one host call, each under its predecessor's tail. A large call is bound by its products: 4096 x 4096 (1.37 TFLOP in five steps) 1.22 ms in a row under the power cap:
 // its gram product and square 57 us each at 80 % of the tensor pipe (136 tiles on 74 pairs), its last product 103 us at 88 %. A launch of one round is bound by its chain, about 3.4 us beside its reduction (first
 // operands 1.0, sums to stores 1.5, end to the next one's start 1.4), and on single CTAs by L2, from which an SM takes 64 bytes a clock: 0.25 us for 64 of the reduction. More epilogue warps (sixteen of
-// 32 columns) made it longer: 688 x 256 88 -> 95 us, 1024 x 1024 121 -> 127.
+// 32 columns) made it longer, 688 x 256 by 8 % and 1024 x 1024 by 5 (77 and 109 us with eight, replayed).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -713,7 +713,8 @@ __global__ void __launch_bounds__(LIN_THREADS) unpad_kernel(const __nv_bfloat16*
   pdl_trigger();
 }
 
-// w <- keep w - step o 2^-p of the padded fp16 rows o, and the working copy.
+// w <- keep w - step o 2^-p of the padded fp16 rows o, and the working copy. (A rounding of o to fp16, 2^-11 of an entry at most, is an eighth of the one to bf16 that an orthogonalised matrix is returned with, and below
+// what the products' own operands leave, 2e-3 of its norm; in fp32 the last product would write, and this read, twice the bytes.)
 __global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ param, const __half* __restrict__ o, int ld, long long rows,
                                                             int cols, int vec, float keep, float step) {
   pdl_wait();
@@ -742,7 +743,8 @@ __global__ void __launch_bounds__(LIN_THREADS) update_kernel(float* __restrict__
 // memory of the cluster), which adds them in the order of the slabs and gives A to all; its square, every CTA for itself; the polynomial over A; the last product and the slab's new hi and lo.
 // A slab of at most 64 (32) rows goes through the last product in two (four) parts side by side: the polynomial stands two (four) times on the diagonal of a 128 x 128 operand, the reduction runs over
 // the parts one behind the other, and each part's columns come out in rows of their own, so that all warps have some. Bound by the chain of
-// those, a step takes 2.0 us for 64 x 64, 2.9 for 32 x 256, 5.3 for 128 x 256 and 8.7 in two slabs of it (the other form's launches 14 to 22): 64 x 64 56 -> 15 us, 128 x 512 88 -> 54, 32 x 2048 74 -> 37, 64 x 8192 100 -> 61.
+// those, a step takes 2.5 us for 64 x 64, 2.9 for 32 x 256 and 5.3 for 128 x 256 (the other form's launches 9 to 16). In the other form and so, by rows of launches: 64 x 64 50 and 17 us, 128 x 256 59 and 37 (46 in two slabs), 128 x 512 64 and
+// 52, 32 x 2048 74 and 35, 64 x 8192 85 and 61.
 constexpr int SMALL_R = 128, SMALL_PARTS = 16, SMALL_THREADS = 512, SMALL_ENTRIES = 128 * 256;   // most of a slab
 constexpr int SMALL_A = 2 * SMALL_R * 128, SMALL_RECV = 16 * 4096;
 constexpr int small_smem(int entries) { return 4 * entries + SMALL_A + SMALL_RECV + 1024 + 256; }
@@ -1165,9 +1167,9 @@ static int resident_clusters(int splits) {
 }
 struct Form { int ctas, splits; };
 // The form of a product by what its rounds of tiles take, in us: 64 of the reduction 0.28 on a single CTA (its operands from L2 at 64 bytes a clock) and 0.30 on a pair, up to 0.36 and 0.43
-// where all SMs multiply at once; and what stands in front of and behind them. Fitted to stacks of 1 to 64 matrices of 64 to 4096: 1024 x 1024 122 us in single CTAs and 201 in pairs, 4096 x 4096 1370 and 1114, 512 x 512 95 and 163, in
-// parts of a half 116 and 157; 1001 x 4097 299 and 327, 239 with the gram product on pairs in four parts; 1536 x 8960 466 and 520, 422 with it on single CTAs in two;
-// 64 x 28672 198 with it in four parts and 147 in eight, 256 x 14336 163 and 139.
+// where all SMs multiply at once; and what stands in front of and behind them. Fitted to stacks of 1 to 64 matrices of 64 to 4096 when each launch took half a microsecond longer than now, so it is the order of the forms that holds: whole calls take 113 us for 1024 x 1024 in
+// single CTAs and 175 in pairs, 4096 x 4096 1512 and 1220, 512 x 512 85 and 151, in parts of a half 106 and 148; 1001 x 4097 209 and 269, 197 with the gram product on pairs in four parts; 1536 x 8960 498 and 495, 426 with the gram
+// product on pairs in two parts and the last on pairs, 470 with it on single CTAs in two; 64 x 28672 188 with it on single CTAs in four parts and 138 in eight, 256 x 14336 154 and 131.
 static Form choose(long long M, long long N, long long K, long long stack, bool sym, int pairs, int sms) {
   constexpr double base[2][4] = {{3.0, 6.0, 6.8, 7.6}, {8.0, 8.7, 9.1, 0.0}};
   auto tiles = [&](long long tile) {
@@ -1237,7 +1239,7 @@ static Layout layout(long long rows, long long cols, long long stack) {
   const long long numel = rows * cols;
   long long most = MOST_CHUNKS / stack;
   if (most < 1) most = 1;
-  l.chunks = (numel + 4095) / 4096;   // (16384 each: a step of 576 x 576 108 us instead of 105, 16 x 512 x 512 154 instead of 149; 2048: level)
+  l.chunks = (numel + 4095) / 4096;   // (16384 each took 3 us longer for a step of 576 x 576, now 94, and 5 for 16 x 512 x 512, now 142; 2048: level)
   if (l.chunks > most) l.chunks = most;
   l.total = 4 * l.xbytes + 2 * l.gbytes + up(stack * l.chunks * 8, 256);
   return l;
@@ -1271,8 +1273,8 @@ static bool small_form(Small& p, long long stack) {
   p.R = p.r <= 32 && p.n > 128 ? 32 : p.r <= 64 && p.n > 64 ? 64 : 128;   // a slab's parts have 64 columns at least
   p.kept = p.steps > 2 ? p.steps - 2 : p.steps - 1;
   const int most = SMALL_ENTRIES / p.R, step = 64 * (SMALL_R / p.R);
-  // Rounds of clusters, of what a slab's size takes and what its exchange does, in us, against fifteen launches that pass over the matrices six times a step: 32 x 2048 47 as two slabs and 37 as eight, 128 x 128 27 as
-  // one and 38 as two, 64 x 128 x 1024 (two rounds of clusters of four) 157 and 130 in the other form.
+  // Rounds of clusters, of what a slab's size takes and what its exchange does, in us, against fifteen launches that pass over the matrices six times a step: 32 x 2048 48 as two slabs and 35 as eight, 128 x 128 28 as
+  // one and 41 as two, 64 x 128 x 1024 (two rounds of clusters of four) 132 and 123 in the other form.
   double least = 75.0 + static_cast<double>(stack) * p.r * p.n * 6.5e-6;
   p.parts = 0;
   for (int parts = 1; parts <= SMALL_PARTS; parts *= 2) {
@@ -1332,8 +1334,8 @@ static int orthogonalise(const Source& src, long long rows, long long cols, long
   const Form fg = choose(r, r, K, stack, true, pairs, sms), fp = choose(r, r, r, stack, true, pairs, sms), fa = choose(rows, cols, r, stack, false, pairs, sms);
 #define PRODUCT(F, A_MN, B_MN, KIND, TURN, ...) (F.ctas == 2 ? launch<2, A_MN, B_MN, KIND, TURN>(__VA_ARGS__, F.splits, pairs, st) : launch<1, A_MN, B_MN, KIND, TURN>(__VA_ARGS__, F.splits, sms, st))
 #define PRODUCT_SYM(F, A_MN, B_MN, KIND, ...) (turn ? PRODUCT(F, A_MN, B_MN, KIND, true, __VA_ARGS__) : PRODUCT(F, A_MN, B_MN, KIND, false, __VA_ARGS__))
-  // Where the matrix is two blocks wide the launches are short, and the transposes cost less than what each of them has to think about: 8 x 2048 x 512 178 us and 183, 4 x 512 x 1376 129 and 131; 64 x 2048 x 1024
-  // 2640 and 2500, 4096 x 4096 1270 and 1206.
+  // Where the matrix is two blocks wide the launches are short, and the transposes cost less than what each of them has to think about: 8 x 2048 x 512 175 us with the transposes and 179 without, 4 x 512 x 1376 120 and 122; larger
+  // ones, in loops at the power cap: 64 x 2048 x 1024 3.00 ms and 2.88, 4096 x 4096 1.26 and 1.22, 5120 x 5120 2.36 and 2.28.
   const bool turn = r > 2 << WHOLE_BITS;
   for (int i = 0; i < steps; ++i) {
     const Matrix& X = xh[i & 1];

@@ -158,7 +158,7 @@ def native_bwd(ops, dloss, x, w, targets, loss, lse, dw_out, accumulate_dw=False
         ldz = -(-n // 64) * 64   # rows of whole 128 bytes
         dz = torch.empty(T, ldz, dtype=torch.bfloat16, device=x.device)
         dx32 = torch.empty(T, H, dtype=torch.float32, device=x.device) if n < V else None
-        form, scale, own = _form(ops, T, H), float(logit_scale), ops.own_counters()   # (64 rows of 1024, 151936 columns, captured: 198 us, and 651 with the sum over the vocabulary in one part)
+        form, scale, own = _form(ops, T, H), float(logit_scale), ops.own_counters()   # (64 rows of 1024, 151936 columns, captured: 202 us, and 650 with the sum over the vocabulary in one part)
         for a in range(0, V, n):
             c = min(n, V - a)
             wc, dwc = (w, dw_out) if c == V else (w[a:a + c], dw_out[a:a + c])
