@@ -4,8 +4,9 @@
 
     ``X = g / (|g| + 1e-7)``, then ``steps`` times ``X <- (a I + b A + c A^2) X`` with ``A = X X^T``, ``(a, b, c) = (3.4445, -4.7750, 2.0315)``:
 
-singular vectors stay, singular values above about a thousandth of the norm end between 0.7 and 1.2. A zero matrix stays zero; what is not finite stays in its matrix. Matrices may be as large as their type allows. A norm far below 1e-7 makes the result itself next to nothing:
-the kernels hold it to 2^-20 of the norm that an orthogonal matrix of that size has, which is less than three digits of the result where the norm is below 1e-12.
+singular vectors stay, singular values above about a thousandth of the norm end between 0.7 and 1.2. A zero matrix stays zero; what is not finite stays in its matrix. Matrices may be as large as their type allows.
+The kernels' result is 2e-3 to 4e-3 of its norm off, the rounding to bf16 included (matrices of a few rows, columns or entries: up to 2e-2). A norm far below 1e-7 makes the result itself next to nothing: they hold it to 2^-20 of
+the norm that an orthogonal matrix of that size has, which is less than three digits of the result where the norm is below 1e-12.
 
 ``muon_step`` is one step of a parameter, or of a stack of parameters of one shape, in place:
 
